@@ -29,6 +29,11 @@ extern "C" {
 #define MOE_Q8_0 0
 #define MOE_Q4_0 1
 #define MOE_AWQ 2
+#define MOE_MXFP4 3 /* OCP Microscaling e2m1, blocks of 32, e8m0 scales */
+
+/* scores of moe_route_scored */
+#define MOE_SCORE_SOFTMAX 0
+#define MOE_SCORE_SIGMOID 1
 
 /* element types of activations, scales and weight inputs */
 #define MOE_F16 0
@@ -41,7 +46,7 @@ typedef struct moe_config {
     int64_t num_experts;       /* experts held by this engine (E, or E/ep_size under EP) */
     int64_t hidden_size;       /* H, multiple of 32 (of the AWQ group for AWQ) */
     int64_t intermediate_size; /* I, multiple of 32 (of the AWQ group for AWQ) */
-    int32_t quant_type;        /* MOE_Q8_0 / MOE_Q4_0 / MOE_AWQ */
+    int32_t quant_type;        /* MOE_Q8_0 / MOE_Q4_0 / MOE_AWQ / MOE_MXFP4 */
     int32_t group_size;        /* AWQ group along K (128); ignored otherwise */
     int32_t device;            /* CUDA device ordinal */
     int32_t expert_offset;     /* global id of this engine's first expert (EP); 0 otherwise */
@@ -66,7 +71,8 @@ int moe_engine_load_quantized(moe_engine* eng, const void* gate_up_qs, const voi
                               int32_t src_on_device, void* stream);
 
 /* Replaces MoEInfer::quantize_and_store_expert (Int8-gemm/moe_infer.cpp:284-360) with
- * quantize_weight_only (Int8-gemm/q8_gemm.cpp:219-260): Q8_0 only, fp16 scales.
+ * quantize_weight_only (Int8-gemm/q8_gemm.cpp:219-260): Q8_0 (fp16 scales) and MXFP4
+ * (by the rule of moe_quantize_rows_mxfp4).
  * proj: 0 = gate_proj [I,H], 1 = up_proj [I,H], 2 = down_proj [H,I];
  * w_dtype MOE_F32 / MOE_F16 / MOE_BF16. */
 int moe_engine_quantize_store_expert(moe_engine* eng, int64_t expert, int32_t proj, const void* w,
@@ -80,6 +86,23 @@ int moe_engine_quantize_store_expert(moe_engine* eng, int64_t expert, int32_t pr
 int moe_engine_load_awq(moe_engine* eng, const void* w13_qweight, const void* w13_scales,
                         const void* w13_qzeros, const void* w2_qweight, const void* w2_scales,
                         const void* w2_qzeros, int32_t src_on_device, void* stream);
+
+/* MXFP4 weights (no counterpart in the reference).  Row-major, host or device memory (device
+ * codes 16-byte aligned):
+ *   w13_q uint8 [E,2I,H/2], w2_q uint8 [E,H,I/2]: e2m1 codes, two a byte, the even element in
+ *   the low half; w13_s uint8 [E,2I,H/32], w2_s uint8 [E,H,I/32]: e8m0 scales.
+ * Rows [0,I) of w13 are gate_proj, rows [I,2I) up_proj.  At most 1024 experts.
+ * The forward of such an engine quantises the token rows and h to MXFP4 too (both by the rule
+ * of moe_quantize_rows_mxfp4) and multiplies codes by codes, accumulating in fp32:
+ *   y = sum_k w_k * down(MX(SiLU(gate MX(x)) * (up MX(x)))).
+ * A token row or an h block with an infinity or a NaN gives NaN.  x and y must be 16-byte
+ * aligned.  The workspace is the engine's: eager calls on different streams are put in order,
+ * replays of captured graphs that hold its calls must not overlap one another or such calls.
+ * A call that is captured needs moe_engine_reserve (or an earlier call of that size) first; the
+ * graph stays valid when the workspace grows later.  The peer combine and the no-allocation
+ * forward refuse such an engine. */
+int moe_engine_load_mxfp4(moe_engine* eng, const uint8_t* w13_q, const uint8_t* w13_s, const uint8_t* w2_q,
+                          const uint8_t* w2_s, int32_t src_on_device, void* stream);
 
 /* Replaces MoEInfer::execute_on_cpu_routed_from_pointers (Int8-gemm/moe_infer.cpp:430-456)
  * -> moe_forward_ptr_impl (Int8-gemm/q8_gemm.cpp:276-646).  All pointers on the engine's
@@ -117,7 +140,8 @@ int moe_engine_device_error(moe_engine* eng, int32_t* code);
  * (bit-exact check of the load-time packing).  which: 0 gate_up (2I rows of H), 1 down
  * (H rows of I).  Q8_0/Q4_0: qs_out / d_out receive the input-contract rows.  AWQ: qs_out
  * receives per row the K/2 bytes of sequential nibbles (element k at byte k/2, low nibble
- * for even k), d_out per row the K/G bf16 scales followed by the K/G zero points (u8). */
+ * for even k), d_out per row the K/G bf16 scales followed by the K/G zero points (u8).
+ * MXFP4: the input-contract rows, K/2 bytes of codes and K/32 scale bytes. */
 int moe_engine_export_expert(moe_engine* eng, int64_t expert, int32_t which, void* qs_out,
                              void* d_out);
 
@@ -138,6 +162,24 @@ int moe_route_gemm_topk(const void* hidden, int32_t act_dtype, const void* route
                         int64_t num_tokens, int64_t hidden_size, int64_t num_experts, int64_t top_k,
                         int32_t renormalize, int32_t* topk_ids, float* topk_w, float* logits, void* stream);
 
+/* Routing by scores (no counterpart in the reference, whose router is a softmax top-k):
+ * logits [T,E] (MOE_F32 / MOE_F16 / MOE_BF16), bias [E] fp32 or null.
+ *   s = sigmoid(logits) or softmax(logits);  c = s + bias
+ *   with num_groups > 1 the experts are num_groups equal consecutive groups; a group's score is
+ *   the sum of its group_top (1 or 2) largest c, and only the experts of the topk_groups best
+ *   groups stay;
+ *   ids = the top_k largest c, descending;  weights = s of those / their sum (renormalize != 0;
+ *   plus 1e-20), times `scale`.
+ * Ties (of groups too) go to the lower index; the order is that of scores in 64 bits.  An expert
+ * is masked where its logit is -infinity or NaN (it then has no part in the softmax) or its
+ * bias is; a group of masked experts is never chosen.  Where fewer than top_k experts remain,
+ * the last ids are -1 with weight 0, which moe_engine_forward skips.  +infinity counts as the
+ * largest float.  E <= 1024, num_groups <= 32, top_k <= min(32, topk_groups * E / num_groups).
+ * Device pointers, stream ordered. */
+int moe_route_scored(const void* logits, int32_t dtype, const float* bias, int64_t num_tokens, int64_t num_experts,
+                     int64_t top_k, int32_t score, int64_t num_groups, int64_t topk_groups, int32_t group_top,
+                     int32_t renormalize, float scale, int32_t* topk_ids, float* topk_w, void* stream);
+
 /* Stable counting sort of routed pairs by expert (Int8-gemm/moe_common.cpp:146-216):
  * counts [E], starts [E+1], token_map [T*K][2] = (t,k) per position, scatter_map [T*K]
  * (-1 for ids outside [0,E)).  Device pointers. */
@@ -150,6 +192,28 @@ int moe_route_permute(const int32_t* topk_ids, int64_t num_tokens, int64_t top_k
  * d fp32 [rows, cols/32].  Device pointers. */
 int moe_quantize_rows_q8_0(const void* x, int32_t dtype, int64_t rows, int64_t cols, int8_t* qs,
                            float* d, void* stream);
+
+/* MXFP4 quantisation of rows (no counterpart in the reference): x [rows, cols] (dtype) ->
+ * codes uint8 [rows, cols/2] (e2m1, the even element in the low half) and one e8m0 scale byte
+ * per 32 elements: s = floor(log2(amax)) - 2 + 127, at least 0; codes = x / 2^(s - 127) rounded
+ * to nearest even, magnitudes above 6 to 6.  A block with an infinity or a NaN gets s = 255 (all
+ * of it decodes to NaN).  scales: row-major [rows, cols/32], or with tiled_scales != 0 the
+ * layout that moe_mxfp4_matmul reads, [ceil(rows/128)][ceil(cols/128)][512] with the scale of
+ * row r and block k of a tile at byte 16 (r % 32) + 4 (r / 32) + k, padding zero.  cols a
+ * multiple of 32; x, codes and tiled scales 16-byte aligned.  Device pointers, stream ordered,
+ * as the three functions below. */
+int moe_quantize_rows_mxfp4(const void* x, int32_t dtype, int64_t rows, int64_t cols, int32_t tiled_scales,
+                            uint8_t* codes, uint8_t* scales, void* stream);
+/* The values of MXFP4 rows in `dtype` (exact in fp32 and bf16; fp16 rounds what it cannot hold). */
+int moe_dequantize_rows_mxfp4(const uint8_t* codes, const uint8_t* scales, int64_t rows, int64_t cols,
+                              int32_t tiled_scales, void* y, int32_t dtype, void* stream);
+/* Row-major scales [rows, cols/32] -> the tiled layout. */
+int moe_mxfp4_tile_scales(const uint8_t* scales, int64_t rows, int64_t cols, uint8_t* tiles, void* stream);
+/* y [M,N] = a [M,K] b [N,K]^T of MXFP4 matrices (codes, tiled scales), fp32 accumulation,
+ * rounded once to out_dtype.  K a multiple of 32; all pointers 16-byte aligned.  A bounded wait
+ * that expires is reported by the next call on the device (MOE_ERR_DEVICE). */
+int moe_mxfp4_matmul(const uint8_t* a, const uint8_t* a_scales, const uint8_t* b, const uint8_t* b_scales, int64_t M,
+                     int64_t N, int64_t K, void* y, int32_t out_dtype, void* stream);
 
 /* Diagnostics (no counterpart in the reference): enable != 0 makes every later decode
  * launch record 20 stamps per CTA (globaltimer ns unless noted).  Persistent decode kernels

@@ -25,6 +25,6 @@ for _p in (LIB_PATH, TORCH_LIB_PATH):
 
 torch.ops.load_library(TORCH_LIB_PATH)
 
-Q8_0, Q4_0, AWQ = 0, 1, 2
+Q8_0, Q4_0, AWQ, MXFP4 = 0, 1, 2, 3
 
 from . import capi  # noqa: E402,F401

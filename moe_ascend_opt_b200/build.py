@@ -44,7 +44,7 @@ def _run(cmd: list[str]) -> None:
 
 def build_capi(verbose_ptxas: bool = False) -> str:
     cu = sorted(glob.glob(os.path.join(CSRC, "*.cu")))
-    headers = sorted(glob.glob(os.path.join(CSRC, "*.cuh"))) + [os.path.join(ROOT, "include", "moe_b200.h")]
+    headers = sorted(glob.glob(os.path.join(CSRC, "*.cuh")) + glob.glob(os.path.join(CSRC, "*.h"))) + [os.path.join(ROOT, "include", "moe_b200.h")]
     os.makedirs(OBJ, exist_ok=True)
     objs = []
     for src in cu:

@@ -13,7 +13,8 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libmoe_b200.so")
 
 MOE_OK, MOE_ERR_INVALID, MOE_ERR_CUDA, MOE_ERR_STATE, MOE_ERR_DEVICE = 0, -1, -2, -3, -4
-Q8_0, Q4_0, AWQ = 0, 1, 2
+Q8_0, Q4_0, AWQ, MXFP4 = 0, 1, 2, 3
+SOFTMAX, SIGMOID = 0, 1
 REPLICATED = 1 << 30
 F16, BF16, F32 = 0, 1, 2
 
@@ -26,6 +27,8 @@ SYMBOLS = [
     "moe_engine_p2p_mailbox", "moe_engine_p2p_connect", "moe_engine_p2p_enable", "moe_engine_p2p_covers",
     "moe_engine_set_expert_map", "moe_route_gemm_topk", "moe_engine_save", "moe_engine_load_file",
     "moe_engine_set_replica_split", "moe_engine_forward_dense",
+    "moe_engine_load_mxfp4", "moe_route_scored", "moe_quantize_rows_mxfp4", "moe_dequantize_rows_mxfp4",
+    "moe_mxfp4_tile_scales", "moe_mxfp4_matmul",
 ]
 
 
@@ -80,6 +83,12 @@ def lib() -> C.CDLL:
             "moe_engine_set_replica_split": [_P, _I32, _I32],
             "moe_engine_forward_dense": [_P, _I64, _P, _P, _I64, _I32, _I32, _P],
             "moe_engine_load_file": [_P, C.c_char_p],
+            "moe_engine_load_mxfp4": [_P, _P, _P, _P, _P, _I32, _P],
+            "moe_route_scored": [_P, _I32, _P, _I64, _I64, _I64, _I32, _I64, _I64, _I32, _I32, C.c_float, _P, _P, _P],
+            "moe_quantize_rows_mxfp4": [_P, _I32, _I64, _I64, _I32, _P, _P, _P],
+            "moe_dequantize_rows_mxfp4": [_P, _P, _I64, _I64, _I32, _P, _I32, _P],
+            "moe_mxfp4_tile_scales": [_P, _I64, _I64, _P, _P],
+            "moe_mxfp4_matmul": [_P, _P, _P, _P, _I64, _I64, _I64, _P, _I32, _P],
         }
         for name, args in sig.items():
             f = getattr(L, name)
@@ -140,6 +149,10 @@ class Engine:
     def load_awq(self, w13_qw, w13_sc, w13_qz, w2_qw, w2_sc, w2_qz, stream=None):
         call("moe_engine_load_awq", self.h, w13_qw.data_ptr(), w13_sc.data_ptr(), w13_qz.data_ptr(),
              w2_qw.data_ptr(), w2_sc.data_ptr(), w2_qz.data_ptr(), int(w13_qw.is_cuda), stream_handle(stream))
+
+    def load_mxfp4(self, w13, w13_scales, w2, w2_scales, stream=None):
+        call("moe_engine_load_mxfp4", self.h, w13.data_ptr(), w13_scales.data_ptr(), w2.data_ptr(), w2_scales.data_ptr(),
+             int(w13.is_cuda), stream_handle(stream))
 
     def forward(self, x, y, ids, w, act_dtype, out_dtype, stream=None):
         call("moe_engine_forward", self.h, x.data_ptr(), y.data_ptr(), ids.data_ptr(), w.data_ptr(),

@@ -13,6 +13,8 @@
 
 #include "../../include/moe_b200.h"
 #include "common.cuh"
+#include "mx_layer.h"
+#include "status.h"
 #include "moe_decode_cl.cuh"
 #include "moe_decode_tp.cuh"
 #include "moe_decode_sk.cuh"
@@ -23,17 +25,10 @@ using namespace moe;
 // ------------------------------------------------------------------ errors
 static thread_local std::string g_last_error;
 
-static int fail(int code, const std::string& msg) {
+int moe::fail(int code, const std::string& msg) {
     g_last_error = msg;
     return code;
 }
-
-#define CUDA_TRY(expr)                                                                       \
-    do {                                                                                     \
-        cudaError_t _e = (expr);                                                             \
-        if (_e != cudaSuccess)                                                               \
-            return fail(MOE_ERR_CUDA, std::string(#expr) + ": " + cudaGetErrorString(_e)); \
-    } while (0)
 
 extern "C" const char* moe_last_error(void) { return g_last_error.c_str(); }
 
@@ -109,6 +104,8 @@ struct moe_engine {
     // grouped-GEMM path workspace (one allocation, carved per call)
     uint8_t* gws = nullptr;
     size_t gws_bytes = 0;
+    MxLayer* mx = nullptr;         // MXFP4: the layer's weights, workspace and kernels (mxfp4.cu)
+    cudaStream_t last_stream = nullptr;  // MXFP4: stream of the last forward (its end is ev1)
     unsigned long long* timeline = nullptr;  // per-CTA phase stamps when enabled
     int timeline_ctas = 0;
 };
@@ -434,6 +431,7 @@ int64_t sk_slice_bytes(const moe_engine* eng) {
 }
 
 int alloc_q_layout(moe_engine* eng) {
+    if (eng->mx) return MOE_OK;  // MXFP4: allocated by mx_create
     const int64_t E = eng->cfg.num_experts, H = eng->cfg.hidden_size, I = eng->cfg.intermediate_size;
     const int qt = eng->cfg.quant_type;
     if (qt == MOE_AWQ) {
@@ -1356,8 +1354,8 @@ extern "C" int moe_engine_create(const moe_config* cfg, moe_engine** out) {
     if (E <= 0 || H <= 0 || I <= 0) return fail(MOE_ERR_INVALID, "E, H, I must be positive");
     if (H % 32 != 0) return fail(MOE_ERR_INVALID, "hidden_size must be multiple of 32");
     if (I % 32 != 0) return fail(MOE_ERR_INVALID, "intermediate_size must be multiple of 32");
-    if (cfg->quant_type < MOE_Q8_0 || cfg->quant_type > MOE_AWQ)
-        return fail(MOE_ERR_INVALID, "quant_type must be 0 (Q8_0), 1 (Q4_0) or 2 (AWQ)");
+    if (cfg->quant_type < MOE_Q8_0 || cfg->quant_type > MOE_MXFP4)
+        return fail(MOE_ERR_INVALID, "quant_type must be 0 (Q8_0), 1 (Q4_0), 2 (AWQ) or 3 (MXFP4)");
     if (cfg->quant_type == MOE_AWQ) {
         const int g = cfg->group_size;
         if (g <= 0 || g % 32 != 0 || H % g != 0 || I % g != 0)
@@ -1404,7 +1402,8 @@ extern "C" int moe_engine_create(const moe_config* cfg, moe_engine** out) {
     if (const char* v = std::getenv("MOE_TP_SLICE_MAX")) eng->tp_slice_max = std::atoi(v);
     if (eng->tp_slice_max < 0) eng->tp_slice_max = cfg->quant_type == MOE_AWQ ? 32 : 0;  // measured crossover
     int rc = MOE_OK;
-    rc = alloc_q_layout(eng);
+    if (cfg->quant_type == MOE_MXFP4) rc = mx_create(*cfg, eng->num_sms, &eng->mx);
+    else rc = alloc_q_layout(eng);
     if (rc == MOE_OK) rc = ensure_workspace(eng, 64);
     if (rc == MOE_OK && (cudaEventCreate(&eng->ev0) != cudaSuccess || cudaEventCreate(&eng->ev1) != cudaSuccess))
         rc = fail(MOE_ERR_CUDA, "cudaEventCreate failed");
@@ -1419,6 +1418,7 @@ extern "C" int moe_engine_create(const moe_config* cfg, moe_engine** out) {
 extern "C" int moe_engine_destroy(moe_engine* eng) {
     if (!eng) return MOE_OK;
     DeviceGuard g(eng->cfg.device);
+    mx_destroy(eng->mx);
     cudaFree(eng->gu);
     cudaFree(eng->dn);
     cudaFree(eng->dk);
@@ -1448,6 +1448,7 @@ extern "C" int moe_engine_load_quantized(moe_engine* eng, const void* gu_qs, con
                                          void* stream) {
     if (int rc = check_engine(eng)) return rc;
     if (eng->cfg.quant_type == MOE_AWQ) return fail(MOE_ERR_STATE, "AWQ engine: use moe_engine_load_awq");
+    if (eng->mx) return fail(MOE_ERR_STATE, "MXFP4 engine: use moe_engine_load_mxfp4");
     if (!gu_qs || !gu_d || !dn_qs || !dn_d) return fail(MOE_ERR_INVALID, "null weight pointer");
     if (scale_dtype != MOE_F16 && scale_dtype != MOE_BF16)
         return fail(MOE_ERR_INVALID, "scales must be float16 or bfloat16");
@@ -1484,8 +1485,8 @@ extern "C" int moe_engine_load_quantized(moe_engine* eng, const void* gu_qs, con
 extern "C" int moe_engine_quantize_store_expert(moe_engine* eng, int64_t expert, int32_t proj, const void* w,
                                                 int32_t w_dtype, int32_t src_on_device, void* stream) {
     if (int rc = check_engine(eng)) return rc;
-    if (eng->cfg.quant_type != MOE_Q8_0)
-        return fail(MOE_ERR_STATE, "online quantization is Q8_0 only; use store_quantized_repack()");
+    if (eng->cfg.quant_type != MOE_Q8_0 && !eng->mx)
+        return fail(MOE_ERR_STATE, "online quantization is Q8_0 and MXFP4 only; use store_quantized_repack()");
     if (!w) return fail(MOE_ERR_INVALID, "null weight");
     if (w_dtype != MOE_F32 && w_dtype != MOE_F16 && w_dtype != MOE_BF16)
         return fail(MOE_ERR_INVALID, "weight must be float32, float16 or bfloat16");
@@ -1500,6 +1501,14 @@ extern "C" int moe_engine_quantize_store_expert(moe_engine* eng, int64_t expert,
     const uint8_t* src = nullptr;
     uint8_t* owned = nullptr;
     if (int rc = stage_to_device(w, (size_t)rows * cols * esz, src_on_device, st, &src, &owned)) return rc;
+    if (eng->mx) {
+        const int rc = mx_quantize_store(eng->mx, expert, proj, src, w_dtype, st);
+        if (owned) CUDA_TRY(cudaFreeAsync(owned, st));
+        if (rc) return rc;
+        CUDA_TRY(cudaStreamSynchronize(st));
+        eng->loaded = true;
+        return MOE_OK;
+    }
     uint8_t *qb, *sb;
     int64_t stride;
     if (proj == 2) {
@@ -1565,6 +1574,29 @@ extern "C" int moe_engine_load_awq(moe_engine* eng, const void* w13_qw, const vo
     if (int rc = build_cl_layout(eng, 0, E, st)) return rc;
     for (int i = 0; i < 6; ++i)
         if (owned[i]) CUDA_TRY(cudaFreeAsync(owned[i], st));
+    CUDA_TRY(cudaStreamSynchronize(st));
+    eng->loaded = true;
+    return MOE_OK;
+}
+
+extern "C" int moe_engine_load_mxfp4(moe_engine* eng, const uint8_t* w13_q, const uint8_t* w13_s, const uint8_t* w2_q,
+                                     const uint8_t* w2_s, int32_t src_on_device, void* stream) {
+    if (int rc = check_engine(eng)) return rc;
+    if (!eng->mx) return fail(MOE_ERR_STATE, "not an MXFP4 engine");
+    if (!w13_q || !w13_s || !w2_q || !w2_s) return fail(MOE_ERR_INVALID, "null weight pointer");
+    DeviceGuard g(eng->cfg.device);
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    const int64_t E = eng->cfg.num_experts, H = eng->cfg.hidden_size, I = eng->cfg.intermediate_size;
+    const void* src[4] = {w13_q, w13_s, w2_q, w2_s};
+    const size_t bytes[4] = {(size_t)E * 2 * I * (H / 2), (size_t)E * 2 * I * (H / 32), (size_t)E * H * (I / 2), (size_t)E * H * (I / 32)};
+    const uint8_t* dev[4] = {};
+    uint8_t* owned[4] = {};
+    int rc = MOE_OK;
+    for (int i = 0; i < 4 && rc == MOE_OK; ++i) rc = stage_to_device(src[i], bytes[i], src_on_device, st, &dev[i], &owned[i]);
+    if (rc == MOE_OK) rc = mx_load(eng->mx, dev[0], dev[1], dev[2], dev[3], st);
+    for (uint8_t* p : owned)
+        if (p) cudaFreeAsync(p, st);
+    if (rc) return rc;
     CUDA_TRY(cudaStreamSynchronize(st));
     eng->loaded = true;
     return MOE_OK;
@@ -1664,6 +1696,10 @@ extern "C" int moe_engine_reserve(moe_engine* eng, int64_t max_tokens, int64_t t
     if (int rc = check_engine(eng)) return rc;
     if (max_tokens < 0 || top_k <= 0) return fail(MOE_ERR_INVALID, "bad reserve size");
     DeviceGuard g(eng->cfg.device);
+    if (eng->mx) {
+        if (top_k > 64) return fail(MOE_ERR_INVALID, "top_k must be at most 64");
+        return mx_reserve(eng->mx, max_tokens, top_k);
+    }
     if ((max_tokens > eng->gemm_min_tokens && gemm_path_ok(eng)) ||
         (max_tokens > eng->awq_gemm_min_tokens && awq_gemm_ok(eng))) {  // the grouped-GEMM path's workspace
         GemmWs w;
@@ -1710,6 +1746,24 @@ extern "C" int moe_engine_forward(moe_engine* eng, const void* x, void* y, const
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     if (int rc = check_sticky_error(eng, st)) return rc;
     if (T == 0) return MOE_OK;
+    if (eng->mx) {
+        cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
+        CUDA_TRY(cudaStreamIsCapturing(st, &cap));
+        const bool timed = cap == cudaStreamCaptureStatusNone;
+        if (timed) {
+            // the workspace is the engine's: a call on another stream follows the last one
+            if (eng->timed && eng->last_stream != st) CUDA_TRY(cudaStreamWaitEvent(st, eng->ev1, 0));
+            CUDA_TRY(cudaEventRecord(eng->ev0, st));
+        }
+        MxForward f{x, y, topk_ids, topk_w, T, K, act_dtype, out_dtype, eng->emap, eng->emap_n, eng->err, eng->pdl};
+        const int rc = mx_forward(eng->mx, f, st);
+        if (timed) {  // after a failure too: what was launched before it still uses the workspace
+            CUDA_TRY(cudaEventRecord(eng->ev1, st));
+            eng->timed = true;
+            eng->last_stream = st;
+        }
+        return rc;
+    }
     const int64_t H = eng->cfg.hidden_size;
     const size_t xe = 2, ye = out_dtype == MOE_F32 ? 4 : 2;
     if (eng->p2p_active && !moe_engine_p2p_covers(eng, T))
@@ -1966,6 +2020,7 @@ extern "C" int moe_engine_export_expert(moe_engine* eng, int64_t expert, int32_t
     if (expert < 0 || expert >= E || (which != 0 && which != 1) || !qs_out || !d_out)
         return fail(MOE_ERR_INVALID, "bad export argument");
     DeviceGuard g(eng->cfg.device);
+    if (eng->mx) return mx_export(eng->mx, expert, which, qs_out, d_out);
     const bool awq = eng->cfg.quant_type == MOE_AWQ;
     const bool q4 = eng->cfg.quant_type == MOE_Q4_0 || awq;
     const int64_t rows = which == 0 ? 2 * I : H;
@@ -2129,6 +2184,7 @@ extern "C" int moe_engine_forward_noalloc(moe_engine* eng, const void* x, void* 
         return fail(MOE_ERR_INVALID, "bad output dtype");
     if (T > 0 && (!x || !y || !topk_ids || !topk_w)) return fail(MOE_ERR_INVALID, "null tensor pointer");
     if (eng->p2p_active) return fail(MOE_ERR_STATE, "the no-allocation forward does not run the peer combine");
+    if (eng->mx) return fail(MOE_ERR_STATE, "MXFP4 engines have no no-allocation forward; reserve and use moe_engine_forward");
     const int64_t I = eng->cfg.intermediate_size;
     const int64_t P = T * K;
     const size_t need = kNoAllocHeader + (size_t)P * I * 4;  // h is requantised in place
@@ -2168,7 +2224,7 @@ extern "C" int moe_engine_forward_noalloc(moe_engine* eng, const void* x, void* 
 
 // =================================================================== peer combine (expert parallel)
 extern "C" int moe_engine_p2p_covers(moe_engine* eng, int64_t num_tokens) {
-    if (!eng) return 0;
+    if (!eng || eng->mx) return 0;
     return !(num_tokens > eng->gemm_min_tokens && gemm_path_ok(eng)) &&
            !(num_tokens > eng->awq_gemm_min_tokens && awq_gemm_ok(eng)) && num_tokens <= std::max<int64_t>(eng->p2p_tcap, 8);
 }
@@ -2177,6 +2233,7 @@ extern "C" int moe_engine_p2p_mailbox(moe_engine* eng, int32_t world, int64_t ma
     if (int rc = check_engine(eng)) return rc;
     if (world < 2 || world > kMaxPeers || max_tokens <= 0 || !ipc_handle_out)
         return fail(MOE_ERR_INVALID, "peer combine needs 2..8 ranks, max_tokens > 0 and a handle buffer");
+    if (eng->mx) return fail(MOE_ERR_STATE, "MXFP4 engines have no peer combine; all-reduce the fp32 partials");
     if (eng->mbox) return fail(MOE_ERR_STATE, "mailbox already created");
     DeviceGuard g(eng->cfg.device);
     const int64_t tcap = std::min<int64_t>(max_tokens, 64);
@@ -2252,6 +2309,12 @@ struct Buf {
 std::vector<Buf> engine_buffers(moe_engine* eng) {
     const int64_t E = eng->cfg.num_experts, H = eng->cfg.hidden_size, I = eng->cfg.intermediate_size;
     std::vector<Buf> v;
+    if (eng->mx) {  // gate_up codes and scale tiles, down codes and scale tiles
+        MxBuffer b[4];
+        mx_buffers(eng->mx, b);
+        for (uint32_t i = 0; i < 4; ++i) v.push_back({6 + i, b[i].ptr, b[i].bytes});
+        return v;
+    }
     v.push_back({1, &eng->gu, (size_t)E * I * eng->unit_bytes()});
     v.push_back({2, &eng->dn, (size_t)E * H * eng->row_bytes()});
     if (eng->dk) v.push_back({3, &eng->dk, (size_t)E * (I / 32) * (H / 32) * sk_slice_bytes(eng)});

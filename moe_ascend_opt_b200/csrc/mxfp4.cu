@@ -1,0 +1,535 @@
+// MXFP4 entry points (include/moe_b200.h) and the MXFP4 expert layer of the engine.
+#include <algorithm>
+#include <mutex>
+#include <new>
+#include <utility>
+#include <vector>
+
+#include "mx_layer.h"
+#include "mxfp4_gemm.cuh"
+#include "status.h"
+
+using namespace moe;
+
+namespace {
+
+inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+// ------------------------------------------------------------------ tensor maps
+using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                              const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                              CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+int encoder(EncodeFn* out) {
+    static EncodeFn fn = nullptr;
+    static std::mutex mu;
+    std::lock_guard<std::mutex> lk(mu);
+    if (!fn) {
+        void* p = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        CUDA_TRY(cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &p, 12000, cudaEnableDefault, &q));
+        if (!p || q != cudaDriverEntryPointSuccess) return fail(MOE_ERR_CUDA, "cuTensorMapEncodeTiled is not available");
+        fn = reinterpret_cast<EncodeFn>(p);
+    }
+    *out = fn;
+    return MOE_OK;
+}
+
+// Codes as bytes [planes][rows][pitch], boxes of 128 bytes x box_rows, 128-byte swizzle; what
+// lies outside reads as zero.  planes 0: a 2-D map.
+int encode(CUtensorMap* m, const void* base, int64_t pitch, int64_t rows, int64_t planes, int box_rows) {
+    EncodeFn fn;
+    if (int rc = encoder(&fn)) return rc;
+    const cuuint64_t dims[3] = {(cuuint64_t)pitch, (cuuint64_t)rows, (cuuint64_t)planes};
+    const cuuint64_t strides[2] = {(cuuint64_t)pitch, (cuuint64_t)(pitch * rows)};
+    const cuuint32_t box[3] = {128, (cuuint32_t)box_rows, 1}, ones[3] = {1, 1, 1};
+    const CUresult r = fn(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, planes ? 3 : 2, const_cast<void*>(base), dims, strides, box, ones,
+                          CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return fail(MOE_ERR_CUDA, "cuTensorMapEncodeTiled failed with " + std::to_string((int)r));
+    return MOE_OK;
+}
+
+// ------------------------------------------------------------------ launches
+// Opt-in shared memory of a kernel, once per kernel and device.
+int allow_smem(const void* fn, int bytes) {
+    static std::mutex mu;
+    static std::vector<std::pair<const void*, int>> done;
+    int dev = 0;
+    CUDA_TRY(cudaGetDevice(&dev));
+    std::lock_guard<std::mutex> lk(mu);
+    for (auto& d : done)
+        if (d.first == fn && d.second == dev) return MOE_OK;
+    CUDA_TRY(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+    done.emplace_back(fn, dev);
+    return MOE_OK;
+}
+
+template <typename... P, typename... A>
+int launch(void (*fn)(P...), unsigned grid, unsigned block, size_t smem, bool pdl, cudaStream_t st, A&&... args) {
+    cudaLaunchConfig_t cfg{};
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(block);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cfg.attrs = attr;
+    cfg.numAttrs = pdl ? 1 : 0;
+    CUDA_TRY(cudaLaunchKernelEx(&cfg, fn, P(args)...));
+    return MOE_OK;
+}
+
+int sm_count(int dev, int* out) {
+    static int n[64] = {};
+    if (dev < 64 && n[dev]) {
+        *out = n[dev];
+        return MOE_OK;
+    }
+    CUDA_TRY(cudaDeviceGetAttribute(out, cudaDevAttrMultiProcessorCount, dev));
+    if (dev < 64) n[dev] = *out;
+    return MOE_OK;
+}
+
+constexpr int kNT = 128, kStages = 6;
+
+template <int MODE>
+int launch_gemm(const CUtensorMap& ta, const CUtensorMap& tb, const mx::GemmParams& p, int64_t tiles, int sms, bool pdl,
+                cudaStream_t st) {
+    auto fn = mx::mx_gemm_kernel<MODE, kNT, kStages>;
+    const int smem = kStages * mx::Shape<kNT>::kStage + 1024;
+    if (int rc = allow_smem(reinterpret_cast<const void*>(fn), smem)) return rc;
+    return launch(fn, (unsigned)std::min<int64_t>(tiles, sms), mx::kGemmThreads, smem, pdl, st, ta, tb, p);
+}
+
+bool dtype_ok(int32_t t) { return t == MOE_F16 || t == MOE_BF16 || t == MOE_F32; }
+bool aligned(const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
+
+// Error word of the products that run without an engine: one per device, in mapped host memory.
+int product_error_word(int dev, int32_t** host, int32_t** device) {
+    static std::mutex mu;
+    static int32_t* words[64] = {};
+    if (dev < 0 || dev >= 64) return fail(MOE_ERR_INVALID, "device ordinal out of range");
+    std::lock_guard<std::mutex> lk(mu);
+    if (!words[dev]) {
+        int32_t* w = nullptr;
+        cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;  // the first call may be a captured one
+        CUDA_TRY(cudaThreadExchangeStreamCaptureMode(&mode));
+        const cudaError_t e = cudaHostAlloc(reinterpret_cast<void**>(&w), 64, cudaHostAllocMapped | cudaHostAllocPortable);
+        cudaThreadExchangeStreamCaptureMode(&mode);
+        if (e != cudaSuccess) return fail(MOE_ERR_CUDA, std::string("cudaHostAlloc: ") + cudaGetErrorString(e));
+        *reinterpret_cast<volatile int32_t*>(w) = 0;
+        words[dev] = w;
+    }
+    *host = words[dev];
+    CUDA_TRY(cudaHostGetDevicePointer(reinterpret_cast<void**>(device), words[dev], 0));
+    return MOE_OK;
+}
+
+template <int DT>
+int quantize_launch(const void* x, int64_t rows, int64_t cols, uint8_t* q, uint8_t* s, bool tiled, int sms, cudaStream_t st) {
+    const unsigned grid = (unsigned)std::min<int64_t>(ceil_div(rows * (cols / 8), 256), (int64_t)sms * 16);
+    if (tiled) mx::quantize_kernel<DT, true><<<grid, 256, 0, st>>>(x, rows, (int)cols, q, s);
+    else mx::quantize_kernel<DT, false><<<grid, 256, 0, st>>>(x, rows, (int)cols, q, s);
+    CUDA_TRY(cudaGetLastError());
+    return MOE_OK;
+}
+
+int quantize(const void* x, int32_t dtype, int64_t rows, int64_t cols, uint8_t* q, uint8_t* s, bool tiled, cudaStream_t st) {
+    int dev = 0, sms = 0;
+    CUDA_TRY(cudaGetDevice(&dev));
+    if (int rc = sm_count(dev, &sms)) return rc;
+    return dtype == MOE_F32    ? quantize_launch<MOE_F32>(x, rows, cols, q, s, tiled, sms, st)
+           : dtype == MOE_BF16 ? quantize_launch<MOE_BF16>(x, rows, cols, q, s, tiled, sms, st)
+                               : quantize_launch<MOE_F16>(x, rows, cols, q, s, tiled, sms, st);
+}
+
+template <int DT>
+int dequantize_launch(const uint8_t* q, const uint8_t* s, int64_t rows, int64_t cols, void* y, bool tiled, int sms, cudaStream_t st) {
+    const unsigned grid = (unsigned)std::min<int64_t>(ceil_div(rows * (cols / 8), 256), (int64_t)sms * 16);
+    if (tiled) mx::dequantize_kernel<DT, true><<<grid, 256, 0, st>>>(q, s, rows, (int)cols, y);
+    else mx::dequantize_kernel<DT, false><<<grid, 256, 0, st>>>(q, s, rows, (int)cols, y);
+    CUDA_TRY(cudaGetLastError());
+    return MOE_OK;
+}
+
+int check_rows(int64_t rows, int64_t cols) {
+    if (rows < 0 || cols <= 0 || cols % 32 != 0) return fail(MOE_ERR_INVALID, "cols must be a positive multiple of 32");
+    if (cols > (int64_t)1 << 30 || rows > (int64_t)1 << 31) return fail(MOE_ERR_INVALID, "rows or cols too large");
+    return MOE_OK;
+}
+
+}  // namespace
+
+// ------------------------------------------------------------------ C ABI
+extern "C" int moe_quantize_rows_mxfp4(const void* x, int32_t dtype, int64_t rows, int64_t cols, int32_t tiled_scales,
+                                       uint8_t* q, uint8_t* scales, void* stream) {
+    if (int rc = check_rows(rows, cols)) return rc;
+    if (!dtype_ok(dtype)) return fail(MOE_ERR_INVALID, "bad dtype");
+    if (rows == 0) return MOE_OK;
+    if (!x || !q || !scales) return fail(MOE_ERR_INVALID, "null pointer");
+    if (!aligned(x, 16) || !aligned(q, 16) || (tiled_scales && !aligned(scales, 16)))
+        return fail(MOE_ERR_INVALID, "x, the codes and tiled scales must be 16-byte aligned");
+    return quantize(x, dtype, rows, cols, q, scales, tiled_scales != 0, static_cast<cudaStream_t>(stream));
+}
+
+extern "C" int moe_dequantize_rows_mxfp4(const uint8_t* q, const uint8_t* scales, int64_t rows, int64_t cols,
+                                         int32_t tiled_scales, void* y, int32_t dtype, void* stream) {
+    if (int rc = check_rows(rows, cols)) return rc;
+    if (!dtype_ok(dtype)) return fail(MOE_ERR_INVALID, "bad dtype");
+    if (rows == 0) return MOE_OK;
+    if (!y || !q || !scales) return fail(MOE_ERR_INVALID, "null pointer");
+    if (!aligned(y, 16) || !aligned(q, 4)) return fail(MOE_ERR_INVALID, "y must be 16-byte, the codes 4-byte aligned");
+    int dev = 0, sms = 0;
+    CUDA_TRY(cudaGetDevice(&dev));
+    if (int rc = sm_count(dev, &sms)) return rc;
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    const bool tiled = tiled_scales != 0;
+    return dtype == MOE_F32    ? dequantize_launch<MOE_F32>(q, scales, rows, cols, y, tiled, sms, st)
+           : dtype == MOE_BF16 ? dequantize_launch<MOE_BF16>(q, scales, rows, cols, y, tiled, sms, st)
+                               : dequantize_launch<MOE_F16>(q, scales, rows, cols, y, tiled, sms, st);
+}
+
+extern "C" int moe_mxfp4_tile_scales(const uint8_t* scales, int64_t rows, int64_t cols, uint8_t* tiles, void* stream) {
+    if (int rc = check_rows(rows, cols)) return rc;
+    if (rows == 0) return MOE_OK;
+    if (!scales || !tiles) return fail(MOE_ERR_INVALID, "null pointer");
+    if (!aligned(tiles, 16)) return fail(MOE_ERR_INVALID, "tiled scales must be 16-byte aligned");
+    const int64_t n = ceil_div(rows, 128) * 128 * ceil_div(cols, 128);
+    mx::tile_scales_kernel<<<(unsigned)std::min<int64_t>(ceil_div(n, 256), 4096), 256, 0, static_cast<cudaStream_t>(stream)>>>(
+        scales, rows, (int)(cols / 32), 0, 0, tiles);
+    CUDA_TRY(cudaGetLastError());
+    return MOE_OK;
+}
+
+extern "C" int moe_mxfp4_matmul(const uint8_t* a, const uint8_t* a_scales, const uint8_t* b, const uint8_t* b_scales,
+                                int64_t M, int64_t N, int64_t K, void* y, int32_t out_dtype, void* stream) {
+    if (M < 0 || N <= 0 || K <= 0 || K % 32 != 0) return fail(MOE_ERR_INVALID, "K must be a positive multiple of 32, N positive");
+    if (M > (int64_t)1 << 30 || N > (int64_t)1 << 30 || K > (int64_t)1 << 30) return fail(MOE_ERR_INVALID, "M, N or K too large");
+    if (!dtype_ok(out_dtype)) return fail(MOE_ERR_INVALID, "bad output dtype");
+    if (M == 0) return MOE_OK;
+    if (!a || !a_scales || !b || !b_scales || !y) return fail(MOE_ERR_INVALID, "null pointer");
+    if (!aligned(a, 16) || !aligned(b, 16) || !aligned(a_scales, 16) || !aligned(b_scales, 16) || !aligned(y, 16))
+        return fail(MOE_ERR_INVALID, "operands, scales and the output must be 16-byte aligned");
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    int dev = 0, sms = 0;
+    CUDA_TRY(cudaGetDevice(&dev));
+    if (int rc = sm_count(dev, &sms)) return rc;
+    mx::GemmParams p{};
+    int32_t* herr = nullptr;
+    if (int rc = product_error_word(dev, &herr, &p.err)) return rc;
+    if (*reinterpret_cast<volatile int32_t*>(herr) != 0) {
+        *reinterpret_cast<volatile int32_t*>(herr) = 0;
+        return fail(MOE_ERR_DEVICE, "an earlier MXFP4 product failed on the device (a bounded wait expired); its output is invalid");
+    }
+    CUtensorMap ta, tb;
+    if (int rc = encode(&ta, a, K / 2, M, 0, mx::kTileM)) return rc;
+    if (int rc = encode(&tb, b, K / 2, N, 1, kNT)) return rc;
+    p.M = (int)M; p.N = (int)N; p.K = (int)K;
+    p.kb = (int)ceil_div(K, 128);
+    p.nt_count = (int)ceil_div(N, kNT);
+    p.mt_count = (int)ceil_div(M, mx::kTileM);
+    p.sfa = a_scales;
+    p.sfb = b_scales;
+    p.out = y;
+    p.out_dtype = out_dtype;
+    return launch_gemm<mx::kDense>(ta, tb, p, (int64_t)p.nt_count * p.mt_count, sms, false, st);
+}
+
+// ------------------------------------------------------------------ expert layer
+namespace moe {
+
+struct MxLayer {
+    moe_config cfg{};
+    int sms = 0;
+    int64_t kb1 = 0, kb2 = 0, nb1 = 0, nb2 = 0;  // scale tiles along K and N of gate_up (1) and down (2)
+    uint8_t *q1 = nullptr, *s1 = nullptr, *q2 = nullptr, *s2 = nullptr;
+    CUtensorMap t1{}, t2{};
+    uint8_t* ws = nullptr;
+    size_t ws_bytes = 0;
+    std::vector<uint8_t*> retired;  // earlier workspaces: captured graphs may still hold them
+    size_t q1_bytes() const { return (size_t)cfg.num_experts * 2 * cfg.intermediate_size * (cfg.hidden_size / 2); }
+    size_t q2_bytes() const { return (size_t)cfg.num_experts * cfg.hidden_size * (cfg.intermediate_size / 2); }
+    size_t s1_bytes() const { return (size_t)cfg.num_experts * nb1 * kb1 * 512; }
+    size_t s2_bytes() const { return (size_t)cfg.num_experts * nb2 * kb2 * 512; }
+};
+
+namespace {
+
+constexpr int64_t kMaxPairs = 1 << 18;  // routed pairs of one pass; longer calls run in slices of tokens
+
+// Rows of a matrix [rows][bytes] between the input contract's order and the layer's: gate_up row
+// r of the layer holds unit 32 (r / 64) + r % 32 of gate (r / 32 even) or up.
+__global__ void mx_rows_kernel(uint8_t* dst, const uint8_t* src, int64_t rows, int64_t bytes, int map, int64_t I, int inverse) {
+    const int64_t n16 = bytes / 16, n = rows * n16, e = blockIdx.y;
+    dst += e * rows * bytes;
+    src += e * rows * bytes;
+    for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (int64_t)gridDim.x * blockDim.x) {
+        const int64_t r = i / n16, c = i - r * n16;
+        const int64_t u = map ? ((r >> 5) & 1) * I + (r >> 6) * 32 + (r & 31) : r;
+        const uint4* s = reinterpret_cast<const uint4*>(src);
+        uint4* d = reinterpret_cast<uint4*>(dst);
+        if (inverse) d[u * n16 + c] = s[i];
+        else d[i] = s[u * n16 + c];
+    }
+}
+
+// Scale tiles of one matrix -> row-major scales (inverse of tile_scales_kernel).
+__global__ void mx_untile_kernel(const uint8_t* tiles, int64_t rows, int nb, int map, int64_t I, uint8_t* s) {
+    const int64_t kb = (nb + 3) >> 2, n = rows * nb;
+    for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (int64_t)gridDim.x * blockDim.x) {
+        const int64_t r = i / nb, b = i - r * nb;
+        const int64_t u = map ? ((r >> 5) & 1) * I + (r >> 6) * 32 + (r & 31) : r;
+        s[u * nb + b] = tiles[mx::tiled_at(r, b, kb)];
+    }
+}
+
+// Online quantisation of rows [n][cols] to layer rows: row j goes to layer row
+// (j / 32) * 64 + 32 * half + j % 32 (gate_up, half 0 gate, 1 up) or j (down, half -1).
+template <int DT>
+__global__ void mx_store_rows_kernel(const void* w, int64_t n, int cols, int half, uint8_t* q, uint8_t* tiles) {
+    const int64_t per = cols >> 3, total = n * per, kb = (cols + 127) >> 7;
+    for (int64_t i0 = (int64_t)blockIdx.x * blockDim.x; i0 < total; i0 += (int64_t)gridDim.x * blockDim.x) {
+        const int64_t i = i0 + threadIdx.x;
+        float v[8] = {};
+        if (i < total) mx::load8<DT>(w, i * 8, v);
+        uint32_t sc;
+        const uint32_t c = mx::quant8(v, sc);
+        if (i >= total) continue;
+        const int64_t j = i / per, k = i - j * per;
+        const int64_t r = half < 0 ? j : (j >> 5) * 64 + 32 * half + (j & 31);
+        reinterpret_cast<uint32_t*>(q)[r * per + k] = c;
+        if ((i & 3) == 0) tiles[mx::tiled_at(r, k >> 2, kb)] = (uint8_t)sc;
+    }
+}
+
+struct Workspace {
+    int32_t *mtiles, *mt_expert, *mt_rows, *rowtok, *ppos;
+    uint8_t *xq, *xs, *hq, *hs;
+    float* part;
+    int64_t mt;  // bound of the number of m tiles
+    size_t bytes;
+};
+
+Workspace carve(const MxLayer* l, int64_t T, int64_t K, uint8_t* base) {
+    Workspace w{};
+    const int64_t P = T * K, H = l->cfg.hidden_size, I = l->cfg.intermediate_size;
+    w.mt = P / mx::kTileM + std::min(P, l->cfg.num_experts);
+    const int64_t rows = w.mt * mx::kTileM;
+    size_t off = 0;
+    auto take = [&](size_t n) {
+        uint8_t* p = base + off;
+        off += (n + 1023) / 1024 * 1024;
+        return p;
+    };
+    w.mtiles = reinterpret_cast<int32_t*>(take(4));
+    w.mt_expert = reinterpret_cast<int32_t*>(take(w.mt * 4));
+    w.mt_rows = reinterpret_cast<int32_t*>(take(w.mt * 4));
+    w.rowtok = reinterpret_cast<int32_t*>(take(rows * 4));
+    w.ppos = reinterpret_cast<int32_t*>(take(P * 4));
+    w.xq = take(T * (H / 2));
+    w.xs = take(w.mt * l->kb1 * 512);
+    w.hq = take(rows * (I / 2));
+    w.hs = take(w.mt * l->kb2 * 512);
+    w.part = reinterpret_cast<float*>(take((size_t)rows * H * 4));
+    w.bytes = off;
+    return w;
+}
+
+int64_t slice_tokens(int64_t T, int64_t K) { return std::min(T, std::max<int64_t>(1, kMaxPairs / K)); }
+
+// A workspace of at least `bytes`.  An outgrown one is kept until the engine goes, since captured
+// graphs refer to it; sizes double, so that all of them hold at most twice the last.
+int grow(MxLayer* l, size_t bytes) {
+    if (bytes <= l->ws_bytes) return MOE_OK;
+    const size_t want = std::max(bytes, 2 * l->ws_bytes);
+    uint8_t* p = nullptr;
+    cudaError_t e = cudaMalloc(&p, want);
+    size_t got = want;
+    if (e != cudaSuccess && want > bytes) {
+        cudaGetLastError();
+        e = cudaMalloc(&p, bytes);
+        got = bytes;
+    }
+    if (e != cudaSuccess) {
+        cudaGetLastError();
+        return fail(MOE_ERR_CUDA, std::string("workspace of ") + std::to_string(bytes) + " bytes: " + cudaGetErrorString(e));
+    }
+    if (l->ws) l->retired.push_back(l->ws);
+    l->ws = p;
+    l->ws_bytes = got;
+    return MOE_OK;
+}
+
+template <int DT>
+int tokens_launch(const MxLayer* l, const MxForward& f, const void* x, const Workspace& w, int64_t T, cudaStream_t st) {
+    const int H = (int)l->cfg.hidden_size;
+    const unsigned block = (unsigned)std::min<int64_t>(256, ceil_div(H / 8, 32) * 32);
+    return launch(mx::mx_tokens_kernel<DT>, (unsigned)T, block, 0, f.pdl, st, x, H, (int)f.K, (const int32_t*)w.ppos, w.xq, w.xs,
+                  (int)l->kb1);
+}
+
+template <int DT>
+int combine_launch(const MxLayer* l, const MxForward& f, const float* tw, void* y, const Workspace& w, int64_t T, cudaStream_t st) {
+    const int H = (int)l->cfg.hidden_size;
+    return launch(mx::mx_combine_kernel<DT>, (unsigned)std::min<int64_t>(ceil_div(T * (H / 4), 256), l->sms * 16), 256, 0, f.pdl, st,
+                  (const float*)w.part, (const int32_t*)w.ppos, tw, (int)T, (int)f.K, H, y);
+}
+
+int forward_slice(MxLayer* l, const MxForward& f, const void* x, void* y, const int32_t* ids, const float* tw, int64_t T,
+                  cudaStream_t st) {
+    const int64_t E = l->cfg.num_experts, H = l->cfg.hidden_size, I = l->cfg.intermediate_size;
+    const Workspace w = carve(l, T, f.K, l->ws);
+    mx::RouteParams r{};
+    r.ids = ids;
+    r.TK = (int)(T * f.K); r.K = (int)f.K; r.E = (int)E; r.e_off = l->cfg.expert_offset;
+    r.emap = f.emap; r.emap_n = f.emap_n;
+    r.mtiles = w.mtiles; r.mt_expert = w.mt_expert; r.mt_rows = w.mt_rows; r.rowtok = w.rowtok; r.ppos = w.ppos;
+    const int rsmem = (int)(32 * E + 32) * 4;
+    if (int rc = allow_smem(reinterpret_cast<const void*>(mx::mx_route_kernel), 33 * 1024 * 4)) return rc;
+    if (int rc = launch(mx::mx_route_kernel, 1, 1024, rsmem, f.pdl, st, r)) return rc;
+    if (int rc = f.act_dtype == MOE_BF16 ? tokens_launch<MOE_BF16>(l, f, x, w, T, st) : tokens_launch<MOE_F16>(l, f, x, w, T, st))
+        return rc;
+    CUtensorMap tx, th;
+    if (int rc = encode(&tx, w.xq, H / 2, T, 0, 1)) return rc;
+    if (int rc = encode(&th, w.hq, I / 2, w.mt * mx::kTileM, 0, 16)) return rc;
+    mx::GemmParams p{};
+    p.mtiles = w.mtiles; p.mt_expert = w.mt_expert; p.mt_rows = w.mt_rows; p.rowtok = w.rowtok;
+    p.err = f.err;
+    p.I = (int)I;
+    mx::GemmParams g1 = p;
+    g1.N = (int)(2 * I); g1.K = (int)H; g1.kb = (int)l->kb1; g1.nt_count = (int)ceil_div(2 * I, kNT);
+    g1.sfa = w.xs; g1.sfb = l->s1; g1.hq = w.hq; g1.hs = w.hs; g1.hkb = (int)l->kb2;
+    if (int rc = launch_gemm<mx::kGateUp>(tx, l->t1, g1, w.mt * g1.nt_count, l->sms, f.pdl, st)) return rc;
+    mx::GemmParams g2 = p;
+    g2.N = (int)H; g2.K = (int)I; g2.kb = (int)l->kb2; g2.nt_count = (int)ceil_div(H, kNT);
+    g2.sfa = w.hs; g2.sfb = l->s2; g2.out = w.part;
+    if (int rc = launch_gemm<mx::kDown>(th, l->t2, g2, w.mt * g2.nt_count, l->sms, f.pdl, st)) return rc;
+    return f.out_dtype == MOE_F32    ? combine_launch<MOE_F32>(l, f, tw, y, w, T, st)
+           : f.out_dtype == MOE_BF16 ? combine_launch<MOE_BF16>(l, f, tw, y, w, T, st)
+                                     : combine_launch<MOE_F16>(l, f, tw, y, w, T, st);
+}
+
+}  // namespace
+
+int mx_create(const moe_config& cfg, int num_sms, MxLayer** out) {
+    *out = nullptr;
+    if (cfg.num_experts > 1024) return fail(MOE_ERR_INVALID, "MXFP4 engines hold at most 1024 experts");
+    if (cfg.hidden_size > 1 << 20 || cfg.intermediate_size > 1 << 20) return fail(MOE_ERR_INVALID, "hidden or intermediate size too large");
+    auto* l = new (std::nothrow) MxLayer();
+    if (!l) return fail(MOE_ERR_STATE, "out of host memory");
+    l->cfg = cfg;
+    l->sms = num_sms;
+    const int64_t E = cfg.num_experts, H = cfg.hidden_size, I = cfg.intermediate_size;
+    l->kb1 = ceil_div(H, 128);
+    l->kb2 = ceil_div(I, 128);
+    l->nb1 = ceil_div(2 * I, 128);
+    l->nb2 = ceil_div(H, 128);
+    MxBuffer b[4];
+    mx_buffers(l, b);
+    for (auto& x : b) {
+        cudaError_t e = cudaMalloc(x.ptr, x.bytes);
+        if (e == cudaSuccess) e = cudaMemset(*x.ptr, 0, x.bytes);
+        if (e != cudaSuccess) {
+            cudaGetLastError();
+            mx_destroy(l);
+            return fail(MOE_ERR_CUDA, std::string("MXFP4 weights: ") + cudaGetErrorString(e));
+        }
+    }
+    int rc = encode(&l->t1, l->q1, H / 2, 2 * I, E, kNT);
+    if (rc == MOE_OK) rc = encode(&l->t2, l->q2, I / 2, H, E, kNT);
+    if (rc != MOE_OK) {
+        mx_destroy(l);
+        return rc;
+    }
+    *out = l;
+    return MOE_OK;
+}
+
+void mx_destroy(MxLayer* l) {
+    if (!l) return;
+    for (uint8_t* p : {l->q1, l->s1, l->q2, l->s2, l->ws}) cudaFree(p);
+    for (uint8_t* p : l->retired) cudaFree(p);
+    delete l;
+}
+
+void mx_buffers(MxLayer* l, MxBuffer (&b)[4]) {
+    b[0] = {&l->q1, l->q1_bytes()};
+    b[1] = {&l->s1, l->s1_bytes()};
+    b[2] = {&l->q2, l->q2_bytes()};
+    b[3] = {&l->s2, l->s2_bytes()};
+}
+
+int mx_load(MxLayer* l, const uint8_t* w13_q, const uint8_t* w13_s, const uint8_t* w2_q, const uint8_t* w2_s, cudaStream_t st) {
+    const int64_t E = l->cfg.num_experts, H = l->cfg.hidden_size, I = l->cfg.intermediate_size;
+    if (!aligned(w13_q, 16) || !aligned(w2_q, 16)) return fail(MOE_ERR_INVALID, "weight codes must be 16-byte aligned");
+    const dim3 g(128, (unsigned)E);
+    mx_rows_kernel<<<g, 256, 0, st>>>(l->q1, w13_q, 2 * I, H / 2, 1, I, 0);
+    mx_rows_kernel<<<g, 256, 0, st>>>(l->q2, w2_q, H, I / 2, 0, I, 0);
+    mx::tile_scales_kernel<<<g, 256, 0, st>>>(w13_s, 2 * I, (int)(H / 32), 1, I, l->s1);
+    mx::tile_scales_kernel<<<g, 256, 0, st>>>(w2_s, H, (int)(I / 32), 0, I, l->s2);
+    CUDA_TRY(cudaGetLastError());
+    return MOE_OK;
+}
+
+int mx_quantize_store(MxLayer* l, int64_t expert, int32_t proj, const void* w, int32_t dtype, cudaStream_t st) {
+    const int64_t H = l->cfg.hidden_size, I = l->cfg.intermediate_size;
+    if (!aligned(w, 16)) return fail(MOE_ERR_INVALID, "weight must be 16-byte aligned");
+    const int64_t n = proj == 2 ? H : I, cols = proj == 2 ? I : H;
+    uint8_t* q = proj == 2 ? l->q2 + expert * H * (I / 2) : l->q1 + expert * 2 * I * (H / 2);
+    uint8_t* s = proj == 2 ? l->s2 + expert * l->nb2 * l->kb2 * 512 : l->s1 + expert * l->nb1 * l->kb1 * 512;
+    const int half = proj == 2 ? -1 : proj;
+    const unsigned grid = (unsigned)std::min<int64_t>(ceil_div(n * (cols / 8), 256), (int64_t)l->sms * 16);
+    if (dtype == MOE_F32) mx_store_rows_kernel<MOE_F32><<<grid, 256, 0, st>>>(w, n, (int)cols, half, q, s);
+    else if (dtype == MOE_BF16) mx_store_rows_kernel<MOE_BF16><<<grid, 256, 0, st>>>(w, n, (int)cols, half, q, s);
+    else mx_store_rows_kernel<MOE_F16><<<grid, 256, 0, st>>>(w, n, (int)cols, half, q, s);
+    CUDA_TRY(cudaGetLastError());
+    return MOE_OK;
+}
+
+int mx_export(MxLayer* l, int64_t expert, int32_t which, void* q_out, void* s_out) {
+    const int64_t H = l->cfg.hidden_size, I = l->cfg.intermediate_size;
+    const int64_t rows = which == 0 ? 2 * I : H, cols = which == 0 ? H : I, nb = cols / 32;
+    const uint8_t* q = which == 0 ? l->q1 + expert * rows * (cols / 2) : l->q2 + expert * rows * (cols / 2);
+    const uint8_t* s = which == 0 ? l->s1 + expert * l->nb1 * l->kb1 * 512 : l->s2 + expert * l->nb2 * l->kb2 * 512;
+    uint8_t* d = nullptr;
+    CUDA_TRY(cudaMalloc(&d, rows * (cols / 2) + rows * nb));
+    uint8_t* ds = d + rows * (cols / 2);
+    mx_rows_kernel<<<128, 256>>>(d, q, rows, cols / 2, which == 0, I, 1);
+    mx_untile_kernel<<<128, 256>>>(s, rows, (int)nb, which == 0, I, ds);
+    cudaError_t e = cudaGetLastError();
+    if (e == cudaSuccess) e = cudaMemcpy(q_out, d, rows * (cols / 2), cudaMemcpyDeviceToHost);
+    if (e == cudaSuccess) e = cudaMemcpy(s_out, ds, rows * nb, cudaMemcpyDeviceToHost);
+    cudaFree(d);
+    CUDA_TRY(e);
+    return MOE_OK;
+}
+
+int mx_reserve(MxLayer* l, int64_t T, int64_t K) {
+    if (T == 0) return MOE_OK;
+    return grow(l, carve(l, slice_tokens(T, K), K, nullptr).bytes);
+}
+
+int mx_forward(MxLayer* l, const MxForward& f, cudaStream_t st) {
+    if (!aligned(f.x, 16) || !aligned(f.y, 16)) return fail(MOE_ERR_INVALID, "hidden and output must be 16-byte aligned");
+    const int64_t S = slice_tokens(f.T, f.K), H = l->cfg.hidden_size;
+    const size_t need = carve(l, S, f.K, nullptr).bytes;
+    if (need > l->ws_bytes) {
+        cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
+        CUDA_TRY(cudaStreamIsCapturing(st, &cap));
+        if (cap != cudaStreamCaptureStatusNone)
+            return fail(MOE_ERR_STATE, "the workspace is too small for this captured call: reserve(max_tokens, top_k) before capture");
+        if (int rc = grow(l, need)) return rc;
+    }
+    const size_t ye = f.out_dtype == MOE_F32 ? 4 : 2;
+    for (int64_t t0 = 0; t0 < f.T; t0 += S) {
+        const int64_t n = std::min(S, f.T - t0);
+        if (int rc = forward_slice(l, f, static_cast<const uint8_t*>(f.x) + (size_t)t0 * H * 2,
+                                   static_cast<uint8_t*>(f.y) + (size_t)t0 * H * ye, f.ids + t0 * f.K, f.tw + t0 * f.K, n, st))
+            return rc;
+    }
+    return MOE_OK;
+}
+
+}  // namespace moe

@@ -7,7 +7,7 @@
 //     .store_quantized_repack(gate_up_qs, gate_up_d, down_qs, down_d)  :366-371
 //     .get_last_run_time_ms() / get_quant_type() / get_num_experts() /
 //      get_hidden_size() / get_intermediate_size()              :372-391
-//     new: store_awq(...), set_expert_parallel(rank, size), set_group_size(g),
+//     new: store_awq(...), store_mxfp4(...), set_expert_parallel(rank, size), set_group_size(g),
 //          p2p_mailbox / p2p_connect / p2p_covers / p2p_enable (peer-memory combine),
 //          reserve(T, K), export_expert(e, which), device_error()
 //   torch.ops.nanovllm.moe_forward(hidden, topk_ids, topk_w, moe)          :402
@@ -16,7 +16,8 @@
 //   torch.classes.nanovllm.MoEGraphContext(moe, num_tokens, top_k, dtype)  :398-399
 //   torch.classes.nanovllm.NpuCallbackManager(stream_ptr, device_id)       :395-396 (no-op)
 //   new: moe_forward_partial, moe_dense_forward, moe_route, moe_route_gemm, moe_route_permute,
-//        quantize_rows_q8_0
+//        quantize_rows_q8_0, moe_route_scored, quantize_rows_mxfp4, dequantize_rows_mxfp4,
+//        mxfp4_tile_scales, mxfp4_matmul
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/custom_class.h>
@@ -54,7 +55,8 @@ struct MoEInferHandle : torch::CustomClassHolder {
     int device = -1;
 
     MoEInferHandle(int64_t E_, int64_t H_, int64_t I_, int64_t qt) : E(E_), H(H_), I(I_), quant_type(qt) {
-        TORCH_CHECK(qt == MOE_Q8_0 || qt == MOE_Q4_0 || qt == MOE_AWQ, "quant_type must be 0 (Q8_0), 1 (Q4_0) or 2 (AWQ)");
+        TORCH_CHECK(qt == MOE_Q8_0 || qt == MOE_Q4_0 || qt == MOE_AWQ || qt == MOE_MXFP4,
+                    "quant_type must be 0 (Q8_0), 1 (Q4_0), 2 (AWQ) or 3 (MXFP4)");
         TORCH_CHECK(H % 32 == 0, "hidden_size must be multiple of 32");
         TORCH_CHECK(I % 32 == 0, "intermediate_size must be multiple of 32");
     }
@@ -138,6 +140,7 @@ struct MoEInferHandle : torch::CustomClassHolder {
     void store_quantized_repack(const at::Tensor& gu_qs, const at::Tensor& gu_d, const at::Tensor& dn_qs,
                                 const at::Tensor& dn_d) {
         TORCH_CHECK(quant_type != MOE_AWQ, "AWQ handle: use store_awq");
+        TORCH_CHECK(quant_type != MOE_MXFP4, "MXFP4 handle: use store_mxfp4");
         TORCH_CHECK(gu_d.scalar_type() == at::kHalf || gu_d.scalar_type() == at::kBFloat16,
                     "gate_up_d must be float16 or bfloat16");
         TORCH_CHECK(dn_d.scalar_type() == gu_d.scalar_type(), "gate_up_d and down_proj_d must have the same dtype");
@@ -172,7 +175,7 @@ struct MoEInferHandle : torch::CustomClassHolder {
     void quantize_and_store_expert(int64_t e, const std::string& proj, const at::Tensor& w) {
         TORCH_CHECK(quant_type != MOE_Q4_0,
                     "Q4_0 does not support online quantization. Use store_quantized_repack() with pre-quantized weights.");
-        TORCH_CHECK(quant_type == MOE_Q8_0, "online quantization is Q8_0 only");
+        TORCH_CHECK(quant_type == MOE_Q8_0 || quant_type == MOE_MXFP4, "online quantization is Q8_0 and MXFP4 only");
         TORCH_CHECK(w.dim() == 2, "Weight must be 2D");
         TORCH_CHECK(w.scalar_type() == at::kFloat || w.scalar_type() == at::kHalf || w.scalar_type() == at::kBFloat16,
                     "Weight must be float32, float16 or bfloat16 for quantize_weight_only");
@@ -227,6 +230,31 @@ struct MoEInferHandle : torch::CustomClassHolder {
                  "store_awq");
     }
 
+    void store_mxfp4(const at::Tensor& w13_q, const at::Tensor& w13_s, const at::Tensor& w2_q, const at::Tensor& w2_s) {
+        TORCH_CHECK(quant_type == MOE_MXFP4, "store_mxfp4 needs quant_type 3 (MXFP4)");
+        auto check = [&](const at::Tensor& t, int64_t rows, int64_t cols, const char* what) {
+            TORCH_CHECK(t.scalar_type() == at::kByte, what, " must be uint8");
+            TORCH_CHECK(t.dim() == 3 && t.size(0) == E && t.size(1) == rows && t.size(2) == cols, what, " must be [", E, ",",
+                        rows, ",", cols, "]");
+            TORCH_CHECK(t.is_cuda() == w13_q.is_cuda(), "weights must all be on the same device type");
+        };
+        check(w13_q, 2 * I, H / 2, "w13");
+        check(w13_s, 2 * I, H / 32, "w13_scales");
+        check(w2_q, H, I / 2, "w2");
+        check(w2_s, H, I / 32, "w2_scales");
+        ensure_engine();
+        c10::cuda::CUDAGuard g(device);
+        at::Tensor t[4] = {local(w13_q), local(w13_s), local(w2_q), local(w2_s)};
+        const bool on_dev = t[0].is_cuda();
+        for (auto& x : t) {
+            TORCH_CHECK(!on_dev || x.get_device() == device, "weights must be on the engine's device");
+            if (on_dev && reinterpret_cast<uintptr_t>(x.data_ptr()) % 16 != 0) x = x.clone();
+        }
+        check_rc(moe_engine_load_mxfp4(eng, t[0].data_ptr<uint8_t>(), t[1].data_ptr<uint8_t>(), t[2].data_ptr<uint8_t>(),
+                                       t[3].data_ptr<uint8_t>(), on_dev ? 1 : 0, cur_stream(device)),
+                 "store_mxfp4");
+    }
+
     void forward_into(const at::Tensor& hidden, const at::Tensor& ids, const at::Tensor& w, at::Tensor& out) {
         TORCH_CHECK(eng, "no weights loaded");
         TORCH_CHECK(hidden.is_cuda() && ids.is_cuda() && w.is_cuda() && out.is_cuda(), "tensors must be CUDA tensors");
@@ -240,6 +268,9 @@ struct MoEInferHandle : torch::CustomClassHolder {
         TORCH_CHECK(hidden.is_contiguous() && ids.is_contiguous() && w.is_contiguous() && out.is_contiguous(),
                     "tensors must be contiguous");
         TORCH_CHECK(out.sizes() == hidden.sizes(), "out must be [T, H]");
+        if (quant_type == MOE_MXFP4)
+            TORCH_CHECK(ids.get_device() == device && w.get_device() == device && out.get_device() == device,
+                        "tensors must be on the engine's device");
         c10::cuda::CUDAGuard g(device);
         check_rc(moe_engine_forward(eng, hidden.data_ptr(), out.data_ptr(), ids.data_ptr<int32_t>(), w.data_ptr<float>(),
                                     hidden.size(0), ids.size(1), dtype_code(hidden.scalar_type()),
@@ -387,6 +418,113 @@ std::tuple<at::Tensor, at::Tensor> quantize_rows(const at::Tensor& x) {
     return {qs, d};
 }
 
+// A contiguous tensor whose data start on 16 bytes.
+at::Tensor packed(const at::Tensor& t) {
+    auto c = t.contiguous();
+    return reinterpret_cast<uintptr_t>(c.data_ptr()) % 16 ? c.clone() : c;
+}
+
+std::tuple<at::Tensor, at::Tensor> route_scored(const at::Tensor& logits, const std::optional<at::Tensor>& bias, int64_t K,
+                                                const std::string& score, int64_t groups, int64_t topk_groups,
+                                                int64_t group_top, bool renormalize, double scale) {
+    TORCH_CHECK(logits.is_cuda() && logits.dim() == 2, "logits must be a CUDA [T,E] tensor");
+    TORCH_CHECK(score == "softmax" || score == "sigmoid", "score must be softmax or sigmoid");
+    auto l = logits.contiguous();
+    at::Tensor b;
+    if (bias.has_value() && bias->defined()) {
+        TORCH_CHECK(bias->is_cuda() && bias->get_device() == l.get_device() && bias->scalar_type() == at::kFloat &&
+                        bias->dim() == 1 && bias->size(0) == l.size(1),
+                    "bias must be float32 [E] on the logits' device");
+        b = bias->contiguous();
+    }
+    TORCH_CHECK(K >= 1 && K <= 32, "need 1 <= top_k <= 32");
+    TORCH_CHECK(groups >= 1 && groups <= 32 && topk_groups >= 1 && topk_groups <= groups,
+                "need 1 <= topk_groups <= num_groups <= 32");
+    TORCH_CHECK(group_top == 1 || group_top == 2, "group_top must be 1 or 2");
+    c10::cuda::CUDAGuard g(l.get_device());
+    auto ids = at::empty({l.size(0), K}, l.options().dtype(at::kInt));
+    auto w = at::empty({l.size(0), K}, l.options().dtype(at::kFloat));
+    check_rc(moe_route_scored(l.data_ptr(), dtype_code(l.scalar_type()), b.defined() ? b.data_ptr<float>() : nullptr,
+                              l.size(0), l.size(1), K, score == "sigmoid" ? MOE_SCORE_SIGMOID : MOE_SCORE_SOFTMAX, groups,
+                              topk_groups, (int32_t)group_top, renormalize ? 1 : 0, (float)scale, ids.data_ptr<int32_t>(),
+                              w.data_ptr<float>(), cur_stream(l.get_device())),
+             "moe_route_scored");
+    return {ids, w};
+}
+
+std::vector<int64_t> tiled_shape(int64_t rows, int64_t cols) { return {(rows + 127) / 128, (cols + 127) / 128, 512}; }
+
+std::tuple<at::Tensor, at::Tensor> quantize_mxfp4(const at::Tensor& x, bool tiled) {
+    TORCH_CHECK(x.is_cuda() && x.dim() == 2, "x must be a CUDA [rows, cols] tensor");
+    TORCH_CHECK(x.size(1) > 0 && x.size(1) % 32 == 0, "cols must be a positive multiple of 32");
+    auto c = packed(x);
+    c10::cuda::CUDAGuard g(c.get_device());
+    auto o = c.options().dtype(at::kByte);
+    auto q = at::empty({c.size(0), c.size(1) / 2}, o);
+    auto s = tiled ? at::empty(tiled_shape(c.size(0), c.size(1)), o) : at::empty({c.size(0), c.size(1) / 32}, o);
+    check_rc(moe_quantize_rows_mxfp4(c.data_ptr(), dtype_code(c.scalar_type()), c.size(0), c.size(1), tiled ? 1 : 0,
+                                     q.data_ptr<uint8_t>(), s.data_ptr<uint8_t>(), cur_stream(c.get_device())),
+             "quantize_rows_mxfp4");
+    return {q, s};
+}
+
+// Codes [rows, cols/2] with row-major or tiled scales; the scales are tiled when they have three dimensions.
+void check_mxfp4(const at::Tensor& q, const at::Tensor& s, bool must_tile, const char* what) {
+    TORCH_CHECK(q.is_cuda() && q.scalar_type() == at::kByte && q.dim() == 2 && q.size(1) > 0 && q.size(1) % 16 == 0, what,
+                ": codes must be CUDA uint8 [rows, cols/2] with cols a multiple of 32");
+    TORCH_CHECK(s.is_cuda() && s.scalar_type() == at::kByte && s.get_device() == q.get_device(), what,
+                ": scales must be uint8 on the codes' device");
+    const int64_t cols = q.size(1) * 2;
+    if (s.dim() == 3 || must_tile) {
+        TORCH_CHECK(s.sizes().vec() == tiled_shape(q.size(0), cols), what,
+                    ": tiled scales must be [ceil(rows/128), ceil(cols/128), 512]");
+    } else {
+        TORCH_CHECK(s.dim() == 2 && s.size(0) == q.size(0) && s.size(1) == cols / 32, what, ": scales must be [rows, cols/32]");
+    }
+}
+
+at::Tensor dequantize_mxfp4(const at::Tensor& q, const at::Tensor& s, std::optional<at::ScalarType> dtype) {
+    check_mxfp4(q, s, false, "dequantize_rows_mxfp4");
+    auto c = packed(q), sc = packed(s);
+    c10::cuda::CUDAGuard g(c.get_device());
+    const auto dt = dtype.value_or(at::kBFloat16);
+    const int32_t code = dtype_code(dt);
+    auto y = at::empty({c.size(0), c.size(1) * 2}, c.options().dtype(dt));
+    check_rc(moe_dequantize_rows_mxfp4(c.data_ptr<uint8_t>(), sc.data_ptr<uint8_t>(), c.size(0), c.size(1) * 2,
+                                       sc.dim() == 3 ? 1 : 0, y.data_ptr(), code, cur_stream(c.get_device())),
+             "dequantize_rows_mxfp4");
+    return y;
+}
+
+at::Tensor tile_scales(const at::Tensor& s) {
+    TORCH_CHECK(s.is_cuda() && s.scalar_type() == at::kByte && s.dim() == 2 && s.size(1) > 0,
+                "scales must be CUDA uint8 [rows, cols/32]");
+    auto c = s.contiguous();
+    c10::cuda::CUDAGuard g(c.get_device());
+    auto t = at::empty(tiled_shape(c.size(0), c.size(1) * 32), c.options());
+    check_rc(moe_mxfp4_tile_scales(c.data_ptr<uint8_t>(), c.size(0), c.size(1) * 32, t.data_ptr<uint8_t>(),
+                                   cur_stream(c.get_device())),
+             "mxfp4_tile_scales");
+    return t;
+}
+
+at::Tensor mxfp4_matmul(const at::Tensor& a, const at::Tensor& as, const at::Tensor& b, const at::Tensor& bs,
+                        std::optional<at::ScalarType> dtype) {
+    check_mxfp4(a, as, true, "mxfp4_matmul a");
+    check_mxfp4(b, bs, true, "mxfp4_matmul b");
+    TORCH_CHECK(a.get_device() == b.get_device() && a.size(1) == b.size(1), "a [M,K] and b [N,K] must agree in K and device");
+    auto ac = packed(a), asc = packed(as), bc = packed(b), bsc = packed(bs);
+    c10::cuda::CUDAGuard g(a.get_device());
+    const auto dt = dtype.value_or(at::kBFloat16);
+    const int32_t code = dtype_code(dt);
+    auto y = at::empty({a.size(0), b.size(0)}, a.options().dtype(dt));
+    if (y.numel() == 0) return y;
+    check_rc(moe_mxfp4_matmul(ac.data_ptr<uint8_t>(), asc.data_ptr<uint8_t>(), bc.data_ptr<uint8_t>(), bsc.data_ptr<uint8_t>(),
+                              a.size(0), b.size(0), a.size(1) * 2, y.data_ptr(), code, cur_stream(a.get_device())),
+             "mxfp4_matmul");
+    return y;
+}
+
 }  // namespace
 
 TORCH_LIBRARY_FRAGMENT(nanovllm, m) {
@@ -395,6 +533,7 @@ TORCH_LIBRARY_FRAGMENT(nanovllm, m) {
         .def("quantize_and_store_expert", &MoEInferHandle::quantize_and_store_expert)
         .def("store_quantized_repack", &MoEInferHandle::store_quantized_repack)
         .def("store_awq", &MoEInferHandle::store_awq)
+        .def("store_mxfp4", &MoEInferHandle::store_mxfp4)
         .def("set_expert_parallel", &MoEInferHandle::set_expert_parallel)
         .def("set_expert_placement", &MoEInferHandle::set_expert_placement)
         .def("set_expert_replicas", &MoEInferHandle::set_expert_replicas)
@@ -421,7 +560,8 @@ TORCH_LIBRARY_FRAGMENT(nanovllm, m) {
         .def("get_last_run_time_ms", [](const c10::intrusive_ptr<MoEInferHandle>& s) { return s->last_ms(); })
         .def("get_quant_type",
              [](const c10::intrusive_ptr<MoEInferHandle>& s) -> std::string {
-                 return s->quant_type == MOE_Q4_0 ? "Q4_0" : (s->quant_type == MOE_AWQ ? "AWQ" : "Q8_0");
+                 const char* names[] = {"Q8_0", "Q4_0", "AWQ", "MXFP4"};
+                 return names[s->quant_type];
              })
         .def("get_num_experts", [](const c10::intrusive_ptr<MoEInferHandle>& s) { return s->E; })
         .def("get_hidden_size", [](const c10::intrusive_ptr<MoEInferHandle>& s) { return s->H; })
@@ -442,6 +582,11 @@ TORCH_LIBRARY_FRAGMENT(nanovllm, m) {
             TORCH_CHECK(s->eng, "no weights loaded");
             const bool q4 = s->quant_type == MOE_Q4_0;
             const int64_t rows = which == 0 ? 2 * s->I : s->H, cols = which == 0 ? s->H : s->I;
+            if (s->quant_type == MOE_MXFP4) {
+                at::Tensor q = at::empty({rows, cols / 2}, at::kByte), sc = at::empty({rows, cols / 32}, at::kByte);
+                check_rc(moe_engine_export_expert(s->eng, e, (int32_t)which, q.data_ptr(), sc.data_ptr()), "export_expert");
+                return std::vector<at::Tensor>{q, sc};
+            }
             at::Tensor qs = q4 ? at::empty({rows, cols / 8}, at::kInt) : at::empty({rows, cols}, at::kChar);
             at::Tensor d = at::empty({rows, cols / 32}, at::kShort);
             check_rc(moe_engine_export_expert(s->eng, e, (int32_t)which, qs.data_ptr(), d.data_ptr()), "export_expert");
@@ -460,6 +605,11 @@ TORCH_LIBRARY_FRAGMENT(nanovllm, m) {
     m.def("moe_route_gemm(Tensor hidden, Tensor router_weight, int top_k, bool renormalize) -> (Tensor, Tensor)");
     m.def("moe_route_permute(Tensor topk_ids, int num_experts) -> (Tensor, Tensor, Tensor, Tensor)");
     m.def("quantize_rows_q8_0(Tensor x) -> (Tensor, Tensor)");
+    m.def("moe_route_scored(Tensor logits, Tensor? bias, int top_k, str score, int num_groups=1, int topk_groups=1, int group_top=1, bool renormalize=True, float scale=1.0) -> (Tensor, Tensor)");
+    m.def("quantize_rows_mxfp4(Tensor x, bool tiled_scales=False) -> (Tensor, Tensor)");
+    m.def("dequantize_rows_mxfp4(Tensor codes, Tensor scales, ScalarType? dtype=None) -> Tensor");
+    m.def("mxfp4_tile_scales(Tensor scales) -> Tensor");
+    m.def("mxfp4_matmul(Tensor a, Tensor a_scales, Tensor b, Tensor b_scales, ScalarType? out_dtype=None) -> Tensor");
 }
 
 TORCH_LIBRARY_IMPL(nanovllm, CUDA, m) {
@@ -472,4 +622,9 @@ TORCH_LIBRARY_IMPL(nanovllm, CUDA, m) {
     m.impl("moe_route_gemm", &moe_route_gemm);
     m.impl("moe_route_permute", &route_permute);
     m.impl("quantize_rows_q8_0", &quantize_rows);
+    m.impl("moe_route_scored", &route_scored);
+    m.impl("quantize_rows_mxfp4", &quantize_mxfp4);
+    m.impl("dequantize_rows_mxfp4", &dequantize_mxfp4);
+    m.impl("mxfp4_tile_scales", &tile_scales);
+    m.impl("mxfp4_matmul", &mxfp4_matmul);
 }

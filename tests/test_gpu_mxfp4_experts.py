@@ -1,0 +1,289 @@
+"""The expert layer on MXFP4 weights against a 64-bit reference, and its entry points."""
+import numpy as np
+import pytest
+import torch
+
+from tests import mx_reference as R
+
+pytestmark = pytest.mark.gpu
+
+if torch.cuda.is_available():
+    import moe_ascend_opt_b200  # noqa: F401
+    from moe_ascend_opt_b200 import capi
+
+ops = torch.ops.nanovllm
+TYPES = {"float32": torch.float32, "bfloat16": torch.bfloat16, "float16": torch.float16}
+
+
+def cuda(a):
+    return torch.from_numpy(np.ascontiguousarray(a)).cuda()
+
+
+def weights(E, H, I, seed):
+    rng = np.random.default_rng(seed)
+    c13, s13 = R.quantize(0.02 * rng.standard_normal((E, 2 * I, H)))
+    c2, s2 = R.quantize(0.02 * rng.standard_normal((E, H, I)))
+    return (R.pack(c13), s13, R.pack(c2), s2), R.decode(c13, s13), R.decode(c2, s2)
+
+
+def handle(E, H, I, packed):
+    h = torch.classes.nanovllm.MoEInfer(E, H, I, 3)
+    h.store_mxfp4(*[torch.from_numpy(p) for p in packed])
+    return h
+
+
+def tokens(T, H, E, K, seed, dtype="bfloat16"):
+    rng = np.random.default_rng(seed + 1)
+    x = cuda(rng.standard_normal((T, H)) * np.exp(0.5 * rng.standard_normal(H))).to(TYPES[dtype])
+    ids = np.stack([rng.permutation(E)[:K] for _ in range(T)]).astype(np.int32).reshape(T, K)
+    w = rng.random((T, K)).astype(np.float32) + 0.05
+    return x, ids, w / w.sum(1, keepdims=True)
+
+
+def close(y, want, tol):
+    y = y.double().cpu().numpy()
+    bad = ~(np.abs(y - want) <= tol)
+    assert not bad.any(), (np.argwhere(bad)[:5], np.abs(y - want).max(), bad.sum())
+
+
+SHAPES = [(4, 64, 32, 2), (8, 256, 96, 3), (16, 512, 160, 8), (3, 96, 64, 3), (1, 128, 128, 1), (40, 320, 224, 6)]
+
+
+@pytest.mark.parametrize("E,H,I,K", SHAPES)
+@pytest.mark.parametrize("T", [1, 2, 7, 33, 150])
+def test_forward(E, H, I, K, T):
+    packed, w13, w2 = weights(E, H, I, E + H)
+    h = handle(E, H, I, packed)
+    for dtype in ("bfloat16", "float16"):
+        x, ids, w = tokens(T, H, E, K, T, dtype)
+        y = ops.moe_forward(x, cuda(ids), cuda(w), h)
+        assert h.device_error() == 0 and y.dtype == x.dtype
+        want, tol = R.experts(x.double().cpu().numpy(), ids, w, w13, w2, dtype)
+        close(y, want, tol)
+    p = ops.moe_forward_partial(x, cuda(ids), cuda(w), h)
+    close(p, want, R.experts(x.double().cpu().numpy(), ids, w, w13, w2, "float32")[1])
+
+
+def test_one_expert_takes_all():
+    """More than one tile of rows for an expert, others empty."""
+    E, H, I, K, T = 6, 128, 64, 2, 300
+    packed, w13, w2 = weights(E, H, I, 3)
+    x, ids, w = tokens(T, H, E, K, 5)
+    ids[:, 0], ids[:, 1] = 4, np.where(np.arange(T) % 97 == 0, 2, 5)
+    want, tol = R.experts(x.double().cpu().numpy(), ids, w, w13, w2, "bfloat16")
+    close(ops.moe_forward(x, cuda(ids), cuda(w), handle(E, H, I, packed)), want, tol)
+
+
+@pytest.mark.parametrize("T", [1, 5, 140])
+def test_skipped_ids(T):
+    """Ids outside the engine's experts are left out; a token that keeps none is zero; an id twice counts twice."""
+    E, H, I, K = 8, 128, 96, 4
+    packed, w13, w2 = weights(E, H, I, 4)
+    h = handle(E, H, I, packed)
+    x, ids, w = tokens(T, H, E, K, 6)
+    ids[0] = [-1, E, 1 << 30, -(1 << 31)]
+    if T > 2:
+        ids[1], ids[2] = [3, 3, 3, -1], [7, -5, 7, 0]
+        ids[T - 1] = -1
+    y = torch.full((T, H), 7.0, device="cuda", dtype=x.dtype)
+    ctx = torch.classes.nanovllm.MoEGraphContext(h, T, K, 1)
+    ops.moe_forward_npu_graph_out(x, cuda(ids), cuda(w), h, ctx, y)
+    want, tol = R.experts(x.double().cpu().numpy(), ids, w, w13, w2, "bfloat16")
+    close(y, want, tol)
+    assert not y[0].any() and (T < 3 or not y[T - 1].any())
+
+
+def test_nan_tokens_stay_apart():
+    E, H, I, K, T = 8, 256, 128, 4, 70
+    packed, _, _ = weights(E, H, I, 7)
+    h = handle(E, H, I, packed)
+    x, ids, w = tokens(T, H, E, K, 8)
+    clean = ops.moe_forward(x, cuda(ids), cuda(w), h)
+    x2 = x.clone()
+    x2[13, 40], x2[60, 3] = float("nan"), float("inf")
+    y = ops.moe_forward(x2, cuda(ids), cuda(w), h)
+    assert y[13].isnan().all() and y[60].isnan().all()
+    keep = torch.ones(T, dtype=torch.bool, device="cuda")
+    keep[13] = keep[60] = False
+    assert torch.equal(y[keep], clean[keep])
+
+
+def test_rows_do_not_depend_on_the_batch():
+    """A token's row is the same whatever else is in the call, and from call to call."""
+    E, H, I, K, T = 16, 256, 160, 4, 400
+    packed, _, _ = weights(E, H, I, 9)
+    h = handle(E, H, I, packed)
+    x, ids, w = tokens(T, H, E, K, 10)
+    idc, wc = cuda(ids), cuda(w)
+    full = ops.moe_forward(x, idc, wc, h)
+    assert torch.equal(full, ops.moe_forward(x, idc, wc, h))
+    for n in (1, 3, 64, 129):
+        assert torch.equal(full[:n], ops.moe_forward(x[:n], idc[:n].contiguous(), wc[:n].contiguous(), h))
+
+
+def test_long_call_in_slices():
+    E, H, I, K, T = 8, 32, 32, 8, 40000
+    packed, w13, w2 = weights(E, H, I, 12)
+    h = handle(E, H, I, packed)
+    x, ids, w = tokens(T, H, E, K, 13)
+    y = ops.moe_forward(x, cuda(ids), cuda(w), h)
+    some = np.concatenate([np.arange(20), np.arange(32760, 32780), np.arange(T - 20, T)])
+    want, tol = R.experts(x.double().cpu().numpy()[some], ids[some], w[some], w13, w2, "bfloat16")
+    close(y[torch.from_numpy(some).cuda()], want, tol)
+
+
+def test_graph_growth_and_streams():
+    """A captured call keeps its results when the workspace grows after the capture; eager calls on two streams."""
+    E, H, I, K = 8, 256, 128, 4
+    packed, _, _ = weights(E, H, I, 14)
+    h = handle(E, H, I, packed)
+    x, ids, w = tokens(9, H, E, K, 15)
+    idc, wc = cuda(ids), cuda(w)
+    ctx = torch.classes.nanovllm.MoEGraphContext(h, 9, K, 1)
+    y = torch.empty_like(x)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        ops.moe_forward_npu_graph_out(x, idc, wc, h, ctx, y)
+    big, bids, bw = tokens(600, H, E, K, 16)
+    bids, bw = cuda(bids), cuda(bw)
+    first = ops.moe_forward(big, bids, bw, h)  # outgrows the captured workspace
+    for seed in (1, 2):
+        x.copy_(tokens(9, H, E, K, 20 + seed)[0])
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(y, ops.moe_forward(x, idc, wc, h))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    outs = []
+    for i in range(6):
+        with torch.cuda.stream(side if i % 2 else torch.cuda.current_stream()):
+            outs.append(ops.moe_forward(big, bids, bw, h))
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, first) for o in outs)
+    with pytest.raises(RuntimeError, match="before capture"):
+        g2 = torch.cuda.CUDAGraph()
+        huge, hids, hw = tokens(3000, H, E, K, 17)
+        hids, hw = cuda(hids), cuda(hw)
+        with torch.cuda.graph(g2):
+            ops.moe_forward(huge, hids, hw, h)
+    torch.cuda.synchronize()
+    assert torch.equal(ops.moe_forward(big, bids, bw, h), first)
+
+
+def test_expert_parallel_parts_sum_to_the_layer():
+    E, H, I, K, T = 12, 128, 96, 4, 50
+    packed, w13, w2 = weights(E, H, I, 18)
+    x, ids, w = tokens(T, H, E, K, 19)
+    idc, wc = cuda(ids), cuda(w)
+    total = torch.zeros(T, H, device="cuda")
+    for part in ([0, 3, 7, 11], [1, 2, 4, 5, 6, 8, 9, 10]):
+        h = torch.classes.nanovllm.MoEInfer(E, H, I, 3)
+        h.set_expert_placement(part)
+        h.store_mxfp4(*[cuda(p) for p in packed])
+        total += ops.moe_forward_partial(x, idc, wc, h)
+    want, tol = R.experts(x.double().cpu().numpy(), ids, w, w13, w2, "float32")
+    close(total, want, 2 * tol)
+    rank = torch.classes.nanovllm.MoEInfer(E, H, I, 3)
+    rank.set_expert_parallel(1, 3)
+    rank.store_mxfp4(*[torch.from_numpy(p) for p in packed])
+    mine = np.where((ids >= 4) & (ids < 8), ids, -1)
+    want, tol = R.experts(x.double().cpu().numpy(), mine, w, w13, w2, "bfloat16")
+    close(ops.moe_forward(x, idc, wc, rank), want, tol)
+
+
+@pytest.mark.parametrize("H,I", [(128, 96), (96, 32), (256, 160)])
+def test_load_export_quantize_file(H, I, tmp_path):
+    """The three ways to fill an engine hold the same bytes and give the same results."""
+    E, K, T = 4, 2, 11
+    rng = np.random.default_rng(21)
+    wg, wu, wd = (0.02 * rng.standard_normal(s).astype(np.float32) for s in ((E, I, H), (E, I, H), (E, H, I)))
+    c13, s13 = R.quantize(np.concatenate([wg, wu], 1))
+    c2, s2 = R.quantize(wd)
+    packed = (R.pack(c13), s13, R.pack(c2), s2)
+    a = handle(E, H, I, packed)
+    b = torch.classes.nanovllm.MoEInfer(E, H, I, 3)
+    for e in range(E):
+        b.quantize_and_store_expert(e, "gate_proj", torch.from_numpy(wg[e]))
+        b.quantize_and_store_expert(e, "up_proj", torch.from_numpy(wu[e]).cuda())
+        b.quantize_and_store_expert(e, "down_proj", torch.from_numpy(wd[e]))
+    a.save(str(tmp_path / "w"))
+    c = torch.classes.nanovllm.MoEInfer(E, H, I, 3)
+    c.load_file(str(tmp_path / "w"))
+    x, ids, w = tokens(T, H, E, K, 22)
+    first = ops.moe_forward(x, cuda(ids), cuda(w), a)
+    for h in (a, b, c):
+        for e in range(E):
+            for which, (q, s) in enumerate(((packed[0], s13), (packed[2], s2))):
+                got = h.export_expert(e, which)
+                np.testing.assert_array_equal(got[0].numpy(), q[e])
+                np.testing.assert_array_equal(got[1].numpy(), s[e])
+        assert torch.equal(ops.moe_forward(x, cuda(ids), cuda(w), h), first)
+    other = torch.classes.nanovllm.MoEInfer(E, H, I, 1)
+    with pytest.raises(RuntimeError, match="differs"):
+        other.load_file(str(tmp_path / "w"))
+
+
+@pytest.mark.parametrize("T", [1, 40, 200])
+def test_dense_forward(T):
+    E, H, I = 3, 256, 128
+    packed, w13, w2 = weights(E, H, I, 23)
+    h = handle(E, H, I, packed)
+    x, _, _ = tokens(T, H, E, 1, 24)
+    for e in (2, 0):
+        want, tol = R.experts(x.double().cpu().numpy(), np.full((T, 1), e, np.int32), np.ones((T, 1)), w13, w2, "bfloat16")
+        close(ops.moe_dense_forward(x, e, h), want, tol)
+
+
+def test_refusals():
+    E, H, I, K = 4, 64, 32, 2
+    packed, _, _ = weights(E, H, I, 25)
+    h = handle(E, H, I, packed)
+    x, ids, w = tokens(5, H, E, K, 26)
+    idc, wc = cuda(ids), cuda(w)
+    with pytest.raises(RuntimeError, match="aligned"):
+        ops.moe_forward(torch.zeros(5 * H + 1, device="cuda", dtype=torch.bfloat16)[1:].view(5, H), idc, wc, h)
+    with pytest.raises(RuntimeError, match="contiguous"):
+        ops.moe_forward(x.repeat(1, 2)[:, ::2], idc, wc, h)
+    with pytest.raises(RuntimeError, match="float16 or bfloat16"):
+        ops.moe_forward(x.float(), idc, wc, h)
+    assert ops.moe_forward(x[:0], idc[:0], wc[:0], h).shape == (0, H)
+    eng = capi.Engine(E, H, I, capi.MXFP4)
+    with pytest.raises(capi.MoeError, match="no weights"):
+        eng.forward(x, x, idc, wc, capi.BF16, capi.BF16)
+    eng.load_mxfp4(*[torch.from_numpy(p) for p in packed])
+    y = torch.empty_like(x)
+    with pytest.raises(capi.MoeError, match="no no-allocation"):
+        eng.forward_noalloc(x, y, idc, wc, capi.BF16, capi.BF16)
+    with pytest.raises(capi.MoeError, match="peer combine"):
+        capi.call("moe_engine_p2p_mailbox", eng.h, 2, 4, y.data_ptr())
+    with pytest.raises(capi.MoeError, match="load_mxfp4"):
+        eng.load_quantized(x, x, x, x, capi.F16)
+    with pytest.raises(capi.MoeError, match="at most 1024"):
+        capi.Engine(1025, 32, 32, capi.MXFP4)
+    eng.forward(x, y, idc, wc, capi.BF16, capi.BF16)
+    assert torch.equal(y, ops.moe_forward(x, idc, wc, h))
+
+
+@pytest.mark.parametrize("T", [1, 6, 90])
+def test_router_to_output(T):
+    """Route by scores, run the routed layer, then a quantised linear layer, as a model's step does."""
+    E, H, I, K, N = 32, 256, 96, 4, 192
+    packed, w13, w2 = weights(E, H, I, 27)
+    h = handle(E, H, I, packed)
+    rng = np.random.default_rng(28)
+    x = cuda(rng.standard_normal((T, H))).bfloat16()
+    logits = cuda(rng.standard_normal((T, E)).astype(np.float32))
+    logits[T - 1] = -float("inf")  # a padding row
+    bias = cuda((0.1 * rng.standard_normal(E)).astype(np.float32))
+    lw, ls = ops.quantize_rows_mxfp4(cuda(0.05 * rng.standard_normal((N, H)).astype(np.float32)), True)
+    ids, w = ops.moe_route_scored(logits, bias, K, "sigmoid", 4, 2, 2, True, 2.5)
+    y = ops.moe_forward(x, ids, w, h)
+    z = ops.mxfp4_matmul(*ops.quantize_rows_mxfp4(y, True), lw, ls, torch.float32)
+    ri, rw = R.route(logits.double().cpu().numpy(), bias.double().cpu().numpy(), K, "sigmoid", 4, 2, 2, True, 2.5)
+    np.testing.assert_array_equal(ids.cpu().numpy(), ri)
+    want, tol = R.experts(x.double().cpu().numpy(), ri, w.double().cpu().numpy(), w13, w2, "bfloat16")
+    close(y, want, tol)
+    assert not y[T - 1].any() and (ri[T - 1] == -1).all()
+    a = R.decode(*R.quantize(y.double().cpu().numpy()))
+    b = ops.dequantize_rows_mxfp4(lw, ls, torch.float32).double().cpu().numpy()
+    close(z, a @ b.T, R.product_error(a, b) + R.HALF["float32"] * np.abs(a @ b.T))
