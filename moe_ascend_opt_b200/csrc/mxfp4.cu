@@ -92,15 +92,25 @@ int sm_count(int dev, int* out) {
     return MOE_OK;
 }
 
-constexpr int kNT = 128, kStages = 6;
+// Tiles of 128 x 256 (a CTA per SM), or of 128 x 64 (two) for products with few rows.
+constexpr int kWide = 256, kWideStages = 4, kNarrow = 64, kNarrowStages = 4;
+
+template <int MODE, int NT, int STAGES>
+int launch_gemm_nt(const CUtensorMap& ta, const CUtensorMap& tb, mx::GemmParams& p, int64_t m_tiles, int sms, bool pdl,
+                   cudaStream_t st) {
+    using S = mx::Shape<NT>;
+    auto fn = mx::mx_gemm_kernel<MODE, NT, STAGES>;
+    const int smem = STAGES * S::kStage + 1024;
+    if (int rc = allow_smem(reinterpret_cast<const void*>(fn), smem)) return rc;
+    p.nt_count = (int)ceil_div(p.N, NT);
+    return launch(fn, (unsigned)std::min<int64_t>(m_tiles * p.nt_count, sms * S::kCtas), S::kThreads, smem, pdl, st, ta, tb, p);
+}
 
 template <int MODE>
-int launch_gemm(const CUtensorMap& ta, const CUtensorMap& tb, const mx::GemmParams& p, int64_t tiles, int sms, bool pdl,
+int launch_gemm(const CUtensorMap& ta, const CUtensorMap& tb, mx::GemmParams& p, int64_t m_tiles, int sms, bool wide, bool pdl,
                 cudaStream_t st) {
-    auto fn = mx::mx_gemm_kernel<MODE, kNT, kStages>;
-    const int smem = kStages * mx::Shape<kNT>::kStage + 1024;
-    if (int rc = allow_smem(reinterpret_cast<const void*>(fn), smem)) return rc;
-    return launch(fn, (unsigned)std::min<int64_t>(tiles, sms), mx::kGemmThreads, smem, pdl, st, ta, tb, p);
+    return wide ? launch_gemm_nt<MODE, kWide, kWideStages>(ta, tb, p, m_tiles, sms, pdl, st)
+                : launch_gemm_nt<MODE, kNarrow, kNarrowStages>(ta, tb, p, m_tiles, sms, pdl, st);
 }
 
 bool dtype_ok(int32_t t) { return t == MOE_F16 || t == MOE_BF16 || t == MOE_F32; }
@@ -225,16 +235,16 @@ extern "C" int moe_mxfp4_matmul(const uint8_t* a, const uint8_t* a_scales, const
     }
     CUtensorMap ta, tb;
     if (int rc = encode(&ta, a, K / 2, M, 0, mx::kTileM)) return rc;
-    if (int rc = encode(&tb, b, K / 2, N, 1, kNT)) return rc;
+    p.mt_count = (int)ceil_div(M, mx::kTileM);
+    const bool wide = p.mt_count * ceil_div(N, kWide) >= sms;
+    if (int rc = encode(&tb, b, K / 2, N, 1, wide ? kWide : kNarrow)) return rc;
     p.M = (int)M; p.N = (int)N; p.K = (int)K;
     p.kb = (int)ceil_div(K, 128);
-    p.nt_count = (int)ceil_div(N, kNT);
-    p.mt_count = (int)ceil_div(M, mx::kTileM);
     p.sfa = a_scales;
     p.sfb = b_scales;
     p.out = y;
     p.out_dtype = out_dtype;
-    return launch_gemm<mx::kDense>(ta, tb, p, (int64_t)p.nt_count * p.mt_count, sms, false, st);
+    return launch_gemm<mx::kDense>(ta, tb, p, p.mt_count, sms, wide, false, st);
 }
 
 // ------------------------------------------------------------------ expert layer
@@ -245,7 +255,7 @@ struct MxLayer {
     int sms = 0;
     int64_t kb1 = 0, kb2 = 0, nb1 = 0, nb2 = 0;  // scale tiles along K and N of gate_up (1) and down (2)
     uint8_t *q1 = nullptr, *s1 = nullptr, *q2 = nullptr, *s2 = nullptr;
-    CUtensorMap t1{}, t2{};
+    CUtensorMap t1[2]{}, t2[2]{};  // narrow and wide boxes
     uint8_t* ws = nullptr;
     size_t ws_bytes = 0;
     std::vector<uint8_t*> retired;  // earlier workspaces: captured graphs may still hold them
@@ -305,12 +315,20 @@ __global__ void mx_store_rows_kernel(const void* w, int64_t n, int cols, int hal
 }
 
 struct Workspace {
-    int32_t *mtiles, *mt_expert, *mt_rows, *rowtok, *ppos;
+    int32_t *mtiles, *mt_expert, *mt_rows, *ppos, *counts;
     uint8_t *xq, *xs, *hq, *hs;
     float* part;
     int64_t mt;  // bound of the number of m tiles
     size_t bytes;
 };
+
+// Tokens of one CTA of the token kernel: runs of 256 pairs or more and at most 512 runs in long
+// calls (every CTA reads all runs' counts), one token or a share of 2 x 148 CTAs in short ones.
+int64_t prep_tokens(int64_t T, int64_t K) {
+    const int64_t P = T * K;
+    if (P <= mx::kPrepSelf) return ceil_div(T, 296);
+    return std::max<int64_t>(ceil_div(256, K), ceil_div(T, 512));
+}
 
 Workspace carve(const MxLayer* l, int64_t T, int64_t K, uint8_t* base) {
     Workspace w{};
@@ -326,9 +344,9 @@ Workspace carve(const MxLayer* l, int64_t T, int64_t K, uint8_t* base) {
     w.mtiles = reinterpret_cast<int32_t*>(take(4));
     w.mt_expert = reinterpret_cast<int32_t*>(take(w.mt * 4));
     w.mt_rows = reinterpret_cast<int32_t*>(take(w.mt * 4));
-    w.rowtok = reinterpret_cast<int32_t*>(take(rows * 4));
     w.ppos = reinterpret_cast<int32_t*>(take(P * 4));
-    w.xq = take(T * (H / 2));
+    w.counts = reinterpret_cast<int32_t*>(take(P > mx::kPrepSelf ? ceil_div(T, prep_tokens(T, K)) * l->cfg.num_experts * 4 : 0));
+    w.xq = take(rows * (H / 2));
     w.xs = take(w.mt * l->kb1 * 512);
     w.hq = take(rows * (I / 2));
     w.hs = take(w.mt * l->kb2 * 512);
@@ -363,14 +381,6 @@ int grow(MxLayer* l, size_t bytes) {
 }
 
 template <int DT>
-int tokens_launch(const MxLayer* l, const MxForward& f, const void* x, const Workspace& w, int64_t T, cudaStream_t st) {
-    const int H = (int)l->cfg.hidden_size;
-    const unsigned block = (unsigned)std::min<int64_t>(256, ceil_div(H / 8, 32) * 32);
-    return launch(mx::mx_tokens_kernel<DT>, (unsigned)T, block, 0, f.pdl, st, x, H, (int)f.K, (const int32_t*)w.ppos, w.xq, w.xs,
-                  (int)l->kb1);
-}
-
-template <int DT>
 int combine_launch(const MxLayer* l, const MxForward& f, const float* tw, void* y, const Workspace& w, int64_t T, cudaStream_t st) {
     const int H = (int)l->cfg.hidden_size;
     return launch(mx::mx_combine_kernel<DT>, (unsigned)std::min<int64_t>(ceil_div(T * (H / 4), 256), l->sms * 16), 256, 0, f.pdl, st,
@@ -381,31 +391,39 @@ int forward_slice(MxLayer* l, const MxForward& f, const void* x, void* y, const 
                   cudaStream_t st) {
     const int64_t E = l->cfg.num_experts, H = l->cfg.hidden_size, I = l->cfg.intermediate_size;
     const Workspace w = carve(l, T, f.K, l->ws);
-    mx::RouteParams r{};
-    r.ids = ids;
-    r.TK = (int)(T * f.K); r.K = (int)f.K; r.E = (int)E; r.e_off = l->cfg.expert_offset;
+    mx::PrepParams r{};
+    r.x = x; r.ids = ids;
+    r.T = (int)T; r.K = (int)f.K; r.H = (int)H; r.E = (int)E; r.e_off = l->cfg.expert_offset;
     r.emap = f.emap; r.emap_n = f.emap_n;
-    r.mtiles = w.mtiles; r.mt_expert = w.mt_expert; r.mt_rows = w.mt_rows; r.rowtok = w.rowtok; r.ppos = w.ppos;
-    const int rsmem = (int)(32 * E + 32) * 4;
-    if (int rc = allow_smem(reinterpret_cast<const void*>(mx::mx_route_kernel), 33 * 1024 * 4)) return rc;
-    if (int rc = launch(mx::mx_route_kernel, 1, 1024, rsmem, f.pdl, st, r)) return rc;
-    if (int rc = f.act_dtype == MOE_BF16 ? tokens_launch<MOE_BF16>(l, f, x, w, T, st) : tokens_launch<MOE_F16>(l, f, x, w, T, st))
-        return rc;
+    r.tokens = (int)prep_tokens(T, f.K);
+    r.mtiles = w.mtiles; r.mt_expert = w.mt_expert; r.mt_rows = w.mt_rows; r.ppos = w.ppos;
+    r.xq = w.xq; r.xs = w.xs; r.kb = (int)l->kb1;
+    const unsigned runs = (unsigned)ceil_div(T, r.tokens);
+    const bool self = T * f.K <= mx::kPrepSelf;
+    if (!self) {
+        r.counts = w.counts;
+        if (int rc = launch(mx::mx_count_kernel, runs, mx::kPrepThreads, (size_t)E * 4, f.pdl, st, r, w.counts)) return rc;
+    }
+    const size_t psmem = ((size_t)(mx::kPrepWarps + 1) * E + (self ? T : r.tokens) * f.K) * 4;
+    auto prep = f.act_dtype == MOE_BF16 ? mx::mx_prep_kernel<MOE_BF16> : mx::mx_prep_kernel<MOE_F16>;
+    if (int rc = allow_smem(reinterpret_cast<const void*>(prep), 128 * 1024)) return rc;
+    if (int rc = launch(prep, runs, mx::kPrepThreads, psmem, f.pdl, st, r)) return rc;
     CUtensorMap tx, th;
-    if (int rc = encode(&tx, w.xq, H / 2, T, 0, 1)) return rc;
+    if (int rc = encode(&tx, w.xq, H / 2, w.mt * mx::kTileM, 0, 16)) return rc;
     if (int rc = encode(&th, w.hq, I / 2, w.mt * mx::kTileM, 0, 16)) return rc;
     mx::GemmParams p{};
-    p.mtiles = w.mtiles; p.mt_expert = w.mt_expert; p.mt_rows = w.mt_rows; p.rowtok = w.rowtok;
+    p.mtiles = w.mtiles; p.mt_expert = w.mt_expert; p.mt_rows = w.mt_rows;
     p.err = f.err;
     p.I = (int)I;
+    const bool wide = T * f.K >= 32 * std::min<int64_t>(E, T * f.K);
     mx::GemmParams g1 = p;
-    g1.N = (int)(2 * I); g1.K = (int)H; g1.kb = (int)l->kb1; g1.nt_count = (int)ceil_div(2 * I, kNT);
+    g1.N = (int)(2 * I); g1.K = (int)H; g1.kb = (int)l->kb1;
     g1.sfa = w.xs; g1.sfb = l->s1; g1.hq = w.hq; g1.hs = w.hs; g1.hkb = (int)l->kb2;
-    if (int rc = launch_gemm<mx::kGateUp>(tx, l->t1, g1, w.mt * g1.nt_count, l->sms, f.pdl, st)) return rc;
+    if (int rc = launch_gemm<mx::kGateUp>(tx, l->t1[wide], g1, w.mt, l->sms, wide, f.pdl, st)) return rc;
     mx::GemmParams g2 = p;
-    g2.N = (int)H; g2.K = (int)I; g2.kb = (int)l->kb2; g2.nt_count = (int)ceil_div(H, kNT);
+    g2.N = (int)H; g2.K = (int)I; g2.kb = (int)l->kb2;
     g2.sfa = w.hs; g2.sfb = l->s2; g2.out = w.part;
-    if (int rc = launch_gemm<mx::kDown>(th, l->t2, g2, w.mt * g2.nt_count, l->sms, f.pdl, st)) return rc;
+    if (int rc = launch_gemm<mx::kDown>(th, l->t2[wide], g2, w.mt, l->sms, wide, f.pdl, st)) return rc;
     return f.out_dtype == MOE_F32    ? combine_launch<MOE_F32>(l, f, tw, y, w, T, st)
            : f.out_dtype == MOE_BF16 ? combine_launch<MOE_BF16>(l, f, tw, y, w, T, st)
                                      : combine_launch<MOE_F16>(l, f, tw, y, w, T, st);
@@ -437,8 +455,11 @@ int mx_create(const moe_config& cfg, int num_sms, MxLayer** out) {
             return fail(MOE_ERR_CUDA, std::string("MXFP4 weights: ") + cudaGetErrorString(e));
         }
     }
-    int rc = encode(&l->t1, l->q1, H / 2, 2 * I, E, kNT);
-    if (rc == MOE_OK) rc = encode(&l->t2, l->q2, I / 2, H, E, kNT);
+    int rc = MOE_OK;
+    for (int w = 0; w < 2 && rc == MOE_OK; ++w) {
+        rc = encode(&l->t1[w], l->q1, H / 2, 2 * I, E, w ? kWide : kNarrow);
+        if (rc == MOE_OK) rc = encode(&l->t2[w], l->q2, I / 2, H, E, w ? kWide : kNarrow);
+    }
     if (rc != MOE_OK) {
         mx_destroy(l);
         return rc;

@@ -1,14 +1,15 @@
 // Products of MXFP4 matrices on the tensor cores (tcgen05.mma kind::mxf4, block scales applied
 // by the MMA): the dense product a b^T, and the gate_up and down products of the expert layer.
 //
-// One persistent, warp-specialised kernel: a CTA per SM walks over the (128 x NT) output tiles.
+// One persistent, warp-specialised kernel: its CTAs walk over the (128 x NT) output tiles.
 //   warp 0      TMA producer: a stage is 256 elements of K, i.e. 128 bytes (one swizzle atom) of
 //               each of the 128 rows of A and NT rows of B, and their scale tiles (512 bytes hold
 //               128 rows x 128 elements);
-//   warp 1      one thread copies the stage's scales to TMEM (tcgen05.cp) and issues its MMAs
-//               (K = 64 each), fp32 accumulators in TMEM, two of them so that the epilogue of a
-//               tile overlaps the products of the next;
-//   warps 4-7   epilogue, a thread per row of the tile.
+//   warp 1      copies the stage's scales to TMEM (tcgen05.cp) and issues its MMAs (K = 64 each),
+//               fp32 accumulators in TMEM;
+//   warps 4-    epilogue, a thread per row of the tile and NT or NT / 2 columns; it takes its
+//               accumulators to registers and gives the TMEM back at once, so that its arithmetic
+//               and stores overlap the products of the next tile.
 // The rows of A are tokens, so a thread of the epilogue holds whole 32-blocks of its token: the
 // gate_up epilogue forms SiLU(gate) * up and quantises it without a word to other threads.
 // gate_up weights lie in 64-row groups of 32 gate rows and the 32 up rows of the same units.
@@ -23,7 +24,7 @@ namespace moe {
 namespace mx {
 
 enum Mode { kDense = 0, kGateUp = 1, kDown = 2 };
-constexpr int kTileM = 128, kStageK = 256, kGemmThreads = 256;
+constexpr int kTileM = 128, kStageK = 256;
 
 struct GemmParams {
     int M, N, K;         // dense: rows of a; N rows of b (of one expert); depth
@@ -34,7 +35,6 @@ struct GemmParams {
     const int32_t* mtiles;     // experts: number of m tiles, then expert and rows of each
     const int32_t* mt_expert;
     const int32_t* mt_rows;
-    const int32_t* rowtok;     // token of each row of the m tiles
     void* out;           // dense [M][N] (out_dtype); down fp32 [m tiles * 128][N]
     int out_dtype;
     int I;               // gate_up: hq [m tiles * 128][I / 2], hs tiled with hkb tiles along I
@@ -46,10 +46,15 @@ struct GemmParams {
 
 template <int NT>
 struct Shape {
+    static constexpr int kSfTiles = (NT + 127) / 128;  // scale tiles (128 rows) that cover a stage's B rows
     static constexpr int kA = kTileM * 128, kB = NT * 128;
-    static constexpr int kSfB = (NT + 127) / 128 * 1024;
-    static constexpr int kStage = kA + kB + 1024 + kSfB;
-    static constexpr int kSfCols = 8 + kSfB / 128;  // TMEM columns of a stage's scales
+    static constexpr int kStage = kA + kB + 1024 * (1 + kSfTiles);
+    static constexpr int kSfCols = 8 * (1 + kSfTiles);  // TMEM columns of a stage's scales
+    static constexpr int kAcc = NT <= 128 ? 2 : 1;      // accumulators
+    static constexpr int kEpiWarps = NT >= 256 ? 8 : 4;
+    static constexpr int kCols = NT / (kEpiWarps / 4);  // columns of an epilogue thread
+    static constexpr int kThreads = 128 + 32 * kEpiWarps;
+    static constexpr int kCtas = NT <= 64 ? 2 : 1;      // per SM
 };
 
 // Descriptor of a 512-byte scale tile for tcgen05.cp: no swizzle, 8-row groups of 128 bytes.
@@ -77,6 +82,13 @@ MOE_DEV void cp_scales(uint32_t taddr, uint64_t desc) {
     asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
 }
 
+// One lane of a converged warp.
+MOE_DEV bool elect_one() {
+    uint32_t r;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
+    return r != 0;
+}
+
 MOE_DEV void tma_2d(uint32_t dst, const CUtensorMap* m, int x, int y, uint64_t* bar) {
     asm volatile(
         "cp.async.bulk.tensor.2d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
@@ -89,14 +101,6 @@ MOE_DEV void tma_3d(uint32_t dst, const CUtensorMap* m, int x, int y, int z, uin
         "l"(m), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar))
         : "memory");
 }
-// Four rows (the map's box is one row), 128 bytes of each.
-MOE_DEV void tma_gather4(uint32_t dst, const CUtensorMap* m, int x, int4 r, uint64_t* bar) {
-    asm volatile(
-        "cp.async.bulk.tensor.2d.shared::cta.global.tile::gather4.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5, %6}], [%7];"
-        ::"r"(dst), "l"(m), "r"(x), "r"(r.x), "r"(r.y), "r"(r.z), "r"(r.w), "r"(smem_u32(bar))
-        : "memory");
-}
-
 // Bounded wait that also ends when another role of the CTA has given up.
 MOE_DEV bool wait_or_fail(uint64_t* bar, uint32_t parity, volatile int* failed) {
     for (uint32_t it = 0; it < kSpinLimit; ++it) {
@@ -106,6 +110,31 @@ MOE_DEV bool wait_or_fail(uint64_t* bar, uint32_t parity, volatile int* failed) 
     }
     *failed = 1;
     return false;
+}
+
+// The same by a whole warp, which goes on or leaves together.
+MOE_DEV bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* failed) {
+    return __all_sync(0xffffffffu, wait_or_fail(bar, parity, failed));
+}
+
+// N consecutive fp32 columns of this thread's TMEM lane.
+template <int N>
+MOE_DEV void load_columns(uint32_t taddr, float (&v)[N]) {
+    uint32_t r[N];
+#pragma unroll
+    for (int c = 0; c < N; c += 16)
+        asm volatile(
+            "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+            : "=r"(r[c]), "=r"(r[c + 1]), "=r"(r[c + 2]), "=r"(r[c + 3]), "=r"(r[c + 4]), "=r"(r[c + 5]), "=r"(r[c + 6]),
+              "=r"(r[c + 7]), "=r"(r[c + 8]), "=r"(r[c + 9]), "=r"(r[c + 10]), "=r"(r[c + 11]), "=r"(r[c + 12]),
+              "=r"(r[c + 13]), "=r"(r[c + 14]), "=r"(r[c + 15])
+            : "r"(taddr + c));
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+    // the registers hold their values from the wait on: tie every use to it
+#pragma unroll
+    for (int c = 0; c < N; ++c) asm volatile("" : "+r"(r[c]));
+#pragma unroll
+    for (int c = 0; c < N; ++c) v[c] = __uint_as_float(r[c]);
 }
 
 template <int DT>
@@ -121,7 +150,7 @@ MOE_DEV uint32_t pack16(float a, float b) {
 // 32 columns of a row to global memory; n of them exist.  Rows whose pitch is a multiple of 16
 // bytes take 16-byte stores (n is then a multiple of a store's elements).
 template <int DT>
-MOE_DEV void store_row(void* out, int64_t at, const float (&v)[32], int n, bool vec) {
+MOE_DEV void store_row(void* out, int64_t at, const float* v, int n, bool vec) {
     if (DT == MOE_F32) {
         float* o = reinterpret_cast<float*>(out) + at;
         if (vec) {
@@ -150,14 +179,26 @@ MOE_DEV void store_row(void* out, int64_t at, const float (&v)[32], int n, bool 
     }
 }
 
+// SiLU(g) * u.  exp(-g) = 2^t (1 + r ln 2) with t = -g log2(e) rounded and r what the rounding and
+// the constant lost, so that a large |g| costs no accuracy; below g = -88 exp overflows.
+MOE_DEV float silu_up(float g, float u) {
+    const float t = -1.44269502f * g;
+    const float r = fmaf(g, -1.92596299e-8f, fmaf(g, -1.44269502f, -t));
+    float e;
+    asm("ex2.approx.f32 %0, %1;" : "=f"(e) : "f"(t));
+    e = g < -88.f ? INFINITY : fmaf(e, 0.693147181f * r, e);
+    float q;
+    asm("rcp.approx.f32 %0, %1;" : "=f"(q) : "f"(1.f + e));
+    return g * q * u;
+}
+
 template <int MODE, int NT, int STAGES>
-__global__ void __launch_bounds__(kGemmThreads, 1) mx_gemm_kernel(const __grid_constant__ CUtensorMap ta,
-                                                                  const __grid_constant__ CUtensorMap tb,
-                                                                  const GemmParams p) {
+__global__ void __launch_bounds__(Shape<NT>::kThreads, Shape<NT>::kCtas)
+    mx_gemm_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtensorMap tb, const GemmParams p) {
     using S = Shape<NT>;
-    constexpr int kSfBase = 2 * NT;  // TMEM: two accumulators, then each stage's scales
+    constexpr int kSfBase = S::kAcc * NT;  // TMEM: the accumulators, then each stage's scales
     constexpr int kTmemCols = kSfBase + STAGES * S::kSfCols <= 256 ? 256 : 512;
-    static_assert(kSfBase + STAGES * S::kSfCols <= 512, "TMEM");
+    static_assert(kSfBase + STAGES * S::kSfCols <= 512 && kTmemCols * S::kCtas <= 512, "TMEM");
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     __shared__ __align__(8) uint64_t s_full[STAGES], s_empty[STAGES], s_accfull[2], s_accempty[2], s_done;
@@ -172,7 +213,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) mx_gemm_kernel(const __grid_c
         }
         for (int a = 0; a < 2; ++a) {
             mbar_init(&s_accfull[a], 1);
-            mbar_init(&s_accempty[a], 4);
+            mbar_init(&s_accempty[a], S::kEpiWarps);
         }
         mbar_init(&s_done, 1);
         s_failed = 0;
@@ -188,61 +229,64 @@ __global__ void __launch_bounds__(kGemmThreads, 1) mx_gemm_kernel(const __grid_c
     gemm::tc_fence_after();
     const uint32_t tmem = s_tmem;
     volatile int* failed = &s_failed;
-    asm volatile("griddepcontrol.wait;" ::: "memory");
+    // down: the tiles' list was complete before gate_up started (which lets this kernel start
+    // after its own wait), so the weights are fetched before the wait for gate_up's output
+    if (MODE != kDown) asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
     const int mt_count = MODE == kDense ? p.mt_count : p.mtiles[0];
     const int64_t tiles = (int64_t)mt_count * p.nt_count;
     const int nstages = (p.K + kStageK - 1) / kStageK, k64 = (p.K + 63) / 64;
     const int nb128 = (p.N + 127) / 128;
-    uint32_t it = 0;  // stages so far (producer and MMA thread)
 
     if (warp == 0) {
         bool ok = true;
+        uint32_t it = 0, st = 0, parity = 1;  // stages so far; stage and phase of the ring
+        // the A rows of a stage: one copy of 128 rows, or 16-row copies of the rows that exist
+        auto load_a = [&](uint32_t to, int mt, int s, int copies) {
+            uint8_t* base = smem + (size_t)to * S::kStage;
+            if (MODE == kDense) {
+                if (lane == 0) tma_2d(smem_u32(base), &ta, s * 128, mt * kTileM, &s_full[to]);
+            } else if (lane < copies) {
+                tma_2d(smem_u32(base) + lane * 2048, &ta, s * 128, mt * kTileM + lane * 16, &s_full[to]);
+            }
+            if (lane == 0) bulk_g2s(base + S::kA + S::kB, p.sfa + ((int64_t)mt * p.kb + 2 * s) * 512, min(2, p.kb - 2 * s) * 512, &s_full[to]);
+        };
         for (int64_t tile = blockIdx.x; ok && tile < tiles; tile += gridDim.x) {
             const int mt = (int)(tile / p.nt_count), nt = (int)(tile - (int64_t)mt * p.nt_count);
             const int e = MODE == kDense ? 0 : p.mt_expert[mt];
-            const int mrows = MODE == kDense ? kTileM : p.mt_rows[mt];
-            int copies = 1, abytes = S::kA;
-            int4 rows = make_int4(0, 0, 0, 0);
-            if (MODE == kGateUp) {  // 4 rows a copy; rows past the tile's last repeat it
-                copies = (mrows + 3) >> 2;
-                abytes = copies * 512;
-                const int32_t* rt = p.rowtok + (int64_t)mt * kTileM;
-                rows.x = rt[min(4 * lane, mrows - 1)];
-                rows.y = rt[min(4 * lane + 1, mrows - 1)];
-                rows.z = rt[min(4 * lane + 2, mrows - 1)];
-                rows.w = rt[min(4 * lane + 3, mrows - 1)];
-            } else if (MODE == kDown) {  // 16 rows a copy
-                copies = (mrows + 15) >> 4;
-                abytes = copies * 2048;
-            }
-            const uint8_t* sfa = p.sfa + (int64_t)mt * p.kb * 512;
-            const uint8_t* sfb = p.sfb + ((int64_t)e * nb128 + (int64_t)nt * NT / 128) * p.kb * 512;
+            const int copies = MODE == kDense ? 8 : (p.mt_rows[mt] + 15) >> 4;
+            const int sft = min(S::kSfTiles, nb128 - nt * NT / 128);
+            const uint8_t* sfb = p.sfb + ((int64_t)e * nb128 + nt * NT / 128) * p.kb * 512;
+            const bool early = MODE == kDown && it == 0;
+            const int first = early ? min(STAGES, nstages) : 0;
             for (int s = 0; s < nstages; ++s, ++it) {
-                const int st = it % STAGES;
-                if (!wait_or_fail(&s_empty[st], (it / STAGES & 1) ^ 1, failed)) { ok = false; break; }
+                if (!warp_wait(&s_empty[st], parity, failed)) { ok = false; break; }
                 uint8_t* base = smem + (size_t)st * S::kStage;
                 const int sfn = min(2, p.kb - 2 * s) * 512;
                 if (lane == 0) {
-                    mbar_arrive_expect_tx(&s_full[st], abytes + S::kB + sfn * (1 + S::kSfB / 1024));
+                    mbar_arrive_expect_tx(&s_full[st], copies * 2048 + S::kB + sfn * (1 + sft));
                     tma_3d(smem_u32(base + S::kA), &tb, s * 128, nt * NT, e, &s_full[st]);
-                    uint8_t* sf = base + S::kA + S::kB;
-                    bulk_g2s(sf, sfa + (int64_t)s * 1024, sfn, &s_full[st]);
-#pragma unroll
-                    for (int b = 0; b < S::kSfB / 1024; ++b)
-                        bulk_g2s(sf + 1024 + b * 1024, sfb + ((int64_t)b * p.kb + 2 * s) * 512, sfn, &s_full[st]);
-                    if (MODE == kDense) tma_2d(smem_u32(base), &ta, s * 128, mt * kTileM, &s_full[st]);
+                    for (int b = 0; b < sft; ++b)
+                        bulk_g2s(base + S::kA + S::kB + 1024 * (1 + b), sfb + ((int64_t)b * p.kb + 2 * s) * 512, sfn, &s_full[st]);
                 }
                 __syncwarp();
-                if (MODE == kGateUp && lane < copies) tma_gather4(smem_u32(base) + lane * 512, &ta, s * 128, rows, &s_full[st]);
-                if (MODE == kDown && lane < copies)
-                    tma_2d(smem_u32(base) + lane * 2048, &ta, s * 128, mt * kTileM + lane * 16, &s_full[st]);
+                if (s >= first) {
+                    load_a(st, mt, s, copies);
+                } else if (s == first - 1) {
+                    asm volatile("griddepcontrol.wait;" ::: "memory");
+                    for (int a = 0; a < first; ++a) load_a(a, mt, a, copies);
+                }
                 __syncwarp();
+                if (++st == STAGES) {
+                    st = 0;
+                    parity ^= 1;
+                }
             }
         }
+        if (MODE == kDown && it == 0) asm volatile("griddepcontrol.wait;" ::: "memory");
         // leave only when the copies have landed: a later owner of this shared memory must not be hit
-        if (lane == 0 && it > 0) {
+        if (lane == 0) {
             for (uint32_t b = 0; b < STAGES && b < it; ++b) {
                 const uint32_t j = it - 1 - b;
                 bool in = false;
@@ -251,68 +295,84 @@ __global__ void __launch_bounds__(kGemmThreads, 1) mx_gemm_kernel(const __grid_c
             }
         }
     } else if (warp == 1) {
-        if (lane == 0) {
-            constexpr uint32_t idesc = idesc_mxf4(kTileM, NT);
-            uint32_t n = 0;  // tiles so far
-            bool ok = true;
-            for (int64_t tile = blockIdx.x; ok && tile < tiles; tile += gridDim.x, ++n) {
-                const uint32_t acc = n & 1, d = tmem + acc * NT;
-                if (!wait_or_fail(&s_accempty[acc], (n >> 1 & 1) ^ 1, failed)) break;
+        // The whole warp walks the loop, so that addresses and descriptors stay in uniform
+        // registers, and one elected lane issues.
+        constexpr uint32_t idesc = idesc_mxf4(kTileM, NT);
+        const uint32_t utmem = __shfl_sync(0xffffffffu, tmem, 0), usmem = __shfl_sync(0xffffffffu, smem_u32(smem), 0);
+        const bool issue = elect_one();
+        uint32_t n = 0, st = 0, parity = 0;  // tiles so far; stage and phase of the ring
+        bool ok = true;
+        for (int64_t tile = blockIdx.x; ok && tile < tiles; tile += gridDim.x, ++n) {
+            const uint32_t acc = n % S::kAcc, d = utmem + acc * NT;
+            // half a scale tile (NT = 64): its rows' columns are 0-1 or 2-3 of the tile's four
+            const uint32_t half = NT == 64 ? (uint32_t)(tile % p.nt_count & 1) * 2 : 0;
+            if (!warp_wait(&s_accempty[acc], (n / S::kAcc & 1) ^ 1, failed)) break;
+            gemm::tc_fence_after();
+            for (int s = 0; s < nstages; ++s) {
+                if (!warp_wait(&s_full[st], parity, failed)) { ok = false; break; }
                 gemm::tc_fence_after();
-                for (int s = 0; s < nstages; ++s, ++it) {
-                    const int st = it % STAGES;
-                    if (!wait_or_fail(&s_full[st], it / STAGES & 1, failed)) { ok = false; break; }
-                    gemm::tc_fence_after();
-                    const uint32_t sa = smem_u32(smem + (size_t)st * S::kStage), sb = sa + S::kA, sf = sb + S::kB;
-                    const uint32_t tsa = tmem + kSfBase + st * S::kSfCols, tsb = tsa + 8;
-                    const int nkb = min(2, p.kb - 2 * s);
-                    for (int i = 0; i < nkb; ++i) {
-                        cp_scales(tsa + 4 * i, sf_desc(sf + 512 * i));
+                const uint32_t sa = usmem + st * S::kStage, sf = sa + S::kA + S::kB;
+                const uint64_t da = gemm::tc_desc_sw128(sa), db = gemm::tc_desc_sw128(sa + S::kA), ds = sf_desc(sf);
+                const uint32_t tsa = utmem + kSfBase + st * S::kSfCols, tsb = tsa + 8;
+                const int nkb = min(2, p.kb - 2 * s), nk = min(4, k64 - 4 * s);
+                if (issue) {
 #pragma unroll
-                        for (int b = 0; b < S::kSfB / 1024; ++b)
-                            cp_scales(tsb + (S::kSfB / 256) * i + 4 * b, sf_desc(sf + 1024 + 1024 * b + 512 * i));
-                    }
-                    const int nk = min(4, k64 - 4 * s);
-                    for (int j = 0; j < nk; ++j) {
-                        const uint32_t id = (uint32_t)(j & 1) * 2;
-                        mma_mxf4(d, gemm::tc_desc_sw128(sa + 32 * j), gemm::tc_desc_sw128(sb + 32 * j),
-                                 idesc | id << 4 | id << 29, tsa + 4 * (j >> 1), tsb + (S::kSfB / 256) * (j >> 1), s > 0 || j > 0);
-                    }
+                    for (int i = 0; i < 2; ++i)
+                        if (i < nkb) {
+                            cp_scales(tsa + 4 * i, ds + 32 * i);
+#pragma unroll
+                            for (int b = 0; b < S::kSfTiles; ++b)
+                                cp_scales(tsb + 4 * S::kSfTiles * i + 4 * b, ds + 64 + 64 * b + 32 * i);
+                        }
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        if (j < nk)  // 64 elements are 32 bytes inside the swizzle atom
+                            mma_mxf4(d, da + 2 * j, db + 2 * j, idesc | (uint32_t)(j & 1) * 2 << 4 | (uint32_t)(j & 1) * 2 << 29,
+                                     tsa + 4 * (j >> 1), tsb + 4 * S::kSfTiles * (j >> 1) + half, s > 0 || j > 0);
                     gemm::tc_commit(&s_empty[st]);
                 }
-                if (ok) gemm::tc_commit(&s_accfull[acc]);
+                __syncwarp();
+                if (++st == STAGES) {
+                    st = 0;
+                    parity ^= 1;
+                }
             }
-            if (*failed) {  // the MMAs in flight end before the accumulators are given back
-                gemm::tc_commit(&s_done);
-                for (uint32_t w = 0; w < kSpinLimit && !mbar_try_wait(&s_done, 0); ++w) {}
-            }
+            if (ok && issue) gemm::tc_commit(&s_accfull[acc]);
+            __syncwarp();
+        }
+        if (*failed && issue) {  // the MMAs in flight end before the accumulators are given back
+            gemm::tc_commit(&s_done);
+            for (uint32_t w = 0; w < kSpinLimit && !mbar_try_wait(&s_done, 0); ++w) {}
         }
         __syncwarp();
     } else if (warp >= 4) {
-        const int r = (warp & 3) * 32 + lane;
+        const int r = (warp & 3) * 32 + lane, c0 = ((warp - 4) >> 2) * S::kCols;
         uint32_t n = 0;
         for (int64_t tile = blockIdx.x; tile < tiles; tile += gridDim.x, ++n) {
             const int mt = (int)(tile / p.nt_count), nt = (int)(tile - (int64_t)mt * p.nt_count);
-            const uint32_t acc = n & 1;
-            if (!wait_or_fail(&s_accfull[acc], n >> 1 & 1, failed)) break;
-            gemm::tc_fence_after();
-            const uint32_t taddr = tmem + acc * NT + ((uint32_t)((warp & 3) * 32) << 16);
+            const uint32_t acc = n % S::kAcc;
             const int mrows = MODE == kDense ? p.M - mt * kTileM : p.mt_rows[mt];
-            const bool live = r < mrows;
+            if (!warp_wait(&s_accfull[acc], n / S::kAcc & 1, failed)) break;
+            gemm::tc_fence_after();
+            float v[S::kCols];
+            const bool any = (warp & 3) * 32 < mrows;  // rows of this warp's quarter exist
+            if (any) load_columns<S::kCols>(tmem + acc * NT + c0 + ((uint32_t)((warp & 3) * 32) << 16), v);
+            gemm::tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&s_accempty[acc]);
+            if (r >= mrows) continue;
             const int64_t row = (int64_t)mt * kTileM + r;
             if (MODE == kGateUp) {
 #pragma unroll
-                for (int b = 0; b < NT / 64; ++b) {
-                    const int i0 = nt * (NT / 2) + b * 32;
+                for (int b = 0; b < S::kCols / 64; ++b) {
+                    const int i0 = (nt * NT + c0) / 2 + b * 32;
                     if (i0 >= p.I) break;
-                    float g[32], u[32];
-                    gemm::tc_ld32(taddr + 64 * b, g);
-                    gemm::tc_ld32(taddr + 64 * b + 32, u);
+                    float h[32];
                     uint32_t m = 0;
 #pragma unroll
                     for (int j = 0; j < 32; ++j) {
-                        g[j] = silu_mul(g[j], u[j]);
-                        m = max(m, __float_as_uint(g[j]) & 0x7fffffffu);
+                        h[j] = silu_up(v[64 * b + j], v[64 * b + 32 + j]);
+                        m = max(m, __float_as_uint(h[j]) & 0x7fffffffu);
                     }
                     const uint32_t sc = scale_of_amax(m);
                     const float k = inv_scale(sc);
@@ -321,34 +381,25 @@ __global__ void __launch_bounds__(kGemmThreads, 1) mx_gemm_kernel(const __grid_c
                     for (int w = 0; w < 4; ++w) {
                         q[w] = 0;
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) q[w] |= cvt_e2m1x2(g[8 * w + 2 * j] * k, g[8 * w + 2 * j + 1] * k) << (8 * j);
+                        for (int j = 0; j < 4; ++j) q[w] |= cvt_e2m1x2(h[8 * w + 2 * j] * k, h[8 * w + 2 * j + 1] * k) << (8 * j);
                     }
-                    if (live) {
-                        *reinterpret_cast<uint4*>(p.hq + row * (p.I / 2) + i0 / 2) = make_uint4(q[0], q[1], q[2], q[3]);
-                        p.hs[tiled_at(row, i0 >> 5, p.hkb)] = (uint8_t)sc;
-                        // the MMAs take K in steps of 64: the scale behind an odd last block must be a number
-                        if (i0 + 32 == p.I && (p.I & 32)) p.hs[tiled_at(row, (i0 >> 5) + 1, p.hkb)] = 0;
-                    }
+                    *reinterpret_cast<uint4*>(p.hq + row * (p.I / 2) + i0 / 2) = make_uint4(q[0], q[1], q[2], q[3]);
+                    p.hs[tiled_at(row, i0 >> 5, p.hkb)] = (uint8_t)sc;
+                    // the MMAs take K in steps of 64: the scale behind an odd last block must be a number
+                    if (i0 + 32 == p.I && (p.I & 32)) p.hs[tiled_at(row, (i0 >> 5) + 1, p.hkb)] = 0;
                 }
             } else {
                 const int esz = MODE == kDown || p.out_dtype == MOE_F32 ? 4 : 2;
                 const bool vec = (int64_t)p.N * esz % 16 == 0;
 #pragma unroll
-                for (int c = 0; c < NT; c += 32) {
-                    const int n0 = nt * NT + c;
-                    if (n0 >= p.N) break;
-                    float v[32];
-                    gemm::tc_ld32(taddr + c, v);
-                    if (!live) continue;
-                    const int left = min(32, p.N - n0);
-                    if (MODE == kDown || p.out_dtype == MOE_F32) store_row<MOE_F32>(p.out, row * p.N + n0, v, left, vec);
-                    else if (p.out_dtype == MOE_BF16) store_row<MOE_BF16>(p.out, row * p.N + n0, v, left, vec);
-                    else store_row<MOE_F16>(p.out, row * p.N + n0, v, left, vec);
+                for (int c = 0; c < S::kCols; c += 32) {
+                    const int n0 = nt * NT + c0 + c, left = min(32, p.N - n0);
+                    if (left <= 0) break;
+                    if (MODE == kDown || p.out_dtype == MOE_F32) store_row<MOE_F32>(p.out, row * p.N + n0, v + c, left, vec);
+                    else if (p.out_dtype == MOE_BF16) store_row<MOE_BF16>(p.out, row * p.N + n0, v + c, left, vec);
+                    else store_row<MOE_F16>(p.out, row * p.N + n0, v + c, left, vec);
                 }
             }
-            gemm::tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&s_accempty[acc]);
         }
     }
     __syncthreads();
@@ -361,120 +412,151 @@ __global__ void __launch_bounds__(kGemmThreads, 1) mx_gemm_kernel(const __grid_c
     }
 }
 
-// ------------------------------------------------------------------ expert layer: routing
-// Stable order of the routed pairs by expert, in tiles of 128 rows, by one CTA of 32 warps: each
-// warp counts its run of pairs per expert, the counts are summed over the warps and scanned over
-// the experts, and each warp places its run (ranks by __match_any_sync).
-struct RouteParams {
+// ------------------------------------------------------------------ expert layer: tokens
+// Routed pairs in a stable order by expert, each expert's in tiles of 128 rows; the token rows
+// quantised into the rows of their pairs.  A CTA takes a run of `tokens` tokens.  It needs, per
+// expert, the pairs before its run and the pairs in all: for short calls it counts all pairs
+// itself, for long ones the runs' counts come from mx_count_kernel.
+constexpr int kPrepThreads = 256, kPrepWarps = kPrepThreads / 32, kPrepSelf = 1024;
+
+struct PrepParams {
+    const void* x;
     const int32_t* ids;
-    int TK, K, E, e_off, emap_n;
+    int T, K, H, E, e_off, emap_n, tokens;
     const int32_t* emap;
+    const int32_t* counts;  // [runs][E], or null: at most kPrepSelf pairs
     int32_t* mtiles;
     int32_t* mt_expert;
     int32_t* mt_rows;
-    int32_t* rowtok;
     int32_t* ppos;  // row of each pair, -1 for pairs of other engines
+    uint8_t* xq;    // [rows][H / 2]
+    uint8_t* xs;    // scale tiles, kb along H
+    int kb;
 };
 
-__global__ void __launch_bounds__(1024) mx_route_kernel(const RouteParams p) {
-    extern __shared__ int32_t rsm[];  // [32][E] counts | [32] warp sums
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, E = p.E;
-    int32_t* hist = rsm + warp * E;
-    int32_t* sums = rsm + 32 * E;
-    for (int e = lane; e < E; e += 32) hist[e] = 0;
-    __syncwarp();
+// Pairs of each expert in a run of tokens.
+__global__ void __launch_bounds__(kPrepThreads) mx_count_kernel(const PrepParams p, int32_t* counts) {
+    extern __shared__ int32_t csm[];
+    for (int e = threadIdx.x; e < p.E; e += kPrepThreads) csm[e] = 0;
+    __syncthreads();
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    const int run = ((p.TK + 31) / 32 + 31) / 32 * 32;
-    const int i0 = min(p.TK, warp * run), i1 = min(p.TK, i0 + run);
-    for (int i = i0 + lane; i - lane < i1; i += 32) {
-        const int e = i < i1 ? local_expert(p.ids[i], p.e_off, E, p.emap, p.emap_n, i, p.K) : -1;
-        const unsigned peers = __match_any_sync(0xffffffffu, e);
-        if (e >= 0 && (peers & ((1u << lane) - 1u)) == 0) hist[e] += __popc(peers);
-        __syncwarp();
+    const int i0 = blockIdx.x * p.tokens * p.K, i1 = min(p.T * p.K, i0 + p.tokens * p.K);
+    for (int i = i0 + threadIdx.x; i < i1; i += kPrepThreads) {
+        const int e = local_expert(p.ids[i], p.e_off, p.E, p.emap, p.emap_n, i, p.K);
+        if (e >= 0) atomicAdd(&csm[e], 1);
     }
     __syncthreads();
-    int cnt = 0;
-    if (tid < E)
-        for (int w = 0; w < 32; ++w) {
-            const int c = rsm[w * E + tid];
-            rsm[w * E + tid] = cnt;
-            cnt += c;
-        }
-    const int nt = (cnt + kTileM - 1) / kTileM;
-    int incl = nt;
-    for (int o = 1; o < 32; o <<= 1) {
-        const int v = __shfl_up_sync(0xffffffffu, incl, o);
-        if (lane >= o) incl += v;
-    }
-    if (lane == 31) sums[warp] = incl;
+    for (int e = threadIdx.x; e < p.E; e += kPrepThreads) counts[(int64_t)blockIdx.x * p.E + e] = csm[e];
+}
+
+template <int DT>
+__global__ void __launch_bounds__(kPrepThreads) mx_prep_kernel(const PrepParams p) {
+    // [warps][E] pairs of each warp's share, then their first rows | [E] first tile | rows of the run's pairs
+    extern __shared__ int32_t psm[];
+    __shared__ int32_t s_sum[kPrepWarps];
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, E = p.E;
+    int32_t* first = psm + kPrepWarps * E;
+    int32_t* pos = first + E;
+    for (int e = tid; e < kPrepWarps * E; e += kPrepThreads) psm[e] = 0;
     __syncthreads();
-    if (warp == 0) {
-        int v = sums[lane];
-        for (int o = 1; o < 32; o <<= 1) {
-            const int u = __shfl_up_sync(0xffffffffu, v, o);
-            if (lane >= o) v += u;
-        }
-        sums[lane] = v;
-    }
-    __syncthreads();
-    const int first = incl - nt + (warp ? sums[warp - 1] : 0);
-    if (tid < E) {
-        for (int m = 0; m < nt; ++m) {
-            p.mt_expert[first + m] = tid;
-            p.mt_rows[first + m] = min(kTileM, cnt - m * kTileM);
-        }
-        for (int w = 0; w < 32; ++w) rsm[w * E + tid] += first * kTileM;
-    }
-    if (tid == 0) p.mtiles[0] = sums[31];
-    __syncthreads();
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    const int t0 = blockIdx.x * p.tokens, t1 = min(p.T, t0 + p.tokens), TK = p.T * p.K;
+    // the pairs whose order this CTA works out: all (short calls) or its own run's
+    const int a0 = p.counts ? t0 * p.K : 0, a1 = p.counts ? t1 * p.K : TK;
+    const int share = ((a1 - a0 + kPrepWarps - 1) / kPrepWarps + 31) / 32 * 32;
+    const int i0 = min(a1, a0 + warp * share), i1 = min(a1, i0 + share);
+    int32_t* hist = psm + warp * E;
     for (int i = i0 + lane; i - lane < i1; i += 32) {
         const int e = i < i1 ? local_expert(p.ids[i], p.e_off, E, p.emap, p.emap_n, i, p.K) : -1;
         const unsigned peers = __match_any_sync(0xffffffffu, e);
         const int rank = __popc(peers & ((1u << lane) - 1u));
-        const int base = e >= 0 ? hist[e] : 0;
+        const int before = e >= 0 ? hist[e] : 0;
         __syncwarp();
-        if (i < i1) {
-            p.ppos[i] = e >= 0 ? base + rank : -1;
-            if (e >= 0) p.rowtok[base + rank] = i / p.K;
-        }
-        if (e >= 0 && rank == 0) hist[e] = base + __popc(peers);
+        if (i < i1) pos[i - a0] = e >= 0 ? (before + rank) << 10 | e : -1;  // rank within the warp's share
+        if (e >= 0 && rank == 0) hist[e] = before + __popc(peers);
         __syncwarp();
     }
-}
-
-// Token rows -> codes [T][H / 2], and each block's scale to the scale tiles of the rows that hold
-// the token: a CTA per token.
-template <int DT>
-__global__ void __launch_bounds__(256) mx_tokens_kernel(const void* x, int H, int K, const int32_t* ppos, uint8_t* xq,
-                                                        uint8_t* xs, int kb) {
-    __shared__ int32_t s_pos[64];
-    const int64_t t = blockIdx.x;
-    const int tid = threadIdx.x;
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    for (int k = tid; k < K; k += blockDim.x) s_pos[k] = ppos[t * K + k];
     __syncthreads();
-    const int n = H >> 3, nb = H >> 5;
-    for (int i0 = 0; i0 < n; i0 += blockDim.x) {
-        const int i = i0 + tid;
+    // per expert: rows before each warp's share, tiles; scan of the tiles over the experts
+    int carry = 0;
+    for (int e0 = 0; e0 < E; e0 += kPrepThreads) {
+        const int e = e0 + tid;
+        int base = 0, total = 0;
+        if (e < E) {
+            if (p.counts) {
+                const int runs = gridDim.x;
+#pragma unroll 16
+                for (int c = 0; c < runs; ++c) {
+                    const int n = __ldcg(p.counts + (int64_t)c * E + e);
+                    if (c < (int)blockIdx.x) base += n;
+                    total += n;
+                }
+            }
+            int run = base;
+            for (int w = 0; w < kPrepWarps; ++w) {
+                const int n = psm[w * E + e];
+                psm[w * E + e] = run;
+                run += n;
+            }
+            if (!p.counts) total = run;
+        }
+        const int nt = (total + kTileM - 1) / kTileM;
+        int incl = nt;
+        for (int o = 1; o < 32; o <<= 1) {
+            const int v = __shfl_up_sync(0xffffffffu, incl, o);
+            if (lane >= o) incl += v;
+        }
+        if (lane == 31) s_sum[warp] = incl;
+        __syncthreads();
+        int all = 0;
+        for (int w = 0; w < kPrepWarps; ++w) {
+            if (w < warp) incl += s_sum[w];
+            all += s_sum[w];
+        }
+        __syncthreads();
+        const int tile = carry + incl - nt;
+        if (e < E) {
+            first[e] = tile * kTileM;
+            if (blockIdx.x == 0)
+                for (int m = 0; m < nt; ++m) {
+                    p.mt_expert[tile + m] = e;
+                    p.mt_rows[tile + m] = min(kTileM, total - m * kTileM);
+                }
+        }
+        carry += all;
+    }
+    if (blockIdx.x == 0 && tid == 0) p.mtiles[0] = carry;
+    __syncthreads();
+    for (int i = i0 + lane; i < i1; i += 32) {
+        const int v = pos[i - a0], e = v & 1023;
+        pos[i - a0] = v < 0 ? -1 : first[e] + hist[e] + (v >> 10);
+    }
+    __syncthreads();
+    pos += t0 * p.K - a0;  // the run's own pairs
+    for (int i = tid; i < (t1 - t0) * p.K; i += kPrepThreads) p.ppos[t0 * p.K + i] = pos[i];
+    const int n = p.H >> 3, nb = p.H >> 5, n16 = (n + 15) & ~15;  // a scale word's 16 threads stay together
+    const int units = (t1 - t0) * n16;
+    for (int u0 = 0; u0 < units; u0 += kPrepThreads) {
+        const int u = u0 + tid, t = u / n16, i = u - t * n16;
+        const bool in = u < units && i < n;
         float v[8] = {};
-        if (i < n) load8<DT>(x, t * H + i * 8, v);
+        if (in) load8<DT>(p.x, (int64_t)(t0 + t) * p.H + i * 8, v);
         uint32_t sc;
         const uint32_t c = quant8(v, sc);
-        // the four blocks of a scale word lie in 16 neighbouring lanes
         uint32_t w = sc;
         w |= __shfl_down_sync(0xffffffffu, sc, 4, 16) << 8;
         w |= __shfl_down_sync(0xffffffffu, sc, 8, 16) << 16;
         w |= __shfl_down_sync(0xffffffffu, sc, 12, 16) << 24;
-        if (i < n) {
-            reinterpret_cast<uint32_t*>(xq + t * (H / 2))[i] = c;
-            if ((i & 15) == 0) {
-                const int b = i >> 2, left = nb - b;
-                if (left < 4) w &= (1u << (8 * left)) - 1u;
-                for (int k = 0; k < K; ++k)
-                    if (s_pos[k] >= 0) *reinterpret_cast<uint32_t*>(xs + tiled_at(s_pos[k], b, kb)) = w;
-            }
+        if (!in) continue;
+        const int left = nb - (i >> 2);
+        if (left < 4) w &= (1u << (8 * left)) - 1u;
+        for (int k = 0; k < p.K; ++k) {
+            const int row = pos[t * p.K + k];
+            if (row < 0) continue;
+            reinterpret_cast<uint32_t*>(p.xq + (int64_t)row * (p.H / 2))[i] = c;
+            if ((i & 15) == 0) *reinterpret_cast<uint32_t*>(p.xs + tiled_at(row, i >> 2, p.kb)) = w;
         }
     }
 }
