@@ -10,6 +10,7 @@ using namespace moe;
 namespace {
 
 constexpr int kRouteWarps = 4;
+constexpr float kMostFloat = 3.402823466e38f;
 constexpr int kRouteMaxTopk = 32, kRouteMaxGroups = 32, kRouteMaxExperts = 1024;
 
 struct RouteScoredParams {
@@ -36,14 +37,11 @@ MOE_DEV void warp_argmax(double& v, int& i) {
     }
 }
 
-// One warp per token; lane l holds experts l, l + 32, ...  The order of the scores is formed
-// in 64 bits (near ties of 32-bit scores would depend on the rounding of exp), or, without a
-// bias, by the logits themselves, which have the scores' order exactly.
+// A row by the definition in 64 bits; lane l holds experts l, l + 32, ...  For rows whose order
+// 32 bits do not settle, and for group sizes that the kernel below has no lane layout for.
 template <int NPL>
-__global__ void __launch_bounds__(kRouteWarps * 32) route_scored_kernel(const RouteScoredParams p) {
-    const int64_t t = (int64_t)blockIdx.x * kRouteWarps + (threadIdx.x >> 5);
+__device__ __noinline__ void route_row_exact(const RouteScoredParams& p, int64_t t) {
     const int lane = threadIdx.x & 31;
-    if (t >= p.T) return;
     const int E = p.E, per = E / p.groups;
     const int64_t base = t * E;
     float l[NPL];
@@ -54,7 +52,7 @@ __global__ void __launch_bounds__(kRouteWarps * 32) route_scored_kernel(const Ro
         const int e = i * 32 + lane;
         l[i] = e < E ? load_logit(p.logits, base + e, p.dtype) : -INFINITY;
         if (!(l[i] > -INFINITY)) l[i] = -INFINITY;  // NaN: masked
-        l[i] = fminf(l[i], 3.402823466e38f);
+        l[i] = fminf(l[i], kMostFloat);
         top = fmaxf(top, l[i]);
         any |= l[i] > -INFINITY;
     }
@@ -83,7 +81,7 @@ __global__ void __launch_bounds__(kRouteWarps * 32) route_scored_kernel(const Ro
             key[i] = (double)l[i];
             if (p.bias) {
                 const float b = p.bias[e];  // -infinity or NaN: never chosen
-                key[i] = b > -INFINITY ? score_of(l[i]) + (double)fminf(b, 3.402823466e38f) : -INFINITY;
+                key[i] = b > -INFINITY ? score_of(l[i]) + (double)fminf(b, kMostFloat) : -INFINITY;
             }
         }
     }
@@ -137,7 +135,7 @@ __global__ void __launch_bounds__(kRouteWarps * 32) route_scored_kernel(const Ro
             if (i * 32 + lane == bi) key[i] = -INFINITY;
     }
     double s = 0.0;
-    if (mine >= 0) s = score_of(fminf(load_logit(p.logits, base + mine, p.dtype), 3.402823466e38f));
+    if (mine >= 0) s = score_of(fminf(load_logit(p.logits, base + mine, p.dtype), kMostFloat));
     if (p.renorm) {
         double sum = s;
 #pragma unroll
@@ -148,6 +146,260 @@ __global__ void __launch_bounds__(kRouteWarps * 32) route_scored_kernel(const Ro
         p.ids[t * p.K + lane] = mine;
         p.w[t * p.K + lane] = (float)(s * (double)p.scale);
     }
+}
+
+
+// Floats as unsigned integers of the same order; 0 is below all of them.
+MOE_DEV uint32_t ordered(float v) {
+    const uint32_t b = __float_as_uint(v);
+    return b & 0x80000000u ? ~b : b | 0x80000000u;
+}
+MOE_DEV float unordered(uint32_t k) { return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k); }
+
+// Whether approximate choices a >= b are in this order for certain: scores off by less than tol / 2,
+// sums with the bias by 6e-8 of themselves, keys without their lowest bits by `cut` of themselves.
+MOE_DEV bool apart(float a, float b, float tol, float cut) {
+    return a - b > tol + (2.4e-7f + cut) * fmaxf(fabsf(a), fabsf(b));
+}
+
+// Descending order of N (a power of two) keys: Batcher's odd-even merge sort.
+template <int N>
+MOE_DEV void sort_keys(uint32_t (&k)[N]) {
+#pragma unroll
+    for (int p = 1; p < N; p *= 2)
+#pragma unroll
+        for (int q = p; q >= 1; q /= 2)
+#pragma unroll
+            for (int j = q % p; j + q < N; j += 2 * q)
+#pragma unroll
+                for (int i = 0; i < q; ++i)
+                    if (i + j + q < N && (i + j) / (2 * p) == (i + j + q) / (2 * p)) {
+                        const uint32_t a = k[i + j], b = k[i + j + q];
+                        k[i + j] = max(a, b);
+                        k[i + j + q] = min(a, b);
+                    }
+}
+
+// One warp per token, lane l holding the NPL neighbouring experts from l * NPL on (wide loads; the
+// lower lane is the lower index, so that a ballot breaks ties).  An expert's key is its choice as a
+// 32-bit integer of the same order, the lowest log2(NPL) bits replaced by its place in the lane.
+// Each lane sorts its keys once; a round of the top-k is then redux.sync over the lanes' heads, a
+// ballot for the owner, and the owner's step to its next.  Two rounds more than top_k show
+// whether the order is certain: neighbouring choices that the keys do not settle (scores are 32-bit
+// approximations, keys lack their last bits) are compared exactly by two lanes, and what that does not
+// settle (three in a row, groups at the border, a softmax with a bias) goes to route_row_exact.
+// Of 256 sigmoid scores with a bias about two rows in a hundred have such a pair.  Without a bias
+// the logits decide, which have the scores' order; 16-bit ones lose nothing in the keys.
+//
+// Bound: the instructions, about 500 a row (16384 x 256 bf16 logits are 8.9 MB, 1.4 us of traffic).
+template <int NPL>
+__global__ void __launch_bounds__(kRouteWarps * 32) route_scored_kernel(const RouteScoredParams p) {
+    constexpr uint32_t kPlace = NPL - 1;
+    constexpr float kCut = NPL * 1.2e-7f;
+    const int64_t t = (int64_t)blockIdx.x * kRouteWarps + (threadIdx.x >> 5);
+    const int lane = threadIdx.x & 31;
+    if (t >= p.T) return;
+    const int E = p.E, per = E / p.groups, e0 = lane * NPL;
+    const int64_t base = t * E;
+    float l[NPL];
+    const int esz = p.dtype == MOE_F32 ? 4 : 2;
+    const bool wide = NPL >= 4 && E % 4 == 0;
+    if (wide && (reinterpret_cast<uintptr_t>(p.logits) & 15) == 0) {
+#pragma unroll
+        for (int i = 0; i < NPL; i += 4) {
+            float v[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+            if (e0 + i < E) {
+                const uint8_t* q = static_cast<const uint8_t*>(p.logits) + (base + e0 + i) * esz;
+                if (p.dtype == MOE_F32) {
+                    const float4 a = __ldg(reinterpret_cast<const float4*>(q));
+                    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+                } else {
+                    const uint2 a = __ldg(reinterpret_cast<const uint2*>(q));
+                    const uint32_t w[2] = {a.x, a.y};
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) v[j] = scale_to_f32((uint16_t)(w[j / 2] >> (16 * (j & 1))), p.dtype == MOE_BF16);
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j) l[(i + j) % NPL] = v[j];
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < NPL; ++i) l[i] = e0 + i < E ? load_logit(p.logits, base + e0 + i, p.dtype) : -INFINITY;
+    }
+#pragma unroll
+    for (int i = 0; i < NPL; ++i) l[i] = l[i] > -INFINITY ? fminf(l[i], kMostFloat) : -INFINITY;  // NaN: masked
+    const bool sigmoid = p.score == MOE_SCORE_SIGMOID, sums = p.groups > 1 && p.group_top > 1, scored = p.bias || sums;
+    float top = 0.f, den = 1.f;
+    if (!sigmoid) {
+        uint32_t m = 0;
+#pragma unroll
+        for (int i = 0; i < NPL; ++i) m = max(m, l[i] > -INFINITY ? ordered(l[i]) : 0u);
+        m = __reduce_max_sync(0xffffffffu, m);
+        top = m ? unordered(m) : 0.f;
+        if (scored || !p.renorm) {
+            den = 0.f;
+#pragma unroll
+            for (int i = 0; i < NPL; ++i) den += l[i] > -INFINITY ? expf(l[i] - top) : 0.f;
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) den += __shfl_xor_sync(0xffffffffu, den, o);
+        }
+    }
+    // keys of the choices; with `sums` and no bias the scores first, for the groups
+    uint32_t key[NPL];
+    float tol = 0.f;
+    if (scored) {
+        const float r = 1.f / den;
+        float most = 0.f;  // largest score
+        float bias[NPL];
+        if (!p.bias) {
+#pragma unroll
+            for (int i = 0; i < NPL; ++i) bias[i] = 0.f;
+        } else if (wide && (reinterpret_cast<uintptr_t>(p.bias) & 15) == 0) {
+#pragma unroll
+            for (int i = 0; i < NPL; i += 4) {
+                const float4 a = e0 + i < E ? __ldg(reinterpret_cast<const float4*>(p.bias + e0 + i)) : make_float4(0.f, 0.f, 0.f, 0.f);
+                bias[i % NPL] = a.x; bias[(i + 1) % NPL] = a.y; bias[(i + 2) % NPL] = a.z; bias[(i + 3) % NPL] = a.w;
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < NPL; ++i) bias[i] = e0 + i < E ? __ldg(p.bias + e0 + i) : 0.f;
+        }
+#pragma unroll
+        for (int i = 0; i < NPL; ++i) {
+            // exp's argument and result lose 2e-7 of e and |v| 6e-8 of it, the reciprocal 1.2e-7 of s
+            float s, e;
+            asm("ex2.approx.f32 %0, %1;" : "=f"(e) : "f"((sigmoid ? -l[i] : l[i] - top) * 1.44269504f));
+            if (sigmoid) asm("rcp.approx.f32 %0, %1;" : "=f"(s) : "f"(1.f + e));
+            else s = e * r;
+            const bool live = l[i] > -INFINITY && bias[i] > -INFINITY;  // a bias of -infinity or NaN: never chosen
+            most = fmaxf(most, live ? s : 0.f);
+            key[i] = live ? (ordered(fminf(s + fminf(bias[i], kMostFloat), kMostFloat)) & ~kPlace) | (kPlace - i) : 0u;
+        }
+        most = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(most)));
+        tol = (sigmoid ? 1.4e-6f : 2.8e-6f) * most;
+    } else {
+#pragma unroll
+        for (int i = 0; i < NPL; ++i) key[i] = l[i] > -INFINITY ? (ordered(l[i]) & ~kPlace) | (kPlace - i) : 0u;
+    }
+    sort_keys(key);
+    bool settled = true;
+    const bool exact_keys = !p.bias && p.dtype != MOE_F32;  // of the logits
+    if (p.groups > 1) {
+        // a lane's experts are of one group, which is held by 2^n neighbouring lanes
+        const int lanes = per / NPL;
+        uint32_t a = key[0], b = NPL > 1 ? key[NPL > 1] : 0u;  // the group's two largest
+        for (int o = 1; o < lanes; o <<= 1) {
+            const uint32_t oa = __shfl_xor_sync(0xffffffffu, a, o), ob = __shfl_xor_sync(0xffffffffu, b, o);
+            b = max(max(b, ob), min(a, oa));
+            a = max(a, oa);
+        }
+        uint32_t left = 0;
+        if (e0 % per == 0 && e0 < E && a) {
+            left = a & ~kPlace;
+            if (sums && b) left = ordered(unordered(a & ~kPlace) + unordered(b & ~kPlace));
+        }
+        uint32_t keep = 0, last = 0;
+        const uint32_t members = lanes < 32 ? (1u << lanes) - 1u : 0xffffffffu;
+        for (int r = 0; r <= p.topk_groups; ++r) {
+            const uint32_t best = __reduce_max_sync(0xffffffffu, left);
+            if (best == 0) break;
+            if (r == p.topk_groups) {  // the first group that is left out
+                if (scored || !exact_keys) settled = apart(unordered(last), unordered(best), 2.f * tol, 2.f * kCut);
+                break;
+            }
+            last = best;
+            const int owner = __ffs(__ballot_sync(0xffffffffu, left == best)) - 1;
+            if (lane == owner) left = 0;
+            keep |= members << owner;
+        }
+        const bool kept = keep >> lane & 1u;
+        if (sums && !p.bias) {  // the logits decide within the groups
+#pragma unroll
+            for (int i = 0; i < NPL; ++i) key[i] = l[i] > -INFINITY ? (ordered(l[i]) & ~kPlace) | (kPlace - i) : 0u;
+            sort_keys(key);
+        }
+        if (!kept) {
+#pragma unroll
+            for (int i = 0; i < NPL; ++i) key[i] = 0;
+        }
+    }
+    int mine = -1;  // lane k: the k-th choice
+    float before = 0.f;
+    uint32_t near = 0;  // bit k: choices k and k + 1 are not settled
+    const int rounds = p.K + (exact_keys ? 0 : 2);
+    const float order_tol = p.bias ? tol : 0.f;
+    for (int k = 0; k < rounds; ++k) {
+        const uint32_t head = key[0] & ~kPlace, best = __reduce_max_sync(0xffffffffu, head);
+        if (best == 0) break;  // nothing is left: id -1, weight 0
+        const int owner = __ffs(__ballot_sync(0xffffffffu, head == best)) - 1;
+        const int e = owner * NPL + (int)(kPlace - (__shfl_sync(0xffffffffu, key[0], owner) & kPlace));
+        if (!exact_keys) {
+            const float c = unordered(best);
+            if (k > 0 && !apart(before, c, order_tol, kCut)) near |= 1u << (k - 1);
+            before = c;
+        }
+        if (lane == k) mine = e;
+        if (lane == owner) {
+#pragma unroll
+            for (int i = 0; i + 1 < NPL; ++i) key[i] = key[i + 1];
+            key[NPL - 1] = 0;
+        }
+    }
+    float v = mine >= 0 ? fminf(load_logit(p.logits, base + mine, p.dtype), kMostFloat) : 0.f;
+    if (near) {
+        if ((near & near >> 1) || (p.bias && !sigmoid)) {
+            settled = false;
+        } else {
+            double c = (double)v;
+            if (p.bias && mine >= 0) c = 1.0 / (1.0 + exp(-c)) + (double)fminf(p.bias[mine], kMostFloat);
+            const bool first = near >> lane & 1u, second = lane > 0 && (near >> (lane - 1) & 1u);
+            const int other = lane + (first ? 1 : 0) - (second ? 1 : 0);
+            const double oc = __shfl_sync(0xffffffffu, c, other);
+            const int oe = __shfl_sync(0xffffffffu, mine, other);
+            const float ov = __shfl_sync(0xffffffffu, v, other);
+            const bool less = c < oc || (c == oc && mine > oe);
+            if ((first && less) || (second && !less)) {
+                mine = oe;
+                v = ov;
+            }
+        }
+    }
+    if (!settled) {
+        route_row_exact<NPL>(p, t);
+        return;
+    }
+    if (lane >= p.K) mine = -1;
+    float s = 0.f;
+    if (mine >= 0) s = sigmoid ? 1.f / (1.f + expf(-v)) : expf(v - top) / den;
+    if (p.renorm) {
+        float sum = s;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        s = s / (sum + 1e-20f);
+    }
+    if (lane < p.K) {
+        p.ids[t * p.K + lane] = mine;
+        p.w[t * p.K + lane] = s * p.scale;
+    }
+}
+
+// The rows of a call whose groups do not fall on whole lanes, or whose top_k takes every lane.
+template <int NPL>
+__global__ void __launch_bounds__(kRouteWarps * 32) route_scored_exact_kernel(const RouteScoredParams p) {
+    const int64_t t = (int64_t)blockIdx.x * kRouteWarps + (threadIdx.x >> 5);
+    if (t < p.T) route_row_exact<NPL>(p, t);
+}
+
+template <int NPL>
+void route_launch(const RouteScoredParams& p, cudaStream_t st) {
+    const unsigned grid = (unsigned)((p.T + kRouteWarps - 1) / kRouteWarps);
+    const int per = p.E / p.groups, lanes = per / NPL;
+    // the two rounds past top_k need a lane each
+    if (p.K <= 30 && (p.groups == 1 || (per % NPL == 0 && (lanes & (lanes - 1)) == 0)))
+        route_scored_kernel<NPL><<<grid, kRouteWarps * 32, 0, st>>>(p);
+    else
+        route_scored_exact_kernel<NPL><<<grid, kRouteWarps * 32, 0, st>>>(p);
 }
 
 }  // namespace
@@ -173,14 +425,13 @@ extern "C" int moe_route_scored(const void* logits, int32_t dtype, const float* 
     if (!logits || !ids || !w) return fail(MOE_ERR_INVALID, "null pointer");
     RouteScoredParams p{logits, bias, T, (int)E, (int)K, dtype, score, (int)num_groups, (int)topk_groups,
                         group_top, renormalize, scale, ids, w};
-    const unsigned grid = (unsigned)((T + kRouteWarps - 1) / kRouteWarps);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    const int npl = (int)((E + 31) / 32);
-    if (npl <= 2) route_scored_kernel<2><<<grid, kRouteWarps * 32, 0, st>>>(p);
-    else if (npl <= 4) route_scored_kernel<4><<<grid, kRouteWarps * 32, 0, st>>>(p);
-    else if (npl <= 8) route_scored_kernel<8><<<grid, kRouteWarps * 32, 0, st>>>(p);
-    else if (npl <= 16) route_scored_kernel<16><<<grid, kRouteWarps * 32, 0, st>>>(p);
-    else route_scored_kernel<32><<<grid, kRouteWarps * 32, 0, st>>>(p);
+    if (E <= 32) route_launch<1>(p, st);
+    else if (E <= 64) route_launch<2>(p, st);
+    else if (E <= 128) route_launch<4>(p, st);
+    else if (E <= 256) route_launch<8>(p, st);
+    else if (E <= 512) route_launch<16>(p, st);
+    else route_launch<32>(p, st);
     CUDA_TRY(cudaGetLastError());
     return MOE_OK;
 }

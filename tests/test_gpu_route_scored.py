@@ -32,7 +32,7 @@ def check(logits, bias, K, score, groups=1, topk_groups=1, group_top=1, renorm=T
 
 
 @pytest.mark.parametrize("score", ["softmax", "sigmoid"])
-@pytest.mark.parametrize("T,E,K", [(1, 1, 1), (1, 8, 8), (3, 33, 5), (257, 128, 8), (64, 250, 16), (5, 1024, 32), (2, 31, 31)])
+@pytest.mark.parametrize("T,E,K", [(1, 1, 1), (1, 8, 8), (3, 33, 5), (257, 128, 8), (64, 250, 16), (5, 1024, 32), (2, 31, 31), (9, 200, 30), (40, 64, 1)])
 @pytest.mark.parametrize("biased", [False, True])
 def test_plain(T, E, K, score, biased):
     g = torch.Generator("cuda").manual_seed(T + E)
@@ -95,6 +95,30 @@ def test_near_ties(score):
     s = torch.sigmoid(logits[0].double()) if score == "sigmoid" else torch.softmax(logits[0].double(), -1)
     check(logits, (0.6 - s).float(), 8, score)
     check(logits[:1].expand(9, E), (0.6 - s).float(), 8, score, 8, 3, 2)
+
+
+@pytest.mark.parametrize("E,groups", [(128, 1), (256, 8), (512, 4)])
+@pytest.mark.parametrize("biased", [False, True])
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+def test_clusters_of_near_ties(score, biased, E, groups):
+    """Pairs and triples of choices that differ by a few units in the last place, at every rank and at the border
+    of the top-k and of the groups."""
+    g = torch.Generator("cuda").manual_seed(E)
+    logits = torch.randn(64, E, generator=g, device="cuda")
+    for t in range(64):
+        order = torch.randperm(E, generator=g, device="cuda")
+        for r in range(2 + t % 3):
+            a, b, c = order[3 * r], order[3 * r + 1], order[3 * r + 2]
+            logits[t, a] = 2.0 - 0.1 * r
+            logits[t, b] = logits[t, a] * (1 + (t % 5 - 2) * 2.0 ** -23)
+            if t % 2:
+                logits[t, c] = logits[t, a] * (1 - (t % 7 - 3) * 2.0 ** -23)
+    bias = torch.zeros(E, device="cuda") if biased else None
+    if biased:
+        bias += 0.25
+    for K in (1, 4, 8):
+        check(logits, bias, K, score, groups, max(1, groups // 2), 2 if groups > 1 else 1)
+    check(torch.zeros(5, E, device="cuda"), bias, 8, score, groups, max(1, groups // 2), 1)
 
 
 def test_strides_streams_and_graph():
