@@ -193,7 +193,7 @@ MOE_DEV void sort_keys(uint32_t (&k)[N]) {
 //
 // Bound: the instructions, about 500 a row (16384 x 256 bf16 logits are 8.9 MB, 1.4 us of traffic).
 template <int NPL>
-__global__ void __launch_bounds__(kRouteWarps * 32) route_scored_kernel(const RouteScoredParams p) {
+__global__ void __launch_bounds__(kRouteWarps * 32) route_scored_kernel(const __grid_constant__ RouteScoredParams p) {
     constexpr uint32_t kPlace = NPL - 1;
     constexpr float kCut = NPL * 1.2e-7f;
     const int64_t t = (int64_t)blockIdx.x * kRouteWarps + (threadIdx.x >> 5);
@@ -269,8 +269,8 @@ __global__ void __launch_bounds__(kRouteWarps * 32) route_scored_kernel(const Ro
         for (int i = 0; i < NPL; ++i) {
             // exp's argument and result lose 2e-7 of e and |v| 6e-8 of it, the reciprocal 1.2e-7 of s
             float s, e;
-            asm("ex2.approx.f32 %0, %1;" : "=f"(e) : "f"((sigmoid ? -l[i] : l[i] - top) * 1.44269504f));
-            if (sigmoid) asm("rcp.approx.f32 %0, %1;" : "=f"(s) : "f"(1.f + e));
+            asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"((sigmoid ? -l[i] : l[i] - top) * 1.44269504f));
+            if (sigmoid) asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(s) : "f"(1.f + e));
             else s = e * r;
             const bool live = l[i] > -INFINITY && bias[i] > -INFINITY;  // a bias of -infinity or NaN: never chosen
             most = fmaxf(most, live ? s : 0.f);
@@ -324,27 +324,29 @@ __global__ void __launch_bounds__(kRouteWarps * 32) route_scored_kernel(const Ro
             for (int i = 0; i < NPL; ++i) key[i] = 0;
         }
     }
-    int mine = -1;  // lane k: the k-th choice
-    float before = 0.f;
-    uint32_t near = 0;  // bit k: choices k and k + 1 are not settled
+    int owner_of = 0, count = 0;  // lane k: owner and key of the k-th choice
+    uint32_t key_of = 0;
     const int rounds = p.K + (exact_keys ? 0 : 2);
-    const float order_tol = p.bias ? tol : 0.f;
-    for (int k = 0; k < rounds; ++k) {
+    for (; count < rounds; ++count) {
         const uint32_t head = key[0] & ~kPlace, best = __reduce_max_sync(0xffffffffu, head);
         if (best == 0) break;  // nothing is left: id -1, weight 0
         const int owner = __ffs(__ballot_sync(0xffffffffu, head == best)) - 1;
-        const int e = owner * NPL + (int)(kPlace - (__shfl_sync(0xffffffffu, key[0], owner) & kPlace));
-        if (!exact_keys) {
-            const float c = unordered(best);
-            if (k > 0 && !apart(before, c, order_tol, kCut)) near |= 1u << (k - 1);
-            before = c;
+        const uint32_t k = __shfl_sync(0xffffffffu, key[0], owner);
+        if (lane == count) {
+            owner_of = owner;
+            key_of = k;
         }
-        if (lane == k) mine = e;
         if (lane == owner) {
 #pragma unroll
             for (int i = 0; i + 1 < NPL; ++i) key[i] = key[i + 1];
             key[NPL - 1] = 0;
         }
+    }
+    int mine = lane < count ? owner_of * NPL + (int)(kPlace - (key_of & kPlace)) : -1;
+    uint32_t near = 0;  // bit k: choices k and k + 1 are not settled
+    if (!exact_keys) {
+        const float c = unordered(key_of & ~kPlace), next = __shfl_down_sync(0xffffffffu, c, 1);
+        near = __ballot_sync(0xffffffffu, lane + 1 < count && !apart(c, next, p.bias ? tol : 0.f, kCut));
     }
     float v = mine >= 0 ? fminf(load_logit(p.logits, base + mine, p.dtype), kMostFloat) : 0.f;
     if (near) {
@@ -386,7 +388,7 @@ __global__ void __launch_bounds__(kRouteWarps * 32) route_scored_kernel(const Ro
 
 // The rows of a call whose groups do not fall on whole lanes, or whose top_k takes every lane.
 template <int NPL>
-__global__ void __launch_bounds__(kRouteWarps * 32) route_scored_exact_kernel(const RouteScoredParams p) {
+__global__ void __launch_bounds__(kRouteWarps * 32) route_scored_exact_kernel(const __grid_constant__ RouteScoredParams p) {
     const int64_t t = (int64_t)blockIdx.x * kRouteWarps + (threadIdx.x >> 5);
     if (t < p.T) route_row_exact<NPL>(p, t);
 }
