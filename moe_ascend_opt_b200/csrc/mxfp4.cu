@@ -35,19 +35,30 @@ int encoder(EncodeFn* out) {
     return MOE_OK;
 }
 
-// Codes as bytes [planes][rows][pitch], boxes of 128 bytes x box_rows, 128-byte swizzle; what
-// lies outside reads as zero.  planes 0: a 2-D map.
-int encode(CUtensorMap* m, const void* base, int64_t pitch, int64_t rows, int64_t planes, int box_rows) {
+int encode_map(CUtensorMap* m, CUtensorMapDataType type, CUtensorMapSwizzle swizzle, const void* base, int64_t esz, int64_t cols,
+               int64_t rows, int64_t planes, int box_cols, int box_rows) {
     EncodeFn fn;
     if (int rc = encoder(&fn)) return rc;
-    const cuuint64_t dims[3] = {(cuuint64_t)pitch, (cuuint64_t)rows, (cuuint64_t)planes};
-    const cuuint64_t strides[2] = {(cuuint64_t)pitch, (cuuint64_t)(pitch * rows)};
-    const cuuint32_t box[3] = {128, (cuuint32_t)box_rows, 1}, ones[3] = {1, 1, 1};
-    const CUresult r = fn(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, planes ? 3 : 2, const_cast<void*>(base), dims, strides, box, ones,
-                          CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+    const cuuint64_t dims[3] = {(cuuint64_t)cols, (cuuint64_t)rows, (cuuint64_t)planes};
+    const cuuint64_t strides[2] = {(cuuint64_t)(cols * esz), (cuuint64_t)(cols * esz * rows)};
+    const cuuint32_t box[3] = {(cuuint32_t)box_cols, (cuuint32_t)box_rows, 1}, ones[3] = {1, 1, 1};
+    const CUresult r = fn(m, type, planes ? 3 : 2, const_cast<void*>(base), dims, strides, box, ones,
+                          CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                           CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS) return fail(MOE_ERR_CUDA, "cuTensorMapEncodeTiled failed with " + std::to_string((int)r));
     return MOE_OK;
+}
+
+// Codes as bytes [planes][rows][pitch], boxes of 128 bytes x box_rows, 128-byte swizzle; what
+// lies outside reads as zero.  planes 0: a 2-D map.
+int encode(CUtensorMap* m, const void* base, int64_t pitch, int64_t rows, int64_t planes, int box_rows) {
+    return encode_map(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, CU_TENSOR_MAP_SWIZZLE_128B, base, 1, pitch, rows, planes, 128, box_rows);
+}
+
+// An output [rows][cols] of 2- or 4-byte elements, stored in boxes of 32 rows x 64 bytes.
+int encode_out(CUtensorMap* m, void* base, int64_t esz, int64_t cols, int64_t rows) {
+    return encode_map(m, esz == 4 ? CU_TENSOR_MAP_DATA_TYPE_UINT32 : CU_TENSOR_MAP_DATA_TYPE_UINT16, CU_TENSOR_MAP_SWIZZLE_64B, base,
+                      esz, cols, rows, 0, (int)(64 / esz), 32);
 }
 
 // ------------------------------------------------------------------ launches
@@ -96,21 +107,21 @@ int sm_count(int dev, int* out) {
 constexpr int kWide = 256, kWideStages = 4, kNarrow = 64, kNarrowStages = 4;
 
 template <int MODE, int NT, int STAGES>
-int launch_gemm_nt(const CUtensorMap& ta, const CUtensorMap& tb, mx::GemmParams& p, int64_t m_tiles, int sms, bool pdl,
+int launch_gemm_nt(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& to, mx::GemmParams& p, int64_t m_tiles, int sms, bool pdl,
                    cudaStream_t st) {
     using S = mx::Shape<NT>;
     auto fn = mx::mx_gemm_kernel<MODE, NT, STAGES>;
-    const int smem = STAGES * S::kStage + 1024;
+    const int smem = STAGES * S::kStage + S::kStaging + 1024;
     if (int rc = allow_smem(reinterpret_cast<const void*>(fn), smem)) return rc;
     p.nt_count = (int)ceil_div(p.N, NT);
-    return launch(fn, (unsigned)std::min<int64_t>(m_tiles * p.nt_count, sms * S::kCtas), S::kThreads, smem, pdl, st, ta, tb, p);
+    return launch(fn, (unsigned)std::min<int64_t>(m_tiles * p.nt_count, sms * S::kCtas), S::kThreads, smem, pdl, st, ta, tb, to, p);
 }
 
 template <int MODE>
-int launch_gemm(const CUtensorMap& ta, const CUtensorMap& tb, mx::GemmParams& p, int64_t m_tiles, int sms, bool wide, bool pdl,
-                cudaStream_t st) {
-    return wide ? launch_gemm_nt<MODE, kWide, kWideStages>(ta, tb, p, m_tiles, sms, pdl, st)
-                : launch_gemm_nt<MODE, kNarrow, kNarrowStages>(ta, tb, p, m_tiles, sms, pdl, st);
+int launch_gemm(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& to, mx::GemmParams& p, int64_t m_tiles, int sms,
+                bool wide, bool pdl, cudaStream_t st) {
+    return wide ? launch_gemm_nt<MODE, kWide, kWideStages>(ta, tb, to, p, m_tiles, sms, pdl, st)
+                : launch_gemm_nt<MODE, kNarrow, kNarrowStages>(ta, tb, to, p, m_tiles, sms, pdl, st);
 }
 
 bool dtype_ok(int32_t t) { return t == MOE_F16 || t == MOE_BF16 || t == MOE_F32; }
@@ -244,7 +255,12 @@ extern "C" int moe_mxfp4_matmul(const uint8_t* a, const uint8_t* a_scales, const
     p.sfb = b_scales;
     p.out = y;
     p.out_dtype = out_dtype;
-    return launch_gemm<mx::kDense>(ta, tb, p, p.mt_count, sms, wide, false, st);
+    CUtensorMap to = ta;  // unused unless tma_out
+    const int64_t esz = out_dtype == MOE_F32 ? 4 : 2;
+    p.tma_out = wide && N * esz % 16 == 0;
+    if (p.tma_out)
+        if (int rc = encode_out(&to, y, esz, N, M)) return rc;
+    return launch_gemm<mx::kDense>(ta, tb, to, p, p.mt_count, sms, wide, false, st);
 }
 
 // ------------------------------------------------------------------ expert layer
@@ -317,7 +333,7 @@ __global__ void mx_store_rows_kernel(const void* w, int64_t n, int cols, int hal
 struct Workspace {
     int32_t *mtiles, *mt_expert, *mt_rows, *ppos, *counts;
     uint8_t *xq, *xs, *hq, *hs;
-    float* part;
+    uint8_t *part, *pexp;  // fp32 [rows][H], or 16-bit integers and exponents [rows][H / 32]
     int64_t mt;  // bound of the number of m tiles
     size_t bytes;
 };
@@ -350,7 +366,8 @@ Workspace carve(const MxLayer* l, int64_t T, int64_t K, uint8_t* base) {
     w.xs = take(w.mt * l->kb1 * 512);
     w.hq = take(rows * (I / 2));
     w.hs = take(w.mt * l->kb2 * 512);
-    w.part = reinterpret_cast<float*>(take((size_t)rows * H * 4));
+    w.part = take((size_t)rows * H * 4);
+    w.pexp = take((size_t)rows * (H / 32));
     w.bytes = off;
     return w;
 }
@@ -380,11 +397,11 @@ int grow(MxLayer* l, size_t bytes) {
     return MOE_OK;
 }
 
-template <int DT>
+template <int DT, bool PART16>
 int combine_launch(const MxLayer* l, const MxForward& f, const float* tw, void* y, const Workspace& w, int64_t T, cudaStream_t st) {
     const int H = (int)l->cfg.hidden_size;
-    return launch(mx::mx_combine_kernel<DT>, (unsigned)std::min<int64_t>(ceil_div(T * (H / 4), 256), l->sms * 16), 256, 0, f.pdl, st,
-                  (const float*)w.part, (const int32_t*)w.ppos, tw, (int)T, (int)f.K, H, y);
+    return launch(mx::mx_combine_kernel<DT, PART16>, (unsigned)std::min<int64_t>(ceil_div(T * (H / 8), 256), l->sms * 16), 256, 0,
+                  f.pdl, st, (const void*)w.part, (const uint8_t*)w.pexp, (const int32_t*)w.ppos, tw, (int)T, (int)f.K, H, y);
 }
 
 int forward_slice(MxLayer* l, const MxForward& f, const void* x, void* y, const int32_t* ids, const float* tw, int64_t T,
@@ -419,14 +436,20 @@ int forward_slice(MxLayer* l, const MxForward& f, const void* x, void* y, const 
     mx::GemmParams g1 = p;
     g1.N = (int)(2 * I); g1.K = (int)H; g1.kb = (int)l->kb1;
     g1.sfa = w.xs; g1.sfb = l->s1; g1.hq = w.hq; g1.hs = w.hs; g1.hkb = (int)l->kb2;
-    if (int rc = launch_gemm<mx::kGateUp>(tx, l->t1[wide], g1, w.mt, l->sms, wide, f.pdl, st)) return rc;
+    if (int rc = launch_gemm<mx::kGateUp>(tx, l->t1[wide], tx, g1, w.mt, l->sms, wide, f.pdl, st)) return rc;
     mx::GemmParams g2 = p;
     g2.N = (int)H; g2.K = (int)I; g2.kb = (int)l->kb2;
-    g2.sfa = w.hs; g2.sfb = l->s2; g2.out = w.part;
-    if (int rc = launch_gemm<mx::kDown>(th, l->t2[wide], g2, w.mt, l->sms, wide, f.pdl, st)) return rc;
-    return f.out_dtype == MOE_F32    ? combine_launch<MOE_F32>(l, f, tw, y, w, T, st)
-           : f.out_dtype == MOE_BF16 ? combine_launch<MOE_BF16>(l, f, tw, y, w, T, st)
-                                     : combine_launch<MOE_F16>(l, f, tw, y, w, T, st);
+    g2.sfa = w.hs; g2.sfb = l->s2; g2.out = w.part; g2.pexp = w.pexp;
+    const bool part16 = wide && f.out_dtype != MOE_F32;
+    g2.out_dtype = part16 ? MOE_F16 : MOE_F32;
+    CUtensorMap tp = th;  // unused by narrow tiles
+    if (wide)
+        if (int rc = encode_out(&tp, w.part, part16 ? 2 : 4, H, w.mt * mx::kTileM)) return rc;
+    if (int rc = launch_gemm<mx::kDown>(th, l->t2[wide], tp, g2, w.mt, l->sms, wide, f.pdl, st)) return rc;
+    if (f.out_dtype == MOE_F32) return combine_launch<MOE_F32, false>(l, f, tw, y, w, T, st);
+    if (f.out_dtype == MOE_BF16)
+        return part16 ? combine_launch<MOE_BF16, true>(l, f, tw, y, w, T, st) : combine_launch<MOE_BF16, false>(l, f, tw, y, w, T, st);
+    return part16 ? combine_launch<MOE_F16, true>(l, f, tw, y, w, T, st) : combine_launch<MOE_F16, false>(l, f, tw, y, w, T, st);
 }
 
 }  // namespace

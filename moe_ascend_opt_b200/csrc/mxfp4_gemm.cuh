@@ -35,8 +35,10 @@ struct GemmParams {
     const int32_t* mtiles;     // experts: number of m tiles, then expert and rows of each
     const int32_t* mt_expert;
     const int32_t* mt_rows;
-    void* out;           // dense [M][N] (out_dtype); down fp32 [m tiles * 128][N]
+    void* out;           // dense [M][N] (out_dtype); down [m tiles * 128][N], fp32 or 16-bit parts
     int out_dtype;
+    int tma_out;         // dense, wide tiles: store through the map (rows of a multiple of 16 bytes)
+    uint8_t* pexp;       // down, 16-bit parts: exponent of each 32 columns [m tiles * 128][ceil(N / 32)]
     int I;               // gate_up: hq [m tiles * 128][I / 2], hs tiled with hkb tiles along I
     int hkb;
     uint8_t* hq;
@@ -55,6 +57,8 @@ struct Shape {
     static constexpr int kCols = NT / (kEpiWarps / 4);  // columns of an epilogue thread
     static constexpr int kThreads = 128 + 32 * kEpiWarps;
     static constexpr int kCtas = NT <= 64 ? 2 : 1;      // per SM
+    // wide tiles leave through shared memory: 32 rows x 64 bytes per epilogue warp, stored by TMA
+    static constexpr int kStaging = NT >= 256 ? kEpiWarps * 2048 : 0;
 };
 
 // Descriptor of a 512-byte scale tile for tcgen05.cp: no swizzle, 8-row groups of 128 bytes.
@@ -94,6 +98,12 @@ MOE_DEV void tma_2d(uint32_t dst, const CUtensorMap* m, int x, int y, uint64_t* 
         "cp.async.bulk.tensor.2d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
         "l"(m), "r"(x), "r"(y), "r"(smem_u32(bar))
         : "memory");
+}
+// 32 rows x 64 bytes of shared memory (64-byte swizzle) to global memory; what lies outside the map is dropped.
+MOE_DEV void tma_store_2d(const CUtensorMap* m, uint32_t src, int x, int y) {
+    asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%1, %2}], [%3];" ::"l"(m), "r"(x), "r"(y), "r"(src)
+                 : "memory");
+    asm volatile("cp.async.bulk.commit_group;" ::: "memory");
 }
 MOE_DEV void tma_3d(uint32_t dst, const CUtensorMap* m, int x, int y, int z, uint64_t* bar) {
     asm volatile(
@@ -179,6 +189,24 @@ MOE_DEV void store_row(void* out, int64_t at, const float* v, int n, bool vec) {
     }
 }
 
+// A down row leaves wide tiles as 16-bit integers with one exponent per 32 columns: v = m 2^(e - 141),
+// e the exponent byte of the block's largest magnitude, so m is off by half a step of 2^-15 of that
+// power of two.  A sum of a token's parts so loses 2^-16 of the largest magnitude near each element where a
+// 16-bit output rounds to 2^-9 or 2^-12 of the element, and the parts' traffic is half of fp32's (which an
+// fp32 output keeps).  e = 255: the block held an infinity or a NaN, and is NaN.
+MOE_DEV uint32_t part_exponent(const float* v) {
+    uint32_t m = 0;
+#pragma unroll
+    for (int j = 0; j < 32; ++j) m = max(m, __float_as_uint(v[j]) & 0x7fffffffu);
+    return m >> 23;
+}
+// 2^(141 - e) as a product of two normal factors: e from 0 (subnormal block) to 254
+MOE_DEV int part_round(float v, float k) { return __float2int_rn(fminf(fmaxf(v * k, -32767.f), 32767.f)); }
+MOE_DEV float part_scale(uint32_t e) { return __uint_as_float(min(268u - max(e, 15u), 253u) << 23); }
+MOE_DEV float part_unscale(uint32_t e) {
+    return e == 255u ? __uint_as_float(0x7fc00000u) : __uint_as_float((max(e, 15u) - 14u) << 23);
+}
+
 // SiLU(g) * u.  exp(-g) = 2^t (1 + r ln 2) with t = -g log2(e) rounded and r what the rounding and
 // the constant lost, so that a large |g| costs no accuracy; below g = -88 exp overflows.
 MOE_DEV float silu_up(float g, float u) {
@@ -194,7 +222,8 @@ MOE_DEV float silu_up(float g, float u) {
 
 template <int MODE, int NT, int STAGES>
 __global__ void __launch_bounds__(Shape<NT>::kThreads, Shape<NT>::kCtas)
-    mx_gemm_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtensorMap tb, const GemmParams p) {
+    mx_gemm_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtensorMap tb,
+                   const __grid_constant__ CUtensorMap to, const GemmParams p) {
     using S = Shape<NT>;
     constexpr int kSfBase = S::kAcc * NT;  // TMEM: the accumulators, then each stage's scales
     constexpr int kTmemCols = kSfBase + STAGES * S::kSfCols <= 256 ? 256 : 512;
@@ -347,6 +376,18 @@ __global__ void __launch_bounds__(Shape<NT>::kThreads, Shape<NT>::kCtas)
         __syncwarp();
     } else if (warp >= 4) {
         const int r = (warp & 3) * 32 + lane, c0 = ((warp - 4) >> 2) * S::kCols;
+        uint8_t* const staging = smem + STAGES * S::kStage + (warp - 4) * 2048;
+        // this lane's 64 bytes of the staging area, its four 16-byte pieces swizzled as the map says
+        auto stage_row = [&](const uint32_t (&w)[16]) {
+            asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");  // the last store has read the area (lane 0's)
+            __syncwarp();
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                *reinterpret_cast<uint4*>(staging + lane * 64 + ((j ^ (lane >> 1 & 3)) << 4)) =
+                    make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+        };
         uint32_t n = 0;
         for (int64_t tile = blockIdx.x; tile < tiles; tile += gridDim.x, ++n) {
             const int mt = (int)(tile / p.nt_count), nt = (int)(tile - (int64_t)mt * p.nt_count);
@@ -360,8 +401,44 @@ __global__ void __launch_bounds__(Shape<NT>::kThreads, Shape<NT>::kCtas)
             gemm::tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(&s_accempty[acc]);
-            if (r >= mrows) continue;
             const int64_t row = (int64_t)mt * kTileM + r;
+            const int y0 = mt * kTileM + (warp & 3) * 32;
+            if (S::kStaging && MODE != kGateUp && any && (MODE == kDown || p.tma_out)) {
+#pragma unroll
+                for (int c = 0; c < S::kCols; c += 32) {
+                    const int n0 = nt * NT + c0 + c;
+                    if (n0 >= p.N) break;
+                    uint32_t w[16];
+                    if (p.out_dtype == MOE_F32) {
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            if (n0 + 16 * h >= p.N) break;
+#pragma unroll
+                            for (int j = 0; j < 16; ++j) w[j] = __float_as_uint(v[c + 16 * h + j]);
+                            stage_row(w);
+                            if (lane == 0) tma_store_2d(&to, smem_u32(staging), n0 + 16 * h, y0);
+                        }
+                        continue;
+                    }
+                    if (MODE == kDown) {
+                        const uint32_t e = part_exponent(v + c);
+                        const float k = part_scale(e);
+#pragma unroll
+                        for (int j = 0; j < 16; ++j)
+                            w[j] = (uint32_t)part_round(v[c + 2 * j], k) & 0xffffu | (uint32_t)part_round(v[c + 2 * j + 1], k) << 16;
+                        if (r < mrows) p.pexp[row * ((p.N + 31) >> 5) + (n0 >> 5)] = (uint8_t)e;
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < 16; ++j)
+                            w[j] = p.out_dtype == MOE_BF16 ? pack16<MOE_BF16>(v[c + 2 * j], v[c + 2 * j + 1])
+                                                           : pack16<MOE_F16>(v[c + 2 * j], v[c + 2 * j + 1]);
+                    }
+                    stage_row(w);
+                    if (lane == 0) tma_store_2d(&to, smem_u32(staging), n0, y0);
+                }
+                continue;
+            }
+            if (r >= mrows) continue;
             if (MODE == kGateUp) {
 #pragma unroll
                 for (int b = 0; b < S::kCols / 64; ++b) {
@@ -402,6 +479,7 @@ __global__ void __launch_bounds__(Shape<NT>::kThreads, Shape<NT>::kCtas)
             }
         }
     }
+    if (S::kStaging && warp >= 4 && lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
     __syncthreads();
     if (s_failed && tid == 0) set_err(p.err, kErrFullWait);
     gemm::tc_fence_before();
@@ -417,7 +495,7 @@ __global__ void __launch_bounds__(Shape<NT>::kThreads, Shape<NT>::kCtas)
 // quantised into the rows of their pairs.  A CTA takes a run of `tokens` tokens.  It needs, per
 // expert, the pairs before its run and the pairs in all: for short calls it counts all pairs
 // itself, for long ones the runs' counts come from mx_count_kernel.
-constexpr int kPrepThreads = 256, kPrepWarps = kPrepThreads / 32, kPrepSelf = 1024;
+constexpr int kPrepThreads = 512, kPrepWarps = kPrepThreads / 32, kPrepSelf = 4096;
 
 struct PrepParams {
     const void* x;
@@ -538,52 +616,95 @@ __global__ void __launch_bounds__(kPrepThreads) mx_prep_kernel(const PrepParams 
     for (int i = tid; i < (t1 - t0) * p.K; i += kPrepThreads) p.ppos[t0 * p.K + i] = pos[i];
     const int n = p.H >> 3, nb = p.H >> 5, n16 = (n + 15) & ~15;  // a scale word's 16 threads stay together
     const int units = (t1 - t0) * n16;
-    for (int u0 = 0; u0 < units; u0 += kPrepThreads) {
-        const int u = u0 + tid, t = u / n16, i = u - t * n16;
-        const bool in = u < units && i < n;
-        float v[8] = {};
-        if (in) load8<DT>(p.x, (int64_t)(t0 + t) * p.H + i * 8, v);
-        uint32_t sc;
-        const uint32_t c = quant8(v, sc);
-        uint32_t w = sc;
-        w |= __shfl_down_sync(0xffffffffu, sc, 4, 16) << 8;
-        w |= __shfl_down_sync(0xffffffffu, sc, 8, 16) << 16;
-        w |= __shfl_down_sync(0xffffffffu, sc, 12, 16) << 24;
-        if (!in) continue;
-        const int left = nb - (i >> 2);
-        if (left < 4) w &= (1u << (8 * left)) - 1u;
-        for (int k = 0; k < p.K; ++k) {
-            const int row = pos[t * p.K + k];
-            if (row < 0) continue;
-            reinterpret_cast<uint32_t*>(p.xq + (int64_t)row * (p.H / 2))[i] = c;
-            if ((i & 15) == 0) *reinterpret_cast<uint32_t*>(p.xs + tiled_at(row, i >> 2, p.kb)) = w;
+    constexpr int kFly = 4;  // loads in flight of a thread
+    for (int u0 = 0; u0 < units; u0 += kFly * kPrepThreads) {
+        float v[kFly][8];
+        int t[kFly], i[kFly];
+#pragma unroll
+        for (int f = 0; f < kFly; ++f) {
+            const int u = u0 + f * kPrepThreads + tid;
+            t[f] = u / n16;
+            i[f] = u < units ? u - t[f] * n16 : n;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[f][j] = 0.f;
+            if (i[f] < n) load8<DT>(p.x, (int64_t)(t0 + t[f]) * p.H + i[f] * 8, v[f]);
+        }
+#pragma unroll
+        for (int f = 0; f < kFly; ++f) {
+            uint32_t sc;
+            const uint32_t c = quant8(v[f], sc);
+            uint32_t w = sc;
+            w |= __shfl_down_sync(0xffffffffu, sc, 4, 16) << 8;
+            w |= __shfl_down_sync(0xffffffffu, sc, 8, 16) << 16;
+            w |= __shfl_down_sync(0xffffffffu, sc, 12, 16) << 24;
+            if (i[f] >= n) continue;
+            const int left = nb - (i[f] >> 2);
+            if (left < 4) w &= (1u << (8 * left)) - 1u;
+            const bool word = (i[f] & 15) == 0;
+#pragma unroll 8
+            for (int k = 0; k < p.K; ++k) {
+                const int row = pos[t[f] * p.K + k];
+                if (row >= 0) {
+                    reinterpret_cast<uint32_t*>(p.xq + (int64_t)row * (p.H / 2))[i[f]] = c;
+                    if (word) *reinterpret_cast<uint32_t*>(p.xs + tiled_at(row, i[f] >> 2, p.kb)) = w;
+                }
+            }
         }
     }
 }
 
-// y[t] = sum over the token's pairs, in their order, of w * part[row]
-template <int DT>
-__global__ void __launch_bounds__(256) mx_combine_kernel(const float* part, const int32_t* ppos, const float* tw, int T, int K,
-                                                         int H, void* y) {
+// y[t] = sum over the token's pairs, in their order, of w * part[row]: a thread takes 8 columns and
+// fetches up to 8 parts at a time.
+template <int DT, bool PART16>
+__global__ void __launch_bounds__(256) mx_combine_kernel(const void* part, const uint8_t* pexp, const int32_t* ppos,
+                                                         const float* tw, int T, int K, int H, void* y) {
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    const int64_t total = (int64_t)T * (H / 4);
+    constexpr int kFly = 8;
+    const int h8 = H >> 3, nb = H >> 5;
+    const int64_t total = (int64_t)T * h8;
     for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < total; i += (int64_t)gridDim.x * blockDim.x) {
-        const int64_t t = i / (H / 4);
-        const int n = (int)(i - t * (H / 4)) * 4;
-        float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (int k = 0; k < K; ++k) {
-            const int pos = __ldg(ppos + t * K + k);
-            if (pos < 0) continue;
-            const float w = __ldg(tw + t * K + k);
-            const float4 v = __ldcg(reinterpret_cast<const float4*>(part + (int64_t)pos * H + n));
-            a.x = fmaf(w, v.x, a.x);
-            a.y = fmaf(w, v.y, a.y);
-            a.z = fmaf(w, v.z, a.z);
-            a.w = fmaf(w, v.w, a.w);
+        const int64_t t = i / h8;
+        const int n = (int)(i - t * h8) * 8;
+        float a[8] = {};
+        for (int k0 = 0; k0 < K; k0 += kFly) {
+            uint4 q[kFly][PART16 ? 1 : 2];
+            float w[kFly];
+#pragma unroll
+            for (int f = 0; f < kFly; ++f) {
+                const int pos = k0 + f < K ? __ldg(ppos + t * K + k0 + f) : -1;
+                w[f] = 0.f;
+                q[f][0] = make_uint4(0u, 0u, 0u, 0u);
+                if (!PART16) q[f][PART16 ? 0 : 1] = q[f][0];
+                if (pos < 0) continue;
+                w[f] = __ldg(tw + t * K + k0 + f);
+                if (PART16) {
+                    q[f][0] = __ldcg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(part) + (int64_t)pos * H + n));
+                    w[f] *= part_unscale(__ldcg(pexp + (int64_t)pos * nb + (n >> 5)));
+                } else {
+                    const uint4* src = reinterpret_cast<const uint4*>(static_cast<const float*>(part) + (int64_t)pos * H + n);
+                    q[f][0] = __ldcg(src);
+                    q[f][PART16 ? 0 : 1] = __ldcg(src + 1);
+                }
+            }
+#pragma unroll
+            for (int f = 0; f < kFly; ++f) {
+                const uint32_t* r = reinterpret_cast<const uint32_t*>(&q[f][0]);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const float v = PART16 ? (float)(int16_t)(r[j / 2] >> (16 * (j & 1))) : __uint_as_float(r[j % (PART16 ? 4 : 8)]);
+                    a[j] = fmaf(w[f], v, a[j]);
+                }
+            }
         }
-        if (DT == MOE_F32) reinterpret_cast<float4*>(y)[i] = a;
-        else reinterpret_cast<uint2*>(y)[i] = make_uint2(pack16<DT>(a.x, a.y), pack16<DT>(a.z, a.w));
+        if (DT == MOE_F32) {
+            float4* d = reinterpret_cast<float4*>(y) + 2 * i;
+            d[0] = make_float4(a[0], a[1], a[2], a[3]);
+            d[1] = make_float4(a[4], a[5], a[6], a[7]);
+        } else {
+            reinterpret_cast<uint4*>(y)[i] = make_uint4(pack16<DT>(a[0], a[1]), pack16<DT>(a[2], a[3]), pack16<DT>(a[4], a[5]),
+                                                        pack16<DT>(a[6], a[7]));
+        }
     }
 }
 

@@ -140,6 +140,9 @@ def experts(x, ids, w, w13, w2, out):
             p = wd @ hq
             y[t] += w[t, k] * p
             tol[t] += np.abs(w[t, k]) * (product_error(hq[None], wd)[0] + np.abs(wd) @ step)
+            if out != "float32":  # parts may be kept as 16-bit integers: a step of 2^-14 of the block's power of two
+                amax = np.maximum(np.abs(p).reshape(-1, 32).max(1), 1e-300)
+                tol[t] += np.abs(w[t, k]) * np.repeat(2.0 ** (np.floor(np.log2(amax)) - 14), 32)
             mag[t] += np.abs(w[t, k] * p)
     # the weighted sum in fp32, then one rounding to the output type
     tol += (ids.shape[1] + 2) * 2.0 ** -24 * mag

@@ -50,7 +50,7 @@ SHAPES = [(4, 64, 32, 2), (8, 256, 96, 3), (16, 512, 160, 8), (3, 96, 64, 3), (1
 
 
 @pytest.mark.parametrize("E,H,I,K", SHAPES)
-@pytest.mark.parametrize("T", [1, 2, 7, 33, 150])
+@pytest.mark.parametrize("T", [1, 2, 7, 33, 150, 700])
 def test_forward(E, H, I, K, T):
     packed, w13, w2 = weights(E, H, I, E + H)
     h = handle(E, H, I, packed)
@@ -69,6 +69,7 @@ def test_one_expert_takes_all():
     E, H, I, K, T = 6, 128, 64, 2, 300
     packed, w13, w2 = weights(E, H, I, 3)
     x, ids, w = tokens(T, H, E, K, 5)
+    w *= 1e3  # parts of very different sizes in a sum
     ids[:, 0], ids[:, 1] = 4, np.where(np.arange(T) % 97 == 0, 2, 5)
     want, tol = R.experts(x.double().cpu().numpy(), ids, w, w13, w2, "bfloat16")
     close(ops.moe_forward(x, cuda(ids), cuda(w), handle(E, H, I, packed)), want, tol)
@@ -115,10 +116,12 @@ def test_rows_do_not_depend_on_the_batch():
     h = handle(E, H, I, packed)
     x, ids, w = tokens(T, H, E, K, 10)
     idc, wc = cuda(ids), cuda(w)
-    full = ops.moe_forward(x, idc, wc, h)
-    assert torch.equal(full, ops.moe_forward(x, idc, wc, h))
+    full = ops.moe_forward_partial(x, idc, wc, h)
+    assert torch.equal(full, ops.moe_forward_partial(x, idc, wc, h))
+    half = ops.moe_forward(x, idc, wc, h)
+    assert torch.equal(half, ops.moe_forward(x, idc, wc, h))
     for n in (1, 3, 64, 129):
-        assert torch.equal(full[:n], ops.moe_forward(x[:n], idc[:n].contiguous(), wc[:n].contiguous(), h))
+        assert torch.equal(full[:n], ops.moe_forward_partial(x[:n], idc[:n].contiguous(), wc[:n].contiguous(), h))
 
 
 def test_long_call_in_slices():
