@@ -1755,7 +1755,8 @@ extern "C" int moe_engine_forward(moe_engine* eng, const void* x, void* y, const
             if (eng->timed && eng->last_stream != st) CUDA_TRY(cudaStreamWaitEvent(st, eng->ev1, 0));
             CUDA_TRY(cudaEventRecord(eng->ev0, st));
         }
-        MxForward f{x, y, topk_ids, topk_w, T, K, act_dtype, out_dtype, eng->emap, eng->emap_n, eng->err, eng->pdl};
+        MxForward f{x, y, topk_ids, topk_w, T, K, act_dtype, out_dtype, eng->emap, eng->emap_n, eng->err,
+                    reinterpret_cast<unsigned int*>(reinterpret_cast<uint8_t*>(eng->bar) + 256), eng->pdl};
         const int rc = mx_forward(eng->mx, f, st);
         if (timed) {  // after a failure too: what was launched before it still uses the workspace
             CUDA_TRY(cudaEventRecord(eng->ev1, st));

@@ -25,6 +25,7 @@ struct MxForward {
     const int32_t* emap;
     int32_t emap_n;
     int32_t* err;
+    unsigned int* cnt;  // counters [H / 64 or more], zero between calls
     bool pdl;
 };
 

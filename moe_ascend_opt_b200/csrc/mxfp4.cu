@@ -36,29 +36,29 @@ int encoder(EncodeFn* out) {
 }
 
 int encode_map(CUtensorMap* m, CUtensorMapDataType type, CUtensorMapSwizzle swizzle, const void* base, int64_t esz, int64_t cols,
-               int64_t rows, int64_t planes, int box_cols, int box_rows) {
+               int64_t rows, int box_cols, int box_rows) {
     EncodeFn fn;
     if (int rc = encoder(&fn)) return rc;
-    const cuuint64_t dims[3] = {(cuuint64_t)cols, (cuuint64_t)rows, (cuuint64_t)planes};
-    const cuuint64_t strides[2] = {(cuuint64_t)(cols * esz), (cuuint64_t)(cols * esz * rows)};
-    const cuuint32_t box[3] = {(cuuint32_t)box_cols, (cuuint32_t)box_rows, 1}, ones[3] = {1, 1, 1};
-    const CUresult r = fn(m, type, planes ? 3 : 2, const_cast<void*>(base), dims, strides, box, ones,
+    const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
+    const cuuint64_t strides[1] = {(cuuint64_t)(cols * esz)};
+    const cuuint32_t box[2] = {(cuuint32_t)box_cols, (cuuint32_t)box_rows}, ones[2] = {1, 1};
+    const CUresult r = fn(m, type, 2, const_cast<void*>(base), dims, strides, box, ones,
                           CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                           CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS) return fail(MOE_ERR_CUDA, "cuTensorMapEncodeTiled failed with " + std::to_string((int)r));
     return MOE_OK;
 }
 
-// Codes as bytes [planes][rows][pitch], boxes of 128 bytes x box_rows, 128-byte swizzle; what
-// lies outside reads as zero.  planes 0: a 2-D map.
-int encode(CUtensorMap* m, const void* base, int64_t pitch, int64_t rows, int64_t planes, int box_rows) {
-    return encode_map(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, CU_TENSOR_MAP_SWIZZLE_128B, base, 1, pitch, rows, planes, 128, box_rows);
+// Codes as bytes [rows][pitch], boxes of 128 bytes x box_rows, 128-byte swizzle; what lies outside
+// reads as zero.
+int encode(CUtensorMap* m, const void* base, int64_t pitch, int64_t rows, int box_rows) {
+    return encode_map(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, CU_TENSOR_MAP_SWIZZLE_128B, base, 1, pitch, rows, 128, box_rows);
 }
 
 // An output [rows][cols] of 2- or 4-byte elements, stored in boxes of 32 rows x 64 bytes.
 int encode_out(CUtensorMap* m, void* base, int64_t esz, int64_t cols, int64_t rows) {
     return encode_map(m, esz == 4 ? CU_TENSOR_MAP_DATA_TYPE_UINT32 : CU_TENSOR_MAP_DATA_TYPE_UINT16, CU_TENSOR_MAP_SWIZZLE_64B, base,
-                      esz, cols, rows, 0, (int)(64 / esz), 32);
+                      esz, cols, rows, (int)(64 / esz), 32);
 }
 
 // ------------------------------------------------------------------ launches
@@ -103,25 +103,26 @@ int sm_count(int dev, int* out) {
     return MOE_OK;
 }
 
-// Tiles of 128 x 256 (a CTA per SM), or of 128 x 64 (two) for products with few rows.
-constexpr int kWide = 256, kWideStages = 4, kNarrow = 64, kNarrowStages = 4;
+// Kernel shapes.  Wide: 128 x 256 tiles, a CTA per SM, for many rows (the tiles' loads from L2 bound
+// it, which fall with the tile's width).  Narrow: 128 x 64, two CTAs per SM, for dense products of too few
+// wide tiles to fill the GPU.  Slim: 32 x 64, for experts with few rows each, where the weights' stream from
+// memory bounds the kernel and a small A leaves room for more of them in flight.
+using Wide = mx::Shape<256, 128, 4, 8, 1>;
+using Narrow = mx::Shape<64, 128, 4, 4, 2>;
+using Slim = mx::Shape<64, 32, 7, 1, 2>;
+using Fused = mx::Shape<64, 8, 8, 1, 2, true>;
 
-template <int MODE, int NT, int STAGES>
-int launch_gemm_nt(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& to, mx::GemmParams& p, int64_t m_tiles, int sms, bool pdl,
-                   cudaStream_t st) {
-    using S = mx::Shape<NT>;
-    auto fn = mx::mx_gemm_kernel<MODE, NT, STAGES>;
-    const int smem = STAGES * S::kStage + S::kStaging + 1024;
-    if (int rc = allow_smem(reinterpret_cast<const void*>(fn), smem)) return rc;
-    p.nt_count = (int)ceil_div(p.N, NT);
-    return launch(fn, (unsigned)std::min<int64_t>(m_tiles * p.nt_count, sms * S::kCtas), S::kThreads, smem, pdl, st, ta, tb, to, p);
-}
+constexpr int kFusedStages = 32;  // depth of fused calls: their A buffers hold it whole
 
-template <int MODE>
+template <int MODE, class S>
 int launch_gemm(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& to, mx::GemmParams& p, int64_t m_tiles, int sms,
-                bool wide, bool pdl, cudaStream_t st) {
-    return wide ? launch_gemm_nt<MODE, kWide, kWideStages>(ta, tb, to, p, m_tiles, sms, pdl, st)
-                : launch_gemm_nt<MODE, kNarrow, kNarrowStages>(ta, tb, to, p, m_tiles, sms, pdl, st);
+                bool pdl, cudaStream_t st) {
+    auto fn = mx::mx_gemm_kernel<MODE, S>;
+    constexpr bool WA = S::FUSED && MODE == mx::kGateUp;
+    const int smem = S::smem(WA, (int)ceil_div(p.K, mx::kStageK));
+    if (int rc = allow_smem(reinterpret_cast<const void*>(fn), S::smem(WA, kFusedStages))) return rc;
+    p.nt_count = (int)ceil_div(p.N, S::NT);
+    return launch(fn, (unsigned)std::min<int64_t>(m_tiles * p.nt_count, sms * S::kCtas), S::kThreads, smem, pdl, st, ta, tb, to, p);
 }
 
 bool dtype_ok(int32_t t) { return t == MOE_F16 || t == MOE_BF16 || t == MOE_F32; }
@@ -219,7 +220,7 @@ extern "C" int moe_mxfp4_tile_scales(const uint8_t* scales, int64_t rows, int64_
     if (!aligned(tiles, 16)) return fail(MOE_ERR_INVALID, "tiled scales must be 16-byte aligned");
     const int64_t n = ceil_div(rows, 128) * 128 * ceil_div(cols, 128);
     mx::tile_scales_kernel<<<(unsigned)std::min<int64_t>(ceil_div(n, 256), 4096), 256, 0, static_cast<cudaStream_t>(stream)>>>(
-        scales, rows, (int)(cols / 32), 0, 0, tiles);
+        scales, rows, (int)(cols / 32), tiles);
     CUDA_TRY(cudaGetLastError());
     return MOE_OK;
 }
@@ -245,10 +246,10 @@ extern "C" int moe_mxfp4_matmul(const uint8_t* a, const uint8_t* a_scales, const
         return fail(MOE_ERR_DEVICE, "an earlier MXFP4 product failed on the device (a bounded wait expired); its output is invalid");
     }
     CUtensorMap ta, tb;
-    if (int rc = encode(&ta, a, K / 2, M, 0, mx::kTileM)) return rc;
-    p.mt_count = (int)ceil_div(M, mx::kTileM);
-    const bool wide = p.mt_count * ceil_div(N, kWide) >= sms;
-    if (int rc = encode(&tb, b, K / 2, N, 1, wide ? kWide : kNarrow)) return rc;
+    if (int rc = encode(&ta, a, K / 2, M, 128)) return rc;
+    p.mt_count = (int)ceil_div(M, 128);
+    const bool wide = p.mt_count * ceil_div(N, Wide::NT) >= sms;
+    if (int rc = encode(&tb, b, K / 2, N, wide ? Wide::NT : Narrow::NT)) return rc;
     p.M = (int)M; p.N = (int)N; p.K = (int)K;
     p.kb = (int)ceil_div(K, 128);
     p.sfa = a_scales;
@@ -260,7 +261,8 @@ extern "C" int moe_mxfp4_matmul(const uint8_t* a, const uint8_t* a_scales, const
     p.tma_out = wide && N * esz % 16 == 0;
     if (p.tma_out)
         if (int rc = encode_out(&to, y, esz, N, M)) return rc;
-    return launch_gemm<mx::kDense>(ta, tb, to, p, p.mt_count, sms, wide, false, st);
+    return wide ? launch_gemm<mx::kDense, Wide>(ta, tb, to, p, p.mt_count, sms, false, st)
+                : launch_gemm<mx::kDense, Narrow>(ta, tb, to, p, p.mt_count, sms, false, st);
 }
 
 // ------------------------------------------------------------------ expert layer
@@ -270,52 +272,65 @@ struct MxLayer {
     moe_config cfg{};
     int sms = 0;
     int64_t kb1 = 0, kb2 = 0, nb1 = 0, nb2 = 0;  // scale tiles along K and N of gate_up (1) and down (2)
+    int64_t st1 = 0, st2 = 0, pn1 = 0, pn2 = 0;  // panels along K and N
+    // panels (codes and scales), and the scales again in tiles, which wide tiles read
     uint8_t *q1 = nullptr, *s1 = nullptr, *q2 = nullptr, *s2 = nullptr;
-    CUtensorMap t1[2]{}, t2[2]{};  // narrow and wide boxes
     uint8_t* ws = nullptr;
     size_t ws_bytes = 0;
     std::vector<uint8_t*> retired;  // earlier workspaces: captured graphs may still hold them
-    size_t q1_bytes() const { return (size_t)cfg.num_experts * 2 * cfg.intermediate_size * (cfg.hidden_size / 2); }
-    size_t q2_bytes() const { return (size_t)cfg.num_experts * cfg.hidden_size * (cfg.intermediate_size / 2); }
+    size_t q1_expert() const { return (size_t)pn1 * st1 * mx::kPanel; }
+    size_t q2_expert() const { return (size_t)pn2 * st2 * mx::kPanel; }
     size_t s1_bytes() const { return (size_t)cfg.num_experts * nb1 * kb1 * 512; }
     size_t s2_bytes() const { return (size_t)cfg.num_experts * nb2 * kb2 * 512; }
 };
 
-namespace {
+namespace layer {
 
 constexpr int64_t kMaxPairs = 1 << 18;  // routed pairs of one pass; longer calls run in slices of tokens
 
-// Rows of a matrix [rows][bytes] between the input contract's order and the layer's: gate_up row
-// r of the layer holds unit 32 (r / 64) + r % 32 of gate (r / 32 even) or up.
-__global__ void mx_rows_kernel(uint8_t* dst, const uint8_t* src, int64_t rows, int64_t bytes, int map, int64_t I, int inverse) {
+// Row of the input contract for row r of the layer: gate_up (map) rows lie in groups of 32 gate rows
+// and the 32 up rows of the same units.
+MOE_DEV int64_t source_row(int64_t r, int map, int64_t I) { return map ? ((r >> 5) & 1) * I + (r >> 6) * 32 + (r & 31) : r; }
+
+// Codes of a matrix [rows][bytes] between the input contract and the layer's panels, 16 bytes a thread.
+__global__ void mx_panel_codes_kernel(uint8_t* panels, uint8_t* codes, int64_t rows, int64_t bytes, int64_t stages, int64_t expert,
+                                      int map, int64_t I, int to_panels) {
     const int64_t n16 = bytes / 16, n = rows * n16, e = blockIdx.y;
-    dst += e * rows * bytes;
-    src += e * rows * bytes;
+    panels += e * expert;
+    codes += e * rows * bytes;
     for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (int64_t)gridDim.x * blockDim.x) {
         const int64_t r = i / n16, c = i - r * n16;
-        const int64_t u = map ? ((r >> 5) & 1) * I + (r >> 6) * 32 + (r & 31) : r;
-        const uint4* s = reinterpret_cast<const uint4*>(src);
-        uint4* d = reinterpret_cast<uint4*>(dst);
-        if (inverse) d[u * n16 + c] = s[i];
-        else d[i] = s[u * n16 + c];
+        uint4* a = reinterpret_cast<uint4*>(panels + mx::panel_code_at(r, c * 16, stages));
+        uint4* b = reinterpret_cast<uint4*>(codes) + source_row(r, map, I) * n16 + c;
+        if (to_panels) *a = *b;
+        else *b = *a;
     }
 }
 
-// Scale tiles of one matrix -> row-major scales (inverse of tile_scales_kernel).
-__global__ void mx_untile_kernel(const uint8_t* tiles, int64_t rows, int nb, int map, int64_t I, uint8_t* s) {
-    const int64_t kb = (nb + 3) >> 2, n = rows * nb;
+// Scales [rows][nb] between the input contract and the layer's panels and tiles.
+__global__ void mx_panel_scales_kernel(uint8_t* panels, uint8_t* tiles, uint8_t* s, int64_t rows, int nb, int64_t stages, int64_t expert,
+                                       int64_t tiles_expert, int map, int64_t I, int to_panels) {
+    const int64_t n = rows * nb, kb = (nb + 3) >> 2, e = blockIdx.y;
+    panels += e * expert;
+    tiles += e * tiles_expert;
+    s += e * n;
     for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (int64_t)gridDim.x * blockDim.x) {
         const int64_t r = i / nb, b = i - r * nb;
-        const int64_t u = map ? ((r >> 5) & 1) * I + (r >> 6) * 32 + (r & 31) : r;
-        s[u * nb + b] = tiles[mx::tiled_at(r, b, kb)];
+        uint8_t* v = s + source_row(r, map, I) * nb + b;
+        if (to_panels) {
+            panels[mx::panel_scale_at(r, b, stages)] = *v;
+            tiles[mx::tiled_at(r, b, kb)] = *v;
+        } else {
+            *v = tiles[mx::tiled_at(r, b, kb)];
+        }
     }
 }
 
 // Online quantisation of rows [n][cols] to layer rows: row j goes to layer row
 // (j / 32) * 64 + 32 * half + j % 32 (gate_up, half 0 gate, 1 up) or j (down, half -1).
 template <int DT>
-__global__ void mx_store_rows_kernel(const void* w, int64_t n, int cols, int half, uint8_t* q, uint8_t* tiles) {
-    const int64_t per = cols >> 3, total = n * per, kb = (cols + 127) >> 7;
+__global__ void mx_store_rows_kernel(const void* w, int64_t n, int cols, int half, uint8_t* panels, uint8_t* tiles) {
+    const int64_t per = cols >> 3, total = n * per, kb = (cols + 127) >> 7, stages = (cols + 255) >> 8;
     for (int64_t i0 = (int64_t)blockIdx.x * blockDim.x; i0 < total; i0 += (int64_t)gridDim.x * blockDim.x) {
         const int64_t i = i0 + threadIdx.x;
         float v[8] = {};
@@ -325,9 +340,22 @@ __global__ void mx_store_rows_kernel(const void* w, int64_t n, int cols, int hal
         if (i >= total) continue;
         const int64_t j = i / per, k = i - j * per;
         const int64_t r = half < 0 ? j : (j >> 5) * 64 + 32 * half + (j & 31);
-        reinterpret_cast<uint32_t*>(q)[r * per + k] = c;
-        if ((i & 3) == 0) tiles[mx::tiled_at(r, k >> 2, kb)] = (uint8_t)sc;
+        *reinterpret_cast<uint32_t*>(panels + mx::panel_code_at(r, k * 4, stages)) = c;
+        if ((i & 3) == 0) {
+            panels[mx::panel_scale_at(r, k >> 2, stages)] = (uint8_t)sc;
+            tiles[mx::tiled_at(r, k >> 2, kb)] = (uint8_t)sc;
+        }
     }
+}
+
+// How a call of T tokens runs.  Fused: two kernels that route for themselves, where the launches and
+// their latencies are what counts; slim or wide tiles after a kernel that places the token rows, by the
+// rows that an expert can expect.
+enum Plan { kPlanFused, kPlanSlim, kPlanWide };
+Plan plan_of(const MxLayer* l, int64_t T, int64_t K) {
+    const int64_t P = T * K;
+    if (P <= mx::kFusedPairs && l->st1 <= kFusedStages) return kPlanFused;
+    return P >= 32 * std::min(l->cfg.num_experts, P) ? kPlanWide : kPlanSlim;
 }
 
 struct Workspace {
@@ -335,6 +363,7 @@ struct Workspace {
     uint8_t *xq, *xs, *hq, *hs;
     uint8_t *part, *pexp;  // fp32 [rows][H], or 16-bit integers and exponents [rows][H / 32]
     int64_t mt;  // bound of the number of m tiles
+    int tile;    // their rows
     size_t bytes;
 };
 
@@ -349,25 +378,29 @@ int64_t prep_tokens(int64_t T, int64_t K) {
 Workspace carve(const MxLayer* l, int64_t T, int64_t K, uint8_t* base) {
     Workspace w{};
     const int64_t P = T * K, H = l->cfg.hidden_size, I = l->cfg.intermediate_size;
-    w.mt = P / mx::kTileM + std::min(P, l->cfg.num_experts);
-    const int64_t rows = w.mt * mx::kTileM;
+    const Plan plan = plan_of(l, T, K);
+    w.tile = plan == kPlanWide ? 128 : (plan == kPlanFused ? Fused::TM : Slim::TM);
+    w.mt = plan == kPlanFused ? P : P / w.tile + std::min(P, l->cfg.num_experts);
+    const int64_t rows = w.mt * w.tile;
     size_t off = 0;
     auto take = [&](size_t n) {
         uint8_t* p = base + off;
         off += (n + 1023) / 1024 * 1024;
         return p;
     };
-    w.mtiles = reinterpret_cast<int32_t*>(take(4));
-    w.mt_expert = reinterpret_cast<int32_t*>(take(w.mt * 4));
-    w.mt_rows = reinterpret_cast<int32_t*>(take(w.mt * 4));
-    w.ppos = reinterpret_cast<int32_t*>(take(P * 4));
-    w.counts = reinterpret_cast<int32_t*>(take(P > mx::kPrepSelf ? ceil_div(T, prep_tokens(T, K)) * l->cfg.num_experts * 4 : 0));
-    w.xq = take(rows * (H / 2));
-    w.xs = take(w.mt * l->kb1 * 512);
     w.hq = take(rows * (I / 2));
     w.hs = take(w.mt * l->kb2 * 512);
-    w.part = take((size_t)rows * H * 4);
-    w.pexp = take((size_t)rows * (H / 32));
+    w.part = take((size_t)(plan == kPlanFused ? P : rows) * H * 4);
+    if (plan != kPlanFused) {
+        w.pexp = take((size_t)rows * (H / 32));
+        w.mtiles = reinterpret_cast<int32_t*>(take(4));
+        w.mt_expert = reinterpret_cast<int32_t*>(take(w.mt * 4));
+        w.mt_rows = reinterpret_cast<int32_t*>(take(w.mt * 4));
+        w.ppos = reinterpret_cast<int32_t*>(take(P * 4));
+        w.counts = reinterpret_cast<int32_t*>(take(P > mx::kPrepSelf ? ceil_div(T, prep_tokens(T, K)) * l->cfg.num_experts * 4 : 0));
+        w.xq = take(rows * (H / 2));
+        w.xs = take(w.mt * l->kb1 * 512);
+    }
     w.bytes = off;
     return w;
 }
@@ -400,19 +433,47 @@ int grow(MxLayer* l, size_t bytes) {
 template <int DT, bool PART16>
 int combine_launch(const MxLayer* l, const MxForward& f, const float* tw, void* y, const Workspace& w, int64_t T, cudaStream_t st) {
     const int H = (int)l->cfg.hidden_size;
-    return launch(mx::mx_combine_kernel<DT, PART16>, (unsigned)std::min<int64_t>(ceil_div(T * (H / 8), 256), l->sms * 16), 256, 0,
+    return launch(mx::mx_combine_kernel<DT, PART16>, (unsigned)std::min<int64_t>(ceil_div(T * ceil_div(H, 256), 8), l->sms * 16), 256, 0,
                   f.pdl, st, (const void*)w.part, (const uint8_t*)w.pexp, (const int32_t*)w.ppos, tw, (int)T, (int)f.K, H, y);
+}
+
+// Two kernels: gate_up (routing, token rows quantised as they are needed), down with the weighted sum.
+int forward_fused(MxLayer* l, const MxForward& f, const void* x, void* y, const int32_t* ids, const float* tw, int64_t T,
+                  cudaStream_t st) {
+    const int64_t H = l->cfg.hidden_size, I = l->cfg.intermediate_size;
+    const Workspace w = carve(l, T, f.K, l->ws);
+    CUtensorMap th;
+    if (int rc = encode(&th, w.hq, I / 2, w.mt * w.tile, w.tile)) return rc;
+    mx::GemmParams p{};
+    p.err = f.err;
+    p.x = x; p.ids = ids; p.tw = tw;
+    p.T = (int)T; p.topk = (int)f.K; p.E = (int)l->cfg.num_experts; p.e_off = l->cfg.expert_offset;
+    p.emap = f.emap; p.emap_n = f.emap_n; p.act_bf16 = f.act_dtype == MOE_BF16;
+    p.I = (int)I;
+    mx::GemmParams g1 = p;
+    g1.N = (int)(2 * I); g1.K = (int)H; g1.kb = (int)l->kb1;
+    g1.sfb = l->s1; g1.panels = l->q1; g1.hq = w.hq; g1.hs = w.hs; g1.hkb = (int)l->kb2;
+    if (int rc = launch_gemm<mx::kGateUp, Fused>(th, th, th, g1, w.mt, l->sms, f.pdl, st)) return rc;
+    mx::GemmParams g2 = p;
+    g2.N = (int)H; g2.K = (int)I; g2.kb = (int)l->kb2;
+    g2.sfa = w.hs; g2.sfb = l->s2; g2.panels = l->q2; g2.out = w.part; g2.out_dtype = MOE_F32;
+    g2.y = y; g2.y_dtype = f.out_dtype; g2.cnt = f.cnt;
+    return launch_gemm<mx::kDown, Fused>(th, th, th, g2, w.mt, l->sms, f.pdl, st);
 }
 
 int forward_slice(MxLayer* l, const MxForward& f, const void* x, void* y, const int32_t* ids, const float* tw, int64_t T,
                   cudaStream_t st) {
     const int64_t E = l->cfg.num_experts, H = l->cfg.hidden_size, I = l->cfg.intermediate_size;
+    const Plan plan = plan_of(l, T, f.K);
+    if (plan == kPlanFused) return forward_fused(l, f, x, y, ids, tw, T, st);
+    const bool wide = plan == kPlanWide;
     const Workspace w = carve(l, T, f.K, l->ws);
     mx::PrepParams r{};
     r.x = x; r.ids = ids;
     r.T = (int)T; r.K = (int)f.K; r.H = (int)H; r.E = (int)E; r.e_off = l->cfg.expert_offset;
     r.emap = f.emap; r.emap_n = f.emap_n;
     r.tokens = (int)prep_tokens(T, f.K);
+    r.tile_log2 = wide ? 7 : 5;
     r.mtiles = w.mtiles; r.mt_expert = w.mt_expert; r.mt_rows = w.mt_rows; r.ppos = w.ppos;
     r.xq = w.xq; r.xs = w.xs; r.kb = (int)l->kb1;
     const unsigned runs = (unsigned)ceil_div(T, r.tokens);
@@ -425,34 +486,43 @@ int forward_slice(MxLayer* l, const MxForward& f, const void* x, void* y, const 
     auto prep = f.act_dtype == MOE_BF16 ? mx::mx_prep_kernel<MOE_BF16> : mx::mx_prep_kernel<MOE_F16>;
     if (int rc = allow_smem(reinterpret_cast<const void*>(prep), 128 * 1024)) return rc;
     if (int rc = launch(prep, runs, mx::kPrepThreads, psmem, f.pdl, st, r)) return rc;
-    CUtensorMap tx, th;
-    if (int rc = encode(&tx, w.xq, H / 2, w.mt * mx::kTileM, 0, 16)) return rc;
-    if (int rc = encode(&th, w.hq, I / 2, w.mt * mx::kTileM, 0, 16)) return rc;
+    CUtensorMap tx, th, tx32, th32;  // boxes of a whole tile, and of 32 rows for tiles that are not full
+    if (int rc = encode(&tx, w.xq, H / 2, w.mt * w.tile, w.tile)) return rc;
+    if (int rc = encode(&th, w.hq, I / 2, w.mt * w.tile, w.tile)) return rc;
+    tx32 = tx, th32 = th;
+    if (wide) {
+        if (int rc = encode(&tx32, w.xq, H / 2, w.mt * w.tile, 32)) return rc;
+        if (int rc = encode(&th32, w.hq, I / 2, w.mt * w.tile, 32)) return rc;
+    }
     mx::GemmParams p{};
     p.mtiles = w.mtiles; p.mt_expert = w.mt_expert; p.mt_rows = w.mt_rows;
     p.err = f.err;
     p.I = (int)I;
-    const bool wide = T * f.K >= 32 * std::min<int64_t>(E, T * f.K);
     mx::GemmParams g1 = p;
     g1.N = (int)(2 * I); g1.K = (int)H; g1.kb = (int)l->kb1;
-    g1.sfa = w.xs; g1.sfb = l->s1; g1.hq = w.hq; g1.hs = w.hs; g1.hkb = (int)l->kb2;
-    if (int rc = launch_gemm<mx::kGateUp>(tx, l->t1[wide], tx, g1, w.mt, l->sms, wide, f.pdl, st)) return rc;
+    g1.sfa = w.xs; g1.sfb = l->s1; g1.panels = l->q1; g1.hq = w.hq; g1.hs = w.hs; g1.hkb = (int)l->kb2;
+    if (int rc = wide ? launch_gemm<mx::kGateUp, Wide>(tx, tx32, tx, g1, w.mt, l->sms, f.pdl, st)
+                      : launch_gemm<mx::kGateUp, Slim>(tx, tx, tx, g1, w.mt, l->sms, f.pdl, st))
+        return rc;
     mx::GemmParams g2 = p;
     g2.N = (int)H; g2.K = (int)I; g2.kb = (int)l->kb2;
-    g2.sfa = w.hs; g2.sfb = l->s2; g2.out = w.part; g2.pexp = w.pexp;
+    g2.sfa = w.hs; g2.sfb = l->s2; g2.panels = l->q2; g2.out = w.part; g2.pexp = w.pexp;
     const bool part16 = wide && f.out_dtype != MOE_F32;
     g2.out_dtype = part16 ? MOE_F16 : MOE_F32;
-    CUtensorMap tp = th;  // unused by narrow tiles
+    CUtensorMap tp = th;  // used by wide tiles
     if (wide)
-        if (int rc = encode_out(&tp, w.part, part16 ? 2 : 4, H, w.mt * mx::kTileM)) return rc;
-    if (int rc = launch_gemm<mx::kDown>(th, l->t2[wide], tp, g2, w.mt, l->sms, wide, f.pdl, st)) return rc;
+        if (int rc = encode_out(&tp, w.part, part16 ? 2 : 4, H, w.mt * w.tile)) return rc;
+    if (int rc = wide ? launch_gemm<mx::kDown, Wide>(th, th32, tp, g2, w.mt, l->sms, f.pdl, st)
+                      : launch_gemm<mx::kDown, Slim>(th, th, tp, g2, w.mt, l->sms, f.pdl, st))
+        return rc;
     if (f.out_dtype == MOE_F32) return combine_launch<MOE_F32, false>(l, f, tw, y, w, T, st);
     if (f.out_dtype == MOE_BF16)
         return part16 ? combine_launch<MOE_BF16, true>(l, f, tw, y, w, T, st) : combine_launch<MOE_BF16, false>(l, f, tw, y, w, T, st);
     return part16 ? combine_launch<MOE_F16, true>(l, f, tw, y, w, T, st) : combine_launch<MOE_F16, false>(l, f, tw, y, w, T, st);
 }
 
-}  // namespace
+}  // namespace layer
+using namespace layer;
 
 int mx_create(const moe_config& cfg, int num_sms, MxLayer** out) {
     *out = nullptr;
@@ -462,11 +532,15 @@ int mx_create(const moe_config& cfg, int num_sms, MxLayer** out) {
     if (!l) return fail(MOE_ERR_STATE, "out of host memory");
     l->cfg = cfg;
     l->sms = num_sms;
-    const int64_t E = cfg.num_experts, H = cfg.hidden_size, I = cfg.intermediate_size;
+    const int64_t H = cfg.hidden_size, I = cfg.intermediate_size;
     l->kb1 = ceil_div(H, 128);
     l->kb2 = ceil_div(I, 128);
     l->nb1 = ceil_div(2 * I, 128);
     l->nb2 = ceil_div(H, 128);
+    l->st1 = ceil_div(H, 256);
+    l->st2 = ceil_div(I, 256);
+    l->pn1 = ceil_div(2 * I, 64);
+    l->pn2 = ceil_div(H, 64);
     MxBuffer b[4];
     mx_buffers(l, b);
     for (auto& x : b) {
@@ -477,15 +551,6 @@ int mx_create(const moe_config& cfg, int num_sms, MxLayer** out) {
             mx_destroy(l);
             return fail(MOE_ERR_CUDA, std::string("MXFP4 weights: ") + cudaGetErrorString(e));
         }
-    }
-    int rc = MOE_OK;
-    for (int w = 0; w < 2 && rc == MOE_OK; ++w) {
-        rc = encode(&l->t1[w], l->q1, H / 2, 2 * I, E, w ? kWide : kNarrow);
-        if (rc == MOE_OK) rc = encode(&l->t2[w], l->q2, I / 2, H, E, w ? kWide : kNarrow);
-    }
-    if (rc != MOE_OK) {
-        mx_destroy(l);
-        return rc;
     }
     *out = l;
     return MOE_OK;
@@ -499,9 +564,9 @@ void mx_destroy(MxLayer* l) {
 }
 
 void mx_buffers(MxLayer* l, MxBuffer (&b)[4]) {
-    b[0] = {&l->q1, l->q1_bytes()};
+    b[0] = {&l->q1, l->cfg.num_experts * l->q1_expert()};
     b[1] = {&l->s1, l->s1_bytes()};
-    b[2] = {&l->q2, l->q2_bytes()};
+    b[2] = {&l->q2, l->cfg.num_experts * l->q2_expert()};
     b[3] = {&l->s2, l->s2_bytes()};
 }
 
@@ -509,10 +574,11 @@ int mx_load(MxLayer* l, const uint8_t* w13_q, const uint8_t* w13_s, const uint8_
     const int64_t E = l->cfg.num_experts, H = l->cfg.hidden_size, I = l->cfg.intermediate_size;
     if (!aligned(w13_q, 16) || !aligned(w2_q, 16)) return fail(MOE_ERR_INVALID, "weight codes must be 16-byte aligned");
     const dim3 g(128, (unsigned)E);
-    mx_rows_kernel<<<g, 256, 0, st>>>(l->q1, w13_q, 2 * I, H / 2, 1, I, 0);
-    mx_rows_kernel<<<g, 256, 0, st>>>(l->q2, w2_q, H, I / 2, 0, I, 0);
-    mx::tile_scales_kernel<<<g, 256, 0, st>>>(w13_s, 2 * I, (int)(H / 32), 1, I, l->s1);
-    mx::tile_scales_kernel<<<g, 256, 0, st>>>(w2_s, H, (int)(I / 32), 0, I, l->s2);
+    const int64_t t1 = l->nb1 * l->kb1 * 512, t2 = l->nb2 * l->kb2 * 512;
+    mx_panel_codes_kernel<<<g, 256, 0, st>>>(l->q1, const_cast<uint8_t*>(w13_q), 2 * I, H / 2, l->st1, l->q1_expert(), 1, I, 1);
+    mx_panel_codes_kernel<<<g, 256, 0, st>>>(l->q2, const_cast<uint8_t*>(w2_q), H, I / 2, l->st2, l->q2_expert(), 0, I, 1);
+    mx_panel_scales_kernel<<<g, 256, 0, st>>>(l->q1, l->s1, const_cast<uint8_t*>(w13_s), 2 * I, (int)(H / 32), l->st1, l->q1_expert(), t1, 1, I, 1);
+    mx_panel_scales_kernel<<<g, 256, 0, st>>>(l->q2, l->s2, const_cast<uint8_t*>(w2_s), H, (int)(I / 32), l->st2, l->q2_expert(), t2, 0, I, 1);
     CUDA_TRY(cudaGetLastError());
     return MOE_OK;
 }
@@ -521,7 +587,7 @@ int mx_quantize_store(MxLayer* l, int64_t expert, int32_t proj, const void* w, i
     const int64_t H = l->cfg.hidden_size, I = l->cfg.intermediate_size;
     if (!aligned(w, 16)) return fail(MOE_ERR_INVALID, "weight must be 16-byte aligned");
     const int64_t n = proj == 2 ? H : I, cols = proj == 2 ? I : H;
-    uint8_t* q = proj == 2 ? l->q2 + expert * H * (I / 2) : l->q1 + expert * 2 * I * (H / 2);
+    uint8_t* q = proj == 2 ? l->q2 + expert * l->q2_expert() : l->q1 + expert * l->q1_expert();
     uint8_t* s = proj == 2 ? l->s2 + expert * l->nb2 * l->kb2 * 512 : l->s1 + expert * l->nb1 * l->kb1 * 512;
     const int half = proj == 2 ? -1 : proj;
     const unsigned grid = (unsigned)std::min<int64_t>(ceil_div(n * (cols / 8), 256), (int64_t)l->sms * 16);
@@ -535,13 +601,14 @@ int mx_quantize_store(MxLayer* l, int64_t expert, int32_t proj, const void* w, i
 int mx_export(MxLayer* l, int64_t expert, int32_t which, void* q_out, void* s_out) {
     const int64_t H = l->cfg.hidden_size, I = l->cfg.intermediate_size;
     const int64_t rows = which == 0 ? 2 * I : H, cols = which == 0 ? H : I, nb = cols / 32;
-    const uint8_t* q = which == 0 ? l->q1 + expert * rows * (cols / 2) : l->q2 + expert * rows * (cols / 2);
-    const uint8_t* s = which == 0 ? l->s1 + expert * l->nb1 * l->kb1 * 512 : l->s2 + expert * l->nb2 * l->kb2 * 512;
+    uint8_t* q = which == 0 ? l->q1 + expert * l->q1_expert() : l->q2 + expert * l->q2_expert();
+    uint8_t* s = which == 0 ? l->s1 + expert * l->nb1 * l->kb1 * 512 : l->s2 + expert * l->nb2 * l->kb2 * 512;
     uint8_t* d = nullptr;
     CUDA_TRY(cudaMalloc(&d, rows * (cols / 2) + rows * nb));
     uint8_t* ds = d + rows * (cols / 2);
-    mx_rows_kernel<<<128, 256>>>(d, q, rows, cols / 2, which == 0, I, 1);
-    mx_untile_kernel<<<128, 256>>>(s, rows, (int)nb, which == 0, I, ds);
+    const int64_t stages = which == 0 ? l->st1 : l->st2;
+    mx_panel_codes_kernel<<<128, 256>>>(q, d, rows, cols / 2, stages, 0, which == 0, I, 0);
+    mx_panel_scales_kernel<<<128, 256>>>(q, s, ds, rows, (int)nb, stages, 0, 0, which == 0, I, 0);
     cudaError_t e = cudaGetLastError();
     if (e == cudaSuccess) e = cudaMemcpy(q_out, d, rows * (cols / 2), cudaMemcpyDeviceToHost);
     if (e == cudaSuccess) e = cudaMemcpy(s_out, ds, rows * nb, cudaMemcpyDeviceToHost);
@@ -552,7 +619,12 @@ int mx_export(MxLayer* l, int64_t expert, int32_t which, void* q_out, void* s_ou
 
 int mx_reserve(MxLayer* l, int64_t T, int64_t K) {
     if (T == 0) return MOE_OK;
-    return grow(l, carve(l, slice_tokens(T, K), K, nullptr).bytes);
+    // a shorter call may take another plan: the longest of each plan up to T
+    const int64_t S = slice_tokens(T, K), E = l->cfg.num_experts;
+    size_t bytes = 0;
+    for (int64_t t : {S, std::min(S, std::max<int64_t>(1, mx::kFusedPairs / K)), std::min(S, std::max<int64_t>(1, (32 * E - 1) / K))})
+        bytes = std::max(bytes, carve(l, t, K, nullptr).bytes);
+    return grow(l, bytes);
 }
 
 int mx_forward(MxLayer* l, const MxForward& f, cudaStream_t st) {

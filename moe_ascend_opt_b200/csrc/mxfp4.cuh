@@ -46,6 +46,25 @@ MOE_DEV int64_t tiled_at(int64_t row, int64_t block, int64_t kb) {
     return ((row >> 7) * kb + (block >> 2)) * 512 + (row & 31) * 16 + ((row >> 5) & 3) * 4 + (block & 3);
 }
 
+// Expert weights lie in panels of 64 rows x 256 elements (one stage of a product), so that a panel is one
+// contiguous copy whatever the matrix's row pitch: 64 x 128 bytes of codes, swizzled as the MMA reads them
+// (16-byte piece c of row r at c ^ (r % 8)), then 512 bytes of scales, 16 for each r % 32: the words (4
+// blocks) of rows r, r + 32 for the first 128 elements, then for the others.  [ceil(rows / 64)][stages]
+// panels; what lies past the matrix is zero.
+constexpr int kPanelCodes = 64 * 128, kPanel = kPanelCodes + 512;
+MOE_DEV int64_t panel_code_at(int64_t row, int64_t byte, int64_t stages) {
+    return ((row >> 6) * stages + (byte >> 7)) * kPanel + (row & 63) * 128 + (((byte >> 4 & 7) ^ (row & 7)) << 4) + (byte & 15);
+}
+MOE_DEV int64_t panel_scale_at(int64_t row, int64_t block, int64_t stages) {
+    return ((row >> 6) * stages + (block >> 3)) * kPanel + kPanelCodes + (row & 31) * 16 + ((block >> 2 & 1) * 2 + (row >> 5 & 1)) * 4 +
+           (block & 3);
+}
+
+// tiled_at for row r (below 128) of scale tile row `tile`, which need not be full.
+MOE_DEV int64_t tile_row_at(int64_t tile, int r, int64_t block, int64_t kb) {
+    return (tile * kb + (block >> 2)) * 512 + (r & 31) * 16 + (r >> 5) * 4 + (block & 3);
+}
+
 template <int DT>  // MOE_F16 / MOE_BF16 / MOE_F32: 8 consecutive values, 16-byte aligned
 MOE_DEV void load8(const void* x, int64_t i, float (&v)[8]) {
     if (DT == MOE_F32) {
@@ -114,22 +133,15 @@ __global__ void __launch_bounds__(256) quantize_kernel(const void* x, int64_t ro
     }
 }
 
-// Row-major scales -> tiled (one thread a word of 4 blocks).  `map` 1: the rows of a gate_up
-// matrix [2I] in the order of the experts' layout, 32 gate rows and 32 up rows in turn.
-__global__ void tile_scales_kernel(const uint8_t* s, int64_t rows, int nb, int map, int64_t I, uint8_t* out) {
-    const int64_t kb = (nb + 3) >> 2, rb = (rows + 127) >> 7;
-    const int64_t n = rb * 128 * kb;
-    const int64_t e = blockIdx.y;
-    s += e * rows * nb;
-    out += e * rb * kb * 512;
+// Row-major scales -> tiled (one thread a word of 4 blocks).
+__global__ void tile_scales_kernel(const uint8_t* s, int64_t rows, int nb, uint8_t* out) {
+    const int64_t kb = (nb + 3) >> 2, n = ((rows + 127) >> 7) * 128 * kb;
     for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (int64_t)gridDim.x * blockDim.x) {
         const int64_t r = i / kb, k = i - r * kb;
         uint32_t w = 0;
-        if (r < rows) {
-            const int64_t src = map ? ((r >> 5) & 1) * I + (r >> 6) * 32 + (r & 31) : r;
+        if (r < rows)
             for (int j = 0; j < 4; ++j)
-                if (4 * k + j < nb) w |= (uint32_t)s[src * nb + 4 * k + j] << (8 * j);
-        }
+                if (4 * k + j < nb) w |= (uint32_t)s[r * nb + 4 * k + j] << (8 * j);
         *reinterpret_cast<uint32_t*>(out + tiled_at(r, 4 * k, kb)) = w;
     }
 }

@@ -24,41 +24,71 @@ namespace moe {
 namespace mx {
 
 enum Mode { kDense = 0, kGateUp = 1, kDown = 2 };
-constexpr int kTileM = 128, kStageK = 256;
+constexpr int kStageK = 256;
+constexpr int kFusedPairs = 64;  // routed pairs of the calls whose two kernels route for themselves
 
 struct GemmParams {
     int M, N, K;         // dense: rows of a; N rows of b (of one expert); depth
     int kb;              // scale tiles along K
     int nt_count, mt_count;
     const uint8_t* sfa;  // [m tiles][kb][512]
-    const uint8_t* sfb;  // [experts][ceil(N / 128)][kb][512]
+    const uint8_t* sfb;  // [experts][ceil(N / 128)][kb][512]: dense and wide tiles
+    const uint8_t* panels;     // experts: [experts][ceil(N / 64)][stages][kPanel]
     const int32_t* mtiles;     // experts: number of m tiles, then expert and rows of each
     const int32_t* mt_expert;
     const int32_t* mt_rows;
-    void* out;           // dense [M][N] (out_dtype); down [m tiles * 128][N], fp32 or 16-bit parts
+    void* out;           // dense [M][N] (out_dtype); down [m tile rows][N], fp32 or 16-bit parts
     int out_dtype;
     int tma_out;         // dense, wide tiles: store through the map (rows of a multiple of 16 bytes)
-    uint8_t* pexp;       // down, 16-bit parts: exponent of each 32 columns [m tiles * 128][ceil(N / 32)]
-    int I;               // gate_up: hq [m tiles * 128][I / 2], hs tiled with hkb tiles along I
+    uint8_t* pexp;       // down, 16-bit parts: exponent of each 32 columns [m tile rows][ceil(N / 32)]
+    int I;               // gate_up: hq [m tile rows][I / 2], hs tiles with hkb tiles along I
     int hkb;
     uint8_t* hq;
     uint8_t* hs;
     int32_t* err;
+    // fused calls: the routing, the tokens, and down's weighted sum
+    const void* x;
+    const int32_t* ids;
+    const float* tw;
+    int T, topk, E, e_off, emap_n, act_bf16;
+    const int32_t* emap;
+    void* y;
+    int y_dtype;
+    unsigned int* cnt;   // down parts finished per column tile, zero between calls
 };
 
-template <int NT>
+// A kernel's shape: NT columns and TM rows of a tile (the MMA always takes 128 rows; of a tile of fewer it
+// reads whatever lies behind them in shared memory, and those lanes are never read back), STAGES of the
+// ring, EPI epilogue warps, CTAS per SM.
+template <int NT_, int TM_, int STAGES_, int EPI_, int CTAS_, bool FUSED_ = false>
 struct Shape {
+    static constexpr int NT = NT_, TM = TM_, STAGES = STAGES_, kEpiWarps = EPI_, kCtas = CTAS_;
+    static constexpr bool FUSED = FUSED_;
     static constexpr int kSfTiles = (NT + 127) / 128;  // scale tiles (128 rows) that cover a stage's B rows
-    static constexpr int kA = kTileM * 128, kB = NT * 128;
-    static constexpr int kStage = kA + kB + 1024 * (1 + kSfTiles);
+    static constexpr bool PANEL = TM < 128;            // B and its scales by the panel, else scale tiles
+    static constexpr int kA = TM * 128, kB = NT * 128;
+    static constexpr int kSfaKg = TM == 8 ? 128 : 512;  // scales of A for 128 elements: those of 8 rows, or a tile
+    static constexpr int kSfbBytes = PANEL ? 512 : 1024 * kSfTiles;
+    // A stage of the ring: A | B | scales of B | scales of A, the first and the last not where the kernel
+    // writes A itself (WA): A and its scales for the whole depth then lie in two buffers before the ring.
+    __host__ __device__ static constexpr int off_b(bool wa) { return wa ? 0 : kA; }
+    __host__ __device__ static constexpr int off_sfb(bool wa) { return off_b(wa) + kB; }
+    __host__ __device__ static constexpr int off_sfa(bool wa) { return off_sfb(wa) + kSfbBytes; }
+    __host__ __device__ static constexpr int stage(bool wa) { return (off_sfa(wa) + (wa ? 0 : 2 * kSfaKg) + 1023) / 1024 * 1024; }
+    __host__ __device__ static constexpr int a_buffer(int stages) { return stages * kA + (stages * 2 * kSfaKg + 1023) / 1024 * 1024; }
     static constexpr int kSfCols = 8 * (1 + kSfTiles);  // TMEM columns of a stage's scales
     static constexpr int kAcc = NT <= 128 ? 2 : 1;      // accumulators
-    static constexpr int kEpiWarps = NT >= 256 ? 8 : 4;
-    static constexpr int kCols = NT / (kEpiWarps / 4);  // columns of an epilogue thread
+    static constexpr int kCols = TM < 128 ? NT : NT / (kEpiWarps / 4);  // columns of an epilogue thread
     static constexpr int kThreads = 128 + 32 * kEpiWarps;
-    static constexpr int kCtas = NT <= 64 ? 2 : 1;      // per SM
     // wide tiles leave through shared memory: 32 rows x 64 bytes per epilogue warp, stored by TMA
     static constexpr int kStaging = NT >= 256 ? kEpiWarps * 2048 : 0;
+    // Dynamic shared memory for `stages` of depth.  The MMA's 128 rows of the last A stay inside, so do
+    // the 512 bytes that a copy of its scales takes.
+    __host__ __device__ static constexpr int smem(bool wa, int stages) {
+        const int ring = STAGES * stage(wa), buffers = wa ? 2 * a_buffer(stages) : 0;
+        const int tail = wa ? 0 : (stage(wa) < 16384 + 512 ? 16384 + 512 - stage(wa) : 0);
+        return buffers + ring + (tail + 1023) / 1024 * 1024 + kStaging + 1024;
+    }
 };
 
 // Descriptor of a 512-byte scale tile for tcgen05.cp: no swizzle, 8-row groups of 128 bytes.
@@ -93,23 +123,22 @@ MOE_DEV bool elect_one() {
     return r != 0;
 }
 
-MOE_DEV void tma_2d(uint32_t dst, const CUtensorMap* m, int x, int y, uint64_t* bar) {
+MOE_DEV void tma_2d(uint32_t dst, const CUtensorMap* m, int x, int y, uint32_t bar) {
     asm volatile(
         "cp.async.bulk.tensor.2d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
-        "l"(m), "r"(x), "r"(y), "r"(smem_u32(bar))
+        "l"(m), "r"(x), "r"(y), "r"(bar)
         : "memory");
+}
+MOE_DEV void bulk_copy(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+    asm volatile("cp.async.bulk.shared::cta.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src),
+                 "r"(bytes), "r"(bar)
+                 : "memory");
 }
 // 32 rows x 64 bytes of shared memory (64-byte swizzle) to global memory; what lies outside the map is dropped.
 MOE_DEV void tma_store_2d(const CUtensorMap* m, uint32_t src, int x, int y) {
     asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%1, %2}], [%3];" ::"l"(m), "r"(x), "r"(y), "r"(src)
                  : "memory");
     asm volatile("cp.async.bulk.commit_group;" ::: "memory");
-}
-MOE_DEV void tma_3d(uint32_t dst, const CUtensorMap* m, int x, int y, int z, uint64_t* bar) {
-    asm volatile(
-        "cp.async.bulk.tensor.3d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
-        "l"(m), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar))
-        : "memory");
 }
 // Bounded wait that also ends when another role of the CTA has given up.
 MOE_DEV bool wait_or_fail(uint64_t* bar, uint32_t parity, volatile int* failed) {
@@ -220,19 +249,116 @@ MOE_DEV float silu_up(float g, float u) {
     return g * q * u;
 }
 
-template <int MODE, int NT, int STAGES>
-__global__ void __launch_bounds__(Shape<NT>::kThreads, Shape<NT>::kCtas)
+// Routing of a fused call by the CTA itself: pieces of up to 8 pairs of one expert, in the order of
+// their first pairs, the pairs of a piece in their own order.
+struct FusedRoute {
+    int np;
+    int e[kFusedPairs];                  // local expert of each pair, -1: another engine's
+    int rank[kFusedPairs];               // among the pairs of its expert
+    int piece_e[kFusedPairs], rows[kFusedPairs];
+    uint8_t pair[kFusedPairs * 8];       // pair of each row
+};
+
+template <bool FUSED>
+struct RouteStore {
+    using type = int;
+};
+template <>
+struct RouteStore<true> {
+    using type = FusedRoute;
+};
+
+MOE_DEV void fused_route(FusedRoute& f, const GemmParams& p, int threads) {
+    const int P = p.T * p.topk, tid = threadIdx.x;
+    for (int i = tid; i < P; i += threads) {
+        f.e[i] = local_expert(__ldcg(p.ids + i), p.e_off, p.E, p.emap, p.emap_n, i, p.topk);
+        f.rows[i] = 0;
+    }
+    if (tid == 0) f.np = 0;
+    __syncthreads();
+    for (int i = tid; i < P; i += threads) {
+        const int e = f.e[i];
+        int rank = 0;
+#pragma unroll 8
+        for (int j = 0; j < i; ++j) rank += f.e[j] == e;
+        f.rank[i] = e >= 0 ? rank : -1;
+    }
+    __syncthreads();
+    for (int i = tid; i < P; i += threads) {
+        const int e = f.e[i], rank = f.rank[i];
+        if (e < 0) continue;
+        int heads = 0, piece = 0;
+#pragma unroll 8
+        for (int j = 0; j <= i; ++j) {  // the piece's first pair comes at or before i
+            const int rj = f.rank[j];
+            if (f.e[j] == e && rj == (rank & ~7)) piece = heads;
+            heads += rj >= 0 && (rj & 7) == 0;
+        }
+        f.pair[piece * 8 + (rank & 7)] = (uint8_t)i;
+        atomicMax(&f.rows[piece], (rank & 7) + 1);
+        if ((rank & 7) == 0) {
+            f.piece_e[piece] = e;
+            atomicAdd(&f.np, 1);
+        }
+    }
+    __syncthreads();
+}
+
+// Columns [n0, n0 + 64) of y from the parts of every pair, a half-warp per token, in the order of
+// the token's pairs.
+template <int DT>
+MOE_DEV void fused_combine(const FusedRoute& f, const GemmParams& p, int n0) {
+    const int lane = threadIdx.x & 31, n = n0 + (lane & 15) * 4, K = p.topk;
+    const float* part = static_cast<const float*>(p.out);
+    if (n >= p.N) return;
+    for (int t = lane >> 4; t < p.T; t += 2) {
+        float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int k0 = 0; k0 < K; k0 += 8) {
+            float4 v[8];
+            float w[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                const int i = t * K + k0 + k;
+                const bool have = k0 + k < K && f.e[min(i, p.T * K - 1)] >= 0;
+                v[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+                w[k] = 0.f;
+                if (have) {
+                    v[k] = __ldcg(reinterpret_cast<const float4*>(part + (int64_t)i * p.N + n));
+                    w[k] = __ldg(p.tw + i);
+                }
+            }
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                a.x = fmaf(w[k], v[k].x, a.x);
+                a.y = fmaf(w[k], v[k].y, a.y);
+                a.z = fmaf(w[k], v[k].z, a.z);
+                a.w = fmaf(w[k], v[k].w, a.w);
+            }
+        }
+        const int64_t at = (int64_t)t * p.N + n;
+        if (DT == MOE_F32) *reinterpret_cast<float4*>(static_cast<float*>(p.y) + at) = a;
+        else *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.y) + at) = make_uint2(pack16<DT>(a.x, a.y), pack16<DT>(a.z, a.w));
+    }
+}
+
+template <int MODE, class S>
+__global__ void __launch_bounds__(S::kThreads, S::kCtas)
     mx_gemm_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtensorMap tb,
-                   const __grid_constant__ CUtensorMap to, const GemmParams p) {
-    using S = Shape<NT>;
+                   const __grid_constant__ CUtensorMap to, const __grid_constant__ GemmParams p) {
+    constexpr int NT = S::NT, TM = S::TM, STAGES = S::STAGES;
+    constexpr bool FUSED = S::FUSED, WRITE_A = FUSED && MODE == kGateUp;  // A from the token rows, by warps 2 and 3
     constexpr int kSfBase = S::kAcc * NT;  // TMEM: the accumulators, then each stage's scales
     constexpr int kTmemCols = kSfBase + STAGES * S::kSfCols <= 256 ? 256 : 512;
     static_assert(kSfBase + STAGES * S::kSfCols <= 512 && kTmemCols * S::kCtas <= 512, "TMEM");
     extern __shared__ __align__(1024) uint8_t smem_raw[];
-    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    __shared__ __align__(8) uint64_t s_full[STAGES], s_empty[STAGES], s_accfull[2], s_accempty[2], s_done;
+    constexpr int kStage = S::stage(WRITE_A), oB = S::off_b(WRITE_A), oSfB = S::off_sfb(WRITE_A), oSfA = S::off_sfa(WRITE_A);
+    uint8_t* abuf = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    const int nstages = (p.K + kStageK - 1) / kStageK, k64 = (p.K + 63) / 64;
+    uint8_t* smem = abuf + (WRITE_A ? 2 * S::a_buffer(nstages) : 0);  // the ring
+    __shared__ __align__(8) uint64_t s_full[STAGES], s_empty[STAGES], s_accfull[2], s_accempty[2], s_afull[2], s_done;
     __shared__ uint32_t s_tmem;
     __shared__ int s_failed;
+    __shared__ typename RouteStore<FUSED>::type s_route;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
     if (tid == 0) {
@@ -243,6 +369,7 @@ __global__ void __launch_bounds__(Shape<NT>::kThreads, Shape<NT>::kCtas)
         for (int a = 0; a < 2; ++a) {
             mbar_init(&s_accfull[a], 1);
             mbar_init(&s_accempty[a], S::kEpiWarps);
+            mbar_init(&s_afull[a], 2);
         }
         mbar_init(&s_done, 1);
         s_failed = 0;
@@ -258,55 +385,75 @@ __global__ void __launch_bounds__(Shape<NT>::kThreads, Shape<NT>::kCtas)
     gemm::tc_fence_after();
     const uint32_t tmem = s_tmem;
     volatile int* failed = &s_failed;
-    // down: the tiles' list was complete before gate_up started (which lets this kernel start
-    // after its own wait), so the weights are fetched before the wait for gate_up's output
+    // down: the routing (ids, or the tiles' list) was complete before gate_up passed its own wait and let
+    // this kernel start, so the weights are fetched before the wait for gate_up's output
     if (MODE != kDown) asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    FusedRoute& route = reinterpret_cast<FusedRoute&>(s_route);  // an int where nothing is fused, never read
+    if (FUSED) fused_route(route, p, S::kThreads);
 
-    const int mt_count = MODE == kDense ? p.mt_count : p.mtiles[0];
+    const int mt_count = FUSED ? route.np : (MODE == kDense ? p.mt_count : p.mtiles[0]);
     const int64_t tiles = (int64_t)mt_count * p.nt_count;
-    const int nstages = (p.K + kStageK - 1) / kStageK, k64 = (p.K + 63) / 64;
     const int nb128 = (p.N + 127) / 128;
+    auto expert_of = [&](int mt) { return FUSED ? route.piece_e[mt] : (MODE == kDense ? 0 : p.mt_expert[mt]); };
+    auto rows_of = [&](int mt) { return FUSED ? route.rows[mt] : (MODE == kDense ? min(TM, p.M - mt * TM) : p.mt_rows[mt]); };
 
     if (warp == 0) {
+        // As for the MMAs: the warp walks the loop with uniform operands and one elected lane issues (a
+        // copy issued under a lane test, with operands that could differ by lane, takes about 100 ns).
+        const uint32_t usmem = __shfl_sync(0xffffffffu, smem_u32(smem), 0);
+        const bool issue = elect_one();
         bool ok = true;
         uint32_t it = 0, st = 0, parity = 1;  // stages so far; stage and phase of the ring
-        // the A rows of a stage: one copy of 128 rows, or 16-row copies of the rows that exist
-        auto load_a = [&](uint32_t to, int mt, int s, int copies) {
-            uint8_t* base = smem + (size_t)to * S::kStage;
-            if (MODE == kDense) {
-                if (lane == 0) tma_2d(smem_u32(base), &ta, s * 128, mt * kTileM, &s_full[to]);
-            } else if (lane < copies) {
-                tma_2d(smem_u32(base) + lane * 2048, &ta, s * 128, mt * kTileM + lane * 16, &s_full[to]);
+        // the A rows of a stage and their scales: all rows of the tile in one copy, or, of a tile of 128
+        // rows that is not full, 32 rows a copy
+        auto load_a = [&](uint32_t to_st, int mt, int s, int copies) {
+            const uint32_t base = usmem + to_st * kStage, bar = smem_u32(&s_full[to_st]);
+            if (TM < 128 || MODE == kDense || copies == 4) {
+                tma_2d(base, &ta, s * 128, mt * TM, bar);
+            } else {
+                for (int c = 0; c < copies; ++c) tma_2d(base + c * 4096, &tb, s * 128, mt * TM + c * 32, bar);
             }
-            if (lane == 0) bulk_g2s(base + S::kA + S::kB, p.sfa + ((int64_t)mt * p.kb + 2 * s) * 512, min(2, p.kb - 2 * s) * 512, &s_full[to]);
+            bulk_copy(base + oSfA, p.sfa + ((int64_t)mt * p.kb + 2 * s) * S::kSfaKg, min(2, p.kb - 2 * s) * S::kSfaKg, bar);
         };
         for (int64_t tile = blockIdx.x; ok && tile < tiles; tile += gridDim.x) {
             const int mt = (int)(tile / p.nt_count), nt = (int)(tile - (int64_t)mt * p.nt_count);
-            const int e = MODE == kDense ? 0 : p.mt_expert[mt];
-            const int copies = MODE == kDense ? 8 : (p.mt_rows[mt] + 15) >> 4;
-            const int sft = min(S::kSfTiles, nb128 - nt * NT / 128);
+            const int e = __shfl_sync(0xffffffffu, expert_of(mt), 0), rows = __shfl_sync(0xffffffffu, rows_of(mt), 0);
+            const int copies = MODE == kDense || TM < 128 ? 4 : (rows + 31) >> 5;  // quarters of a 128-row tile
+            const int sft = S::PANEL ? 0 : min(S::kSfTiles, nb128 - nt * NT / 128);
             const uint8_t* sfb = p.sfb + ((int64_t)e * nb128 + nt * NT / 128) * p.kb * 512;
+            const int nb64 = (p.N + 63) / 64, panels = min(NT / 64, nb64 - nt * (NT / 64));
+            const uint8_t* panel = p.panels + ((int64_t)e * nb64 + nt * (NT / 64)) * nstages * kPanel;
+            const int bbytes = MODE == kDense ? S::kB : panels * (S::PANEL ? kPanel : kPanelCodes);
             const bool early = MODE == kDown && it == 0;
             const int first = early ? min(STAGES, nstages) : 0;
             for (int s = 0; s < nstages; ++s, ++it) {
                 if (!warp_wait(&s_empty[st], parity, failed)) { ok = false; break; }
-                uint8_t* base = smem + (size_t)st * S::kStage;
-                const int sfn = min(2, p.kb - 2 * s) * 512;
-                if (lane == 0) {
-                    mbar_arrive_expect_tx(&s_full[st], copies * 2048 + S::kB + sfn * (1 + sft));
-                    tma_3d(smem_u32(base + S::kA), &tb, s * 128, nt * NT, e, &s_full[st]);
-                    for (int b = 0; b < sft; ++b)
-                        bulk_g2s(base + S::kA + S::kB + 1024 * (1 + b), sfb + ((int64_t)b * p.kb + 2 * s) * 512, sfn, &s_full[st]);
+                const uint32_t base = usmem + st * kStage, bar = smem_u32(&s_full[st]);
+                const int kgs = min(2, p.kb - 2 * s), sfn = kgs * 512;
+                if (issue) {
+                    mbar_arrive_expect_tx(&s_full[st], (WRITE_A ? 0 : copies * (S::kA / 4) + kgs * S::kSfaKg) + bbytes + sfn * sft);
+                    if (MODE == kDense) {
+                        tma_2d(base + oB, &tb, s * 128, nt * NT, bar);
+                    } else {
+#pragma unroll
+                        for (int b = 0; b < NT / 64; ++b)
+                            if (b < panels)
+                                bulk_copy(base + oB + b * kPanelCodes, panel + ((int64_t)b * nstages + s) * kPanel,
+                                          S::PANEL ? kPanel : kPanelCodes, bar);
+                    }
+#pragma unroll
+                    for (int b = 0; b < S::kSfTiles; ++b)
+                        if (b < sft) bulk_copy(base + oSfB + 1024 * b, sfb + ((int64_t)b * p.kb + 2 * s) * 512, sfn, bar);
+                    if (!WRITE_A && s >= first) load_a(st, mt, s, copies);
                 }
                 __syncwarp();
-                if (s >= first) {
-                    load_a(st, mt, s, copies);
-                } else if (s == first - 1) {
+                if (!WRITE_A && s < first && s == first - 1) {
                     asm volatile("griddepcontrol.wait;" ::: "memory");
-                    for (int a = 0; a < first; ++a) load_a(a, mt, a, copies);
+                    if (issue)
+                        for (int a = 0; a < first; ++a) load_a(a, mt, a, copies);
+                    __syncwarp();
                 }
-                __syncwarp();
                 if (++st == STAGES) {
                     st = 0;
                     parity ^= 1;
@@ -315,7 +462,7 @@ __global__ void __launch_bounds__(Shape<NT>::kThreads, Shape<NT>::kCtas)
         }
         if (MODE == kDown && it == 0) asm volatile("griddepcontrol.wait;" ::: "memory");
         // leave only when the copies have landed: a later owner of this shared memory must not be hit
-        if (lane == 0) {
+        if (issue) {
             for (uint32_t b = 0; b < STAGES && b < it; ++b) {
                 const uint32_t j = it - 1 - b;
                 bool in = false;
@@ -323,41 +470,50 @@ __global__ void __launch_bounds__(Shape<NT>::kThreads, Shape<NT>::kCtas)
                 if (!in) *failed = 1;
             }
         }
+        __syncwarp();
     } else if (warp == 1) {
         // The whole warp walks the loop, so that addresses and descriptors stay in uniform
         // registers, and one elected lane issues.
-        constexpr uint32_t idesc = idesc_mxf4(kTileM, NT);
+        constexpr uint32_t idesc = idesc_mxf4(128, NT);
         const uint32_t utmem = __shfl_sync(0xffffffffu, tmem, 0), usmem = __shfl_sync(0xffffffffu, smem_u32(smem), 0);
+        const uint32_t uabuf = __shfl_sync(0xffffffffu, smem_u32(abuf), 0);
         const bool issue = elect_one();
         uint32_t n = 0, st = 0, parity = 0;  // tiles so far; stage and phase of the ring
         bool ok = true;
         for (int64_t tile = blockIdx.x; ok && tile < tiles; tile += gridDim.x, ++n) {
             const uint32_t acc = n % S::kAcc, d = utmem + acc * NT;
             // half a scale tile (NT = 64): its rows' columns are 0-1 or 2-3 of the tile's four
-            const uint32_t half = NT == 64 ? (uint32_t)(tile % p.nt_count & 1) * 2 : 0;
+            const uint32_t half = NT == 64 && !S::PANEL ? (uint32_t)(tile % p.nt_count & 1) * 2 : 0;
             if (!warp_wait(&s_accempty[acc], (n / S::kAcc & 1) ^ 1, failed)) break;
+            if (WRITE_A && !warp_wait(&s_afull[n & 1], n >> 1 & 1, failed)) break;
             gemm::tc_fence_after();
             for (int s = 0; s < nstages; ++s) {
                 if (!warp_wait(&s_full[st], parity, failed)) { ok = false; break; }
                 gemm::tc_fence_after();
-                const uint32_t sa = usmem + st * S::kStage, sf = sa + S::kA + S::kB;
-                const uint64_t da = gemm::tc_desc_sw128(sa), db = gemm::tc_desc_sw128(sa + S::kA), ds = sf_desc(sf);
+                const uint32_t ring = usmem + st * kStage, buf = uabuf + (n & 1) * S::a_buffer(nstages);
+                const uint32_t sa = WRITE_A ? buf + s * S::kA : ring;
+                const uint32_t sfa = WRITE_A ? buf + nstages * S::kA + s * 2 * S::kSfaKg : ring + oSfA;
+                const uint64_t da = gemm::tc_desc_sw128(sa), db = gemm::tc_desc_sw128(ring + oB);
+                const uint64_t dsa = sf_desc(sfa), dsb = sf_desc(ring + oSfB);
                 const uint32_t tsa = utmem + kSfBase + st * S::kSfCols, tsb = tsa + 8;
+                constexpr int kColsB = S::PANEL ? 2 : 4 * S::kSfTiles;  // TMEM columns of B's scales per 128 elements
                 const int nkb = min(2, p.kb - 2 * s), nk = min(4, k64 - 4 * s);
                 if (issue) {
+                    if (S::PANEL) cp_scales(tsb, dsb);
 #pragma unroll
                     for (int i = 0; i < 2; ++i)
                         if (i < nkb) {
-                            cp_scales(tsa + 4 * i, ds + 32 * i);
+                            cp_scales(tsa + 4 * i, dsa + S::kSfaKg / 16 * i);
+                            if (!S::PANEL) {
 #pragma unroll
-                            for (int b = 0; b < S::kSfTiles; ++b)
-                                cp_scales(tsb + 4 * S::kSfTiles * i + 4 * b, ds + 64 + 64 * b + 32 * i);
+                                for (int b = 0; b < S::kSfTiles; ++b) cp_scales(tsb + kColsB * i + 4 * b, dsb + 64 * b + 32 * i);
+                            }
                         }
 #pragma unroll
                     for (int j = 0; j < 4; ++j)
                         if (j < nk)  // 64 elements are 32 bytes inside the swizzle atom
                             mma_mxf4(d, da + 2 * j, db + 2 * j, idesc | (uint32_t)(j & 1) * 2 << 4 | (uint32_t)(j & 1) * 2 << 29,
-                                     tsa + 4 * (j >> 1), tsb + 4 * S::kSfTiles * (j >> 1) + half, s > 0 || j > 0);
+                                     tsa + 4 * (j >> 1), tsb + kColsB * (j >> 1) + half, s > 0 || j > 0);
                     gemm::tc_commit(&s_empty[st]);
                 }
                 __syncwarp();
@@ -374,9 +530,57 @@ __global__ void __launch_bounds__(Shape<NT>::kThreads, Shape<NT>::kCtas)
             for (uint32_t w = 0; w < kSpinLimit && !mbar_try_wait(&s_done, 0); ++w) {}
         }
         __syncwarp();
+    } else if (WRITE_A && warp < 4) {
+        // The rows of each tile's piece, quantised for the whole depth into one of the two buffers while the
+        // MMAs read the other; a thread takes 8 elements, four loads in flight.  A buffer is free when the tile
+        // before the last has been read, i.e. its accumulators are full.
+        constexpr int kFly = 4;
+        const int t64 = tid - 64;
+        uint32_t n = 0;
+        for (int64_t tile = blockIdx.x; tile < tiles; tile += gridDim.x, ++n) {
+            const int mt = (int)(tile / p.nt_count);
+            if (n >= 2 && !warp_wait(&s_accfull[n & 1], (n - 2) >> 1 & 1, failed)) break;
+            uint8_t* codes = abuf + (n & 1) * S::a_buffer(nstages);
+            uint8_t* scales = codes + nstages * S::kA;
+            const int per = nstages * 32, units = route.rows[mt] * per;  // a multiple of 32: a warp is in or out as a whole
+            for (int u0 = t64; u0 - (t64 & 31) < units; u0 += 64 * kFly) {
+                uint4 q[kFly];
+#pragma unroll
+                for (int f = 0; f < kFly; ++f) {
+                    const int u = u0 + 64 * f, r = u / per, k = (u - r * per) * 8;
+                    q[f] = make_uint4(0u, 0u, 0u, 0u);
+                    if (u < units && k < p.K) {
+                        const int64_t t = route.pair[mt * 8 + r] / p.topk;
+                        q[f] = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.x) + t * p.K + k));
+                    }
+                }
+#pragma unroll
+                for (int f = 0; f < kFly; ++f) {
+                    const int u = u0 + 64 * f, r = u / per, i = u - r * per;  // element 8 i of row r
+                    if (u >= units) break;
+                    float v[8];
+                    const uint32_t w4[4] = {q[f].x, q[f].y, q[f].z, q[f].w};
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        v[2 * j] = scale_to_f32((uint16_t)(w4[j] & 0xffffu), p.act_bf16);
+                        v[2 * j + 1] = scale_to_f32((uint16_t)(w4[j] >> 16), p.act_bf16);
+                    }
+                    uint32_t sc;
+                    const uint32_t c = quant8(v, sc);
+                    const int st = i >> 5, piece = i >> 2 & 7;  // 16-byte piece of the stage's 128 bytes
+                    *reinterpret_cast<uint32_t*>(codes + st * S::kA + r * 128 + ((piece ^ r) << 4) + (i & 3) * 4) = c;
+                    if ((i & 3) == 0) scales[(st * 2 + (piece >> 2)) * S::kSfaKg + r * 16 + (piece & 3)] = (uint8_t)sc;
+                }
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&s_afull[n & 1]);
+        }
     } else if (warp >= 4) {
-        const int r = (warp & 3) * 32 + lane, c0 = ((warp - 4) >> 2) * S::kCols;
-        uint8_t* const staging = smem + STAGES * S::kStage + (warp - 4) * 2048;
+        const int r = TM == 128 ? (warp & 3) * 32 + lane : lane, c0 = TM == 128 ? ((warp - 4) >> 2) * S::kCols : 0;
+        const uint32_t quarter = TM == 128 ? (uint32_t)((warp & 3) * 32) : 0u;
+        static_assert(TM == 128 || S::kEpiWarps == 1, "a tile of up to 32 rows has one epilogue warp, on TMEM lanes 0-31");
+        uint8_t* const staging = smem + STAGES * kStage + (warp - 4) * 2048;  // wide tiles only: no tail
         // this lane's 64 bytes of the staging area, its four 16-byte pieces swizzled as the map says
         auto stage_row = [&](const uint32_t (&w)[16]) {
             asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");  // the last store has read the area (lane 0's)
@@ -392,54 +596,18 @@ __global__ void __launch_bounds__(Shape<NT>::kThreads, Shape<NT>::kCtas)
         for (int64_t tile = blockIdx.x; tile < tiles; tile += gridDim.x, ++n) {
             const int mt = (int)(tile / p.nt_count), nt = (int)(tile - (int64_t)mt * p.nt_count);
             const uint32_t acc = n % S::kAcc;
-            const int mrows = MODE == kDense ? p.M - mt * kTileM : p.mt_rows[mt];
+            const int mrows = rows_of(mt);
             if (!warp_wait(&s_accfull[acc], n / S::kAcc & 1, failed)) break;
             gemm::tc_fence_after();
             float v[S::kCols];
-            const bool any = (warp & 3) * 32 < mrows;  // rows of this warp's quarter exist
-            if (any) load_columns<S::kCols>(tmem + acc * NT + c0 + ((uint32_t)((warp & 3) * 32) << 16), v);
+            const bool any = (int)quarter < mrows;  // rows of this warp's quarter exist
+            if (any) load_columns<S::kCols>(tmem + acc * NT + c0 + (quarter << 16), v);
             gemm::tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(&s_accempty[acc]);
-            const int64_t row = (int64_t)mt * kTileM + r;
-            const int y0 = mt * kTileM + (warp & 3) * 32;
-            if (S::kStaging && MODE != kGateUp && any && (MODE == kDown || p.tma_out)) {
-#pragma unroll
-                for (int c = 0; c < S::kCols; c += 32) {
-                    const int n0 = nt * NT + c0 + c;
-                    if (n0 >= p.N) break;
-                    uint32_t w[16];
-                    if (p.out_dtype == MOE_F32) {
-#pragma unroll
-                        for (int h = 0; h < 2; ++h) {
-                            if (n0 + 16 * h >= p.N) break;
-#pragma unroll
-                            for (int j = 0; j < 16; ++j) w[j] = __float_as_uint(v[c + 16 * h + j]);
-                            stage_row(w);
-                            if (lane == 0) tma_store_2d(&to, smem_u32(staging), n0 + 16 * h, y0);
-                        }
-                        continue;
-                    }
-                    if (MODE == kDown) {
-                        const uint32_t e = part_exponent(v + c);
-                        const float k = part_scale(e);
-#pragma unroll
-                        for (int j = 0; j < 16; ++j)
-                            w[j] = (uint32_t)part_round(v[c + 2 * j], k) & 0xffffu | (uint32_t)part_round(v[c + 2 * j + 1], k) << 16;
-                        if (r < mrows) p.pexp[row * ((p.N + 31) >> 5) + (n0 >> 5)] = (uint8_t)e;
-                    } else {
-#pragma unroll
-                        for (int j = 0; j < 16; ++j)
-                            w[j] = p.out_dtype == MOE_BF16 ? pack16<MOE_BF16>(v[c + 2 * j], v[c + 2 * j + 1])
-                                                           : pack16<MOE_F16>(v[c + 2 * j], v[c + 2 * j + 1]);
-                    }
-                    stage_row(w);
-                    if (lane == 0) tma_store_2d(&to, smem_u32(staging), n0, y0);
-                }
-                continue;
-            }
-            if (r >= mrows) continue;
+            const int64_t row = (int64_t)mt * TM + r;
             if (MODE == kGateUp) {
+                if (r >= mrows) continue;
 #pragma unroll
                 for (int b = 0; b < S::kCols / 64; ++b) {
                     const int i0 = (nt * NT + c0) / 2 + b * 32;
@@ -461,23 +629,87 @@ __global__ void __launch_bounds__(Shape<NT>::kThreads, Shape<NT>::kCtas)
                         for (int j = 0; j < 4; ++j) q[w] |= cvt_e2m1x2(h[8 * w + 2 * j] * k, h[8 * w + 2 * j + 1] * k) << (8 * j);
                     }
                     *reinterpret_cast<uint4*>(p.hq + row * (p.I / 2) + i0 / 2) = make_uint4(q[0], q[1], q[2], q[3]);
-                    p.hs[tiled_at(row, i0 >> 5, p.hkb)] = (uint8_t)sc;
+                    uint8_t* hs = p.hs + (TM == 8 ? ((int64_t)mt * p.hkb + (i0 >> 7)) * 128 + r * 16 + (i0 >> 5 & 3) : tile_row_at(mt, r, i0 >> 5, p.hkb));
+                    hs[0] = (uint8_t)sc;
                     // the MMAs take K in steps of 64: the scale behind an odd last block must be a number
-                    if (i0 + 32 == p.I && (p.I & 32)) p.hs[tiled_at(row, (i0 >> 5) + 1, p.hkb)] = 0;
+                    if (i0 + 32 == p.I && (p.I & 32)) hs[1] = 0;
                 }
-            } else {
+                continue;
+            }
+            if (S::kStaging && any && (MODE == kDown || p.tma_out)) {
+                const int y0 = mt * TM + (int)quarter;
+#pragma unroll
+                for (int c = 0; c < S::kCols; c += 32) {
+                    const int n0 = nt * NT + c0 + c;
+                    if (n0 >= p.N) break;
+                    uint32_t w[16];
+                    if (p.out_dtype == MOE_F32) {
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            if (n0 + 16 * h >= p.N) break;
+#pragma unroll
+                            for (int j = 0; j < 16; ++j) w[j] = __float_as_uint(v[c + 16 * h + j]);
+                            stage_row(w);
+                            if (lane == 0) tma_store_2d(&to, smem_u32(staging), n0 + 16 * h, y0);
+                        }
+                        continue;
+                    }
+                    if (MODE == kDown) {
+                        const uint32_t e = part_exponent(v + c);
+                        const float k = part_scale(e);
+#pragma unroll
+                        for (int j = 0; j < 16; ++j)
+                            w[j] = ((uint32_t)part_round(v[c + 2 * j], k) & 0xffffu) | (uint32_t)part_round(v[c + 2 * j + 1], k) << 16;
+                        if (r < mrows) p.pexp[row * ((p.N + 31) >> 5) + (n0 >> 5)] = (uint8_t)e;
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < 16; ++j)
+                            w[j] = p.out_dtype == MOE_BF16 ? pack16<MOE_BF16>(v[c + 2 * j], v[c + 2 * j + 1])
+                                                           : pack16<MOE_F16>(v[c + 2 * j], v[c + 2 * j + 1]);
+                    }
+                    stage_row(w);
+                    if (lane == 0) tma_store_2d(&to, smem_u32(staging), n0, y0);
+                }
+                continue;
+            }
+            if (r < mrows) {
+                const int64_t to_row = FUSED ? (int64_t)route.pair[mt * 8 + r] : row;  // fused parts lie by pair
                 const int esz = MODE == kDown || p.out_dtype == MOE_F32 ? 4 : 2;
                 const bool vec = (int64_t)p.N * esz % 16 == 0;
 #pragma unroll
                 for (int c = 0; c < S::kCols; c += 32) {
                     const int n0 = nt * NT + c0 + c, left = min(32, p.N - n0);
                     if (left <= 0) break;
-                    if (MODE == kDown || p.out_dtype == MOE_F32) store_row<MOE_F32>(p.out, row * p.N + n0, v + c, left, vec);
-                    else if (p.out_dtype == MOE_BF16) store_row<MOE_BF16>(p.out, row * p.N + n0, v + c, left, vec);
-                    else store_row<MOE_F16>(p.out, row * p.N + n0, v + c, left, vec);
+                    if (MODE == kDown || p.out_dtype == MOE_F32) store_row<MOE_F32>(p.out, to_row * p.N + n0, v + c, left, vec);
+                    else if (p.out_dtype == MOE_BF16) store_row<MOE_BF16>(p.out, to_row * p.N + n0, v + c, left, vec);
+                    else store_row<MOE_F16>(p.out, to_row * p.N + n0, v + c, left, vec);
                 }
             }
+            if (FUSED && MODE == kDown) {
+                // the CTA that finishes a column tile's last part sums them
+                __syncwarp();
+                unsigned int done = 0;
+                if (lane == 0) {
+                    __threadfence();
+                    done = atomicAdd(p.cnt + nt, 1u);
+                    __threadfence();
+                }
+                done = __shfl_sync(0xffffffffu, done, 0);
+                if (done + 1 == (unsigned int)mt_count) {
+                    if (lane == 0) p.cnt[nt] = 0;
+                    if (p.y_dtype == MOE_F32) fused_combine<MOE_F32>(route, p, nt * NT);
+                    else if (p.y_dtype == MOE_BF16) fused_combine<MOE_BF16>(route, p, nt * NT);
+                    else fused_combine<MOE_F16>(route, p, nt * NT);
+                }
+                __syncwarp();
+            }
         }
+        if (FUSED && MODE == kDown && mt_count == 0)  // no pair is this engine's
+            for (int nt = blockIdx.x; nt < p.nt_count; nt += gridDim.x) {
+                if (p.y_dtype == MOE_F32) fused_combine<MOE_F32>(route, p, nt * NT);
+                else if (p.y_dtype == MOE_BF16) fused_combine<MOE_BF16>(route, p, nt * NT);
+                else fused_combine<MOE_F16>(route, p, nt * NT);
+            }
     }
     if (S::kStaging && warp >= 4 && lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
     __syncthreads();
@@ -491,7 +723,7 @@ __global__ void __launch_bounds__(Shape<NT>::kThreads, Shape<NT>::kCtas)
 }
 
 // ------------------------------------------------------------------ expert layer: tokens
-// Routed pairs in a stable order by expert, each expert's in tiles of 128 rows; the token rows
+// Routed pairs in a stable order by expert, each expert's in tiles of 32 or 128 rows; the token rows
 // quantised into the rows of their pairs.  A CTA takes a run of `tokens` tokens.  It needs, per
 // expert, the pairs before its run and the pairs in all: for short calls it counts all pairs
 // itself, for long ones the runs' counts come from mx_count_kernel.
@@ -501,6 +733,7 @@ struct PrepParams {
     const void* x;
     const int32_t* ids;
     int T, K, H, E, e_off, emap_n, tokens;
+    int tile_log2;  // rows of an m tile: 32 or 128
     const int32_t* emap;
     const int32_t* counts;  // [runs][E], or null: at most kPrepSelf pairs
     int32_t* mtiles;
@@ -580,7 +813,7 @@ __global__ void __launch_bounds__(kPrepThreads) mx_prep_kernel(const PrepParams 
             }
             if (!p.counts) total = run;
         }
-        const int nt = (total + kTileM - 1) / kTileM;
+        const int tile_rows = 1 << p.tile_log2, nt = (total + tile_rows - 1) >> p.tile_log2;
         int incl = nt;
         for (int o = 1; o < 32; o <<= 1) {
             const int v = __shfl_up_sync(0xffffffffu, incl, o);
@@ -596,11 +829,11 @@ __global__ void __launch_bounds__(kPrepThreads) mx_prep_kernel(const PrepParams 
         __syncthreads();
         const int tile = carry + incl - nt;
         if (e < E) {
-            first[e] = tile * kTileM;
+            first[e] = tile << p.tile_log2;
             if (blockIdx.x == 0)
                 for (int m = 0; m < nt; ++m) {
                     p.mt_expert[tile + m] = e;
-                    p.mt_rows[tile + m] = min(kTileM, total - m * kTileM);
+                    p.mt_rows[tile + m] = min(tile_rows, total - (m << p.tile_log2));
                 }
         }
         carry += all;
@@ -646,64 +879,69 @@ __global__ void __launch_bounds__(kPrepThreads) mx_prep_kernel(const PrepParams 
                 const int row = pos[t[f] * p.K + k];
                 if (row >= 0) {
                     reinterpret_cast<uint32_t*>(p.xq + (int64_t)row * (p.H / 2))[i[f]] = c;
-                    if (word) *reinterpret_cast<uint32_t*>(p.xs + tiled_at(row, i[f] >> 2, p.kb)) = w;
+                    if (word) *reinterpret_cast<uint32_t*>(p.xs + tile_row_at(row >> p.tile_log2, row & ((1 << p.tile_log2) - 1), i[f] >> 2, p.kb)) = w;
                 }
             }
         }
     }
 }
 
-// y[t] = sum over the token's pairs, in their order, of w * part[row]: a thread takes 8 columns and
-// fetches up to 8 parts at a time.
+// y[t] = sum over the token's pairs, in their order, of w * part[row].  A warp takes 256 columns of a
+// token, a lane 8 of them; lane k holds the k-th pair's row and weight, and 8 parts are in flight.
 template <int DT, bool PART16>
 __global__ void __launch_bounds__(256) mx_combine_kernel(const void* part, const uint8_t* pexp, const int32_t* ppos,
                                                          const float* tw, int T, int K, int H, void* y) {
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     constexpr int kFly = 8;
-    const int h8 = H >> 3, nb = H >> 5;
-    const int64_t total = (int64_t)T * h8;
-    for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < total; i += (int64_t)gridDim.x * blockDim.x) {
-        const int64_t t = i / h8;
-        const int n = (int)(i - t * h8) * 8;
+    const int lane = threadIdx.x & 31, chunks = (H + 255) >> 8, nb = H >> 5;
+    const int64_t total = (int64_t)T * chunks;
+    for (int64_t i = (blockIdx.x * (int64_t)blockDim.x + threadIdx.x) >> 5; i < total; i += (int64_t)gridDim.x * blockDim.x >> 5) {
+        const int64_t t = i / chunks;
+        const int n = ((int)(i - t * chunks) << 8) + lane * 8;
+        const bool in = n < H;
         float a[8] = {};
-        for (int k0 = 0; k0 < K; k0 += kFly) {
-            uint4 q[kFly][PART16 ? 1 : 2];
-            float w[kFly];
+        for (int k0 = 0; k0 < K; k0 += 32) {
+            const int mypos = k0 + lane < K ? __ldg(ppos + t * K + k0 + lane) : -1;
+            const float myw = k0 + lane < K ? __ldg(tw + t * K + k0 + lane) : 0.f;
+            for (int k1 = 0; k1 < min(32, K - k0); k1 += kFly) {
+                uint4 q[kFly][PART16 ? 1 : 2];
+                float w[kFly];
 #pragma unroll
-            for (int f = 0; f < kFly; ++f) {
-                const int pos = k0 + f < K ? __ldg(ppos + t * K + k0 + f) : -1;
-                w[f] = 0.f;
-                q[f][0] = make_uint4(0u, 0u, 0u, 0u);
-                if (!PART16) q[f][PART16 ? 0 : 1] = q[f][0];
-                if (pos < 0) continue;
-                w[f] = __ldg(tw + t * K + k0 + f);
-                if (PART16) {
-                    q[f][0] = __ldcg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(part) + (int64_t)pos * H + n));
-                    w[f] *= part_unscale(__ldcg(pexp + (int64_t)pos * nb + (n >> 5)));
-                } else {
-                    const uint4* src = reinterpret_cast<const uint4*>(static_cast<const float*>(part) + (int64_t)pos * H + n);
-                    q[f][0] = __ldcg(src);
-                    q[f][PART16 ? 0 : 1] = __ldcg(src + 1);
+                for (int f = 0; f < kFly; ++f) {
+                    const int pos = __shfl_sync(0xffffffffu, mypos, k1 + f);
+                    w[f] = pos >= 0 ? __shfl_sync(0xffffffffu, myw, k1 + f) : 0.f;
+                    q[f][0] = q[f][PART16 ? 0 : 1] = make_uint4(0u, 0u, 0u, 0u);
+                    if (pos < 0 || !in) continue;
+                    if (PART16) {
+                        q[f][0] = __ldcs(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(part) + (int64_t)pos * H + n));
+                        w[f] *= part_unscale(__ldcg(pexp + (int64_t)pos * nb + (n >> 5)));
+                    } else {
+                        const uint4* src = reinterpret_cast<const uint4*>(static_cast<const float*>(part) + (int64_t)pos * H + n);
+                        q[f][0] = __ldcs(src);
+                        q[f][PART16 ? 0 : 1] = __ldcs(src + 1);
+                    }
                 }
-            }
 #pragma unroll
-            for (int f = 0; f < kFly; ++f) {
-                const uint32_t* r = reinterpret_cast<const uint32_t*>(&q[f][0]);
+                for (int f = 0; f < kFly; ++f) {
+                    const uint32_t* r = reinterpret_cast<const uint32_t*>(&q[f][0]);
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const float v = PART16 ? (float)(int16_t)(r[j / 2] >> (16 * (j & 1))) : __uint_as_float(r[j % (PART16 ? 4 : 8)]);
-                    a[j] = fmaf(w[f], v, a[j]);
+                    for (int j = 0; j < 8; ++j) {
+                        const float v = PART16 ? (float)(int16_t)(r[j / 2] >> (16 * (j & 1))) : __uint_as_float(r[j % (PART16 ? 4 : 8)]);
+                        a[j] = fmaf(w[f], v, a[j]);
+                    }
                 }
             }
         }
+        if (!in) continue;
+        const int64_t at = (t * H + n) >> 3;
         if (DT == MOE_F32) {
-            float4* d = reinterpret_cast<float4*>(y) + 2 * i;
+            float4* d = reinterpret_cast<float4*>(y) + 2 * at;
             d[0] = make_float4(a[0], a[1], a[2], a[3]);
             d[1] = make_float4(a[4], a[5], a[6], a[7]);
         } else {
-            reinterpret_cast<uint4*>(y)[i] = make_uint4(pack16<DT>(a[0], a[1]), pack16<DT>(a[2], a[3]), pack16<DT>(a[4], a[5]),
-                                                        pack16<DT>(a[6], a[7]));
+            reinterpret_cast<uint4*>(y)[at] = make_uint4(pack16<DT>(a[0], a[1]), pack16<DT>(a[2], a[3]), pack16<DT>(a[4], a[5]),
+                                                         pack16<DT>(a[6], a[7]));
         }
     }
 }
