@@ -2310,10 +2310,10 @@ struct Buf {
 std::vector<Buf> engine_buffers(moe_engine* eng) {
     const int64_t E = eng->cfg.num_experts, H = eng->cfg.hidden_size, I = eng->cfg.intermediate_size;
     std::vector<Buf> v;
-    if (eng->mx) {  // gate_up codes and scale tiles, down codes and scale tiles
-        MxBuffer b[4];
+    if (eng->mx) {
+        MxBuffer b[kMxBuffers];
         mx_buffers(eng->mx, b);
-        for (uint32_t i = 0; i < 4; ++i) v.push_back({6 + i, b[i].ptr, b[i].bytes});
+        for (uint32_t i = 0; i < kMxBuffers; ++i) v.push_back({6 + i, b[i].ptr, b[i].bytes});
         return v;
     }
     v.push_back({1, &eng->gu, (size_t)E * I * eng->unit_bytes()});

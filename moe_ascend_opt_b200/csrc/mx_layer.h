@@ -9,7 +9,9 @@ namespace moe {
 
 struct MxLayer;
 
-// Device-resident weights of one engine: gate_up codes and scale tiles, down codes and scale tiles.
+// Device-resident weights of one engine: for gate_up, then for down, panels of codes and their scales in two
+// orders.
+constexpr int kMxBuffers = 6;
 struct MxBuffer {
     uint8_t** ptr;
     size_t bytes;
@@ -34,7 +36,7 @@ void mx_destroy(MxLayer* l);
 int mx_load(MxLayer* l, const uint8_t* w13_q, const uint8_t* w13_s, const uint8_t* w2_q, const uint8_t* w2_s, cudaStream_t st);
 int mx_quantize_store(MxLayer* l, int64_t expert, int32_t proj, const void* w, int32_t dtype, cudaStream_t st);
 int mx_export(MxLayer* l, int64_t expert, int32_t which, void* q_out, void* s_out);
-void mx_buffers(MxLayer* l, MxBuffer (&b)[4]);
+void mx_buffers(MxLayer* l, MxBuffer (&b)[kMxBuffers]);
 int mx_reserve(MxLayer* l, int64_t T, int64_t K);
 int mx_forward(MxLayer* l, const MxForward& f, cudaStream_t st);
 

@@ -115,14 +115,14 @@ using Fused = mx::Shape<64, 8, 8, 1, 2, true>;
 constexpr int kFusedStages = 32;  // depth of fused calls: their A buffers hold it whole
 
 template <int MODE, class S>
-int launch_gemm(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& to, mx::GemmParams& p, int64_t m_tiles, int sms,
+int launch_gemm(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& ta32, const CUtensorMap& to, mx::GemmParams& p, int64_t m_tiles, int sms,
                 bool pdl, cudaStream_t st) {
     auto fn = mx::mx_gemm_kernel<MODE, S>;
     constexpr bool WA = S::FUSED && MODE == mx::kGateUp;
     const int smem = S::smem(WA, (int)ceil_div(p.K, mx::kStageK));
     if (int rc = allow_smem(reinterpret_cast<const void*>(fn), S::smem(WA, kFusedStages))) return rc;
     p.nt_count = (int)ceil_div(p.N, S::NT);
-    return launch(fn, (unsigned)std::min<int64_t>(m_tiles * p.nt_count, sms * S::kCtas), S::kThreads, smem, pdl, st, ta, tb, to, p);
+    return launch(fn, (unsigned)std::min<int64_t>(m_tiles * p.nt_count, sms * S::kCtas), S::kThreads, smem, pdl, st, ta, tb, ta32, to, p);
 }
 
 bool dtype_ok(int32_t t) { return t == MOE_F16 || t == MOE_BF16 || t == MOE_F32; }
@@ -261,8 +261,8 @@ extern "C" int moe_mxfp4_matmul(const uint8_t* a, const uint8_t* a_scales, const
     p.tma_out = wide && N * esz % 16 == 0;
     if (p.tma_out)
         if (int rc = encode_out(&to, y, esz, N, M)) return rc;
-    return wide ? launch_gemm<mx::kDense, Wide>(ta, tb, to, p, p.mt_count, sms, false, st)
-                : launch_gemm<mx::kDense, Narrow>(ta, tb, to, p, p.mt_count, sms, false, st);
+    return wide ? launch_gemm<mx::kDense, Wide>(ta, tb, ta, to, p, p.mt_count, sms, false, st)
+                : launch_gemm<mx::kDense, Narrow>(ta, tb, ta, to, p, p.mt_count, sms, false, st);
 }
 
 // ------------------------------------------------------------------ expert layer
@@ -271,17 +271,21 @@ namespace moe {
 struct MxLayer {
     moe_config cfg{};
     int sms = 0;
-    int64_t kb1 = 0, kb2 = 0, nb1 = 0, nb2 = 0;  // scale tiles along K and N of gate_up (1) and down (2)
+    int64_t kb1 = 0, kb2 = 0;  // scale tiles along K of gate_up (1) and down (2)
     int64_t st1 = 0, st2 = 0, pn1 = 0, pn2 = 0;  // panels along K and N
-    // panels (codes and scales), and the scales again in tiles, which wide tiles read
-    uint8_t *q1 = nullptr, *s1 = nullptr, *q2 = nullptr, *s2 = nullptr;
+    // panels of codes, their scales in slim and in wide order; maps of 64 and of 256 rows
+    uint8_t *q1 = nullptr, *ss1 = nullptr, *sw1 = nullptr, *q2 = nullptr, *ss2 = nullptr, *sw2 = nullptr;
+    CUtensorMap t1[2]{}, t2[2]{};
     uint8_t* ws = nullptr;
     size_t ws_bytes = 0;
     std::vector<uint8_t*> retired;  // earlier workspaces: captured graphs may still hold them
     size_t q1_expert() const { return (size_t)pn1 * st1 * mx::kPanel; }
     size_t q2_expert() const { return (size_t)pn2 * st2 * mx::kPanel; }
-    size_t s1_bytes() const { return (size_t)cfg.num_experts * nb1 * kb1 * 512; }
-    size_t s2_bytes() const { return (size_t)cfg.num_experts * nb2 * kb2 * 512; }
+    // scales of an expert: slim [ceil(rows / 64)][stages][512], wide [panels][stages][2048]
+    size_t ss1_expert() const { return (size_t)(2 * cfg.intermediate_size / 64) * st1 * 512; }
+    size_t ss2_expert() const { return (size_t)((cfg.hidden_size + 63) / 64) * st2 * 512; }
+    size_t sw1_expert() const { return (size_t)pn1 * st1 * 2048; }
+    size_t sw2_expert() const { return (size_t)pn2 * st2 * 2048; }
 };
 
 namespace layer {
@@ -307,21 +311,21 @@ __global__ void mx_panel_codes_kernel(uint8_t* panels, uint8_t* codes, int64_t r
     }
 }
 
-// Scales [rows][nb] between the input contract and the layer's panels and tiles.
-__global__ void mx_panel_scales_kernel(uint8_t* panels, uint8_t* tiles, uint8_t* s, int64_t rows, int nb, int64_t stages, int64_t expert,
-                                       int64_t tiles_expert, int map, int64_t I, int to_panels) {
-    const int64_t n = rows * nb, kb = (nb + 3) >> 2, e = blockIdx.y;
-    panels += e * expert;
-    tiles += e * tiles_expert;
+// Scales [rows][nb] between the input contract and the layer's two orders.
+__global__ void mx_panel_scales_kernel(uint8_t* slim, uint8_t* wide, uint8_t* s, int64_t rows, int nb, int64_t stages, int64_t slim_expert,
+                                       int64_t wide_expert, int map, int64_t I, int to_panels) {
+    const int64_t n = rows * nb, e = blockIdx.y;
+    slim += e * slim_expert;
+    wide += e * wide_expert;
     s += e * n;
     for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (int64_t)gridDim.x * blockDim.x) {
         const int64_t r = i / nb, b = i - r * nb;
         uint8_t* v = s + source_row(r, map, I) * nb + b;
         if (to_panels) {
-            panels[mx::panel_scale_at(r, b, stages)] = *v;
-            tiles[mx::tiled_at(r, b, kb)] = *v;
+            slim[mx::slim_scale_at(r, b, stages)] = *v;
+            wide[mx::wide_scale_at(r, b, stages)] = *v;
         } else {
-            *v = tiles[mx::tiled_at(r, b, kb)];
+            *v = slim[mx::slim_scale_at(r, b, stages)];
         }
     }
 }
@@ -329,8 +333,8 @@ __global__ void mx_panel_scales_kernel(uint8_t* panels, uint8_t* tiles, uint8_t*
 // Online quantisation of rows [n][cols] to layer rows: row j goes to layer row
 // (j / 32) * 64 + 32 * half + j % 32 (gate_up, half 0 gate, 1 up) or j (down, half -1).
 template <int DT>
-__global__ void mx_store_rows_kernel(const void* w, int64_t n, int cols, int half, uint8_t* panels, uint8_t* tiles) {
-    const int64_t per = cols >> 3, total = n * per, kb = (cols + 127) >> 7, stages = (cols + 255) >> 8;
+__global__ void mx_store_rows_kernel(const void* w, int64_t n, int cols, int half, uint8_t* panels, uint8_t* slim, uint8_t* wide) {
+    const int64_t per = cols >> 3, total = n * per, stages = (cols + 255) >> 8;
     for (int64_t i0 = (int64_t)blockIdx.x * blockDim.x; i0 < total; i0 += (int64_t)gridDim.x * blockDim.x) {
         const int64_t i = i0 + threadIdx.x;
         float v[8] = {};
@@ -342,8 +346,8 @@ __global__ void mx_store_rows_kernel(const void* w, int64_t n, int cols, int hal
         const int64_t r = half < 0 ? j : (j >> 5) * 64 + 32 * half + (j & 31);
         *reinterpret_cast<uint32_t*>(panels + mx::panel_code_at(r, k * 4, stages)) = c;
         if ((i & 3) == 0) {
-            panels[mx::panel_scale_at(r, k >> 2, stages)] = (uint8_t)sc;
-            tiles[mx::tiled_at(r, k >> 2, kb)] = (uint8_t)sc;
+            slim[mx::slim_scale_at(r, k >> 2, stages)] = (uint8_t)sc;
+            wide[mx::wide_scale_at(r, k >> 2, stages)] = (uint8_t)sc;
         }
     }
 }
@@ -452,13 +456,13 @@ int forward_fused(MxLayer* l, const MxForward& f, const void* x, void* y, const 
     p.I = (int)I;
     mx::GemmParams g1 = p;
     g1.N = (int)(2 * I); g1.K = (int)H; g1.kb = (int)l->kb1;
-    g1.sfb = l->s1; g1.panels = l->q1; g1.hq = w.hq; g1.hs = w.hs; g1.hkb = (int)l->kb2;
-    if (int rc = launch_gemm<mx::kGateUp, Fused>(th, th, th, g1, w.mt, l->sms, f.pdl, st)) return rc;
+    g1.sfb = l->ss1; g1.hq = w.hq; g1.hs = w.hs; g1.hkb = (int)l->kb2;
+    if (int rc = launch_gemm<mx::kGateUp, Fused>(th, l->t1[0], th, th, g1, w.mt, l->sms, f.pdl, st)) return rc;
     mx::GemmParams g2 = p;
     g2.N = (int)H; g2.K = (int)I; g2.kb = (int)l->kb2;
-    g2.sfa = w.hs; g2.sfb = l->s2; g2.panels = l->q2; g2.out = w.part; g2.out_dtype = MOE_F32;
+    g2.sfa = w.hs; g2.sfb = l->ss2; g2.out = w.part; g2.out_dtype = MOE_F32;
     g2.y = y; g2.y_dtype = f.out_dtype; g2.cnt = f.cnt;
-    return launch_gemm<mx::kDown, Fused>(th, th, th, g2, w.mt, l->sms, f.pdl, st);
+    return launch_gemm<mx::kDown, Fused>(th, l->t2[0], th, th, g2, w.mt, l->sms, f.pdl, st);
 }
 
 int forward_slice(MxLayer* l, const MxForward& f, const void* x, void* y, const int32_t* ids, const float* tw, int64_t T,
@@ -482,7 +486,7 @@ int forward_slice(MxLayer* l, const MxForward& f, const void* x, void* y, const 
         r.counts = w.counts;
         if (int rc = launch(mx::mx_count_kernel, runs, mx::kPrepThreads, (size_t)E * 4, f.pdl, st, r, w.counts)) return rc;
     }
-    const size_t psmem = ((size_t)(mx::kPrepWarps + 1) * E + (self ? T : r.tokens) * f.K) * 4;
+    const size_t psmem = ((size_t)(mx::kPrepWarps + 1) * E + (self ? T * f.K : r.tokens * f.K + 2 * E)) * 4;
     auto prep = f.act_dtype == MOE_BF16 ? mx::mx_prep_kernel<MOE_BF16> : mx::mx_prep_kernel<MOE_F16>;
     if (int rc = allow_smem(reinterpret_cast<const void*>(prep), 128 * 1024)) return rc;
     if (int rc = launch(prep, runs, mx::kPrepThreads, psmem, f.pdl, st, r)) return rc;
@@ -500,20 +504,20 @@ int forward_slice(MxLayer* l, const MxForward& f, const void* x, void* y, const 
     p.I = (int)I;
     mx::GemmParams g1 = p;
     g1.N = (int)(2 * I); g1.K = (int)H; g1.kb = (int)l->kb1;
-    g1.sfa = w.xs; g1.sfb = l->s1; g1.panels = l->q1; g1.hq = w.hq; g1.hs = w.hs; g1.hkb = (int)l->kb2;
-    if (int rc = wide ? launch_gemm<mx::kGateUp, Wide>(tx, tx32, tx, g1, w.mt, l->sms, f.pdl, st)
-                      : launch_gemm<mx::kGateUp, Slim>(tx, tx, tx, g1, w.mt, l->sms, f.pdl, st))
+    g1.sfa = w.xs; g1.sfb = wide ? l->sw1 : l->ss1; g1.hq = w.hq; g1.hs = w.hs; g1.hkb = (int)l->kb2;
+    if (int rc = wide ? launch_gemm<mx::kGateUp, Wide>(tx, l->t1[1], tx32, tx, g1, w.mt, l->sms, f.pdl, st)
+                      : launch_gemm<mx::kGateUp, Slim>(tx, l->t1[0], tx, tx, g1, w.mt, l->sms, f.pdl, st))
         return rc;
     mx::GemmParams g2 = p;
     g2.N = (int)H; g2.K = (int)I; g2.kb = (int)l->kb2;
-    g2.sfa = w.hs; g2.sfb = l->s2; g2.panels = l->q2; g2.out = w.part; g2.pexp = w.pexp;
+    g2.sfa = w.hs; g2.sfb = wide ? l->sw2 : l->ss2; g2.out = w.part; g2.pexp = w.pexp;
     const bool part16 = wide && f.out_dtype != MOE_F32;
     g2.out_dtype = part16 ? MOE_F16 : MOE_F32;
     CUtensorMap tp = th;  // used by wide tiles
     if (wide)
         if (int rc = encode_out(&tp, w.part, part16 ? 2 : 4, H, w.mt * w.tile)) return rc;
-    if (int rc = wide ? launch_gemm<mx::kDown, Wide>(th, th32, tp, g2, w.mt, l->sms, f.pdl, st)
-                      : launch_gemm<mx::kDown, Slim>(th, th, tp, g2, w.mt, l->sms, f.pdl, st))
+    if (int rc = wide ? launch_gemm<mx::kDown, Wide>(th, l->t2[1], th32, tp, g2, w.mt, l->sms, f.pdl, st)
+                      : launch_gemm<mx::kDown, Slim>(th, l->t2[0], th, tp, g2, w.mt, l->sms, f.pdl, st))
         return rc;
     if (f.out_dtype == MOE_F32) return combine_launch<MOE_F32, false>(l, f, tw, y, w, T, st);
     if (f.out_dtype == MOE_BF16)
@@ -535,13 +539,16 @@ int mx_create(const moe_config& cfg, int num_sms, MxLayer** out) {
     const int64_t H = cfg.hidden_size, I = cfg.intermediate_size;
     l->kb1 = ceil_div(H, 128);
     l->kb2 = ceil_div(I, 128);
-    l->nb1 = ceil_div(2 * I, 128);
-    l->nb2 = ceil_div(H, 128);
     l->st1 = ceil_div(H, 256);
     l->st2 = ceil_div(I, 256);
-    l->pn1 = ceil_div(2 * I, 64);
-    l->pn2 = ceil_div(H, 64);
-    MxBuffer b[4];
+    l->pn1 = ceil_div(2 * I, mx::kPanelRows);
+    l->pn2 = ceil_div(H, mx::kPanelRows);
+    // the maps' row coordinates are 32-bit integers
+    if (cfg.num_experts * std::max(l->pn1 * l->st1, l->pn2 * l->st2) * mx::kPanelRows > (int64_t)1 << 31) {
+        mx_destroy(l);
+        return fail(MOE_ERR_INVALID, "MXFP4 weights too large for one engine");
+    }
+    MxBuffer b[kMxBuffers];
     mx_buffers(l, b);
     for (auto& x : b) {
         cudaError_t e = cudaMalloc(x.ptr, x.bytes);
@@ -552,33 +559,47 @@ int mx_create(const moe_config& cfg, int num_sms, MxLayer** out) {
             return fail(MOE_ERR_CUDA, std::string("MXFP4 weights: ") + cudaGetErrorString(e));
         }
     }
+    int rc = MOE_OK;
+    for (int w = 0; w < 2 && rc == MOE_OK; ++w) {
+        const int box = w ? Wide::NT : Slim::NT;
+        rc = encode(&l->t1[w], l->q1, 128, cfg.num_experts * l->pn1 * l->st1 * mx::kPanelRows, box);
+        if (rc == MOE_OK) rc = encode(&l->t2[w], l->q2, 128, cfg.num_experts * l->pn2 * l->st2 * mx::kPanelRows, box);
+    }
+    if (rc != MOE_OK) {
+        mx_destroy(l);
+        return rc;
+    }
     *out = l;
     return MOE_OK;
 }
 
 void mx_destroy(MxLayer* l) {
     if (!l) return;
-    for (uint8_t* p : {l->q1, l->s1, l->q2, l->s2, l->ws}) cudaFree(p);
+    for (uint8_t* p : {l->q1, l->ss1, l->sw1, l->q2, l->ss2, l->sw2, l->ws}) cudaFree(p);
     for (uint8_t* p : l->retired) cudaFree(p);
     delete l;
 }
 
-void mx_buffers(MxLayer* l, MxBuffer (&b)[4]) {
-    b[0] = {&l->q1, l->cfg.num_experts * l->q1_expert()};
-    b[1] = {&l->s1, l->s1_bytes()};
-    b[2] = {&l->q2, l->cfg.num_experts * l->q2_expert()};
-    b[3] = {&l->s2, l->s2_bytes()};
+void mx_buffers(MxLayer* l, MxBuffer (&b)[kMxBuffers]) {
+    const size_t E = l->cfg.num_experts;
+    b[0] = {&l->q1, E * l->q1_expert()};
+    b[1] = {&l->ss1, E * l->ss1_expert()};
+    b[2] = {&l->sw1, E * l->sw1_expert()};
+    b[3] = {&l->q2, E * l->q2_expert()};
+    b[4] = {&l->ss2, E * l->ss2_expert()};
+    b[5] = {&l->sw2, E * l->sw2_expert()};
 }
 
 int mx_load(MxLayer* l, const uint8_t* w13_q, const uint8_t* w13_s, const uint8_t* w2_q, const uint8_t* w2_s, cudaStream_t st) {
     const int64_t E = l->cfg.num_experts, H = l->cfg.hidden_size, I = l->cfg.intermediate_size;
     if (!aligned(w13_q, 16) || !aligned(w2_q, 16)) return fail(MOE_ERR_INVALID, "weight codes must be 16-byte aligned");
     const dim3 g(128, (unsigned)E);
-    const int64_t t1 = l->nb1 * l->kb1 * 512, t2 = l->nb2 * l->kb2 * 512;
     mx_panel_codes_kernel<<<g, 256, 0, st>>>(l->q1, const_cast<uint8_t*>(w13_q), 2 * I, H / 2, l->st1, l->q1_expert(), 1, I, 1);
     mx_panel_codes_kernel<<<g, 256, 0, st>>>(l->q2, const_cast<uint8_t*>(w2_q), H, I / 2, l->st2, l->q2_expert(), 0, I, 1);
-    mx_panel_scales_kernel<<<g, 256, 0, st>>>(l->q1, l->s1, const_cast<uint8_t*>(w13_s), 2 * I, (int)(H / 32), l->st1, l->q1_expert(), t1, 1, I, 1);
-    mx_panel_scales_kernel<<<g, 256, 0, st>>>(l->q2, l->s2, const_cast<uint8_t*>(w2_s), H, (int)(I / 32), l->st2, l->q2_expert(), t2, 0, I, 1);
+    mx_panel_scales_kernel<<<g, 256, 0, st>>>(l->ss1, l->sw1, const_cast<uint8_t*>(w13_s), 2 * I, (int)(H / 32), l->st1,
+                                              l->ss1_expert(), l->sw1_expert(), 1, I, 1);
+    mx_panel_scales_kernel<<<g, 256, 0, st>>>(l->ss2, l->sw2, const_cast<uint8_t*>(w2_s), H, (int)(I / 32), l->st2,
+                                              l->ss2_expert(), l->sw2_expert(), 0, I, 1);
     CUDA_TRY(cudaGetLastError());
     return MOE_OK;
 }
@@ -588,12 +609,13 @@ int mx_quantize_store(MxLayer* l, int64_t expert, int32_t proj, const void* w, i
     if (!aligned(w, 16)) return fail(MOE_ERR_INVALID, "weight must be 16-byte aligned");
     const int64_t n = proj == 2 ? H : I, cols = proj == 2 ? I : H;
     uint8_t* q = proj == 2 ? l->q2 + expert * l->q2_expert() : l->q1 + expert * l->q1_expert();
-    uint8_t* s = proj == 2 ? l->s2 + expert * l->nb2 * l->kb2 * 512 : l->s1 + expert * l->nb1 * l->kb1 * 512;
+    uint8_t* ss = proj == 2 ? l->ss2 + expert * l->ss2_expert() : l->ss1 + expert * l->ss1_expert();
+    uint8_t* sw = proj == 2 ? l->sw2 + expert * l->sw2_expert() : l->sw1 + expert * l->sw1_expert();
     const int half = proj == 2 ? -1 : proj;
     const unsigned grid = (unsigned)std::min<int64_t>(ceil_div(n * (cols / 8), 256), (int64_t)l->sms * 16);
-    if (dtype == MOE_F32) mx_store_rows_kernel<MOE_F32><<<grid, 256, 0, st>>>(w, n, (int)cols, half, q, s);
-    else if (dtype == MOE_BF16) mx_store_rows_kernel<MOE_BF16><<<grid, 256, 0, st>>>(w, n, (int)cols, half, q, s);
-    else mx_store_rows_kernel<MOE_F16><<<grid, 256, 0, st>>>(w, n, (int)cols, half, q, s);
+    if (dtype == MOE_F32) mx_store_rows_kernel<MOE_F32><<<grid, 256, 0, st>>>(w, n, (int)cols, half, q, ss, sw);
+    else if (dtype == MOE_BF16) mx_store_rows_kernel<MOE_BF16><<<grid, 256, 0, st>>>(w, n, (int)cols, half, q, ss, sw);
+    else mx_store_rows_kernel<MOE_F16><<<grid, 256, 0, st>>>(w, n, (int)cols, half, q, ss, sw);
     CUDA_TRY(cudaGetLastError());
     return MOE_OK;
 }
@@ -602,13 +624,13 @@ int mx_export(MxLayer* l, int64_t expert, int32_t which, void* q_out, void* s_ou
     const int64_t H = l->cfg.hidden_size, I = l->cfg.intermediate_size;
     const int64_t rows = which == 0 ? 2 * I : H, cols = which == 0 ? H : I, nb = cols / 32;
     uint8_t* q = which == 0 ? l->q1 + expert * l->q1_expert() : l->q2 + expert * l->q2_expert();
-    uint8_t* s = which == 0 ? l->s1 + expert * l->nb1 * l->kb1 * 512 : l->s2 + expert * l->nb2 * l->kb2 * 512;
+    uint8_t* s = which == 0 ? l->ss1 + expert * l->ss1_expert() : l->ss2 + expert * l->ss2_expert();
     uint8_t* d = nullptr;
     CUDA_TRY(cudaMalloc(&d, rows * (cols / 2) + rows * nb));
     uint8_t* ds = d + rows * (cols / 2);
     const int64_t stages = which == 0 ? l->st1 : l->st2;
     mx_panel_codes_kernel<<<128, 256>>>(q, d, rows, cols / 2, stages, 0, which == 0, I, 0);
-    mx_panel_scales_kernel<<<128, 256>>>(q, s, ds, rows, (int)nb, stages, 0, 0, which == 0, I, 0);
+    mx_panel_scales_kernel<<<128, 256>>>(s, nullptr, ds, rows, (int)nb, stages, 0, 0, which == 0, I, 0);
     cudaError_t e = cudaGetLastError();
     if (e == cudaSuccess) e = cudaMemcpy(q_out, d, rows * (cols / 2), cudaMemcpyDeviceToHost);
     if (e == cudaSuccess) e = cudaMemcpy(s_out, ds, rows * nb, cudaMemcpyDeviceToHost);

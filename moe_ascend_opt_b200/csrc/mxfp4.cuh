@@ -46,18 +46,22 @@ MOE_DEV int64_t tiled_at(int64_t row, int64_t block, int64_t kb) {
     return ((row >> 7) * kb + (block >> 2)) * 512 + (row & 31) * 16 + ((row >> 5) & 3) * 4 + (block & 3);
 }
 
-// Expert weights lie in panels of 64 rows x 256 elements (one stage of a product), so that a panel is one
-// contiguous copy whatever the matrix's row pitch: 64 x 128 bytes of codes, swizzled as the MMA reads them
-// (16-byte piece c of row r at c ^ (r % 8)), then 512 bytes of scales, 16 for each r % 32: the words (4
-// blocks) of rows r, r + 32 for the first 128 elements, then for the others.  [ceil(rows / 64)][stages]
-// panels; what lies past the matrix is zero.
-constexpr int kPanelCodes = 64 * 128, kPanel = kPanelCodes + 512;
+// Expert weights lie in panels of 256 rows x 256 elements (128 bytes), one stage of a wide product, so that
+// a stage is one contiguous copy whatever the matrix's row pitch; a slim product takes 64 rows of a
+// panel.  [ceil(rows / 256)][stages] panels; what lies past the matrix is zero.
+constexpr int kPanelRows = 256, kPanel = kPanelRows * 128;
 MOE_DEV int64_t panel_code_at(int64_t row, int64_t byte, int64_t stages) {
-    return ((row >> 6) * stages + (byte >> 7)) * kPanel + (row & 63) * 128 + (((byte >> 4 & 7) ^ (row & 7)) << 4) + (byte & 15);
+    return ((row >> 8) * stages + (byte >> 7)) * kPanel + (row & 255) * 128 + (byte & 127);
 }
-MOE_DEV int64_t panel_scale_at(int64_t row, int64_t block, int64_t stages) {
-    return ((row >> 6) * stages + (block >> 3)) * kPanel + kPanelCodes + (row & 31) * 16 + ((block >> 2 & 1) * 2 + (row >> 5 & 1)) * 4 +
-           (block & 3);
+// Their scales, in two orders of TMEM columns (words of 4 blocks for 32 rows).  Slim: 512 bytes for 64 rows of
+// a panel, rows 0-31 and 32-63 for the first 128 elements, then for the others.  Wide: 2048 bytes for a
+// panel, two scale tiles for rows 0-127, two for rows 128-255.
+MOE_DEV int64_t slim_scale_at(int64_t row, int64_t block, int64_t stages) {
+    return ((row >> 6) * stages + (block >> 3)) * 512 + (row & 31) * 16 + ((block >> 2 & 1) * 2 + (row >> 5 & 1)) * 4 + (block & 3);
+}
+MOE_DEV int64_t wide_scale_at(int64_t row, int64_t block, int64_t stages) {
+    return ((row >> 8) * stages + (block >> 3)) * 2048 + (row >> 7 & 1) * 1024 + (block >> 2 & 1) * 512 + (row & 31) * 16 +
+           (row >> 5 & 3) * 4 + (block & 3);
 }
 
 // tiled_at for row r (below 128) of scale tile row `tile`, which need not be full.

@@ -25,15 +25,14 @@ namespace mx {
 
 enum Mode { kDense = 0, kGateUp = 1, kDown = 2 };
 constexpr int kStageK = 256;
-constexpr int kFusedPairs = 64;  // routed pairs of the calls whose two kernels route for themselves
+constexpr int kFusedPairs = 16;  // routed pairs of the calls whose two kernels route for themselves
 
 struct GemmParams {
     int M, N, K;         // dense: rows of a; N rows of b (of one expert); depth
     int kb;              // scale tiles along K
     int nt_count, mt_count;
     const uint8_t* sfa;  // [m tiles][kb][512]
-    const uint8_t* sfb;  // [experts][ceil(N / 128)][kb][512]: dense and wide tiles
-    const uint8_t* panels;     // experts: [experts][ceil(N / 64)][stages][kPanel]
+    const uint8_t* sfb;  // dense [ceil(N / 128)][kb][512]; experts [experts][stage rows][stages], slim or wide order
     const int32_t* mtiles;     // experts: number of m tiles, then expert and rows of each
     const int32_t* mt_expert;
     const int32_t* mt_rows;
@@ -344,7 +343,8 @@ MOE_DEV void fused_combine(const FusedRoute& f, const GemmParams& p, int n0) {
 template <int MODE, class S>
 __global__ void __launch_bounds__(S::kThreads, S::kCtas)
     mx_gemm_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtensorMap tb,
-                   const __grid_constant__ CUtensorMap to, const __grid_constant__ GemmParams p) {
+                   const __grid_constant__ CUtensorMap ta32, const __grid_constant__ CUtensorMap to,
+                   const __grid_constant__ GemmParams p) {
     constexpr int NT = S::NT, TM = S::TM, STAGES = S::STAGES;
     constexpr bool FUSED = S::FUSED, WRITE_A = FUSED && MODE == kGateUp;  // A from the token rows, by warps 2 and 3
     constexpr int kSfBase = S::kAcc * NT;  // TMEM: the accumulators, then each stage's scales
@@ -412,7 +412,7 @@ __global__ void __launch_bounds__(S::kThreads, S::kCtas)
             if (TM < 128 || MODE == kDense || copies == 4) {
                 tma_2d(base, &ta, s * 128, mt * TM, bar);
             } else {
-                for (int c = 0; c < copies; ++c) tma_2d(base + c * 4096, &tb, s * 128, mt * TM + c * 32, bar);
+                for (int c = 0; c < copies; ++c) tma_2d(base + c * 4096, &ta32, s * 128, mt * TM + c * 32, bar);
             }
             bulk_copy(base + oSfA, p.sfa + ((int64_t)mt * p.kb + 2 * s) * S::kSfaKg, min(2, p.kb - 2 * s) * S::kSfaKg, bar);
         };
@@ -420,11 +420,14 @@ __global__ void __launch_bounds__(S::kThreads, S::kCtas)
             const int mt = (int)(tile / p.nt_count), nt = (int)(tile - (int64_t)mt * p.nt_count);
             const int e = __shfl_sync(0xffffffffu, expert_of(mt), 0), rows = __shfl_sync(0xffffffffu, rows_of(mt), 0);
             const int copies = MODE == kDense || TM < 128 ? 4 : (rows + 31) >> 5;  // quarters of a 128-row tile
-            const int sft = S::PANEL ? 0 : min(S::kSfTiles, nb128 - nt * NT / 128);
-            const uint8_t* sfb = p.sfb + ((int64_t)e * nb128 + nt * NT / 128) * p.kb * 512;
-            const int nb64 = (p.N + 63) / 64, panels = min(NT / 64, nb64 - nt * (NT / 64));
-            const uint8_t* panel = p.panels + ((int64_t)e * nb64 + nt * (NT / 64)) * nstages * kPanel;
-            const int bbytes = MODE == kDense ? S::kB : panels * (S::PANEL ? kPanel : kPanelCodes);
+            // B's scales: of an expert one contiguous piece a stage, of a dense product a piece per 128 rows
+            const int sft = MODE == kDense ? min(S::kSfTiles, nb128 - nt * NT / 128) : 1;
+            const int per_expert = (p.N + NT - 1) / NT;
+            const uint8_t* sfb = MODE == kDense ? p.sfb + (int64_t)(nt * NT / 128) * p.kb * 512
+                                                : p.sfb + ((int64_t)e * per_expert + nt) * nstages * S::kSfbBytes;
+            // B's rows: of an expert those of a panel, whose stages follow one another
+            const int64_t panel0 = ((int64_t)e * ((p.N + kPanelRows - 1) / kPanelRows) + nt * NT / kPanelRows) * nstages;
+            const int in_panel = nt * NT % kPanelRows;
             const bool early = MODE == kDown && it == 0;
             const int first = early ? min(STAGES, nstages) : 0;
             for (int s = 0; s < nstages; ++s, ++it) {
@@ -432,19 +435,17 @@ __global__ void __launch_bounds__(S::kThreads, S::kCtas)
                 const uint32_t base = usmem + st * kStage, bar = smem_u32(&s_full[st]);
                 const int kgs = min(2, p.kb - 2 * s), sfn = kgs * 512;
                 if (issue) {
-                    mbar_arrive_expect_tx(&s_full[st], (WRITE_A ? 0 : copies * (S::kA / 4) + kgs * S::kSfaKg) + bbytes + sfn * sft);
+                    const int sfbytes = MODE == kDense ? sfn * sft : S::kSfbBytes;
+                    mbar_arrive_expect_tx(&s_full[st], (WRITE_A ? 0 : copies * (S::kA / 4) + kgs * S::kSfaKg) + S::kB + sfbytes);
                     if (MODE == kDense) {
                         tma_2d(base + oB, &tb, s * 128, nt * NT, bar);
+#pragma unroll
+                        for (int b = 0; b < S::kSfTiles; ++b)
+                            if (b < sft) bulk_copy(base + oSfB + 1024 * b, sfb + ((int64_t)b * p.kb + 2 * s) * 512, sfn, bar);
                     } else {
-#pragma unroll
-                        for (int b = 0; b < NT / 64; ++b)
-                            if (b < panels)
-                                bulk_copy(base + oB + b * kPanelCodes, panel + ((int64_t)b * nstages + s) * kPanel,
-                                          S::PANEL ? kPanel : kPanelCodes, bar);
+                        tma_2d(base + oB, &tb, 0, (int)((panel0 + s) * kPanelRows) + in_panel, bar);
+                        bulk_copy(base + oSfB, sfb + (int64_t)s * S::kSfbBytes, S::kSfbBytes, bar);
                     }
-#pragma unroll
-                    for (int b = 0; b < S::kSfTiles; ++b)
-                        if (b < sft) bulk_copy(base + oSfB + 1024 * b, sfb + ((int64_t)b * p.kb + 2 * s) * 512, sfn, bar);
                     if (!WRITE_A && s >= first) load_a(st, mt, s, copies);
                 }
                 __syncwarp();
@@ -779,8 +780,20 @@ __global__ void __launch_bounds__(kPrepThreads) mx_prep_kernel(const PrepParams 
     const int share = ((a1 - a0 + kPrepWarps - 1) / kPrepWarps + 31) / 32 * 32;
     const int i0 = min(a1, a0 + warp * share), i1 = min(a1, i0 + share);
     int32_t* hist = psm + warp * E;
-    for (int i = i0 + lane; i - lane < i1; i += 32) {
-        const int e = i < i1 ? local_expert(p.ids[i], p.e_off, E, p.emap, p.emap_n, i, p.K) : -1;
+    constexpr int kIds = kPrepSelf / kPrepThreads;  // a lane's ids in short calls; longer runs reload
+    int mine[kIds];
+#pragma unroll
+    for (int f = 0; f < kIds; ++f) {
+        const int i = i0 + f * 32 + lane;
+        mine[f] = i < i1 ? p.ids[i] : -1;
+    }
+    for (int i = i0 + lane, f = 0; i - lane < i1; i += 32, ++f) {
+        int id = -1;
+#pragma unroll
+        for (int g = 0; g < kIds; ++g)
+            if (g == f) id = mine[g];
+        if (f >= kIds && i < i1) id = p.ids[i];
+        const int e = i < i1 ? local_expert(id, p.e_off, E, p.emap, p.emap_n, i, p.K) : -1;
         const unsigned peers = __match_any_sync(0xffffffffu, e);
         const int rank = __popc(peers & ((1u << lane) - 1u));
         const int before = e >= 0 ? hist[e] : 0;
@@ -790,6 +803,27 @@ __global__ void __launch_bounds__(kPrepThreads) mx_prep_kernel(const PrepParams 
         __syncwarp();
     }
     __syncthreads();
+    // the runs' counts, before this run and in all: groups of threads take every G-th run
+    int32_t* before = pos + (a1 - a0);  // [2][E]
+    if (p.counts) {
+        for (int e = tid; e < 2 * E; e += kPrepThreads) before[e] = 0;
+        __syncthreads();
+        const int pad = (E + 31) & ~31, G = max(1, kPrepThreads / pad), runs = gridDim.x;
+        for (int u = tid; u < G * pad || u < pad; u += kPrepThreads) {
+            const int g = u / pad, e = u - g * pad;
+            if (e >= E) continue;
+            int base = 0, total = 0;
+#pragma unroll 8
+            for (int c = g; c < runs; c += G) {
+                const int n = __ldcg(p.counts + (int64_t)c * E + e);
+                if (c < (int)blockIdx.x) base += n;
+                total += n;
+            }
+            atomicAdd(&before[e], base);
+            atomicAdd(&before[E + e], total);
+        }
+        __syncthreads();
+    }
     // per expert: rows before each warp's share, tiles; scan of the tiles over the experts
     int carry = 0;
     for (int e0 = 0; e0 < E; e0 += kPrepThreads) {
@@ -797,13 +831,8 @@ __global__ void __launch_bounds__(kPrepThreads) mx_prep_kernel(const PrepParams 
         int base = 0, total = 0;
         if (e < E) {
             if (p.counts) {
-                const int runs = gridDim.x;
-#pragma unroll 16
-                for (int c = 0; c < runs; ++c) {
-                    const int n = __ldcg(p.counts + (int64_t)c * E + e);
-                    if (c < (int)blockIdx.x) base += n;
-                    total += n;
-                }
+                base = before[e];
+                total = before[E + e];
             }
             int run = base;
             for (int w = 0; w < kPrepWarps; ++w) {
@@ -889,7 +918,7 @@ __global__ void __launch_bounds__(kPrepThreads) mx_prep_kernel(const PrepParams 
 // y[t] = sum over the token's pairs, in their order, of w * part[row].  A warp takes 256 columns of a
 // token, a lane 8 of them; lane k holds the k-th pair's row and weight, and 8 parts are in flight.
 template <int DT, bool PART16>
-__global__ void __launch_bounds__(256) mx_combine_kernel(const void* part, const uint8_t* pexp, const int32_t* ppos,
+__global__ void __launch_bounds__(256, 4) mx_combine_kernel(const void* part, const uint8_t* pexp, const int32_t* ppos,
                                                          const float* tw, int T, int K, int H, void* y) {
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
