@@ -108,6 +108,7 @@ int sm_count(int dev, int* out) {
 // wide tiles to fill the GPU.  Slim: 32 x 64, for experts with few rows each, where the weights' stream from
 // memory bounds the kernel and a small A leaves room for more of them in flight.
 using Wide = mx::Shape<256, 128, 4, 8, 1>;
+using WideDown = mx::Shape<256, 128, 3, 8, 1, false, 4>;  // down has few stages a tile and many stores
 using Narrow = mx::Shape<64, 128, 4, 4, 2>;
 using Slim = mx::Shape<64, 32, 7, 1, 2>;
 using Fused = mx::Shape<64, 8, 8, 1, 2, true>;
@@ -516,7 +517,7 @@ int forward_slice(MxLayer* l, const MxForward& f, const void* x, void* y, const 
     CUtensorMap tp = th;  // used by wide tiles
     if (wide)
         if (int rc = encode_out(&tp, w.part, part16 ? 2 : 4, H, w.mt * w.tile)) return rc;
-    if (int rc = wide ? launch_gemm<mx::kDown, Wide>(th, l->t2[1], th32, tp, g2, w.mt, l->sms, f.pdl, st)
+    if (int rc = wide ? launch_gemm<mx::kDown, WideDown>(th, l->t2[1], th32, tp, g2, w.mt, l->sms, f.pdl, st)
                       : launch_gemm<mx::kDown, Slim>(th, l->t2[0], th, tp, g2, w.mt, l->sms, f.pdl, st))
         return rc;
     if (f.out_dtype == MOE_F32) return combine_launch<MOE_F32, false>(l, f, tw, y, w, T, st);

@@ -58,11 +58,12 @@ struct GemmParams {
 
 // A kernel's shape: NT columns and TM rows of a tile (the MMA always takes 128 rows; of a tile of fewer it
 // reads whatever lies behind them in shared memory, and those lanes are never read back), STAGES of the
-// ring, EPI epilogue warps, CTAS per SM.
-template <int NT_, int TM_, int STAGES_, int EPI_, int CTAS_, bool FUSED_ = false>
+// ring, EPI epilogue warps, CTAS per SM, BUFS staging buffers of a wide tile's epilogue warp.
+template <int NT_, int TM_, int STAGES_, int EPI_, int CTAS_, bool FUSED_ = false, int BUFS_ = 1>
 struct Shape {
     static constexpr int NT = NT_, TM = TM_, STAGES = STAGES_, kEpiWarps = EPI_, kCtas = CTAS_;
     static constexpr bool FUSED = FUSED_;
+    static constexpr int BUFS = BUFS_;  // staging buffers of an epilogue warp
     static constexpr int kSfTiles = (NT + 127) / 128;  // scale tiles (128 rows) that cover a stage's B rows
     static constexpr bool PANEL = TM < 128;            // B and its scales by the panel, else scale tiles
     static constexpr int kA = TM * 128, kB = NT * 128;
@@ -80,7 +81,7 @@ struct Shape {
     static constexpr int kCols = TM < 128 ? NT : NT / (kEpiWarps / 4);  // columns of an epilogue thread
     static constexpr int kThreads = 128 + 32 * kEpiWarps;
     // wide tiles leave through shared memory: 32 rows x 64 bytes per epilogue warp, stored by TMA
-    static constexpr int kStaging = NT >= 256 ? kEpiWarps * 2048 : 0;
+    static constexpr int kStaging = NT >= 256 ? kEpiWarps * BUFS * 2048 : 0;
     // Dynamic shared memory for `stages` of depth.  The MMA's 128 rows of the last A stay inside, so do
     // the 512 bytes that a copy of its scales takes.
     __host__ __device__ static constexpr int smem(bool wa, int stages) {
@@ -228,12 +229,19 @@ MOE_DEV uint32_t part_exponent(const float* v) {
     for (int j = 0; j < 32; ++j) m = max(m, __float_as_uint(v[j]) & 0x7fffffffu);
     return m >> 23;
 }
-// 2^(141 - e) as a product of two normal factors: e from 0 (subnormal block) to 254
-MOE_DEV int part_round(float v, float k) { return __float2int_rn(fminf(fmaxf(v * k, -32767.f), 32767.f)); }
+// 2^(141 - e) and its inverse, e from 0 (a subnormal block counts as 15) to 254.
 MOE_DEV float part_scale(uint32_t e) { return __uint_as_float(min(268u - max(e, 15u), 253u) << 23); }
 MOE_DEV float part_unscale(uint32_t e) {
     return e == 255u ? __uint_as_float(0x7fc00000u) : __uint_as_float((max(e, 15u) - 14u) << 23);
 }
+// Rounded v k, |v k| < 2^15, as the low 16 bits of a float near 1.5 2^23 (conversions run at an eighth of
+// the rate of sums); two of them a word, and a half of the word back as a float.
+MOE_DEV uint32_t part_pack(float a, float b, float k) {
+    const uint32_t x = __float_as_uint(fminf(a * k, 32767.f) + 12582912.f), y = __float_as_uint(fminf(b * k, 32767.f) + 12582912.f);
+    return __byte_perm(x, y, 0x5410);
+}
+MOE_DEV float part_low(uint32_t flipped) { return __uint_as_float(__byte_perm(flipped, 0x4b00u, 0x5410)) - 8421376.f; }
+MOE_DEV float part_high(uint32_t flipped) { return __uint_as_float(__byte_perm(flipped, 0x4b00u, 0x5432)) - 8421376.f; }
 
 // SiLU(g) * u.  exp(-g) = 2^t (1 + r ln 2) with t = -g log2(e) rounded and r what the rounding and
 // the constant lost, so that a large |g| costs no accuracy; below g = -88 exp overflows.
@@ -581,10 +589,13 @@ __global__ void __launch_bounds__(S::kThreads, S::kCtas)
         const int r = TM == 128 ? (warp & 3) * 32 + lane : lane, c0 = TM == 128 ? ((warp - 4) >> 2) * S::kCols : 0;
         const uint32_t quarter = TM == 128 ? (uint32_t)((warp & 3) * 32) : 0u;
         static_assert(TM == 128 || S::kEpiWarps == 1, "a tile of up to 32 rows has one epilogue warp, on TMEM lanes 0-31");
-        uint8_t* const staging = smem + STAGES * kStage + (warp - 4) * 2048;  // wide tiles only: no tail
+        uint8_t* const staging0 = smem + STAGES * kStage + (warp - 4) * S::BUFS * 2048;  // wide tiles only: no tail
+        uint8_t* staging = staging0;
+        uint32_t stores = 0;
         // this lane's 64 bytes of the staging area, its four 16-byte pieces swizzled as the map says
         auto stage_row = [&](const uint32_t (&w)[16]) {
-            asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");  // the last store has read the area (lane 0's)
+            staging = staging0 + stores++ % S::BUFS * 2048;
+            asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(S::BUFS - 1) : "memory");  // lane 0's store from here is done
             __syncwarp();
 #pragma unroll
             for (int j = 0; j < 4; ++j)
@@ -659,8 +670,7 @@ __global__ void __launch_bounds__(S::kThreads, S::kCtas)
                         const uint32_t e = part_exponent(v + c);
                         const float k = part_scale(e);
 #pragma unroll
-                        for (int j = 0; j < 16; ++j)
-                            w[j] = ((uint32_t)part_round(v[c + 2 * j], k) & 0xffffu) | (uint32_t)part_round(v[c + 2 * j + 1], k) << 16;
+                        for (int j = 0; j < 16; ++j) w[j] = part_pack(v[c + 2 * j], v[c + 2 * j + 1], k);
                         if (r < mrows) p.pexp[row * ((p.N + 31) >> 5) + (n0 >> 5)] = (uint8_t)e;
                     } else {
 #pragma unroll
@@ -956,7 +966,9 @@ __global__ void __launch_bounds__(256, 4) mx_combine_kernel(const void* part, co
                     const uint32_t* r = reinterpret_cast<const uint32_t*>(&q[f][0]);
 #pragma unroll
                     for (int j = 0; j < 8; ++j) {
-                        const float v = PART16 ? (float)(int16_t)(r[j / 2] >> (16 * (j & 1))) : __uint_as_float(r[j % (PART16 ? 4 : 8)]);
+                        const uint32_t word = r[PART16 ? j / 2 : j];
+                        const float v = !PART16 ? __uint_as_float(word)
+                                                : (j & 1 ? part_high(word ^ 0x80008000u) : part_low(word ^ 0x80008000u));
                         a[j] = fmaf(w[f], v, a[j]);
                     }
                 }
