@@ -364,7 +364,8 @@ Plan plan_of(const MxLayer* l, int64_t T, int64_t K) {
 }
 
 struct Workspace {
-    int32_t *mtiles, *mt_expert, *mt_rows, *ppos, *counts;
+    int2* mt_list;
+    int32_t *ppos, *counts;
     uint8_t *xq, *xs, *hq, *hs;
     uint8_t *part, *pexp;  // fp32 [rows][H], or 16-bit integers and exponents [rows][H / 32]
     int64_t mt;  // bound of the number of m tiles
@@ -373,10 +374,10 @@ struct Workspace {
 };
 
 // Tokens of one CTA of the token kernel: runs of 256 pairs or more and at most 512 runs in long
-// calls (every CTA reads all runs' counts), one token or a share of 2 x 148 CTAs in short ones.
+// calls (every CTA reads all runs' counts), a 148th of a short call.
 int64_t prep_tokens(int64_t T, int64_t K) {
     const int64_t P = T * K;
-    if (P <= mx::kPrepSelf) return ceil_div(T, 296);
+    if (P <= mx::kPrepSelf) return ceil_div(T, 148);
     return std::max<int64_t>(ceil_div(256, K), ceil_div(T, 512));
 }
 
@@ -398,9 +399,7 @@ Workspace carve(const MxLayer* l, int64_t T, int64_t K, uint8_t* base) {
     w.part = take((size_t)(plan == kPlanFused ? P : rows) * H * 4);
     if (plan != kPlanFused) {
         w.pexp = take((size_t)rows * (H / 32));
-        w.mtiles = reinterpret_cast<int32_t*>(take(4));
-        w.mt_expert = reinterpret_cast<int32_t*>(take(w.mt * 4));
-        w.mt_rows = reinterpret_cast<int32_t*>(take(w.mt * 4));
+        w.mt_list = reinterpret_cast<int2*>(take(w.mt * 8));
         w.ppos = reinterpret_cast<int32_t*>(take(P * 4));
         w.counts = reinterpret_cast<int32_t*>(take(P > mx::kPrepSelf ? ceil_div(T, prep_tokens(T, K)) * l->cfg.num_experts * 4 : 0));
         w.xq = take(rows * (H / 2));
@@ -479,7 +478,7 @@ int forward_slice(MxLayer* l, const MxForward& f, const void* x, void* y, const 
     r.emap = f.emap; r.emap_n = f.emap_n;
     r.tokens = (int)prep_tokens(T, f.K);
     r.tile_log2 = wide ? 7 : 5;
-    r.mtiles = w.mtiles; r.mt_expert = w.mt_expert; r.mt_rows = w.mt_rows; r.ppos = w.ppos;
+    r.mt_list = w.mt_list; r.mt_bound = (int)w.mt; r.ppos = w.ppos;
     r.xq = w.xq; r.xs = w.xs; r.kb = (int)l->kb1;
     const unsigned runs = (unsigned)ceil_div(T, r.tokens);
     const bool self = T * f.K <= mx::kPrepSelf;
@@ -500,7 +499,7 @@ int forward_slice(MxLayer* l, const MxForward& f, const void* x, void* y, const 
         if (int rc = encode(&th32, w.hq, I / 2, w.mt * w.tile, 32)) return rc;
     }
     mx::GemmParams p{};
-    p.mtiles = w.mtiles; p.mt_expert = w.mt_expert; p.mt_rows = w.mt_rows;
+    p.mt_list = w.mt_list; p.mt_count = (int)w.mt;
     p.err = f.err;
     p.I = (int)I;
     mx::GemmParams g1 = p;

@@ -33,9 +33,7 @@ struct GemmParams {
     int nt_count, mt_count;
     const uint8_t* sfa;  // [m tiles][kb][512]
     const uint8_t* sfb;  // dense [ceil(N / 128)][kb][512]; experts [experts][stage rows][stages], slim or wide order
-    const int32_t* mtiles;     // experts: number of m tiles, then expert and rows of each
-    const int32_t* mt_expert;
-    const int32_t* mt_rows;
+    const int2* mt_list;       // experts: expert and rows of each m tile; rows 0 ends it
     void* out;           // dense [M][N] (out_dtype); down [m tile rows][N], fp32 or 16-bit parts
     int out_dtype;
     int tma_out;         // dense, wide tiles: store through the map (rows of a multiple of 16 bytes)
@@ -400,11 +398,13 @@ __global__ void __launch_bounds__(S::kThreads, S::kCtas)
     FusedRoute& route = reinterpret_cast<FusedRoute&>(s_route);  // an int where nothing is fused, never read
     if (FUSED) fused_route(route, p, S::kThreads);
 
-    const int mt_count = FUSED ? route.np : (MODE == kDense ? p.mt_count : p.mtiles[0]);
+    const int mt_count = FUSED ? route.np : p.mt_count;  // of an expert list its bound
     const int64_t tiles = (int64_t)mt_count * p.nt_count;
     const int nb128 = (p.N + 127) / 128;
-    auto expert_of = [&](int mt) { return FUSED ? route.piece_e[mt] : (MODE == kDense ? 0 : p.mt_expert[mt]); };
-    auto rows_of = [&](int mt) { return FUSED ? route.rows[mt] : (MODE == kDense ? min(TM, p.M - mt * TM) : p.mt_rows[mt]); };
+    auto tile_of = [&](int mt) {  // expert, rows; no rows: past the list's end
+        if (FUSED) return make_int2(route.piece_e[mt], route.rows[mt]);
+        return MODE == kDense ? make_int2(0, min(TM, p.M - mt * TM)) : __ldcg(p.mt_list + mt);
+    };
 
     if (warp == 0) {
         // As for the MMAs: the warp walks the loop with uniform operands and one elected lane issues (a
@@ -426,7 +426,9 @@ __global__ void __launch_bounds__(S::kThreads, S::kCtas)
         };
         for (int64_t tile = blockIdx.x; ok && tile < tiles; tile += gridDim.x) {
             const int mt = (int)(tile / p.nt_count), nt = (int)(tile - (int64_t)mt * p.nt_count);
-            const int e = __shfl_sync(0xffffffffu, expert_of(mt), 0), rows = __shfl_sync(0xffffffffu, rows_of(mt), 0);
+            const int2 of = tile_of(mt);
+            const int e = __shfl_sync(0xffffffffu, of.x, 0), rows = __shfl_sync(0xffffffffu, of.y, 0);
+            if (rows == 0) break;
             const int copies = MODE == kDense || TM < 128 ? 4 : (rows + 31) >> 5;  // quarters of a 128-row tile
             // B's scales: of an expert one contiguous piece a stage, of a dense product a piece per 128 rows
             const int sft = MODE == kDense ? min(S::kSfTiles, nb128 - nt * NT / 128) : 1;
@@ -491,6 +493,7 @@ __global__ void __launch_bounds__(S::kThreads, S::kCtas)
         bool ok = true;
         for (int64_t tile = blockIdx.x; ok && tile < tiles; tile += gridDim.x, ++n) {
             const uint32_t acc = n % S::kAcc, d = utmem + acc * NT;
+            if (MODE != kDense && !FUSED && __shfl_sync(0xffffffffu, tile_of((int)(tile / p.nt_count)).y, 0) == 0) break;
             // half a scale tile (NT = 64): its rows' columns are 0-1 or 2-3 of the tile's four
             const uint32_t half = NT == 64 && !S::PANEL ? (uint32_t)(tile % p.nt_count & 1) * 2 : 0;
             if (!warp_wait(&s_accempty[acc], (n / S::kAcc & 1) ^ 1, failed)) break;
@@ -608,7 +611,8 @@ __global__ void __launch_bounds__(S::kThreads, S::kCtas)
         for (int64_t tile = blockIdx.x; tile < tiles; tile += gridDim.x, ++n) {
             const int mt = (int)(tile / p.nt_count), nt = (int)(tile - (int64_t)mt * p.nt_count);
             const uint32_t acc = n % S::kAcc;
-            const int mrows = rows_of(mt);
+            const int mrows = tile_of(mt).y;
+            if (mrows == 0) break;
             if (!warp_wait(&s_accfull[acc], n / S::kAcc & 1, failed)) break;
             gemm::tc_fence_after();
             float v[S::kCols];
@@ -747,9 +751,8 @@ struct PrepParams {
     int tile_log2;  // rows of an m tile: 32 or 128
     const int32_t* emap;
     const int32_t* counts;  // [runs][E], or null: at most kPrepSelf pairs
-    int32_t* mtiles;
-    int32_t* mt_expert;
-    int32_t* mt_rows;
+    int2* mt_list;  // expert and rows of each m tile, then rows 0 up to the bound
+    int mt_bound;
     int32_t* ppos;  // row of each pair, -1 for pairs of other engines
     uint8_t* xq;    // [rows][H / 2]
     uint8_t* xs;    // scale tiles, kb along H
@@ -870,14 +873,12 @@ __global__ void __launch_bounds__(kPrepThreads) mx_prep_kernel(const PrepParams 
         if (e < E) {
             first[e] = tile << p.tile_log2;
             if (blockIdx.x == 0)
-                for (int m = 0; m < nt; ++m) {
-                    p.mt_expert[tile + m] = e;
-                    p.mt_rows[tile + m] = min(tile_rows, total - (m << p.tile_log2));
-                }
+                for (int m = 0; m < nt; ++m) p.mt_list[tile + m] = make_int2(e, min(tile_rows, total - (m << p.tile_log2)));
         }
         carry += all;
     }
-    if (blockIdx.x == 0 && tid == 0) p.mtiles[0] = carry;
+    if (blockIdx.x == 0)
+        for (int m = carry + tid; m < p.mt_bound; m += kPrepThreads) p.mt_list[m] = make_int2(0, 0);
     __syncthreads();
     for (int i = i0 + lane; i < i1; i += 32) {
         const int v = pos[i - a0], e = v & 1023;
@@ -886,40 +887,44 @@ __global__ void __launch_bounds__(kPrepThreads) mx_prep_kernel(const PrepParams 
     __syncthreads();
     pos += t0 * p.K - a0;  // the run's own pairs
     for (int i = tid; i < (t1 - t0) * p.K; i += kPrepThreads) p.ppos[t0 * p.K + i] = pos[i];
-    const int n = p.H >> 3, nb = p.H >> 5, n16 = (n + 15) & ~15;  // a scale word's 16 threads stay together
-    const int units = (t1 - t0) * n16;
-    constexpr int kFly = 4;  // loads in flight of a thread
-    for (int u0 = 0; u0 < units; u0 += kFly * kPrepThreads) {
+    // A warp takes up to 8 chunks of 256 elements of a token, all loads in flight, a lane 8 elements of each;
+    // then for every pair of the token its row's codes and, by two lanes, the chunks' scale words.
+    constexpr int kFly = 8;
+    const int chunks = (p.H + 255) >> 8, nb = p.H >> 5, ntok = t1 - t0;
+    const int group = max(1, min(kFly, ntok * chunks / kPrepWarps)), groups = (chunks + group - 1) / group;
+    for (int item = warp; item < ntok * groups; item += kPrepWarps) {
+        const int t = item / groups, c0 = (item - t * groups) * group, c1 = min(chunks, c0 + group);
         float v[kFly][8];
-        int t[kFly], i[kFly];
 #pragma unroll
         for (int f = 0; f < kFly; ++f) {
-            const int u = u0 + f * kPrepThreads + tid;
-            t[f] = u / n16;
-            i[f] = u < units ? u - t[f] * n16 : n;
 #pragma unroll
             for (int j = 0; j < 8; ++j) v[f][j] = 0.f;
-            if (i[f] < n) load8<DT>(p.x, (int64_t)(t0 + t[f]) * p.H + i[f] * 8, v[f]);
+            const int i = (c0 + f) * 256 + lane * 8;
+            if (c0 + f < c1 && i < p.H) load8<DT>(p.x, (int64_t)(t0 + t) * p.H + i, v[f]);
         }
+        uint32_t code[kFly], word[kFly];
 #pragma unroll
         for (int f = 0; f < kFly; ++f) {
+            if (c0 + f >= c1) break;
             uint32_t sc;
-            const uint32_t c = quant8(v[f], sc);
-            uint32_t w = sc;
-            w |= __shfl_down_sync(0xffffffffu, sc, 4, 16) << 8;
-            w |= __shfl_down_sync(0xffffffffu, sc, 8, 16) << 16;
-            w |= __shfl_down_sync(0xffffffffu, sc, 12, 16) << 24;
-            if (i[f] >= n) continue;
-            const int left = nb - (i[f] >> 2);
-            if (left < 4) w &= (1u << (8 * left)) - 1u;
-            const bool word = (i[f] & 15) == 0;
-#pragma unroll 8
-            for (int k = 0; k < p.K; ++k) {
-                const int row = pos[t[f] * p.K + k];
-                if (row >= 0) {
-                    reinterpret_cast<uint32_t*>(p.xq + (int64_t)row * (p.H / 2))[i[f]] = c;
-                    if (word) *reinterpret_cast<uint32_t*>(p.xs + tile_row_at(row >> p.tile_log2, row & ((1 << p.tile_log2) - 1), i[f] >> 2, p.kb)) = w;
-                }
+            code[f] = quant8(v[f], sc);
+            word[f] = sc;  // lanes 0 and 16: the scales of 16 neighbouring lanes' four blocks
+            word[f] |= __shfl_down_sync(0xffffffffu, sc, 4, 16) << 8;
+            word[f] |= __shfl_down_sync(0xffffffffu, sc, 8, 16) << 16;
+            word[f] |= __shfl_down_sync(0xffffffffu, sc, 12, 16) << 24;
+            const int left = nb - ((c0 + f) * 8 + (lane >> 4) * 4);
+            if (left < 4) word[f] &= left > 0 ? (1u << (8 * left)) - 1u : 0u;
+        }
+        for (int k = 0; k < p.K; ++k) {
+            const int row = pos[t * p.K + k];
+            if (row < 0) continue;
+            uint32_t* to = reinterpret_cast<uint32_t*>(p.xq + (int64_t)row * (p.H / 2)) + c0 * 32 + lane;
+            uint8_t* sc = p.xs + tile_row_at(row >> p.tile_log2, row & ((1 << p.tile_log2) - 1), c0 * 8 + (lane >> 4) * 4, p.kb);
+#pragma unroll
+            for (int f = 0; f < kFly; ++f) {
+                if (c0 + f >= c1) break;
+                if ((c0 + f) * 256 + lane * 8 < p.H) to[f * 32] = code[f];
+                if ((lane & 15) == 0 && (c0 + f) * 2 + (lane >> 4) < p.kb) *reinterpret_cast<uint32_t*>(sc + f * 1024) = word[f];
             }
         }
     }
@@ -928,7 +933,7 @@ __global__ void __launch_bounds__(kPrepThreads) mx_prep_kernel(const PrepParams 
 // y[t] = sum over the token's pairs, in their order, of w * part[row].  A warp takes 256 columns of a
 // token, a lane 8 of them; lane k holds the k-th pair's row and weight, and 8 parts are in flight.
 template <int DT, bool PART16>
-__global__ void __launch_bounds__(256, 4) mx_combine_kernel(const void* part, const uint8_t* pexp, const int32_t* ppos,
+__global__ void __launch_bounds__(256, PART16 ? 3 : 2) mx_combine_kernel(const void* part, const uint8_t* pexp, const int32_t* ppos,
                                                          const float* tw, int T, int K, int H, void* y) {
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -939,26 +944,38 @@ __global__ void __launch_bounds__(256, 4) mx_combine_kernel(const void* part, co
         const int64_t t = i / chunks;
         const int n = ((int)(i - t * chunks) << 8) + lane * 8;
         const bool in = n < H;
+        const int at8 = in ? n : 0;
         float a[8] = {};
         for (int k0 = 0; k0 < K; k0 += 32) {
             const int mypos = k0 + lane < K ? __ldg(ppos + t * K + k0 + lane) : -1;
             const float myw = k0 + lane < K ? __ldg(tw + t * K + k0 + lane) : 0.f;
             for (int k1 = 0; k1 < min(32, K - k0); k1 += kFly) {
+                // no branch stands between the loads: of an absent pair row 0 is read, and weighs nothing
                 uint4 q[kFly][PART16 ? 1 : 2];
+                int pos[kFly];
+                uint32_t e[kFly];
                 float w[kFly];
 #pragma unroll
                 for (int f = 0; f < kFly; ++f) {
-                    const int pos = __shfl_sync(0xffffffffu, mypos, k1 + f);
-                    w[f] = pos >= 0 ? __shfl_sync(0xffffffffu, myw, k1 + f) : 0.f;
-                    q[f][0] = q[f][PART16 ? 0 : 1] = make_uint4(0u, 0u, 0u, 0u);
-                    if (pos < 0 || !in) continue;
+                    pos[f] = __shfl_sync(0xffffffffu, mypos, k1 + f);
+                    const int64_t row = max(pos[f], 0);
                     if (PART16) {
-                        q[f][0] = __ldcs(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(part) + (int64_t)pos * H + n));
-                        w[f] *= part_unscale(__ldcg(pexp + (int64_t)pos * nb + (n >> 5)));
+                        q[f][0] = __ldcs(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(part) + row * H + at8));
+                        e[f] = __ldcg(pexp + row * nb + (at8 >> 5));
                     } else {
-                        const uint4* src = reinterpret_cast<const uint4*>(static_cast<const float*>(part) + (int64_t)pos * H + n);
+                        const uint4* src = reinterpret_cast<const uint4*>(static_cast<const float*>(part) + row * H + at8);
                         q[f][0] = __ldcs(src);
                         q[f][PART16 ? 0 : 1] = __ldcs(src + 1);
+                        e[f] = 0;
+                    }
+                }
+#pragma unroll
+                for (int f = 0; f < kFly; ++f) {
+                    w[f] = __shfl_sync(0xffffffffu, myw, k1 + f);
+                    if (PART16) w[f] *= part_unscale(e[f]);
+                    if (pos[f] < 0) {
+                        w[f] = 0.f;
+                        q[f][0] = q[f][PART16 ? 0 : 1] = make_uint4(0u, 0u, 0u, 0u);
                     }
                 }
 #pragma unroll
