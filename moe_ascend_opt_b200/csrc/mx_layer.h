@@ -9,9 +9,8 @@ namespace moe {
 
 struct MxLayer;
 
-// Device-resident weights of one engine: for gate_up, then for down, panels of codes and their scales in two
-// orders.
-constexpr int kMxBuffers = 6;
+// Device-resident weights of one engine: for gate_up, then for down, panels of codes and their scales.
+constexpr int kMxBuffers = 4;
 struct MxBuffer {
     uint8_t** ptr;
     size_t bytes;

@@ -103,15 +103,18 @@ int sm_count(int dev, int* out) {
     return MOE_OK;
 }
 
-// Kernel shapes.  Wide: 128 x 256 tiles, a CTA per SM, for many rows (the tiles' loads from L2 bound
-// it, which fall with the tile's width).  Narrow: 128 x 64, two CTAs per SM, for dense products of too few
-// wide tiles to fill the GPU.  Slim: 32 x 64, for experts with few rows each, where the weights' stream from
-// memory bounds the kernel and a small A leaves room for more of them in flight.
-using Wide = mx::Shape<256, 128, 4, 8, 1>;
-using WideDown = mx::Shape<256, 128, 3, 8, 1, false, 4>;  // down has few stages a tile and many stores
-using Narrow = mx::Shape<64, 128, 4, 4, 2>;
-using Slim = mx::Shape<64, 32, 7, 1, 2>;
-using Fused = mx::Shape<64, 8, 8, 1, 2, true>;
+// Kernel shapes.  Wide: 128 x 256 tiles, for many rows (the tiles' loads from L2 bound it, which fall with
+// the tile's width); down has few stages a tile and many stores.  Narrow: 128 x 64, two CTAs per SM, for
+// dense products of too few wide tiles to fill the GPU.  Slim: 32 x 128, for experts with few rows each, where
+// the weights' stream from memory bounds the kernel: an MMA of 64 columns takes as long as one of 128, and two
+// CTAs with 32 x 64 tiles were held up by them.  Fused: 8 x 128, and small enough for a CTA of each
+// kernel on an SM, so that down's first weights arrive while gate_up runs.
+using Wide = mx::Shape<256, 128, 4, 8, 1, 1>;
+using WideDown = mx::Shape<256, 128, 3, 8, 1, 1, false, 4>;
+using Narrow = mx::Shape<64, 128, 4, 4, 2, 2>;
+using Slim = mx::Shape<128, 32, 9, 1, 1, 2>;
+using FusedUp = mx::Shape<128, 8, 6, 1, 1, 1, true>;
+using FusedDown = mx::Shape<128, 8, 4, 1, 1, 1, true>;
 
 constexpr int kFusedStages = 32;  // depth of fused calls: their A buffers hold it whole
 
@@ -274,19 +277,16 @@ struct MxLayer {
     int sms = 0;
     int64_t kb1 = 0, kb2 = 0;  // scale tiles along K of gate_up (1) and down (2)
     int64_t st1 = 0, st2 = 0, pn1 = 0, pn2 = 0;  // panels along K and N
-    // panels of codes, their scales in slim and in wide order; maps of 64 and of 256 rows
-    uint8_t *q1 = nullptr, *ss1 = nullptr, *sw1 = nullptr, *q2 = nullptr, *ss2 = nullptr, *sw2 = nullptr;
+    // panels of codes and their scales; maps of 128 and of 256 rows
+    uint8_t *q1 = nullptr, *s1 = nullptr, *q2 = nullptr, *s2 = nullptr;
     CUtensorMap t1[2]{}, t2[2]{};
     uint8_t* ws = nullptr;
     size_t ws_bytes = 0;
     std::vector<uint8_t*> retired;  // earlier workspaces: captured graphs may still hold them
     size_t q1_expert() const { return (size_t)pn1 * st1 * mx::kPanel; }
     size_t q2_expert() const { return (size_t)pn2 * st2 * mx::kPanel; }
-    // scales of an expert: slim [ceil(rows / 64)][stages][512], wide [panels][stages][2048]
-    size_t ss1_expert() const { return (size_t)(2 * cfg.intermediate_size / 64) * st1 * 512; }
-    size_t ss2_expert() const { return (size_t)((cfg.hidden_size + 63) / 64) * st2 * 512; }
-    size_t sw1_expert() const { return (size_t)pn1 * st1 * 2048; }
-    size_t sw2_expert() const { return (size_t)pn2 * st2 * 2048; }
+    size_t s1_expert() const { return (size_t)pn1 * st1 * mx::kPanelScales; }
+    size_t s2_expert() const { return (size_t)pn2 * st2 * mx::kPanelScales; }
 };
 
 namespace layer {
@@ -312,29 +312,25 @@ __global__ void mx_panel_codes_kernel(uint8_t* panels, uint8_t* codes, int64_t r
     }
 }
 
-// Scales [rows][nb] between the input contract and the layer's two orders.
-__global__ void mx_panel_scales_kernel(uint8_t* slim, uint8_t* wide, uint8_t* s, int64_t rows, int nb, int64_t stages, int64_t slim_expert,
-                                       int64_t wide_expert, int map, int64_t I, int to_panels) {
+// Scales [rows][nb] between the input contract and the panels'.
+__global__ void mx_panel_scales_kernel(uint8_t* scales, uint8_t* s, int64_t rows, int nb, int64_t stages, int64_t expert, int map,
+                                       int64_t I, int to_panels) {
     const int64_t n = rows * nb, e = blockIdx.y;
-    slim += e * slim_expert;
-    wide += e * wide_expert;
+    scales += e * expert;
     s += e * n;
     for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (int64_t)gridDim.x * blockDim.x) {
         const int64_t r = i / nb, b = i - r * nb;
+        uint8_t* p = scales + mx::panel_scale_at(r, b, stages);
         uint8_t* v = s + source_row(r, map, I) * nb + b;
-        if (to_panels) {
-            slim[mx::slim_scale_at(r, b, stages)] = *v;
-            wide[mx::wide_scale_at(r, b, stages)] = *v;
-        } else {
-            *v = slim[mx::slim_scale_at(r, b, stages)];
-        }
+        if (to_panels) *p = *v;
+        else *v = *p;
     }
 }
 
 // Online quantisation of rows [n][cols] to layer rows: row j goes to layer row
 // (j / 32) * 64 + 32 * half + j % 32 (gate_up, half 0 gate, 1 up) or j (down, half -1).
 template <int DT>
-__global__ void mx_store_rows_kernel(const void* w, int64_t n, int cols, int half, uint8_t* panels, uint8_t* slim, uint8_t* wide) {
+__global__ void mx_store_rows_kernel(const void* w, int64_t n, int cols, int half, uint8_t* panels, uint8_t* scales) {
     const int64_t per = cols >> 3, total = n * per, stages = (cols + 255) >> 8;
     for (int64_t i0 = (int64_t)blockIdx.x * blockDim.x; i0 < total; i0 += (int64_t)gridDim.x * blockDim.x) {
         const int64_t i = i0 + threadIdx.x;
@@ -346,10 +342,7 @@ __global__ void mx_store_rows_kernel(const void* w, int64_t n, int cols, int hal
         const int64_t j = i / per, k = i - j * per;
         const int64_t r = half < 0 ? j : (j >> 5) * 64 + 32 * half + (j & 31);
         *reinterpret_cast<uint32_t*>(panels + mx::panel_code_at(r, k * 4, stages)) = c;
-        if ((i & 3) == 0) {
-            slim[mx::slim_scale_at(r, k >> 2, stages)] = (uint8_t)sc;
-            wide[mx::wide_scale_at(r, k >> 2, stages)] = (uint8_t)sc;
-        }
+        if ((i & 3) == 0) scales[mx::panel_scale_at(r, k >> 2, stages)] = (uint8_t)sc;
     }
 }
 
@@ -385,7 +378,7 @@ Workspace carve(const MxLayer* l, int64_t T, int64_t K, uint8_t* base) {
     Workspace w{};
     const int64_t P = T * K, H = l->cfg.hidden_size, I = l->cfg.intermediate_size;
     const Plan plan = plan_of(l, T, K);
-    w.tile = plan == kPlanWide ? 128 : (plan == kPlanFused ? Fused::TM : Slim::TM);
+    w.tile = plan == kPlanWide ? 128 : (plan == kPlanFused ? FusedUp::TM : Slim::TM);
     w.mt = plan == kPlanFused ? P : P / w.tile + std::min(P, l->cfg.num_experts);
     const int64_t rows = w.mt * w.tile;
     size_t off = 0;
@@ -456,13 +449,13 @@ int forward_fused(MxLayer* l, const MxForward& f, const void* x, void* y, const 
     p.I = (int)I;
     mx::GemmParams g1 = p;
     g1.N = (int)(2 * I); g1.K = (int)H; g1.kb = (int)l->kb1;
-    g1.sfb = l->ss1; g1.hq = w.hq; g1.hs = w.hs; g1.hkb = (int)l->kb2;
-    if (int rc = launch_gemm<mx::kGateUp, Fused>(th, l->t1[0], th, th, g1, w.mt, l->sms, f.pdl, st)) return rc;
+    g1.sfb = l->s1; g1.hq = w.hq; g1.hs = w.hs; g1.hkb = (int)l->kb2;
+    if (int rc = launch_gemm<mx::kGateUp, FusedUp>(th, l->t1[0], th, th, g1, w.mt, l->sms, f.pdl, st)) return rc;
     mx::GemmParams g2 = p;
     g2.N = (int)H; g2.K = (int)I; g2.kb = (int)l->kb2;
-    g2.sfa = w.hs; g2.sfb = l->ss2; g2.out = w.part; g2.out_dtype = MOE_F32;
+    g2.sfa = w.hs; g2.sfb = l->s2; g2.out = w.part; g2.out_dtype = MOE_F32;
     g2.y = y; g2.y_dtype = f.out_dtype; g2.cnt = f.cnt;
-    return launch_gemm<mx::kDown, Fused>(th, l->t2[0], th, th, g2, w.mt, l->sms, f.pdl, st);
+    return launch_gemm<mx::kDown, FusedDown>(th, l->t2[0], th, th, g2, w.mt, l->sms, f.pdl, st);
 }
 
 int forward_slice(MxLayer* l, const MxForward& f, const void* x, void* y, const int32_t* ids, const float* tw, int64_t T,
@@ -504,13 +497,13 @@ int forward_slice(MxLayer* l, const MxForward& f, const void* x, void* y, const 
     p.I = (int)I;
     mx::GemmParams g1 = p;
     g1.N = (int)(2 * I); g1.K = (int)H; g1.kb = (int)l->kb1;
-    g1.sfa = w.xs; g1.sfb = wide ? l->sw1 : l->ss1; g1.hq = w.hq; g1.hs = w.hs; g1.hkb = (int)l->kb2;
+    g1.sfa = w.xs; g1.sfb = l->s1; g1.hq = w.hq; g1.hs = w.hs; g1.hkb = (int)l->kb2;
     if (int rc = wide ? launch_gemm<mx::kGateUp, Wide>(tx, l->t1[1], tx32, tx, g1, w.mt, l->sms, f.pdl, st)
                       : launch_gemm<mx::kGateUp, Slim>(tx, l->t1[0], tx, tx, g1, w.mt, l->sms, f.pdl, st))
         return rc;
     mx::GemmParams g2 = p;
     g2.N = (int)H; g2.K = (int)I; g2.kb = (int)l->kb2;
-    g2.sfa = w.hs; g2.sfb = wide ? l->sw2 : l->ss2; g2.out = w.part; g2.pexp = w.pexp;
+    g2.sfa = w.hs; g2.sfb = l->s2; g2.out = w.part; g2.pexp = w.pexp;
     const bool part16 = wide && f.out_dtype != MOE_F32;
     g2.out_dtype = part16 ? MOE_F16 : MOE_F32;
     CUtensorMap tp = th;  // used by wide tiles
@@ -575,7 +568,7 @@ int mx_create(const moe_config& cfg, int num_sms, MxLayer** out) {
 
 void mx_destroy(MxLayer* l) {
     if (!l) return;
-    for (uint8_t* p : {l->q1, l->ss1, l->sw1, l->q2, l->ss2, l->sw2, l->ws}) cudaFree(p);
+    for (uint8_t* p : {l->q1, l->s1, l->q2, l->s2, l->ws}) cudaFree(p);
     for (uint8_t* p : l->retired) cudaFree(p);
     delete l;
 }
@@ -583,11 +576,9 @@ void mx_destroy(MxLayer* l) {
 void mx_buffers(MxLayer* l, MxBuffer (&b)[kMxBuffers]) {
     const size_t E = l->cfg.num_experts;
     b[0] = {&l->q1, E * l->q1_expert()};
-    b[1] = {&l->ss1, E * l->ss1_expert()};
-    b[2] = {&l->sw1, E * l->sw1_expert()};
-    b[3] = {&l->q2, E * l->q2_expert()};
-    b[4] = {&l->ss2, E * l->ss2_expert()};
-    b[5] = {&l->sw2, E * l->sw2_expert()};
+    b[1] = {&l->s1, E * l->s1_expert()};
+    b[2] = {&l->q2, E * l->q2_expert()};
+    b[3] = {&l->s2, E * l->s2_expert()};
 }
 
 int mx_load(MxLayer* l, const uint8_t* w13_q, const uint8_t* w13_s, const uint8_t* w2_q, const uint8_t* w2_s, cudaStream_t st) {
@@ -596,10 +587,8 @@ int mx_load(MxLayer* l, const uint8_t* w13_q, const uint8_t* w13_s, const uint8_
     const dim3 g(128, (unsigned)E);
     mx_panel_codes_kernel<<<g, 256, 0, st>>>(l->q1, const_cast<uint8_t*>(w13_q), 2 * I, H / 2, l->st1, l->q1_expert(), 1, I, 1);
     mx_panel_codes_kernel<<<g, 256, 0, st>>>(l->q2, const_cast<uint8_t*>(w2_q), H, I / 2, l->st2, l->q2_expert(), 0, I, 1);
-    mx_panel_scales_kernel<<<g, 256, 0, st>>>(l->ss1, l->sw1, const_cast<uint8_t*>(w13_s), 2 * I, (int)(H / 32), l->st1,
-                                              l->ss1_expert(), l->sw1_expert(), 1, I, 1);
-    mx_panel_scales_kernel<<<g, 256, 0, st>>>(l->ss2, l->sw2, const_cast<uint8_t*>(w2_s), H, (int)(I / 32), l->st2,
-                                              l->ss2_expert(), l->sw2_expert(), 0, I, 1);
+    mx_panel_scales_kernel<<<g, 256, 0, st>>>(l->s1, const_cast<uint8_t*>(w13_s), 2 * I, (int)(H / 32), l->st1, l->s1_expert(), 1, I, 1);
+    mx_panel_scales_kernel<<<g, 256, 0, st>>>(l->s2, const_cast<uint8_t*>(w2_s), H, (int)(I / 32), l->st2, l->s2_expert(), 0, I, 1);
     CUDA_TRY(cudaGetLastError());
     return MOE_OK;
 }
@@ -609,13 +598,12 @@ int mx_quantize_store(MxLayer* l, int64_t expert, int32_t proj, const void* w, i
     if (!aligned(w, 16)) return fail(MOE_ERR_INVALID, "weight must be 16-byte aligned");
     const int64_t n = proj == 2 ? H : I, cols = proj == 2 ? I : H;
     uint8_t* q = proj == 2 ? l->q2 + expert * l->q2_expert() : l->q1 + expert * l->q1_expert();
-    uint8_t* ss = proj == 2 ? l->ss2 + expert * l->ss2_expert() : l->ss1 + expert * l->ss1_expert();
-    uint8_t* sw = proj == 2 ? l->sw2 + expert * l->sw2_expert() : l->sw1 + expert * l->sw1_expert();
+    uint8_t* s = proj == 2 ? l->s2 + expert * l->s2_expert() : l->s1 + expert * l->s1_expert();
     const int half = proj == 2 ? -1 : proj;
     const unsigned grid = (unsigned)std::min<int64_t>(ceil_div(n * (cols / 8), 256), (int64_t)l->sms * 16);
-    if (dtype == MOE_F32) mx_store_rows_kernel<MOE_F32><<<grid, 256, 0, st>>>(w, n, (int)cols, half, q, ss, sw);
-    else if (dtype == MOE_BF16) mx_store_rows_kernel<MOE_BF16><<<grid, 256, 0, st>>>(w, n, (int)cols, half, q, ss, sw);
-    else mx_store_rows_kernel<MOE_F16><<<grid, 256, 0, st>>>(w, n, (int)cols, half, q, ss, sw);
+    if (dtype == MOE_F32) mx_store_rows_kernel<MOE_F32><<<grid, 256, 0, st>>>(w, n, (int)cols, half, q, s);
+    else if (dtype == MOE_BF16) mx_store_rows_kernel<MOE_BF16><<<grid, 256, 0, st>>>(w, n, (int)cols, half, q, s);
+    else mx_store_rows_kernel<MOE_F16><<<grid, 256, 0, st>>>(w, n, (int)cols, half, q, s);
     CUDA_TRY(cudaGetLastError());
     return MOE_OK;
 }
@@ -624,13 +612,13 @@ int mx_export(MxLayer* l, int64_t expert, int32_t which, void* q_out, void* s_ou
     const int64_t H = l->cfg.hidden_size, I = l->cfg.intermediate_size;
     const int64_t rows = which == 0 ? 2 * I : H, cols = which == 0 ? H : I, nb = cols / 32;
     uint8_t* q = which == 0 ? l->q1 + expert * l->q1_expert() : l->q2 + expert * l->q2_expert();
-    uint8_t* s = which == 0 ? l->ss1 + expert * l->ss1_expert() : l->ss2 + expert * l->ss2_expert();
+    uint8_t* s = which == 0 ? l->s1 + expert * l->s1_expert() : l->s2 + expert * l->s2_expert();
     uint8_t* d = nullptr;
     CUDA_TRY(cudaMalloc(&d, rows * (cols / 2) + rows * nb));
     uint8_t* ds = d + rows * (cols / 2);
     const int64_t stages = which == 0 ? l->st1 : l->st2;
     mx_panel_codes_kernel<<<128, 256>>>(q, d, rows, cols / 2, stages, 0, which == 0, I, 0);
-    mx_panel_scales_kernel<<<128, 256>>>(s, nullptr, ds, rows, (int)nb, stages, 0, 0, which == 0, I, 0);
+    mx_panel_scales_kernel<<<128, 256>>>(s, ds, rows, (int)nb, stages, 0, which == 0, I, 0);
     cudaError_t e = cudaGetLastError();
     if (e == cudaSuccess) e = cudaMemcpy(q_out, d, rows * (cols / 2), cudaMemcpyDeviceToHost);
     if (e == cudaSuccess) e = cudaMemcpy(s_out, ds, rows * nb, cudaMemcpyDeviceToHost);

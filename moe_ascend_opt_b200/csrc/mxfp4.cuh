@@ -47,20 +47,15 @@ MOE_DEV int64_t tiled_at(int64_t row, int64_t block, int64_t kb) {
 }
 
 // Expert weights lie in panels of 256 rows x 256 elements (128 bytes), one stage of a wide product, so that
-// a stage is one contiguous copy whatever the matrix's row pitch; a slim product takes 64 rows of a
-// panel.  [ceil(rows / 256)][stages] panels; what lies past the matrix is zero.
-constexpr int kPanelRows = 256, kPanel = kPanelRows * 128;
+// a stage is one contiguous copy whatever the matrix's row pitch; a slim product takes 128 rows of a
+// panel.  [ceil(rows / 256)][stages] panels; what lies past the matrix is zero.  Their scales: 2048 bytes a
+// panel, two scale tiles (256 elements) for rows 0-127, two for rows 128-255.
+constexpr int kPanelRows = 256, kPanel = kPanelRows * 128, kPanelScales = 2048;
 MOE_DEV int64_t panel_code_at(int64_t row, int64_t byte, int64_t stages) {
     return ((row >> 8) * stages + (byte >> 7)) * kPanel + (row & 255) * 128 + (byte & 127);
 }
-// Their scales, in two orders of TMEM columns (words of 4 blocks for 32 rows).  Slim: 512 bytes for 64 rows of
-// a panel, rows 0-31 and 32-63 for the first 128 elements, then for the others.  Wide: 2048 bytes for a
-// panel, two scale tiles for rows 0-127, two for rows 128-255.
-MOE_DEV int64_t slim_scale_at(int64_t row, int64_t block, int64_t stages) {
-    return ((row >> 6) * stages + (block >> 3)) * 512 + (row & 31) * 16 + ((block >> 2 & 1) * 2 + (row >> 5 & 1)) * 4 + (block & 3);
-}
-MOE_DEV int64_t wide_scale_at(int64_t row, int64_t block, int64_t stages) {
-    return ((row >> 8) * stages + (block >> 3)) * 2048 + (row >> 7 & 1) * 1024 + (block >> 2 & 1) * 512 + (row & 31) * 16 +
+MOE_DEV int64_t panel_scale_at(int64_t row, int64_t block, int64_t stages) {
+    return ((row >> 8) * stages + (block >> 3)) * kPanelScales + (row >> 7 & 1) * 1024 + (block >> 2 & 1) * 512 + (row & 31) * 16 +
            (row >> 5 & 3) * 4 + (block & 3);
 }
 

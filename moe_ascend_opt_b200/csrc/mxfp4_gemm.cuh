@@ -32,7 +32,7 @@ struct GemmParams {
     int kb;              // scale tiles along K
     int nt_count, mt_count;
     const uint8_t* sfa;  // [m tiles][kb][512]
-    const uint8_t* sfb;  // dense [ceil(N / 128)][kb][512]; experts [experts][stage rows][stages], slim or wide order
+    const uint8_t* sfb;  // dense [ceil(N / 128)][kb][512]; experts [experts][ceil(N / 256)][stages][kPanelScales]
     const int2* mt_list;       // experts: expert and rows of each m tile; rows 0 ends it
     void* out;           // dense [M][N] (out_dtype); down [m tile rows][N], fp32 or 16-bit parts
     int out_dtype;
@@ -56,17 +56,16 @@ struct GemmParams {
 
 // A kernel's shape: NT columns and TM rows of a tile (the MMA always takes 128 rows; of a tile of fewer it
 // reads whatever lies behind them in shared memory, and those lanes are never read back), STAGES of the
-// ring, EPI epilogue warps, CTAS per SM, BUFS staging buffers of a wide tile's epilogue warp.
-template <int NT_, int TM_, int STAGES_, int EPI_, int CTAS_, bool FUSED_ = false, int BUFS_ = 1>
+// ring, EPI epilogue warps, CTAS per SM, ACC accumulators, BUFS staging buffers of a wide tile's epilogue warp.
+template <int NT_, int TM_, int STAGES_, int EPI_, int CTAS_, int ACC_, bool FUSED_ = false, int BUFS_ = 1>
 struct Shape {
     static constexpr int NT = NT_, TM = TM_, STAGES = STAGES_, kEpiWarps = EPI_, kCtas = CTAS_;
     static constexpr bool FUSED = FUSED_;
     static constexpr int BUFS = BUFS_;  // staging buffers of an epilogue warp
     static constexpr int kSfTiles = (NT + 127) / 128;  // scale tiles (128 rows) that cover a stage's B rows
-    static constexpr bool PANEL = TM < 128;            // B and its scales by the panel, else scale tiles
     static constexpr int kA = TM * 128, kB = NT * 128;
     static constexpr int kSfaKg = TM == 8 ? 128 : 512;  // scales of A for 128 elements: those of 8 rows, or a tile
-    static constexpr int kSfbBytes = PANEL ? 512 : 1024 * kSfTiles;
+    static constexpr int kSfbBytes = 1024 * kSfTiles;
     // A stage of the ring: A | B | scales of B | scales of A, the first and the last not where the kernel
     // writes A itself (WA): A and its scales for the whole depth then lie in two buffers before the ring.
     __host__ __device__ static constexpr int off_b(bool wa) { return wa ? 0 : kA; }
@@ -75,7 +74,7 @@ struct Shape {
     __host__ __device__ static constexpr int stage(bool wa) { return (off_sfa(wa) + (wa ? 0 : 2 * kSfaKg) + 1023) / 1024 * 1024; }
     __host__ __device__ static constexpr int a_buffer(int stages) { return stages * kA + (stages * 2 * kSfaKg + 1023) / 1024 * 1024; }
     static constexpr int kSfCols = 8 * (1 + kSfTiles);  // TMEM columns of a stage's scales
-    static constexpr int kAcc = NT <= 128 ? 2 : 1;      // accumulators
+    static constexpr int kAcc = ACC_;
     static constexpr int kCols = TM < 128 ? NT : NT / (kEpiWarps / 4);  // columns of an epilogue thread
     static constexpr int kThreads = 128 + 32 * kEpiWarps;
     // wide tiles leave through shared memory: 32 rows x 64 bytes per epilogue warp, stored by TMA
@@ -309,14 +308,14 @@ MOE_DEV void fused_route(FusedRoute& f, const GemmParams& p, int threads) {
     __syncthreads();
 }
 
-// Columns [n0, n0 + 64) of y from the parts of every pair, a half-warp per token, in the order of
-// the token's pairs.
+// Columns [n0, n0 + 128) of y from the parts of every pair, 4 columns a lane, in the order of a
+// token's pairs.
 template <int DT>
 MOE_DEV void fused_combine(const FusedRoute& f, const GemmParams& p, int n0) {
-    const int lane = threadIdx.x & 31, n = n0 + (lane & 15) * 4, K = p.topk;
+    const int n = n0 + (threadIdx.x & 31) * 4, K = p.topk;
     const float* part = static_cast<const float*>(p.out);
     if (n >= p.N) return;
-    for (int t = lane >> 4; t < p.T; t += 2) {
+    for (int t = 0; t < p.T; ++t) {
         float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
         for (int k0 = 0; k0 < K; k0 += 8) {
             float4 v[8];
@@ -361,7 +360,7 @@ __global__ void __launch_bounds__(S::kThreads, S::kCtas)
     uint8_t* abuf = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     const int nstages = (p.K + kStageK - 1) / kStageK, k64 = (p.K + 63) / 64;
     uint8_t* smem = abuf + (WRITE_A ? 2 * S::a_buffer(nstages) : 0);  // the ring
-    __shared__ __align__(8) uint64_t s_full[STAGES], s_empty[STAGES], s_accfull[2], s_accempty[2], s_afull[2], s_done;
+    __shared__ __align__(8) uint64_t s_full[STAGES], s_empty[STAGES], s_accfull[2], s_accempty[2], s_afull[2], s_aempty[2], s_done;
     __shared__ uint32_t s_tmem;
     __shared__ int s_failed;
     __shared__ typename RouteStore<FUSED>::type s_route;
@@ -376,6 +375,7 @@ __global__ void __launch_bounds__(S::kThreads, S::kCtas)
             mbar_init(&s_accfull[a], 1);
             mbar_init(&s_accempty[a], S::kEpiWarps);
             mbar_init(&s_afull[a], 2);
+            mbar_init(&s_aempty[a], 1);
         }
         mbar_init(&s_done, 1);
         s_failed = 0;
@@ -432,12 +432,11 @@ __global__ void __launch_bounds__(S::kThreads, S::kCtas)
             const int copies = MODE == kDense || TM < 128 ? 4 : (rows + 31) >> 5;  // quarters of a 128-row tile
             // B's scales: of an expert one contiguous piece a stage, of a dense product a piece per 128 rows
             const int sft = MODE == kDense ? min(S::kSfTiles, nb128 - nt * NT / 128) : 1;
-            const int per_expert = (p.N + NT - 1) / NT;
-            const uint8_t* sfb = MODE == kDense ? p.sfb + (int64_t)(nt * NT / 128) * p.kb * 512
-                                                : p.sfb + ((int64_t)e * per_expert + nt) * nstages * S::kSfbBytes;
             // B's rows: of an expert those of a panel, whose stages follow one another
             const int64_t panel0 = ((int64_t)e * ((p.N + kPanelRows - 1) / kPanelRows) + nt * NT / kPanelRows) * nstages;
             const int in_panel = nt * NT % kPanelRows;
+            const uint8_t* sfb = MODE == kDense ? p.sfb + (int64_t)(nt * NT / 128) * p.kb * 512
+                                                : p.sfb + panel0 * kPanelScales + in_panel / 128 * 1024;
             const bool early = MODE == kDown && it == 0;
             const int first = early ? min(STAGES, nstages) : 0;
             for (int s = 0; s < nstages; ++s, ++it) {
@@ -454,7 +453,7 @@ __global__ void __launch_bounds__(S::kThreads, S::kCtas)
                             if (b < sft) bulk_copy(base + oSfB + 1024 * b, sfb + ((int64_t)b * p.kb + 2 * s) * 512, sfn, bar);
                     } else {
                         tma_2d(base + oB, &tb, 0, (int)((panel0 + s) * kPanelRows) + in_panel, bar);
-                        bulk_copy(base + oSfB, sfb + (int64_t)s * S::kSfbBytes, S::kSfbBytes, bar);
+                        bulk_copy(base + oSfB, sfb + (int64_t)s * kPanelScales, S::kSfbBytes, bar);
                     }
                     if (!WRITE_A && s >= first) load_a(st, mt, s, copies);
                 }
@@ -495,7 +494,7 @@ __global__ void __launch_bounds__(S::kThreads, S::kCtas)
             const uint32_t acc = n % S::kAcc, d = utmem + acc * NT;
             if (MODE != kDense && !FUSED && __shfl_sync(0xffffffffu, tile_of((int)(tile / p.nt_count)).y, 0) == 0) break;
             // half a scale tile (NT = 64): its rows' columns are 0-1 or 2-3 of the tile's four
-            const uint32_t half = NT == 64 && !S::PANEL ? (uint32_t)(tile % p.nt_count & 1) * 2 : 0;
+            const uint32_t half = NT == 64 ? (uint32_t)(tile % p.nt_count & 1) * 2 : 0;
             if (!warp_wait(&s_accempty[acc], (n / S::kAcc & 1) ^ 1, failed)) break;
             if (WRITE_A && !warp_wait(&s_afull[n & 1], n >> 1 & 1, failed)) break;
             gemm::tc_fence_after();
@@ -508,18 +507,15 @@ __global__ void __launch_bounds__(S::kThreads, S::kCtas)
                 const uint64_t da = gemm::tc_desc_sw128(sa), db = gemm::tc_desc_sw128(ring + oB);
                 const uint64_t dsa = sf_desc(sfa), dsb = sf_desc(ring + oSfB);
                 const uint32_t tsa = utmem + kSfBase + st * S::kSfCols, tsb = tsa + 8;
-                constexpr int kColsB = S::PANEL ? 2 : 4 * S::kSfTiles;  // TMEM columns of B's scales per 128 elements
+                constexpr int kColsB = 4 * S::kSfTiles;  // TMEM columns of B's scales per 128 elements
                 const int nkb = min(2, p.kb - 2 * s), nk = min(4, k64 - 4 * s);
                 if (issue) {
-                    if (S::PANEL) cp_scales(tsb, dsb);
 #pragma unroll
                     for (int i = 0; i < 2; ++i)
                         if (i < nkb) {
                             cp_scales(tsa + 4 * i, dsa + S::kSfaKg / 16 * i);
-                            if (!S::PANEL) {
 #pragma unroll
-                                for (int b = 0; b < S::kSfTiles; ++b) cp_scales(tsb + kColsB * i + 4 * b, dsb + 64 * b + 32 * i);
-                            }
+                            for (int b = 0; b < S::kSfTiles; ++b) cp_scales(tsb + kColsB * i + 4 * b, dsb + 64 * b + 32 * i);
                         }
 #pragma unroll
                     for (int j = 0; j < 4; ++j)
@@ -534,7 +530,10 @@ __global__ void __launch_bounds__(S::kThreads, S::kCtas)
                     parity ^= 1;
                 }
             }
-            if (ok && issue) gemm::tc_commit(&s_accfull[acc]);
+            if (ok && issue) {
+                if (WRITE_A) gemm::tc_commit(&s_aempty[n & 1]);
+                gemm::tc_commit(&s_accfull[acc]);
+            }
             __syncwarp();
         }
         if (*failed && issue) {  // the MMAs in flight end before the accumulators are given back
@@ -544,14 +543,13 @@ __global__ void __launch_bounds__(S::kThreads, S::kCtas)
         __syncwarp();
     } else if (WRITE_A && warp < 4) {
         // The rows of each tile's piece, quantised for the whole depth into one of the two buffers while the
-        // MMAs read the other; a thread takes 8 elements, four loads in flight.  A buffer is free when the tile
-        // before the last has been read, i.e. its accumulators are full.
+        // MMAs read the other; a thread takes 8 elements, four loads in flight.
         constexpr int kFly = 4;
         const int t64 = tid - 64;
         uint32_t n = 0;
         for (int64_t tile = blockIdx.x; tile < tiles; tile += gridDim.x, ++n) {
             const int mt = (int)(tile / p.nt_count);
-            if (n >= 2 && !warp_wait(&s_accfull[n & 1], (n - 2) >> 1 & 1, failed)) break;
+            if (n >= 2 && !warp_wait(&s_aempty[n & 1], (n - 2) >> 1 & 1, failed)) break;
             uint8_t* codes = abuf + (n & 1) * S::a_buffer(nstages);
             uint8_t* scales = codes + nstages * S::kA;
             const int per = nstages * 32, units = route.rows[mt] * per;  // a multiple of 32: a warp is in or out as a whole
