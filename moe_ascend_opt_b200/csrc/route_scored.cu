@@ -186,13 +186,14 @@ MOE_DEV void sort_keys(uint32_t (&k)[N]) {
 // Each lane sorts its keys once; a round of the top-k is then redux.sync over the lanes' heads, a
 // ballot for the owner, and the owner's step to its next.  Two rounds more than top_k show
 // whether the order is certain: neighbouring choices that the keys do not settle (scores are 32-bit
-// approximations, keys lack their last bits) are compared exactly by two lanes, and what that does not
+// approximations, keys lack their last bits) are compared exactly by two lanes, groups at the border of the
+// kept ones by their lanes' exact pairs, and what that does not
 // settle (three in a row, groups at the border, a softmax with a bias) goes to route_row_exact.
 // Of 256 sigmoid scores with a bias about two rows in a hundred have such a pair.  Without a bias
 // the logits decide, which have the scores' order; 16-bit ones lose nothing in the keys.
 //
 // Bound: the instructions, about 500 a row (16384 x 256 bf16 logits are 8.9 MB, 1.4 us of traffic).
-template <int NPL>
+template <int NPL, int DT, bool sigmoid>
 __global__ void __launch_bounds__(kRouteWarps * 32) route_scored_kernel(const __grid_constant__ RouteScoredParams p) {
     constexpr uint32_t kPlace = NPL - 1;
     constexpr float kCut = NPL * 1.2e-7f;
@@ -202,7 +203,7 @@ __global__ void __launch_bounds__(kRouteWarps * 32) route_scored_kernel(const __
     const int E = p.E, per = E / p.groups, e0 = lane * NPL;
     const int64_t base = t * E;
     float l[NPL];
-    const int esz = p.dtype == MOE_F32 ? 4 : 2;
+    constexpr int esz = DT == MOE_F32 ? 4 : 2;
     const bool wide = NPL >= 4 && E % 4 == 0;
     if (wide && (reinterpret_cast<uintptr_t>(p.logits) & 15) == 0) {
 #pragma unroll
@@ -210,14 +211,14 @@ __global__ void __launch_bounds__(kRouteWarps * 32) route_scored_kernel(const __
             float v[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
             if (e0 + i < E) {
                 const uint8_t* q = static_cast<const uint8_t*>(p.logits) + (base + e0 + i) * esz;
-                if (p.dtype == MOE_F32) {
+                if (DT == MOE_F32) {
                     const float4 a = __ldg(reinterpret_cast<const float4*>(q));
                     v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
                 } else {
                     const uint2 a = __ldg(reinterpret_cast<const uint2*>(q));
                     const uint32_t w[2] = {a.x, a.y};
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) v[j] = scale_to_f32((uint16_t)(w[j / 2] >> (16 * (j & 1))), p.dtype == MOE_BF16);
+                    for (int j = 0; j < 4; ++j) v[j] = scale_to_f32((uint16_t)(w[j / 2] >> (16 * (j & 1))), DT == MOE_BF16);
                 }
             }
 #pragma unroll
@@ -225,11 +226,11 @@ __global__ void __launch_bounds__(kRouteWarps * 32) route_scored_kernel(const __
         }
     } else {
 #pragma unroll
-        for (int i = 0; i < NPL; ++i) l[i] = e0 + i < E ? load_logit(p.logits, base + e0 + i, p.dtype) : -INFINITY;
+        for (int i = 0; i < NPL; ++i) l[i] = e0 + i < E ? load_logit(p.logits, base + e0 + i, DT) : -INFINITY;
     }
 #pragma unroll
     for (int i = 0; i < NPL; ++i) l[i] = l[i] > -INFINITY ? fminf(l[i], kMostFloat) : -INFINITY;  // NaN: masked
-    const bool sigmoid = p.score == MOE_SCORE_SIGMOID, sums = p.groups > 1 && p.group_top > 1, scored = p.bias || sums;
+    const bool sums = p.groups > 1 && p.group_top > 1, scored = p.bias || sums;
     float top = 0.f, den = 1.f;
     if (!sigmoid) {
         uint32_t m = 0;
@@ -284,7 +285,7 @@ __global__ void __launch_bounds__(kRouteWarps * 32) route_scored_kernel(const __
     }
     sort_keys(key);
     bool settled = true;
-    const bool exact_keys = !p.bias && p.dtype != MOE_F32;  // of the logits
+    const bool exact_keys = !p.bias && DT != MOE_F32;  // of the logits
     if (p.groups > 1) {
         // a lane's experts are of one group, which is held by 2^n neighbouring lanes
         const int lanes = per / NPL;
@@ -294,26 +295,61 @@ __global__ void __launch_bounds__(kRouteWarps * 32) route_scored_kernel(const __
             b = max(max(b, ob), min(a, oa));
             a = max(a, oa);
         }
-        uint32_t left = 0;
-        if (e0 % per == 0 && e0 < E && a) {
-            left = a & ~kPlace;
-            if (sums && b) left = ordered(unordered(a & ~kPlace) + unordered(b & ~kPlace));
+        uint32_t total = a & ~kPlace;  // in every lane of the group
+        if (sums && a && b) total = ordered(unordered(a & ~kPlace) + unordered(b & ~kPlace));
+        if (e0 >= E) total = 0;
+        // rank of this lane's group among the groups (0 the best), ties to the lower index
+        const int group = lane / lanes;
+        int rank = 0;
+        for (int d = 1; d < p.groups; ++d) {
+            const int other = group + d < p.groups ? group + d : group + d - p.groups;
+            const uint32_t t2 = __shfl_sync(0xffffffffu, total, (other * lanes) & 31);
+            rank += t2 > total || (t2 == total && other < group);
         }
-        uint32_t keep = 0, last = 0;
-        const uint32_t members = lanes < 32 ? (1u << lanes) - 1u : 0xffffffffu;
-        for (int r = 0; r <= p.topk_groups; ++r) {
-            const uint32_t best = __reduce_max_sync(0xffffffffu, left);
-            if (best == 0) break;
-            if (r == p.topk_groups) {  // the first group that is left out
-                if (scored || !exact_keys) settled = apart(unordered(last), unordered(best), 2.f * tol, 2.f * kCut);
-                break;
+        bool kept = total && rank < p.topk_groups;
+        if ((scored || !exact_keys) && p.topk_groups < p.groups) {
+            // the last group that is kept and the first that is left out
+            const uint32_t in = __ballot_sync(0xffffffffu, rank == p.topk_groups - 1 && e0 < E);
+            const uint32_t out = __ballot_sync(0xffffffffu, rank == p.topk_groups && e0 < E);
+            const uint32_t last = __shfl_sync(0xffffffffu, total, __ffs(in) - 1), next = __shfl_sync(0xffffffffu, total, __ffs(out) - 1);
+            if (next && !apart(unordered(last), unordered(next), 2.f * tol, 2.f * kCut)) {
+                // in 64 bits: each lane's two best exactly (if a third is as near as the second, or a softmax has a
+                // bias, the whole row is), the groups' from them, and their ranks again
+                double c[2];
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    const uint32_t k = key[j < NPL ? j : 0];
+                    const int i = kPlace - (k & kPlace);
+                    float v = 0.f;
+#pragma unroll
+                    for (int n = 0; n < NPL; ++n)
+                        if (n == i) v = l[n];
+                    c[j] = -INFINITY;
+                    if (k && j < NPL) {
+                        c[j] = (double)v;
+                        if (scored) c[j] = sigmoid ? 1.0 / (1.0 + exp(-(double)v)) : exp((double)v - (double)top);
+                        if (p.bias) c[j] += (double)fminf(p.bias[e0 + i], kMostFloat);
+                    }
+                }
+                const uint32_t second = NPL > 1 ? key[NPL > 1] : 0u, third = NPL > 2 ? key[NPL > 2 ? 2 : 0] : 0u;
+                const bool sure = !third || apart(unordered(second & ~kPlace), unordered(third & ~kPlace), tol, kCut);
+                if (!__all_sync(0xffffffffu, sure) || (p.bias && !sigmoid)) settled = false;
+                double x = fmax(c[0], c[1]), y = fmin(c[0], c[1]);
+                for (int o = 1; o < lanes; o <<= 1) {
+                    const double ox = __shfl_xor_sync(0xffffffffu, x, o), oy = __shfl_xor_sync(0xffffffffu, y, o);
+                    y = fmax(fmax(y, oy), fmin(x, ox));
+                    x = fmax(x, ox);
+                }
+                const double sum = sums && y > -INFINITY ? x + y : x;
+                rank = 0;
+                for (int d = 1; d < p.groups; ++d) {
+                    const int other = group + d < p.groups ? group + d : group + d - p.groups;
+                    const double s2 = __shfl_sync(0xffffffffu, sum, (other * lanes) & 31);
+                    rank += s2 > sum || (s2 == sum && other < group);
+                }
+                kept = total && rank < p.topk_groups;
             }
-            last = best;
-            const int owner = __ffs(__ballot_sync(0xffffffffu, left == best)) - 1;
-            if (lane == owner) left = 0;
-            keep |= members << owner;
         }
-        const bool kept = keep >> lane & 1u;
         if (sums && !p.bias) {  // the logits decide within the groups
 #pragma unroll
             for (int i = 0; i < NPL; ++i) key[i] = l[i] > -INFINITY ? (ordered(l[i]) & ~kPlace) | (kPlace - i) : 0u;
@@ -324,31 +360,31 @@ __global__ void __launch_bounds__(kRouteWarps * 32) route_scored_kernel(const __
             for (int i = 0; i < NPL; ++i) key[i] = 0;
         }
     }
-    int owner_of = 0, count = 0;  // lane k: owner and key of the k-th choice
+    uint32_t owner_of = 1;  // lane k: holders and key of the k-th choice
+    int count = 0;
+    const uint32_t below = (1u << lane) - 1u;
     uint32_t key_of = 0;
     const int rounds = p.K + (exact_keys ? 0 : 2);
     for (; count < rounds; ++count) {
         const uint32_t head = key[0] & ~kPlace, best = __reduce_max_sync(0xffffffffu, head);
         if (best == 0) break;  // nothing is left: id -1, weight 0
-        const int owner = __ffs(__ballot_sync(0xffffffffu, head == best)) - 1;
-        const uint32_t k = __shfl_sync(0xffffffffu, key[0], owner);
-        if (lane == count) {
-            owner_of = owner;
-            key_of = k;
-        }
-        if (lane == owner) {
+        const uint32_t holders = __ballot_sync(0xffffffffu, head == best);
+        const bool owns = head == best && (holders & below) == 0;  // the lowest of them
+        const uint32_t k = __shfl_sync(0xffffffffu, key[0], __ffs(holders) - 1);
+        const bool here = lane == count;
+        owner_of = here ? holders : owner_of;
+        key_of = here ? k : key_of;
 #pragma unroll
-            for (int i = 0; i + 1 < NPL; ++i) key[i] = key[i + 1];
-            key[NPL - 1] = 0;
-        }
+        for (int i = 0; i + 1 < NPL; ++i) key[i] = owns ? key[i + 1] : key[i];
+        key[NPL - 1] = owns ? 0u : key[NPL - 1];
     }
-    int mine = lane < count ? owner_of * NPL + (int)(kPlace - (key_of & kPlace)) : -1;
+    int mine = lane < count ? (__ffs(owner_of) - 1) * NPL + (int)(kPlace - (key_of & kPlace)) : -1;
     uint32_t near = 0;  // bit k: choices k and k + 1 are not settled
     if (!exact_keys) {
         const float c = unordered(key_of & ~kPlace), next = __shfl_down_sync(0xffffffffu, c, 1);
         near = __ballot_sync(0xffffffffu, lane + 1 < count && !apart(c, next, p.bias ? tol : 0.f, kCut));
     }
-    float v = mine >= 0 ? fminf(load_logit(p.logits, base + mine, p.dtype), kMostFloat) : 0.f;
+    float v = mine >= 0 ? fminf(load_logit(p.logits, base + mine, DT), kMostFloat) : 0.f;
     if (near) {
         if ((near & near >> 1) || (p.bias && !sigmoid)) {
             settled = false;
@@ -393,15 +429,22 @@ __global__ void __launch_bounds__(kRouteWarps * 32) route_scored_exact_kernel(co
     if (t < p.T) route_row_exact<NPL>(p, t);
 }
 
+template <int NPL, int DT>
+void route_launch_as(const RouteScoredParams& p, unsigned grid, cudaStream_t st) {
+    if (p.score == MOE_SCORE_SIGMOID) route_scored_kernel<NPL, DT, true><<<grid, kRouteWarps * 32, 0, st>>>(p);
+    else route_scored_kernel<NPL, DT, false><<<grid, kRouteWarps * 32, 0, st>>>(p);
+}
+
 template <int NPL>
 void route_launch(const RouteScoredParams& p, cudaStream_t st) {
     const unsigned grid = (unsigned)((p.T + kRouteWarps - 1) / kRouteWarps);
     const int per = p.E / p.groups, lanes = per / NPL;
     // the two rounds past top_k need a lane each
-    if (p.K <= 30 && (p.groups == 1 || (per % NPL == 0 && (lanes & (lanes - 1)) == 0)))
-        route_scored_kernel<NPL><<<grid, kRouteWarps * 32, 0, st>>>(p);
-    else
+    if (p.K > 30 || (p.groups > 1 && (per % NPL != 0 || (lanes & (lanes - 1)) != 0)))
         route_scored_exact_kernel<NPL><<<grid, kRouteWarps * 32, 0, st>>>(p);
+    else if (p.dtype == MOE_F32) route_launch_as<NPL, MOE_F32>(p, grid, st);
+    else if (p.dtype == MOE_BF16) route_launch_as<NPL, MOE_BF16>(p, grid, st);
+    else route_launch_as<NPL, MOE_F16>(p, grid, st);
 }
 
 }  // namespace
