@@ -112,9 +112,9 @@ int sm_count(int dev, int* out) {
 using Wide = mx::Shape<256, 128, 4, 8, 1, 1>;
 using WideDown = mx::Shape<256, 128, 3, 8, 1, 1, false, 4>;
 using Narrow = mx::Shape<64, 128, 4, 4, 2, 2>;
-using Slim = mx::Shape<128, 32, 9, 1, 1, 2>;
-using FusedUp = mx::Shape<128, 8, 6, 1, 1, 1, true>;
-using FusedDown = mx::Shape<128, 8, 4, 1, 1, 1, true>;
+using Slim = mx::Shape<128, 32, 9, 4, 1, 2>;
+using FusedUp = mx::Shape<128, 8, 7, 4, 2, 1, true>;
+using FusedDown = mx::Shape<128, 8, 3, 4, 2, 1, true>;
 
 constexpr int kFusedStages = 32;  // depth of fused calls: their A buffers hold it whole
 
@@ -126,7 +126,7 @@ int launch_gemm(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap&
     const int smem = S::smem(WA, (int)ceil_div(p.K, mx::kStageK));
     if (int rc = allow_smem(reinterpret_cast<const void*>(fn), S::smem(WA, kFusedStages))) return rc;
     p.nt_count = (int)ceil_div(p.N, S::NT);
-    return launch(fn, (unsigned)std::min<int64_t>(m_tiles * p.nt_count, sms * S::kCtas), S::kThreads, smem, pdl, st, ta, tb, ta32, to, p);
+    return launch(fn, (unsigned)std::min<int64_t>(m_tiles * p.nt_count, sms * (S::FUSED ? 1 : S::kCtas)), S::kThreads, smem, pdl, st, ta, tb, ta32, to, p);
 }
 
 bool dtype_ok(int32_t t) { return t == MOE_F16 || t == MOE_BF16 || t == MOE_F32; }

@@ -75,16 +75,21 @@ struct Shape {
     __host__ __device__ static constexpr int a_buffer(int stages) { return stages * kA + (stages * 2 * kSfaKg + 1023) / 1024 * 1024; }
     static constexpr int kSfCols = 8 * (1 + kSfTiles);  // TMEM columns of a stage's scales
     static constexpr int kAcc = ACC_;
-    static constexpr int kCols = TM < 128 ? NT : NT / (kEpiWarps / 4);  // columns of an epilogue thread
+    static constexpr int kCols = NT / (kEpiWarps / 4);  // columns of an epilogue thread of a 128-row tile
     static constexpr int kThreads = 128 + 32 * kEpiWarps;
     // wide tiles leave through shared memory: 32 rows x 64 bytes per epilogue warp, stored by TMA
     static constexpr int kStaging = NT >= 256 ? kEpiWarps * BUFS * 2048 : 0;
+    // tiles of few rows pass through shared memory too, from the one warp that can read their TMEM lanes to all
+    static constexpr int kRowPitch = NT + 4;  // floats: 16-byte accesses of neighbouring rows meet no bank twice
+    static constexpr int kRows = TM < 128 ? TM * kRowPitch * 4 : 0;
     // Dynamic shared memory for `stages` of depth.  The MMA's 128 rows of the last A stay inside, so do
     // the 512 bytes that a copy of its scales takes.
+    __host__ __device__ static constexpr int tail(bool wa) {
+        return wa || stage(wa) >= 16384 + 512 ? 0 : (16384 + 512 - stage(wa) + 1023) / 1024 * 1024;
+    }
     __host__ __device__ static constexpr int smem(bool wa, int stages) {
         const int ring = STAGES * stage(wa), buffers = wa ? 2 * a_buffer(stages) : 0;
-        const int tail = wa ? 0 : (stage(wa) < 16384 + 512 ? 16384 + 512 - stage(wa) : 0);
-        return buffers + ring + (tail + 1023) / 1024 * 1024 + kStaging + 1024;
+        return buffers + ring + tail(wa) + kStaging + (kRows + 1023) / 1024 * 1024 + 1024;
     }
 };
 
@@ -308,14 +313,14 @@ MOE_DEV void fused_route(FusedRoute& f, const GemmParams& p, int threads) {
     __syncthreads();
 }
 
-// Columns [n0, n0 + 128) of y from the parts of every pair, 4 columns a lane, in the order of a
-// token's pairs.
+// Columns [n0, n0 + 128) of y from the parts of every pair, 4 columns a lane, in the order of a token's
+// pairs; tokens first, first + step, ...
 template <int DT>
-MOE_DEV void fused_combine(const FusedRoute& f, const GemmParams& p, int n0) {
+MOE_DEV void fused_combine(const FusedRoute& f, const GemmParams& p, int n0, int first, int step) {
     const int n = n0 + (threadIdx.x & 31) * 4, K = p.topk;
     const float* part = static_cast<const float*>(p.out);
     if (n >= p.N) return;
-    for (int t = 0; t < p.T; ++t) {
+    for (int t = first; t < p.T; t += step) {
         float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
         for (int k0 = 0; k0 < K; k0 += 8) {
             float4 v[8];
@@ -362,7 +367,7 @@ __global__ void __launch_bounds__(S::kThreads, S::kCtas)
     uint8_t* smem = abuf + (WRITE_A ? 2 * S::a_buffer(nstages) : 0);  // the ring
     __shared__ __align__(8) uint64_t s_full[STAGES], s_empty[STAGES], s_accfull[2], s_accempty[2], s_afull[2], s_aempty[2], s_done;
     __shared__ uint32_t s_tmem;
-    __shared__ int s_failed;
+    __shared__ int s_failed, s_go, s_last;
     __shared__ typename RouteStore<FUSED>::type s_route;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
@@ -373,7 +378,7 @@ __global__ void __launch_bounds__(S::kThreads, S::kCtas)
         }
         for (int a = 0; a < 2; ++a) {
             mbar_init(&s_accfull[a], 1);
-            mbar_init(&s_accempty[a], S::kEpiWarps);
+            mbar_init(&s_accempty[a], TM < 128 ? 1 : S::kEpiWarps);
             mbar_init(&s_afull[a], 2);
             mbar_init(&s_aempty[a], 1);
         }
@@ -424,9 +429,11 @@ __global__ void __launch_bounds__(S::kThreads, S::kCtas)
             }
             bulk_copy(base + oSfA, p.sfa + ((int64_t)mt * p.kb + 2 * s) * S::kSfaKg, min(2, p.kb - 2 * s) * S::kSfaKg, bar);
         };
+        int2 next = blockIdx.x < tiles ? tile_of((int)(blockIdx.x / p.nt_count)) : make_int2(0, 0);
         for (int64_t tile = blockIdx.x; ok && tile < tiles; tile += gridDim.x) {
             const int mt = (int)(tile / p.nt_count), nt = (int)(tile - (int64_t)mt * p.nt_count);
-            const int2 of = tile_of(mt);
+            const int2 of = next;
+            if (tile + gridDim.x < tiles) next = tile_of((int)((tile + gridDim.x) / p.nt_count));  // a tile ahead of its use
             const int e = __shfl_sync(0xffffffffu, of.x, 0), rows = __shfl_sync(0xffffffffu, of.y, 0);
             if (rows == 0) break;
             const int copies = MODE == kDense || TM < 128 ? 4 : (rows + 31) >> 5;  // quarters of a 128-row tile
@@ -490,9 +497,14 @@ __global__ void __launch_bounds__(S::kThreads, S::kCtas)
         const bool issue = elect_one();
         uint32_t n = 0, st = 0, parity = 0;  // tiles so far; stage and phase of the ring
         bool ok = true;
+        int next = blockIdx.x < tiles ? tile_of((int)(blockIdx.x / p.nt_count)).y : 0;
         for (int64_t tile = blockIdx.x; ok && tile < tiles; tile += gridDim.x, ++n) {
             const uint32_t acc = n % S::kAcc, d = utmem + acc * NT;
-            if (MODE != kDense && !FUSED && __shfl_sync(0xffffffffu, tile_of((int)(tile / p.nt_count)).y, 0) == 0) break;
+            if (MODE != kDense && !FUSED) {
+                const int rows = next;
+                if (tile + gridDim.x < tiles) next = tile_of((int)((tile + gridDim.x) / p.nt_count)).y;
+                if (__shfl_sync(0xffffffffu, rows, 0) == 0) break;
+            }
             // half a scale tile (NT = 64): its rows' columns are 0-1 or 2-3 of the tile's four
             const uint32_t half = NT == 64 ? (uint32_t)(tile % p.nt_count & 1) * 2 : 0;
             if (!warp_wait(&s_accempty[acc], (n / S::kAcc & 1) ^ 1, failed)) break;
@@ -586,10 +598,105 @@ __global__ void __launch_bounds__(S::kThreads, S::kCtas)
             __syncwarp();
             if (lane == 0) mbar_arrive(&s_afull[n & 1]);
         }
+    } else if (TM < 128 && warp >= 4) {
+        // Few rows: warp 4 reads their TMEM lanes into shared memory, and all epilogue threads share the
+        // arithmetic: 8 threads a 32-block of a row (gate_up), a warp a row (down).
+        float* rows = reinterpret_cast<float*>(smem + STAGES * kStage + S::tail(WRITE_A));
+        const int et = tid - 128;
+        constexpr int kEt = 32 * S::kEpiWarps;
+        uint32_t n = 0;
+        int2 of = blockIdx.x < tiles ? tile_of((int)(blockIdx.x / p.nt_count)) : make_int2(0, 0);
+        for (int64_t tile = blockIdx.x; tile < tiles && of.y; tile += gridDim.x, ++n) {
+            const int mt = (int)(tile / p.nt_count), nt = (int)(tile - (int64_t)mt * p.nt_count), mrows = of.y;
+            const uint32_t acc = n % S::kAcc;
+            if (tile + gridDim.x < tiles) of = tile_of((int)((tile + gridDim.x) / p.nt_count));
+            if (warp == 4) {
+                const bool go = warp_wait(&s_accfull[acc], n / S::kAcc & 1, failed);
+                gemm::tc_fence_after();
+                if (go) {
+#pragma unroll
+                    for (int c = 0; c < NT; c += 32) {
+                        float v[32];
+                        load_columns<32>(tmem + acc * NT + c, v);
+                        if (lane < mrows)
+#pragma unroll
+                            for (int j = 0; j < 8; ++j)
+                                *reinterpret_cast<float4*>(rows + lane * S::kRowPitch + c + 4 * j) =
+                                    make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+                    }
+                }
+                gemm::tc_fence_before();
+                __syncwarp();
+                if (lane == 0) {
+                    mbar_arrive(&s_accempty[acc]);
+                    s_go = go;
+                }
+            }
+            named_bar_sync(1, kEt);
+            if (!*reinterpret_cast<volatile int*>(&s_go)) break;
+            if (MODE == kGateUp) {
+                for (int i = et >> 3; i < mrows * (NT / 64); i += kEt / 8) {
+                    const int r = i / (NT / 64), b = i % (NT / 64), i0 = (nt * NT) / 2 + b * 32, j = et & 7;
+                    const float* src = rows + r * S::kRowPitch + 64 * b + 4 * j;
+                    const float4 g = *reinterpret_cast<const float4*>(src), u = *reinterpret_cast<const float4*>(src + 32);
+                    const float h[4] = {silu_up(g.x, u.x), silu_up(g.y, u.y), silu_up(g.z, u.z), silu_up(g.w, u.w)};
+                    uint32_t m = 0;
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) m = max(m, __float_as_uint(h[k]) & 0x7fffffffu);
+                    const uint32_t octet = 0xffu << (lane & 24);
+#pragma unroll
+                    for (int o = 1; o < 8; o <<= 1) m = max(m, __shfl_xor_sync(octet, m, o));
+                    if (i0 >= p.I) continue;
+                    const uint32_t sc = scale_of_amax(m);
+                    const float k = inv_scale(sc);
+                    const int64_t row = (int64_t)mt * TM + r;
+                    *reinterpret_cast<uint16_t*>(p.hq + row * (p.I / 2) + i0 / 2 + 2 * j) =
+                        (uint16_t)(cvt_e2m1x2(h[0] * k, h[1] * k) | cvt_e2m1x2(h[2] * k, h[3] * k) << 8);
+                    if (j == 0) {
+                        uint8_t* hs = p.hs + (TM == 8 ? ((int64_t)mt * p.hkb + (i0 >> 7)) * 128 + r * 16 + (i0 >> 5 & 3)
+                                                      : tile_row_at(mt, r, i0 >> 5, p.hkb));
+                        hs[0] = (uint8_t)sc;
+                        // the MMAs take K in steps of 64: the scale behind an odd last block must be a number
+                        if (i0 + 32 == p.I && (p.I & 32)) hs[1] = 0;
+                    }
+                }
+            } else {
+                for (int r = warp - 4; r < mrows; r += S::kEpiWarps) {
+                    const int64_t row = FUSED ? (int64_t)route.pair[mt * 8 + r] : (int64_t)mt * TM + r;  // fused parts lie by pair
+#pragma unroll
+                    for (int c = lane * 4; c < NT; c += 128)
+                        if (nt * NT + c < p.N)  // rows are multiples of 32
+                            *reinterpret_cast<float4*>(static_cast<float*>(p.out) + row * p.N + nt * NT + c) =
+                                *reinterpret_cast<const float4*>(rows + r * S::kRowPitch + c);
+                }
+            }
+            named_bar_sync(1, kEt);  // the rows are read (and a part is written) before warp 4 goes on
+            if (FUSED && MODE == kDown) {
+                // the CTA that finishes a column tile's last part sums them
+                if (et == 0) {
+                    __threadfence();
+                    const bool last = atomicAdd(p.cnt + nt, 1u) + 1 == (unsigned int)mt_count;
+                    __threadfence();
+                    if (last) p.cnt[nt] = 0;
+                    s_last = last;
+                }
+                named_bar_sync(1, kEt);
+                if (*reinterpret_cast<volatile int*>(&s_last)) {
+                    if (p.y_dtype == MOE_F32) fused_combine<MOE_F32>(route, p, nt * NT, warp - 4, S::kEpiWarps);
+                    else if (p.y_dtype == MOE_BF16) fused_combine<MOE_BF16>(route, p, nt * NT, warp - 4, S::kEpiWarps);
+                    else fused_combine<MOE_F16>(route, p, nt * NT, warp - 4, S::kEpiWarps);
+                }
+            }
+        }
+        if (FUSED && MODE == kDown && mt_count == 0)  // no pair is this engine's
+            for (int nt = blockIdx.x; nt < p.nt_count; nt += gridDim.x) {
+                if (p.y_dtype == MOE_F32) fused_combine<MOE_F32>(route, p, nt * NT, warp - 4, S::kEpiWarps);
+                else if (p.y_dtype == MOE_BF16) fused_combine<MOE_BF16>(route, p, nt * NT, warp - 4, S::kEpiWarps);
+                else fused_combine<MOE_F16>(route, p, nt * NT, warp - 4, S::kEpiWarps);
+            }
     } else if (warp >= 4) {
-        const int r = TM == 128 ? (warp & 3) * 32 + lane : lane, c0 = TM == 128 ? ((warp - 4) >> 2) * S::kCols : 0;
-        const uint32_t quarter = TM == 128 ? (uint32_t)((warp & 3) * 32) : 0u;
-        static_assert(TM == 128 || S::kEpiWarps == 1, "a tile of up to 32 rows has one epilogue warp, on TMEM lanes 0-31");
+        const int r = (warp & 3) * 32 + lane, c0 = ((warp - 4) >> 2) * S::kCols;
+        const uint32_t quarter = (uint32_t)((warp & 3) * 32);
         uint8_t* const staging0 = smem + STAGES * kStage + (warp - 4) * S::BUFS * 2048;  // wide tiles only: no tail
         uint8_t* staging = staging0;
         uint32_t stores = 0;
@@ -643,7 +750,7 @@ __global__ void __launch_bounds__(S::kThreads, S::kCtas)
                         for (int j = 0; j < 4; ++j) q[w] |= cvt_e2m1x2(h[8 * w + 2 * j] * k, h[8 * w + 2 * j + 1] * k) << (8 * j);
                     }
                     *reinterpret_cast<uint4*>(p.hq + row * (p.I / 2) + i0 / 2) = make_uint4(q[0], q[1], q[2], q[3]);
-                    uint8_t* hs = p.hs + (TM == 8 ? ((int64_t)mt * p.hkb + (i0 >> 7)) * 128 + r * 16 + (i0 >> 5 & 3) : tile_row_at(mt, r, i0 >> 5, p.hkb));
+                    uint8_t* hs = p.hs + tile_row_at(mt, r, i0 >> 5, p.hkb);
                     hs[0] = (uint8_t)sc;
                     // the MMAs take K in steps of 64: the scale behind an odd last block must be a number
                     if (i0 + 32 == p.I && (p.I & 32)) hs[1] = 0;
@@ -686,43 +793,18 @@ __global__ void __launch_bounds__(S::kThreads, S::kCtas)
                 continue;
             }
             if (r < mrows) {
-                const int64_t to_row = FUSED ? (int64_t)route.pair[mt * 8 + r] : row;  // fused parts lie by pair
                 const int esz = MODE == kDown || p.out_dtype == MOE_F32 ? 4 : 2;
                 const bool vec = (int64_t)p.N * esz % 16 == 0;
 #pragma unroll
                 for (int c = 0; c < S::kCols; c += 32) {
                     const int n0 = nt * NT + c0 + c, left = min(32, p.N - n0);
                     if (left <= 0) break;
-                    if (MODE == kDown || p.out_dtype == MOE_F32) store_row<MOE_F32>(p.out, to_row * p.N + n0, v + c, left, vec);
-                    else if (p.out_dtype == MOE_BF16) store_row<MOE_BF16>(p.out, to_row * p.N + n0, v + c, left, vec);
-                    else store_row<MOE_F16>(p.out, to_row * p.N + n0, v + c, left, vec);
+                    if (MODE == kDown || p.out_dtype == MOE_F32) store_row<MOE_F32>(p.out, row * p.N + n0, v + c, left, vec);
+                    else if (p.out_dtype == MOE_BF16) store_row<MOE_BF16>(p.out, row * p.N + n0, v + c, left, vec);
+                    else store_row<MOE_F16>(p.out, row * p.N + n0, v + c, left, vec);
                 }
-            }
-            if (FUSED && MODE == kDown) {
-                // the CTA that finishes a column tile's last part sums them
-                __syncwarp();
-                unsigned int done = 0;
-                if (lane == 0) {
-                    __threadfence();
-                    done = atomicAdd(p.cnt + nt, 1u);
-                    __threadfence();
-                }
-                done = __shfl_sync(0xffffffffu, done, 0);
-                if (done + 1 == (unsigned int)mt_count) {
-                    if (lane == 0) p.cnt[nt] = 0;
-                    if (p.y_dtype == MOE_F32) fused_combine<MOE_F32>(route, p, nt * NT);
-                    else if (p.y_dtype == MOE_BF16) fused_combine<MOE_BF16>(route, p, nt * NT);
-                    else fused_combine<MOE_F16>(route, p, nt * NT);
-                }
-                __syncwarp();
             }
         }
-        if (FUSED && MODE == kDown && mt_count == 0)  // no pair is this engine's
-            for (int nt = blockIdx.x; nt < p.nt_count; nt += gridDim.x) {
-                if (p.y_dtype == MOE_F32) fused_combine<MOE_F32>(route, p, nt * NT);
-                else if (p.y_dtype == MOE_BF16) fused_combine<MOE_BF16>(route, p, nt * NT);
-                else fused_combine<MOE_F16>(route, p, nt * NT);
-            }
     }
     if (S::kStaging && warp >= 4 && lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
     __syncthreads();
