@@ -855,6 +855,36 @@ __global__ void __launch_bounds__(kPrepThreads) mx_count_kernel(const PrepParams
     for (int e = threadIdx.x; e < p.E; e += kPrepThreads) counts[(int64_t)blockIdx.x * p.E + e] = csm[e];
 }
 
+// A block of 16-bit values -> its codes, and the scale.
+template <int DT>
+MOE_DEV uint32_t quant32(const uint4 (&raw)[4], uint4& codes) {
+    uint32_t w[16];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        w[4 * j] = raw[j].x;
+        w[4 * j + 1] = raw[j].y;
+        w[4 * j + 2] = raw[j].z;
+        w[4 * j + 3] = raw[j].w;
+    }
+    uint32_t m = 0;  // both types order by their bits, sign apart
+#pragma unroll
+    for (int j = 0; j < 16; ++j) m = __vmaxu2(m, w[j] & 0x7fff7fffu);
+    const uint16_t top = (uint16_t)max(m & 0xffffu, m >> 16);
+    const uint32_t sc = scale_of_amax(__float_as_uint(scale_to_f32(top, DT == MOE_BF16)));
+    const float k = inv_scale(sc);
+    uint32_t q[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        q[j] = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            q[j] |= cvt_e2m1x2(scale_to_f32((uint16_t)(w[4 * j + i] & 0xffffu), DT == MOE_BF16) * k,
+                               scale_to_f32((uint16_t)(w[4 * j + i] >> 16), DT == MOE_BF16) * k) << (8 * i);
+    }
+    codes = make_uint4(q[0], q[1], q[2], q[3]);
+    return sc;
+}
+
 template <int DT>
 __global__ void __launch_bounds__(kPrepThreads) mx_prep_kernel(const PrepParams p) {
     // [warps][E] pairs of each warp's share, then their first rows | [E] first tile | rows of the run's pairs
@@ -868,6 +898,21 @@ __global__ void __launch_bounds__(kPrepThreads) mx_prep_kernel(const PrepParams 
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const int t0 = blockIdx.x * p.tokens, t1 = min(p.T, t0 + p.tokens), TK = p.T * p.K;
+    // The token rows: a lane takes a block, a warp `group` (1 or 2) times 32 blocks of a token; the first are
+    // fetched before the routing.
+    const int nb = p.H >> 5, chunks = (nb + 31) >> 5, group = (t1 - t0) * chunks >= 2 * kPrepWarps ? 2 : 1;
+    const int groups = (chunks + group - 1) / group, items = (t1 - t0) * groups;
+    uint4 raw[2][4];
+    auto fetch = [&](int item) {
+        const int t = item / groups, b0 = (item - t * groups) * 32 * group + lane;
+        const uint4* src = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.x) + (int64_t)(t0 + t) * p.H) + b0 * 4;
+#pragma unroll
+        for (int f = 0; f < 2; ++f)
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                raw[f][j] = f < group && b0 + 32 * f < nb ? __ldg(src + 128 * f + j) : make_uint4(0u, 0u, 0u, 0u);
+    };
+    if (warp < items) fetch(warp);
     // the pairs whose order this CTA works out: all (short calls) or its own run's
     const int a0 = p.counts ? t0 * p.K : 0, a1 = p.counts ? t1 * p.K : TK;
     const int share = ((a1 - a0 + kPrepWarps - 1) / kPrepWarps + 31) / 32 * 32;
@@ -967,44 +1012,27 @@ __global__ void __launch_bounds__(kPrepThreads) mx_prep_kernel(const PrepParams 
     __syncthreads();
     pos += t0 * p.K - a0;  // the run's own pairs
     for (int i = tid; i < (t1 - t0) * p.K; i += kPrepThreads) p.ppos[t0 * p.K + i] = pos[i];
-    // A warp takes up to 8 chunks of 256 elements of a token, all loads in flight, a lane 8 elements of each;
-    // then for every pair of the token its row's codes and, by two lanes, the chunks' scale words.
-    constexpr int kFly = 8;
-    const int chunks = (p.H + 255) >> 8, nb = p.H >> 5, ntok = t1 - t0;
-    const int group = max(1, min(kFly, ntok * chunks / kPrepWarps)), groups = (chunks + group - 1) / group;
-    for (int item = warp; item < ntok * groups; item += kPrepWarps) {
-        const int t = item / groups, c0 = (item - t * groups) * group, c1 = min(chunks, c0 + group);
-        float v[kFly][8];
+    for (int item = warp; item < items; item += kPrepWarps) {
+        const int t = item / groups, b0 = (item - t * groups) * 32 * group + lane;
+        uint4 codes[2];
+        uint32_t words[2];
 #pragma unroll
-        for (int f = 0; f < kFly; ++f) {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) v[f][j] = 0.f;
-            const int i = (c0 + f) * 256 + lane * 8;
-            if (c0 + f < c1 && i < p.H) load8<DT>(p.x, (int64_t)(t0 + t) * p.H + i, v[f]);
+        for (int f = 0; f < 2; ++f) {
+            const uint32_t sc = quant32<DT>(raw[f], codes[f]);
+            words[f] = sc | __shfl_down_sync(0xffffffffu, sc, 1, 4) << 8;  // the scales of four lanes' blocks
+            words[f] |= __shfl_down_sync(0xffffffffu, words[f], 2, 4) << 16;
         }
-        uint32_t code[kFly], word[kFly];
-#pragma unroll
-        for (int f = 0; f < kFly; ++f) {
-            if (c0 + f >= c1) break;
-            uint32_t sc;
-            code[f] = quant8(v[f], sc);
-            word[f] = sc;  // lanes 0 and 16: the scales of 16 neighbouring lanes' four blocks
-            word[f] |= __shfl_down_sync(0xffffffffu, sc, 4, 16) << 8;
-            word[f] |= __shfl_down_sync(0xffffffffu, sc, 8, 16) << 16;
-            word[f] |= __shfl_down_sync(0xffffffffu, sc, 12, 16) << 24;
-            const int left = nb - ((c0 + f) * 8 + (lane >> 4) * 4);
-            if (left < 4) word[f] &= left > 0 ? (1u << (8 * left)) - 1u : 0u;
-        }
+        if (item + kPrepWarps < items) fetch(item + kPrepWarps);
         for (int k = 0; k < p.K; ++k) {
             const int row = pos[t * p.K + k];
             if (row < 0) continue;
-            uint32_t* to = reinterpret_cast<uint32_t*>(p.xq + (int64_t)row * (p.H / 2)) + c0 * 32 + lane;
-            uint8_t* sc = p.xs + tile_row_at(row >> p.tile_log2, row & ((1 << p.tile_log2) - 1), c0 * 8 + (lane >> 4) * 4, p.kb);
+            uint4* to = reinterpret_cast<uint4*>(p.xq + (int64_t)row * (p.H / 2)) + b0;
+            uint8_t* sc = p.xs + tile_row_at(row >> p.tile_log2, row & ((1 << p.tile_log2) - 1), b0, p.kb);
 #pragma unroll
-            for (int f = 0; f < kFly; ++f) {
-                if (c0 + f >= c1) break;
-                if ((c0 + f) * 256 + lane * 8 < p.H) to[f * 32] = code[f];
-                if ((lane & 15) == 0 && (c0 + f) * 2 + (lane >> 4) < p.kb) *reinterpret_cast<uint32_t*>(sc + f * 1024) = word[f];
+            for (int f = 0; f < 2; ++f) {
+                if (f >= group) break;
+                if (b0 + 32 * f < nb) to[32 * f] = codes[f];
+                if ((lane & 3) == 0 && (b0 >> 2) + 8 * f < p.kb) *reinterpret_cast<uint32_t*>(sc + 4096 * f) = words[f];
             }
         }
     }
