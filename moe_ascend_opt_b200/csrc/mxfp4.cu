@@ -1,5 +1,6 @@
 // MXFP4 entry points (include/moe_b200.h) and the MXFP4 expert layer of the engine.
 #include <algorithm>
+#include <atomic>
 #include <mutex>
 #include <new>
 #include <utility>
@@ -21,17 +22,17 @@ using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, voi
                               CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
 
 int encoder(EncodeFn* out) {
-    static EncodeFn fn = nullptr;
-    static std::mutex mu;
-    std::lock_guard<std::mutex> lk(mu);
-    if (!fn) {
+    static std::atomic<EncodeFn> fn{nullptr};
+    EncodeFn f = fn.load(std::memory_order_acquire);
+    if (!f) {
         void* p = nullptr;
         cudaDriverEntryPointQueryResult q;
         CUDA_TRY(cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &p, 12000, cudaEnableDefault, &q));
         if (!p || q != cudaDriverEntryPointSuccess) return fail(MOE_ERR_CUDA, "cuTensorMapEncodeTiled is not available");
-        fn = reinterpret_cast<EncodeFn>(p);
+        f = reinterpret_cast<EncodeFn>(p);
+        fn.store(f, std::memory_order_release);
     }
-    *out = fn;
+    *out = f;
     return MOE_OK;
 }
 
@@ -93,13 +94,10 @@ int launch(void (*fn)(P...), unsigned grid, unsigned block, size_t smem, bool pd
 }
 
 int sm_count(int dev, int* out) {
-    static int n[64] = {};
-    if (dev < 64 && n[dev]) {
-        *out = n[dev];
-        return MOE_OK;
-    }
+    static std::atomic<int> n[64] = {};
+    if (dev < 64 && (*out = n[dev].load(std::memory_order_relaxed))) return MOE_OK;
     CUDA_TRY(cudaDeviceGetAttribute(out, cudaDevAttrMultiProcessorCount, dev));
-    if (dev < 64) n[dev] = *out;
+    if (dev < 64) n[dev].store(*out, std::memory_order_relaxed);
     return MOE_OK;
 }
 
@@ -132,24 +130,30 @@ int launch_gemm(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap&
 bool dtype_ok(int32_t t) { return t == MOE_F16 || t == MOE_BF16 || t == MOE_F32; }
 bool aligned(const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
 
-// Error word of the products that run without an engine: one per device, in mapped host memory.
-int product_error_word(int dev, int32_t** host, int32_t** device) {
+// Error word of the products that run without an engine: one per device, in mapped host memory, whose
+// address is the same on both sides.
+int product_error_word(int dev, int32_t** word) {
     static std::mutex mu;
-    static int32_t* words[64] = {};
+    static std::atomic<int32_t*> words[64] = {};
     if (dev < 0 || dev >= 64) return fail(MOE_ERR_INVALID, "device ordinal out of range");
-    std::lock_guard<std::mutex> lk(mu);
-    if (!words[dev]) {
-        int32_t* w = nullptr;
-        cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;  // the first call may be a captured one
-        CUDA_TRY(cudaThreadExchangeStreamCaptureMode(&mode));
-        const cudaError_t e = cudaHostAlloc(reinterpret_cast<void**>(&w), 64, cudaHostAllocMapped | cudaHostAllocPortable);
-        cudaThreadExchangeStreamCaptureMode(&mode);
-        if (e != cudaSuccess) return fail(MOE_ERR_CUDA, std::string("cudaHostAlloc: ") + cudaGetErrorString(e));
-        *reinterpret_cast<volatile int32_t*>(w) = 0;
-        words[dev] = w;
+    int32_t* w = words[dev].load(std::memory_order_acquire);
+    if (!w) {
+        std::lock_guard<std::mutex> lk(mu);
+        w = words[dev].load();
+        if (!w) {
+            cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;  // the first call may be a captured one
+            CUDA_TRY(cudaThreadExchangeStreamCaptureMode(&mode));
+            cudaError_t e = cudaHostAlloc(reinterpret_cast<void**>(&w), 64, cudaHostAllocMapped | cudaHostAllocPortable);
+            cudaThreadExchangeStreamCaptureMode(&mode);
+            void* d = nullptr;
+            if (e == cudaSuccess) e = cudaHostGetDevicePointer(&d, w, 0);
+            if (e == cudaSuccess && d != w) e = cudaErrorNotSupported;
+            if (e != cudaSuccess) return fail(MOE_ERR_CUDA, std::string("error word: ") + cudaGetErrorString(e));
+            *reinterpret_cast<volatile int32_t*>(w) = 0;
+            words[dev].store(w, std::memory_order_release);
+        }
     }
-    *host = words[dev];
-    CUDA_TRY(cudaHostGetDevicePointer(reinterpret_cast<void**>(device), words[dev], 0));
+    *word = w;
     return MOE_OK;
 }
 
@@ -243,10 +247,9 @@ extern "C" int moe_mxfp4_matmul(const uint8_t* a, const uint8_t* a_scales, const
     CUDA_TRY(cudaGetDevice(&dev));
     if (int rc = sm_count(dev, &sms)) return rc;
     mx::GemmParams p{};
-    int32_t* herr = nullptr;
-    if (int rc = product_error_word(dev, &herr, &p.err)) return rc;
-    if (*reinterpret_cast<volatile int32_t*>(herr) != 0) {
-        *reinterpret_cast<volatile int32_t*>(herr) = 0;
+    if (int rc = product_error_word(dev, &p.err)) return rc;
+    if (*reinterpret_cast<volatile int32_t*>(p.err) != 0) {
+        *reinterpret_cast<volatile int32_t*>(p.err) = 0;
         return fail(MOE_ERR_DEVICE, "an earlier MXFP4 product failed on the device (a bounded wait expired); its output is invalid");
     }
     CUtensorMap ta, tb;

@@ -19,6 +19,7 @@
 //        quantize_rows_q8_0, moe_route_scored, quantize_rows_mxfp4, dequantize_rows_mxfp4,
 //        mxfp4_tile_scales, mxfp4_matmul
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/custom_class.h>
 #include <torch/library.h>
@@ -418,6 +419,11 @@ std::tuple<at::Tensor, at::Tensor> quantize_rows(const at::Tensor& x) {
     return {qs, d};
 }
 
+// A new tensor on like's device, without a pass through the dispatcher.
+at::Tensor fresh(at::IntArrayRef sizes, at::ScalarType dtype, const at::Tensor& like) {
+    return at::detail::empty_cuda(sizes, dtype, like.device(), std::nullopt);
+}
+
 // A contiguous tensor whose data start on 16 bytes.
 at::Tensor packed(const at::Tensor& t) {
     auto c = t.contiguous();
@@ -442,8 +448,8 @@ std::tuple<at::Tensor, at::Tensor> route_scored(const at::Tensor& logits, const 
                 "need 1 <= topk_groups <= num_groups <= 32");
     TORCH_CHECK(group_top == 1 || group_top == 2, "group_top must be 1 or 2");
     c10::cuda::CUDAGuard g(l.get_device());
-    auto ids = at::empty({l.size(0), K}, l.options().dtype(at::kInt));
-    auto w = at::empty({l.size(0), K}, l.options().dtype(at::kFloat));
+    auto ids = fresh({l.size(0), K}, at::kInt, l);
+    auto w = fresh({l.size(0), K}, at::kFloat, l);
     check_rc(moe_route_scored(l.data_ptr(), dtype_code(l.scalar_type()), b.defined() ? b.data_ptr<float>() : nullptr,
                               l.size(0), l.size(1), K, score == "sigmoid" ? MOE_SCORE_SIGMOID : MOE_SCORE_SOFTMAX, groups,
                               topk_groups, (int32_t)group_top, renormalize ? 1 : 0, (float)scale, ids.data_ptr<int32_t>(),
@@ -459,9 +465,8 @@ std::tuple<at::Tensor, at::Tensor> quantize_mxfp4(const at::Tensor& x, bool tile
     TORCH_CHECK(x.size(1) > 0 && x.size(1) % 32 == 0, "cols must be a positive multiple of 32");
     auto c = packed(x);
     c10::cuda::CUDAGuard g(c.get_device());
-    auto o = c.options().dtype(at::kByte);
-    auto q = at::empty({c.size(0), c.size(1) / 2}, o);
-    auto s = tiled ? at::empty(tiled_shape(c.size(0), c.size(1)), o) : at::empty({c.size(0), c.size(1) / 32}, o);
+    auto q = fresh({c.size(0), c.size(1) / 2}, at::kByte, c);
+    auto s = tiled ? fresh(tiled_shape(c.size(0), c.size(1)), at::kByte, c) : fresh({c.size(0), c.size(1) / 32}, at::kByte, c);
     check_rc(moe_quantize_rows_mxfp4(c.data_ptr(), dtype_code(c.scalar_type()), c.size(0), c.size(1), tiled ? 1 : 0,
                                      q.data_ptr<uint8_t>(), s.data_ptr<uint8_t>(), cur_stream(c.get_device())),
              "quantize_rows_mxfp4");
@@ -489,7 +494,7 @@ at::Tensor dequantize_mxfp4(const at::Tensor& q, const at::Tensor& s, std::optio
     c10::cuda::CUDAGuard g(c.get_device());
     const auto dt = dtype.value_or(at::kBFloat16);
     const int32_t code = dtype_code(dt);
-    auto y = at::empty({c.size(0), c.size(1) * 2}, c.options().dtype(dt));
+    auto y = fresh({c.size(0), c.size(1) * 2}, dt, c);
     check_rc(moe_dequantize_rows_mxfp4(c.data_ptr<uint8_t>(), sc.data_ptr<uint8_t>(), c.size(0), c.size(1) * 2,
                                        sc.dim() == 3 ? 1 : 0, y.data_ptr(), code, cur_stream(c.get_device())),
              "dequantize_rows_mxfp4");
@@ -501,7 +506,7 @@ at::Tensor tile_scales(const at::Tensor& s) {
                 "scales must be CUDA uint8 [rows, cols/32]");
     auto c = s.contiguous();
     c10::cuda::CUDAGuard g(c.get_device());
-    auto t = at::empty(tiled_shape(c.size(0), c.size(1) * 32), c.options());
+    auto t = fresh(tiled_shape(c.size(0), c.size(1) * 32), at::kByte, c);
     check_rc(moe_mxfp4_tile_scales(c.data_ptr<uint8_t>(), c.size(0), c.size(1) * 32, t.data_ptr<uint8_t>(),
                                    cur_stream(c.get_device())),
              "mxfp4_tile_scales");
@@ -517,7 +522,7 @@ at::Tensor mxfp4_matmul(const at::Tensor& a, const at::Tensor& as, const at::Ten
     c10::cuda::CUDAGuard g(a.get_device());
     const auto dt = dtype.value_or(at::kBFloat16);
     const int32_t code = dtype_code(dt);
-    auto y = at::empty({a.size(0), b.size(0)}, a.options().dtype(dt));
+    auto y = fresh({a.size(0), b.size(0)}, dt, a);
     if (y.numel() == 0) return y;
     check_rc(moe_mxfp4_matmul(ac.data_ptr<uint8_t>(), asc.data_ptr<uint8_t>(), bc.data_ptr<uint8_t>(), bsc.data_ptr<uint8_t>(),
                               a.size(0), b.size(0), a.size(1) * 2, y.data_ptr(), code, cur_stream(a.get_device())),
