@@ -1961,7 +1961,6 @@ extern "C" int moe_engine_forward_dense(moe_engine* eng, int64_t expert, const v
     if (T > eng->dense_cap) {
         CUDA_TRY(cudaDeviceSynchronize());  // the old buffers may still be in use by queued work
         cudaFree(eng->dense_ids);
-    cudaFree(eng->clmeta);
         eng->dense_ids = nullptr;
         int64_t cap = std::max<int64_t>(64, eng->dense_cap);
         while (cap < T) cap *= 2;

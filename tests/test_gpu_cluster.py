@@ -159,3 +159,15 @@ def test_cluster_kernel_deterministic():
     xb, _, ids, w = tokens(T, H, E, 8, 3)
     outs = [run(eng, xb, ids, w, H) for _ in range(3)]
     assert all(np.array_equal(outs[0], o) for o in outs[1:])
+
+
+def test_decode_after_a_dense_call():
+    """A dense call that grows its own buffers leaves the decode kernel's in place."""
+    E, H, I = 16, 512, 256
+    eng, wts = make_engine(1, E, H, I, 91)
+    xb, xf, ids, w = tokens(4, H, E, 8, 91)
+    before = run(eng, xb, ids, w, H)
+    x = torch.zeros((100, H), dtype=torch.bfloat16, device="cuda")
+    eng.forward_dense(0, x, torch.empty_like(x), capi.BF16, capi.BF16)
+    torch.cuda.synchronize()
+    assert np.array_equal(run(eng, xb, ids, w, H), before)
