@@ -96,8 +96,8 @@ int moe_engine_load_awq(moe_engine* eng, const void* w13_qweight, const void* w1
  * of moe_quantize_rows_mxfp4) and multiplies codes by codes, accumulating in fp32:
  *   y = sum_k w_k * down(MX(SiLU(gate MX(x)) * (up MX(x)))).
  * A token row or an h block with an infinity or a NaN gives NaN.  x and y must be 16-byte
- * aligned.  The workspace is the engine's: eager calls on different streams are put in order,
- * replays of captured graphs that hold its calls must not overlap one another or such calls.
+ * aligned.  The workspace is the engine's: eager calls on different streams, from one thread or
+ * several, are put in order; replays of captured graphs that hold its calls must not overlap one another or such calls.
  * A call that is captured needs moe_engine_reserve (or an earlier call of that size) first; the
  * graph stays valid when the workspace grows later.  The peer combine and the no-allocation
  * forward refuse such an engine. */

@@ -106,6 +106,7 @@ struct moe_engine {
     size_t gws_bytes = 0;
     MxLayer* mx = nullptr;         // MXFP4: the layer's weights, workspace and kernels (mxfp4.cu)
     cudaStream_t last_stream = nullptr;  // MXFP4: stream of the last forward (its end is ev1)
+    std::mutex mx_mu;              // MXFP4: one thread at a time orders its call and launches it
     unsigned long long* timeline = nullptr;  // per-CTA phase stamps when enabled
     int timeline_ctas = 0;
 };
@@ -1698,6 +1699,7 @@ extern "C" int moe_engine_reserve(moe_engine* eng, int64_t max_tokens, int64_t t
     DeviceGuard g(eng->cfg.device);
     if (eng->mx) {
         if (top_k > 64) return fail(MOE_ERR_INVALID, "top_k must be at most 64");
+        std::lock_guard<std::mutex> lk(eng->mx_mu);
         return mx_reserve(eng->mx, max_tokens, top_k);
     }
     if ((max_tokens > eng->gemm_min_tokens && gemm_path_ok(eng)) ||
@@ -1750,9 +1752,11 @@ extern "C" int moe_engine_forward(moe_engine* eng, const void* x, void* y, const
         cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
         CUDA_TRY(cudaStreamIsCapturing(st, &cap));
         const bool timed = cap == cudaStreamCaptureStatusNone;
+        std::lock_guard<std::mutex> lk(eng->mx_mu);
         if (timed) {
-            // the workspace is the engine's: a call on another stream follows the last one
-            if (eng->timed && eng->last_stream != st) CUDA_TRY(cudaStreamWaitEvent(st, eng->ev1, 0));
+            // the workspace is the engine's: a call on another stream follows the last one (the
+            // per-thread stream is another one in each thread)
+            if (eng->timed && (eng->last_stream != st || st == cudaStreamPerThread)) CUDA_TRY(cudaStreamWaitEvent(st, eng->ev1, 0));
             CUDA_TRY(cudaEventRecord(eng->ev0, st));
         }
         MxForward f{x, y, topk_ids, topk_w, T, K, act_dtype, out_dtype, eng->emap, eng->emap_n, eng->err,

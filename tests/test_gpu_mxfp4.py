@@ -147,7 +147,8 @@ def test_product_shapes(M, N):
     check_product(M, N, 320, 1000 * M + N, ("float32",))
 
 
-@pytest.mark.parametrize("M,N,K", [(1000, 1000, 1024), (1, 4096, 2048), (3, 2049, 4096), (2000, 96, 512), (4100, 1288, 288), (2333, 2050, 64), (1300, 4104, 96)])
+@pytest.mark.parametrize("M,N,K", [(1000, 1000, 1024), (1, 4096, 2048), (3, 2049, 4096), (2000, 96, 512), (4100, 1288, 288), (2333, 2050, 64), (1300, 4104, 96),
+                                   (2500, 2050, 320), (5, 40000, 96), (130, 38000, 64)])
 def test_product_large(M, N, K):
     check_product(M, N, K, M, ("bfloat16", "float16", "float32") if K < 1024 else ("bfloat16", "float32"))
 

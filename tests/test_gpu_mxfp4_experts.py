@@ -290,3 +290,111 @@ def test_router_to_output(T):
     a = R.decode(*R.quantize(y.double().cpu().numpy()))
     b = ops.dequantize_rows_mxfp4(lw, ls, torch.float32).double().cpu().numpy()
     close(z, a @ b.T, R.product_error(a, b) + R.HALF["float32"] * np.abs(a @ b.T))
+
+
+@pytest.mark.parametrize("T,K", [(1, 16), (2, 8), (1, 20), (3, 33), (40, 64)])
+def test_same_expert_many_times(T, K):
+    """More pairs of one expert in a token than a tile of few rows holds, and long lists of ids."""
+    E, H, I = 80, 128, 96
+    packed, w13, w2 = weights(E, H, I, 30)
+    h = handle(E, H, I, packed)
+    x, ids, w = tokens(T, H, E, K, 31)
+    for same in (True, False):
+        if same:
+            ids[:, : K - K // 4] = 7
+        want, tol = R.experts(x.double().cpu().numpy(), ids, w, w13, w2, "bfloat16")
+        close(ops.moe_forward(x, cuda(ids), cuda(w), h), want, tol)
+        ids = tokens(T, H, E, K, 32)[1]
+
+
+@pytest.mark.parametrize("E,H,I,K,T", [(1024, 64, 32, 8, 1), (1024, 64, 32, 8, 37), (1024, 64, 32, 8, 5000), (3, 8224, 32, 2, 1),
+                                       (3, 8224, 32, 2, 5), (3, 64, 4128, 2, 2), (2, 32, 32, 1, 1), (2, 32, 32, 1, 513)])
+def test_largest_and_smallest_sizes(E, H, I, K, T):
+    packed, w13, w2 = weights(E, H, I, 33)
+    h = handle(E, H, I, packed)
+    x, ids, w = tokens(T, H, E, K, 34)
+    y = ops.moe_forward(x, cuda(ids), cuda(w), h)
+    some = np.unique(np.linspace(0, T - 1, 300).astype(int))
+    want, tol = R.experts(x.double().cpu().numpy()[some], ids[some], w[some], w13, w2, "bfloat16")
+    close(y[torch.from_numpy(some).cuda()], want, tol)
+
+
+@pytest.mark.parametrize("T", [1, 3, 60, 300])
+def test_replicated_experts(T):
+    """Ranks that share hot experts compute each pair once."""
+    from moe_ascend_opt_b200.ep import replicated_placement
+    E, H, I, K, W = 14, 128, 96, 4, 3
+    packed, w13, w2 = weights(E, H, I, 35)
+    x, ids, w = tokens(T, H, E, K, 36)
+    pl, hot = replicated_placement(np.bincount(ids.ravel(), minlength=E), W, 2)
+    total = torch.zeros(T, H, device="cuda")
+    for r in range(W):
+        h = torch.classes.nanovllm.MoEInfer(E, H, I, 3)
+        h.set_expert_parallel(r, W)
+        h.set_expert_placement(pl[r])
+        h.set_expert_replicas(hot)
+        h.store_mxfp4(*[torch.from_numpy(p) for p in packed])
+        total += ops.moe_forward_partial(x, cuda(ids), cuda(w), h)
+    want, tol = R.experts(x.double().cpu().numpy(), ids, w, w13, w2, "float32")
+    close(total, want, W * tol)
+
+
+@pytest.mark.parametrize("T", [1, 12, 400])
+def test_captured_step_follows_its_routing(T):
+    """Routing, experts and a product in one graph, replayed with other tokens, equal the eager calls."""
+    E, H, I, K, N = 8, 256, 128, 2, 96
+    packed, _, _ = weights(E, H, I, 37)
+    h = handle(E, H, I, packed)
+    x = tokens(T, H, E, K, 38)[0]
+    rng = np.random.default_rng(39)
+    logits = cuda(rng.standard_normal((T, E)).astype(np.float32))
+    lw, ls = ops.quantize_rows_mxfp4(cuda(rng.standard_normal((N, H)).astype(np.float32)), True)
+
+    def step():
+        ids, w = ops.moe_route_scored(logits, None, K, "softmax", 1, 1, 1, True, 1.0)
+        q, s = ops.quantize_rows_mxfp4(ops.moe_forward(x, ids, w, h), True)
+        return ops.mxfp4_matmul(q, s, lw, ls, torch.bfloat16)
+
+    step()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        z = step()
+    for seed in (1, 2, 3):
+        x.copy_(tokens(T, H, E, K, 40 + seed)[0])
+        logits.copy_(cuda(np.random.default_rng(seed).standard_normal((T, E)).astype(np.float32)))
+        if seed == 2:
+            logits[:, 1:] = -float("inf")  # one expert takes every token's first place
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(z, step())
+    assert h.device_error() == 0
+
+
+def test_threads_with_streams_of_their_own():
+    import threading
+    E, H, I, K, T = 8, 256, 128, 4, 150
+    packed, _, _ = weights(E, H, I, 44)
+    x, ids, w = tokens(T, H, E, K, 45)
+    idc, wc = cuda(ids), cuda(w)
+    shared = handle(E, H, I, packed)
+    first = ops.moe_forward(x, idc, wc, shared)
+    q, s = ops.quantize_rows_mxfp4(x, True)
+    product = ops.mxfp4_matmul(q, s, q, s, torch.float32)
+    torch.cuda.synchronize()
+    bad = []
+
+    def work(i):
+        own = handle(E, H, I, packed) if i % 2 else shared
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(20):
+                y = ops.moe_forward(x, idc, wc, own)
+                z = ops.mxfp4_matmul(*ops.quantize_rows_mxfp4(x, True), q, s, torch.float32)
+                if not (torch.equal(y, first) and torch.equal(z, product)):
+                    bad.append(i)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not bad
