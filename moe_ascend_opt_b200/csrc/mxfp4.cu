@@ -50,6 +50,11 @@ int encode_map(CUtensorMap* m, CUtensorMapDataType type, CUtensorMapSwizzle swiz
     return MOE_OK;
 }
 
+// Scales as rows of `words` 32-bit words, boxes of 1 KB (a stage's scales of 128 rows) x box_rows.
+int encode_scales(CUtensorMap* m, const void* base, int64_t words, int64_t rows, int box_rows) {
+    return encode_map(m, CU_TENSOR_MAP_DATA_TYPE_UINT32, CU_TENSOR_MAP_SWIZZLE_NONE, base, 4, words, rows, 256, box_rows);
+}
+
 // Codes as bytes [rows][pitch], boxes of 128 bytes x box_rows, 128-byte swizzle; what lies outside
 // reads as zero.
 int encode(CUtensorMap* m, const void* base, int64_t pitch, int64_t rows, int box_rows) {
@@ -77,10 +82,10 @@ int allow_smem(const void* fn, int bytes) {
     return MOE_OK;
 }
 
-template <typename... P, typename... A>
+template <int CLUSTER = 1, typename... P, typename... A>
 int launch(void (*fn)(P...), unsigned grid, unsigned block, size_t smem, bool pdl, cudaStream_t st, A&&... args) {
     cudaLaunchConfig_t cfg{};
-    cudaLaunchAttribute attr[1];
+    cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.gridDim = dim3(grid);
@@ -89,6 +94,12 @@ int launch(void (*fn)(P...), unsigned grid, unsigned block, size_t smem, bool pd
     cfg.stream = st;
     cfg.attrs = attr;
     cfg.numAttrs = pdl ? 1 : 0;
+    if (CLUSTER > 1) {
+        cudaLaunchAttribute& a = attr[cfg.numAttrs++];
+        a.id = cudaLaunchAttributeClusterDimension;
+        a.val.clusterDim.x = CLUSTER;
+        a.val.clusterDim.y = a.val.clusterDim.z = 1;
+    }
     CUDA_TRY(cudaLaunchKernelEx(&cfg, fn, P(args)...));
     return MOE_OK;
 }
@@ -109,6 +120,7 @@ int sm_count(int dev, int* out) {
 // kernel on an SM, so that down's first weights arrive while gate_up runs.
 using Wide = mx::Shape<256, 128, 4, 8, 1, 1>;
 using WideDown = mx::Shape<256, 128, 3, 8, 1, 1, false, 4>;
+using Pair = mx::Shape<256, 128, 6, 8, 1, 1, false, 1, true>;
 using Narrow = mx::Shape<64, 128, 4, 4, 2, 2>;
 using Slim = mx::Shape<128, 32, 9, 4, 1, 2>;
 using FusedUp = mx::Shape<128, 8, 7, 4, 2, 1, true>;
@@ -117,14 +129,16 @@ using FusedDown = mx::Shape<128, 8, 3, 4, 2, 1, true>;
 constexpr int kFusedStages = 32;  // depth of fused calls: their A buffers hold it whole
 
 template <int MODE, class S>
-int launch_gemm(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& ta32, const CUtensorMap& to, mx::GemmParams& p, int64_t m_tiles, int sms,
-                bool pdl, cudaStream_t st) {
+int launch_gemm(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& ta32, const CUtensorMap& to, const CUtensorMap& tfa,
+                const CUtensorMap& tfb, mx::GemmParams& p, int64_t m_tiles, int sms, bool pdl, cudaStream_t st) {
     auto fn = mx::mx_gemm_kernel<MODE, S>;
     constexpr bool WA = S::FUSED && MODE == mx::kGateUp;
     const int smem = S::smem(WA, (int)ceil_div(p.K, mx::kStageK));
     if (int rc = allow_smem(reinterpret_cast<const void*>(fn), S::smem(WA, kFusedStages))) return rc;
     p.nt_count = (int)ceil_div(p.N, S::NT);
-    return launch(fn, (unsigned)std::min<int64_t>(m_tiles * p.nt_count, sms * (S::FUSED ? 1 : S::kCtas)), S::kThreads, smem, pdl, st, ta, tb, ta32, to, p);
+    const int64_t at_once = S::PAIR ? sms / 2 : sms * (S::FUSED ? 1 : S::kCtas);  // tiles
+    const unsigned grid = (unsigned)(std::min(m_tiles * p.nt_count, at_once) * (S::PAIR ? 2 : 1));
+    return launch<S::PAIR ? 2 : 1>(fn, grid, S::kThreads, smem, pdl, st, ta, tb, ta32, to, tfa, tfb, p);
 }
 
 bool dtype_ok(int32_t t) { return t == MOE_F16 || t == MOE_BF16 || t == MOE_F32; }
@@ -254,9 +268,9 @@ extern "C" int moe_mxfp4_matmul(const uint8_t* a, const uint8_t* a_scales, const
     }
     CUtensorMap ta, tb;
     if (int rc = encode(&ta, a, K / 2, M, 128)) return rc;
-    p.mt_count = (int)ceil_div(M, 128);
-    const bool wide = p.mt_count * ceil_div(N, Wide::NT) >= sms;
-    if (int rc = encode(&tb, b, K / 2, N, wide ? Wide::NT : Narrow::NT)) return rc;
+    const bool wide = ceil_div(M, 128) * ceil_div(N, Pair::NT) >= sms;
+    p.mt_count = (int)ceil_div(M, wide ? Pair::kTileRows : Narrow::kTileRows);
+    if (int rc = encode(&tb, b, K / 2, N, wide ? Pair::NT / 2 : Narrow::NT)) return rc;
     p.M = (int)M; p.N = (int)N; p.K = (int)K;
     p.kb = (int)ceil_div(K, 128);
     p.sfa = a_scales;
@@ -268,8 +282,11 @@ extern "C" int moe_mxfp4_matmul(const uint8_t* a, const uint8_t* a_scales, const
     p.tma_out = wide && N * esz % 16 == 0;
     if (p.tma_out)
         if (int rc = encode_out(&to, y, esz, N, M)) return rc;
-    return wide ? launch_gemm<mx::kDense, Wide>(ta, tb, ta, to, p, p.mt_count, sms, false, st)
-                : launch_gemm<mx::kDense, Narrow>(ta, tb, ta, to, p, p.mt_count, sms, false, st);
+    if (!wide) return launch_gemm<mx::kDense, Narrow>(ta, tb, ta, to, ta, ta, p, p.mt_count, sms, false, st);
+    CUtensorMap tfa, tfb;
+    if (int rc = encode_scales(&tfa, a_scales, p.kb * 128, ceil_div(M, 128), 1)) return rc;
+    if (int rc = encode_scales(&tfb, b_scales, p.kb * 128, ceil_div(N, 128), 2)) return rc;
+    return launch_gemm<mx::kDense, Pair>(ta, tb, ta, to, tfa, tfb, p, p.mt_count, sms, false, st);
 }
 
 // ------------------------------------------------------------------ expert layer
@@ -453,12 +470,12 @@ int forward_fused(MxLayer* l, const MxForward& f, const void* x, void* y, const 
     mx::GemmParams g1 = p;
     g1.N = (int)(2 * I); g1.K = (int)H; g1.kb = (int)l->kb1;
     g1.sfb = l->s1; g1.hq = w.hq; g1.hs = w.hs; g1.hkb = (int)l->kb2;
-    if (int rc = launch_gemm<mx::kGateUp, FusedUp>(th, l->t1[0], th, th, g1, w.mt, l->sms, f.pdl, st)) return rc;
+    if (int rc = launch_gemm<mx::kGateUp, FusedUp>(th, l->t1[0], th, th, th, th, g1, w.mt, l->sms, f.pdl, st)) return rc;
     mx::GemmParams g2 = p;
     g2.N = (int)H; g2.K = (int)I; g2.kb = (int)l->kb2;
     g2.sfa = w.hs; g2.sfb = l->s2; g2.out = w.part; g2.out_dtype = MOE_F32;
     g2.y = y; g2.y_dtype = f.out_dtype; g2.cnt = f.cnt;
-    return launch_gemm<mx::kDown, FusedDown>(th, l->t2[0], th, th, g2, w.mt, l->sms, f.pdl, st);
+    return launch_gemm<mx::kDown, FusedDown>(th, l->t2[0], th, th, th, th, g2, w.mt, l->sms, f.pdl, st);
 }
 
 int forward_slice(MxLayer* l, const MxForward& f, const void* x, void* y, const int32_t* ids, const float* tw, int64_t T,
@@ -501,8 +518,8 @@ int forward_slice(MxLayer* l, const MxForward& f, const void* x, void* y, const 
     mx::GemmParams g1 = p;
     g1.N = (int)(2 * I); g1.K = (int)H; g1.kb = (int)l->kb1;
     g1.sfa = w.xs; g1.sfb = l->s1; g1.hq = w.hq; g1.hs = w.hs; g1.hkb = (int)l->kb2;
-    if (int rc = wide ? launch_gemm<mx::kGateUp, Wide>(tx, l->t1[1], tx32, tx, g1, w.mt, l->sms, f.pdl, st)
-                      : launch_gemm<mx::kGateUp, Slim>(tx, l->t1[0], tx, tx, g1, w.mt, l->sms, f.pdl, st))
+    if (int rc = wide ? launch_gemm<mx::kGateUp, Wide>(tx, l->t1[1], tx32, tx, tx, tx, g1, w.mt, l->sms, f.pdl, st)
+                      : launch_gemm<mx::kGateUp, Slim>(tx, l->t1[0], tx, tx, tx, tx, g1, w.mt, l->sms, f.pdl, st))
         return rc;
     mx::GemmParams g2 = p;
     g2.N = (int)H; g2.K = (int)I; g2.kb = (int)l->kb2;
@@ -512,8 +529,8 @@ int forward_slice(MxLayer* l, const MxForward& f, const void* x, void* y, const 
     CUtensorMap tp = th;  // used by wide tiles
     if (wide)
         if (int rc = encode_out(&tp, w.part, part16 ? 2 : 4, H, w.mt * w.tile)) return rc;
-    if (int rc = wide ? launch_gemm<mx::kDown, WideDown>(th, l->t2[1], th32, tp, g2, w.mt, l->sms, f.pdl, st)
-                      : launch_gemm<mx::kDown, Slim>(th, l->t2[0], th, tp, g2, w.mt, l->sms, f.pdl, st))
+    if (int rc = wide ? launch_gemm<mx::kDown, WideDown>(th, l->t2[1], th32, tp, th, th, g2, w.mt, l->sms, f.pdl, st)
+                      : launch_gemm<mx::kDown, Slim>(th, l->t2[0], th, tp, th, th, g2, w.mt, l->sms, f.pdl, st))
         return rc;
     if (f.out_dtype == MOE_F32) return combine_launch<MOE_F32, false>(l, f, tw, y, w, T, st);
     if (f.out_dtype == MOE_BF16)

@@ -57,13 +57,15 @@ struct GemmParams {
 // A kernel's shape: NT columns and TM rows of a tile (the MMA always takes 128 rows; of a tile of fewer it
 // reads whatever lies behind them in shared memory, and those lanes are never read back), STAGES of the
 // ring, EPI epilogue warps, CTAS per SM, ACC accumulators, BUFS staging buffers of a wide tile's epilogue warp.
-template <int NT_, int TM_, int STAGES_, int EPI_, int CTAS_, int ACC_, bool FUSED_ = false, int BUFS_ = 1>
+// PAIR: the two CTAs of a cluster share a tile of 256 rows, 128 rows (TM) each, and each fetches half of B.
+template <int NT_, int TM_, int STAGES_, int EPI_, int CTAS_, int ACC_, bool FUSED_ = false, int BUFS_ = 1, bool PAIR_ = false>
 struct Shape {
     static constexpr int NT = NT_, TM = TM_, STAGES = STAGES_, kEpiWarps = EPI_, kCtas = CTAS_;
-    static constexpr bool FUSED = FUSED_;
+    static constexpr bool FUSED = FUSED_, PAIR = PAIR_;
     static constexpr int BUFS = BUFS_;  // staging buffers of an epilogue warp
     static constexpr int kSfTiles = (NT + 127) / 128;  // scale tiles (128 rows) that cover a stage's B rows
-    static constexpr int kA = TM * 128, kB = NT * 128;
+    static constexpr int kA = TM * 128, kB = NT * 128 / (PAIR ? 2 : 1);
+    static constexpr int kTileRows = PAIR ? 256 : TM;
     static constexpr int kSfaKg = TM == 8 ? 128 : 512;  // scales of A for 128 elements: those of 8 rows, or a tile
     static constexpr int kSfbBytes = 1024 * kSfTiles;
     // A stage of the ring: A | B | scales of B | scales of A, the first and the last not where the kernel
@@ -89,7 +91,7 @@ struct Shape {
     }
     __host__ __device__ static constexpr int smem(bool wa, int stages) {
         const int ring = STAGES * stage(wa), buffers = wa ? 2 * a_buffer(stages) : 0;
-        return buffers + ring + tail(wa) + kStaging + (kRows + 1023) / 1024 * 1024 + 1024;
+        return buffers + ring + tail(wa) + kStaging + (kRows + 1023) / 1024 * 1024;
     }
 };
 
@@ -105,17 +107,56 @@ __host__ __device__ constexpr uint32_t idesc_mxf4(int M, int N) {
     return (1u << 7) | (1u << 10) | ((uint32_t)(N >> 3) << 17) | (1u << 23) | ((uint32_t)(M >> 4) << 24);
 }
 
+// PAIR: one instruction for the two CTAs of a cluster, 256 rows; each holds its 128 rows of A, its half of
+// B's rows, and its accumulators, at the same addresses.
+template <bool PAIR>
 MOE_DEV void mma_mxf4(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sfa, uint32_t sfb, bool accumulate) {
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %6, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
-        ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"((uint32_t)accumulate)
-        : "memory");
+    if (PAIR)
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "setp.ne.b32 p, %6, 0;\n\t"
+            "tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
+            ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"((uint32_t)accumulate)
+            : "memory");
+    else
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "setp.ne.b32 p, %6, 0;\n\t"
+            "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
+            ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"((uint32_t)accumulate)
+            : "memory");
 }
 
+template <bool PAIR>
 MOE_DEV void cp_scales(uint32_t taddr, uint64_t desc) {
-    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+    if (PAIR) asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+    else asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+}
+
+// Arrival on a barrier (PAIR: on that of both CTAs) when the MMAs issued so far are complete.
+template <bool PAIR>
+MOE_DEV void commit(uint64_t* bar) {
+    if (PAIR)
+        asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+                         smem_u32(bar)),
+                     "h"((uint16_t)3)
+                     : "memory");
+    else
+        gemm::tc_commit(bar);
+}
+
+// Shared memory of CTA 0 of the cluster at the place of this CTA's `addr`, and an arrival there.  tcgen05's own
+// fences order the accumulators' reads before it, so it carries no release (which took about a microsecond).
+MOE_DEV uint32_t in_leader(uint32_t addr) {
+    uint32_t a;
+    asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(a) : "r"(addr));
+    return a;
+}
+MOE_DEV void arrive_leader(uint64_t* bar) {
+    asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(in_leader(smem_u32(bar))) : "memory");
+}
+MOE_DEV void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
 // One lane of a converged warp.
@@ -131,6 +172,13 @@ MOE_DEV void tma_2d(uint32_t dst, const CUtensorMap* m, int x, int y, uint32_t b
         "l"(m), "r"(x), "r"(y), "r"(bar)
         : "memory");
 }
+// PAIR: into this CTA's shared memory, counted by a barrier of CTA 0 of the cluster.
+MOE_DEV void tma_2d_pair(uint32_t dst, const CUtensorMap* m, int x, int y, uint32_t bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
+        "l"(m), "r"(x), "r"(y), "r"(bar)
+        : "memory");
+}
 MOE_DEV void bulk_copy(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
     asm volatile("cp.async.bulk.shared::cta.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src),
                  "r"(bytes), "r"(bar)
@@ -142,10 +190,23 @@ MOE_DEV void tma_store_2d(const CUtensorMap* m, uint32_t src, int x, int y) {
                  : "memory");
     asm volatile("cp.async.bulk.commit_group;" ::: "memory");
 }
+// As mbar_try_wait, for arrivals from the other CTA of the cluster (arrive_leader).
+MOE_DEV bool mbar_try_wait_cluster(uint64_t* bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.relaxed.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(smem_u32(bar)), "r"(parity)
+        : "memory");
+    return ok != 0;
+}
 // Bounded wait that also ends when another role of the CTA has given up.
+template <bool CLUSTER>
 MOE_DEV bool wait_or_fail(uint64_t* bar, uint32_t parity, volatile int* failed) {
     for (uint32_t it = 0; it < kSpinLimit; ++it) {
-        if (mbar_try_wait(bar, parity)) return true;
+        if (CLUSTER ? mbar_try_wait_cluster(bar, parity) : mbar_try_wait(bar, parity)) return true;
         if ((it & 15u) == 15u && *failed) return false;
         if (it > 8192) __nanosleep(128);
     }
@@ -154,8 +215,9 @@ MOE_DEV bool wait_or_fail(uint64_t* bar, uint32_t parity, volatile int* failed) 
 }
 
 // The same by a whole warp, which goes on or leaves together.
+template <bool CLUSTER = false>
 MOE_DEV bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* failed) {
-    return __all_sync(0xffffffffu, wait_or_fail(bar, parity, failed));
+    return __all_sync(0xffffffffu, wait_or_fail<CLUSTER>(bar, parity, failed));
 }
 
 // N consecutive fp32 columns of this thread's TMEM lane.
@@ -354,15 +416,18 @@ template <int MODE, class S>
 __global__ void __launch_bounds__(S::kThreads, S::kCtas)
     mx_gemm_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtensorMap tb,
                    const __grid_constant__ CUtensorMap ta32, const __grid_constant__ CUtensorMap to,
+                   const __grid_constant__ CUtensorMap tfa, const __grid_constant__ CUtensorMap tfb,
                    const __grid_constant__ GemmParams p) {
     constexpr int NT = S::NT, TM = S::TM, STAGES = S::STAGES;
+    constexpr bool PAIR = S::PAIR;
+    static_assert(!PAIR || MODE == kDense, "pairs take dense products");
     constexpr bool FUSED = S::FUSED, WRITE_A = FUSED && MODE == kGateUp;  // A from the token rows, by warps 2 and 3
     constexpr int kSfBase = S::kAcc * NT;  // TMEM: the accumulators, then each stage's scales
     constexpr int kTmemCols = kSfBase + STAGES * S::kSfCols <= 256 ? 256 : 512;
     static_assert(kSfBase + STAGES * S::kSfCols <= 512 && kTmemCols * S::kCtas <= 512, "TMEM");
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     constexpr int kStage = S::stage(WRITE_A), oB = S::off_b(WRITE_A), oSfB = S::off_sfb(WRITE_A), oSfA = S::off_sfa(WRITE_A);
-    uint8_t* abuf = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    uint8_t* abuf = smem_raw;
     const int nstages = (p.K + kStageK - 1) / kStageK, k64 = (p.K + 63) / 64;
     uint8_t* smem = abuf + (WRITE_A ? 2 * S::a_buffer(nstages) : 0);  // the ring
     __shared__ __align__(8) uint64_t s_full[STAGES], s_empty[STAGES], s_accfull[2], s_accempty[2], s_afull[2], s_aempty[2], s_done;
@@ -370,6 +435,10 @@ __global__ void __launch_bounds__(S::kThreads, S::kCtas)
     __shared__ int s_failed, s_go, s_last;
     __shared__ typename RouteStore<FUSED>::type s_route;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    if (smem_u32(smem_raw) & 1023) {  // the swizzled tiles rely on it; in every CTA or in none
+        if (tid == 0) set_err(p.err, kErrFullWait);
+        return;
+    }
 
     if (tid == 0) {
         for (int s = 0; s < STAGES; ++s) {
@@ -378,7 +447,7 @@ __global__ void __launch_bounds__(S::kThreads, S::kCtas)
         }
         for (int a = 0; a < 2; ++a) {
             mbar_init(&s_accfull[a], 1);
-            mbar_init(&s_accempty[a], TM < 128 ? 1 : S::kEpiWarps);
+            mbar_init(&s_accempty[a], TM < 128 ? 1 : S::kEpiWarps * (PAIR ? 2 : 1));
             mbar_init(&s_afull[a], 2);
             mbar_init(&s_aempty[a], 1);
         }
@@ -387,12 +456,19 @@ __global__ void __launch_bounds__(S::kThreads, S::kCtas)
         fence_barrier_init();
     }
     if (warp == 2) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&s_tmem)), "n"(kTmemCols)
-                     : "memory");
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        if (PAIR) {
+            asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&s_tmem)), "n"(kTmemCols)
+                         : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+        } else {
+            asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&s_tmem)), "n"(kTmemCols)
+                         : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        }
     }
     gemm::tc_fence_before();
     __syncthreads();
+    if (PAIR) cluster_sync();  // the peer's barriers are ready
     gemm::tc_fence_after();
     const uint32_t tmem = s_tmem;
     volatile int* failed = &s_failed;
@@ -405,10 +481,12 @@ __global__ void __launch_bounds__(S::kThreads, S::kCtas)
 
     const int mt_count = FUSED ? route.np : p.mt_count;  // of an expert list its bound
     const int64_t tiles = (int64_t)mt_count * p.nt_count;
+    const int rank = PAIR ? (int)(blockIdx.x & 1) : 0;  // in the cluster
+    const int first = PAIR ? blockIdx.x >> 1 : blockIdx.x, step = PAIR ? gridDim.x >> 1 : gridDim.x;
     const int nb128 = (p.N + 127) / 128;
     auto tile_of = [&](int mt) {  // expert, rows; no rows: past the list's end
         if (FUSED) return make_int2(route.piece_e[mt], route.rows[mt]);
-        return MODE == kDense ? make_int2(0, min(TM, p.M - mt * TM)) : __ldcg(p.mt_list + mt);
+        return MODE == kDense ? make_int2(0, min(S::kTileRows, p.M - mt * S::kTileRows)) : __ldcg(p.mt_list + mt);
     };
 
     if (warp == 0) {
@@ -429,11 +507,24 @@ __global__ void __launch_bounds__(S::kThreads, S::kCtas)
             }
             bulk_copy(base + oSfA, p.sfa + ((int64_t)mt * p.kb + 2 * s) * S::kSfaKg, min(2, p.kb - 2 * s) * S::kSfaKg, bar);
         };
-        int2 next = blockIdx.x < tiles ? tile_of((int)(blockIdx.x / p.nt_count)) : make_int2(0, 0);
-        for (int64_t tile = blockIdx.x; ok && tile < tiles; tile += gridDim.x) {
+        // a pair's stage: both CTAs' copies count on CTA 0's barrier; the second 128 rows may not exist
+        auto load_pair = [&](int mt, int nt, int s) {
+            const bool both = p.M - mt * 256 > 128;
+            const uint32_t base = usmem + st * kStage, bar = in_leader(smem_u32(&s_full[st]));
+            if (rank == 0)
+                mbar_arrive_expect_tx(&s_full[st], (both ? 2 : 1) * (S::kA + 2 * S::kSfaKg) + 2 * (S::kB + S::kSfbBytes));
+            tma_2d_pair(base + oB, &tb, s * 128, nt * NT + rank * (NT / 2), bar);
+            tma_2d_pair(base + oSfB, &tfb, s * 256, nt * NT / 128, bar);
+            if (rank == 0 || both) {
+                tma_2d_pair(base, &ta, s * 128, mt * 256 + rank * 128, bar);
+                tma_2d_pair(base + oSfA, &tfa, s * 256, mt * 2 + rank, bar);
+            }
+        };
+        int2 next = first < tiles ? tile_of((int)(first / p.nt_count)) : make_int2(0, 0);
+        for (int64_t tile = first; ok && tile < tiles; tile += step) {
             const int mt = (int)(tile / p.nt_count), nt = (int)(tile - (int64_t)mt * p.nt_count);
             const int2 of = next;
-            if (tile + gridDim.x < tiles) next = tile_of((int)((tile + gridDim.x) / p.nt_count));  // a tile ahead of its use
+            if (tile + step < tiles) next = tile_of((int)((tile + step) / p.nt_count));  // a tile ahead of its use
             const int e = __shfl_sync(0xffffffffu, of.x, 0), rows = __shfl_sync(0xffffffffu, of.y, 0);
             if (rows == 0) break;
             const int copies = MODE == kDense || TM < 128 ? 4 : (rows + 31) >> 5;  // quarters of a 128-row tile
@@ -445,12 +536,14 @@ __global__ void __launch_bounds__(S::kThreads, S::kCtas)
             const uint8_t* sfb = MODE == kDense ? p.sfb + (int64_t)(nt * NT / 128) * p.kb * 512
                                                 : p.sfb + panel0 * kPanelScales + in_panel / 128 * 1024;
             const bool early = MODE == kDown && it == 0;
-            const int first = early ? min(STAGES, nstages) : 0;
+            const int ahead = early ? min(STAGES, nstages) : 0;
             for (int s = 0; s < nstages; ++s, ++it) {
                 if (!warp_wait(&s_empty[st], parity, failed)) { ok = false; break; }
                 const uint32_t base = usmem + st * kStage, bar = smem_u32(&s_full[st]);
                 const int kgs = min(2, p.kb - 2 * s), sfn = kgs * 512;
-                if (issue) {
+                if (PAIR) {
+                    if (issue) load_pair(mt, nt, s);
+                } else if (issue) {
                     const int sfbytes = MODE == kDense ? sfn * sft : S::kSfbBytes;
                     mbar_arrive_expect_tx(&s_full[st], (WRITE_A ? 0 : copies * (S::kA / 4) + kgs * S::kSfaKg) + S::kB + sfbytes);
                     if (MODE == kDense) {
@@ -462,13 +555,13 @@ __global__ void __launch_bounds__(S::kThreads, S::kCtas)
                         tma_2d(base + oB, &tb, 0, (int)((panel0 + s) * kPanelRows) + in_panel, bar);
                         bulk_copy(base + oSfB, sfb + (int64_t)s * kPanelScales, S::kSfbBytes, bar);
                     }
-                    if (!WRITE_A && s >= first) load_a(st, mt, s, copies);
+                    if (!WRITE_A && s >= ahead) load_a(st, mt, s, copies);
                 }
                 __syncwarp();
-                if (!WRITE_A && s < first && s == first - 1) {
+                if (!WRITE_A && s < ahead && s == ahead - 1) {
                     asm volatile("griddepcontrol.wait;" ::: "memory");
                     if (issue)
-                        for (int a = 0; a < first; ++a) load_a(a, mt, a, copies);
+                        for (int a = 0; a < ahead; ++a) load_a(a, mt, a, copies);
                     __syncwarp();
                 }
                 if (++st == STAGES) {
@@ -483,31 +576,33 @@ __global__ void __launch_bounds__(S::kThreads, S::kCtas)
             for (uint32_t b = 0; b < STAGES && b < it; ++b) {
                 const uint32_t j = it - 1 - b;
                 bool in = false;
-                for (uint32_t n = 0; n < kSpinLimit && !in; ++n) in = mbar_try_wait(&s_full[j % STAGES], j / STAGES & 1);
+                // a pair's are complete when its MMAs have read them, which also leaves no arrival to come
+                uint64_t* const bar = PAIR ? &s_empty[j % STAGES] : &s_full[j % STAGES];
+                for (uint32_t n = 0; n < kSpinLimit && !in; ++n) in = mbar_try_wait(bar, j / STAGES & 1);
                 if (!in) *failed = 1;
             }
         }
         __syncwarp();
-    } else if (warp == 1) {
+    } else if (warp == 1 && rank == 0) {  // of a pair, CTA 0 issues for both
         // The whole warp walks the loop, so that addresses and descriptors stay in uniform
         // registers, and one elected lane issues.
-        constexpr uint32_t idesc = idesc_mxf4(128, NT);
+        constexpr uint32_t idesc = idesc_mxf4(PAIR ? 256 : 128, NT);
         const uint32_t utmem = __shfl_sync(0xffffffffu, tmem, 0), usmem = __shfl_sync(0xffffffffu, smem_u32(smem), 0);
         const uint32_t uabuf = __shfl_sync(0xffffffffu, smem_u32(abuf), 0);
         const bool issue = elect_one();
         uint32_t n = 0, st = 0, parity = 0;  // tiles so far; stage and phase of the ring
         bool ok = true;
-        int next = blockIdx.x < tiles ? tile_of((int)(blockIdx.x / p.nt_count)).y : 0;
-        for (int64_t tile = blockIdx.x; ok && tile < tiles; tile += gridDim.x, ++n) {
+        int next = first < tiles ? tile_of((int)(first / p.nt_count)).y : 0;
+        for (int64_t tile = first; ok && tile < tiles; tile += step, ++n) {
             const uint32_t acc = n % S::kAcc, d = utmem + acc * NT;
             if (MODE != kDense && !FUSED) {
                 const int rows = next;
-                if (tile + gridDim.x < tiles) next = tile_of((int)((tile + gridDim.x) / p.nt_count)).y;
+                if (tile + step < tiles) next = tile_of((int)((tile + step) / p.nt_count)).y;
                 if (__shfl_sync(0xffffffffu, rows, 0) == 0) break;
             }
             // half a scale tile (NT = 64): its rows' columns are 0-1 or 2-3 of the tile's four
             const uint32_t half = NT == 64 ? (uint32_t)(tile % p.nt_count & 1) * 2 : 0;
-            if (!warp_wait(&s_accempty[acc], (n / S::kAcc & 1) ^ 1, failed)) break;
+            if (!warp_wait<PAIR>(&s_accempty[acc], (n / S::kAcc & 1) ^ 1, failed)) break;
             if (WRITE_A && !warp_wait(&s_afull[n & 1], n >> 1 & 1, failed)) break;
             gemm::tc_fence_after();
             for (int s = 0; s < nstages; ++s) {
@@ -525,16 +620,16 @@ __global__ void __launch_bounds__(S::kThreads, S::kCtas)
 #pragma unroll
                     for (int i = 0; i < 2; ++i)
                         if (i < nkb) {
-                            cp_scales(tsa + 4 * i, dsa + S::kSfaKg / 16 * i);
+                            cp_scales<PAIR>(tsa + 4 * i, dsa + S::kSfaKg / 16 * i);
 #pragma unroll
-                            for (int b = 0; b < S::kSfTiles; ++b) cp_scales(tsb + kColsB * i + 4 * b, dsb + 64 * b + 32 * i);
+                            for (int b = 0; b < S::kSfTiles; ++b) cp_scales<PAIR>(tsb + kColsB * i + 4 * b, dsb + 64 * b + 32 * i);
                         }
 #pragma unroll
                     for (int j = 0; j < 4; ++j)
                         if (j < nk)  // 64 elements are 32 bytes inside the swizzle atom
-                            mma_mxf4(d, da + 2 * j, db + 2 * j, idesc | (uint32_t)(j & 1) * 2 << 4 | (uint32_t)(j & 1) * 2 << 29,
+                            mma_mxf4<PAIR>(d, da + 2 * j, db + 2 * j, idesc | (uint32_t)(j & 1) * 2 << 4 | (uint32_t)(j & 1) * 2 << 29,
                                      tsa + 4 * (j >> 1), tsb + kColsB * (j >> 1) + half, s > 0 || j > 0);
-                    gemm::tc_commit(&s_empty[st]);
+                    commit<PAIR>(&s_empty[st]);
                 }
                 __syncwarp();
                 if (++st == STAGES) {
@@ -543,13 +638,16 @@ __global__ void __launch_bounds__(S::kThreads, S::kCtas)
                 }
             }
             if (ok && issue) {
-                if (WRITE_A) gemm::tc_commit(&s_aempty[n & 1]);
-                gemm::tc_commit(&s_accfull[acc]);
+                if (WRITE_A) commit<false>(&s_aempty[n & 1]);
+                commit<PAIR>(&s_accfull[acc]);
             }
             __syncwarp();
         }
         if (*failed && issue) {  // the MMAs in flight end before the accumulators are given back
-            gemm::tc_commit(&s_done);
+            if (PAIR)
+                asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(&s_done)) : "memory");
+            else
+                gemm::tc_commit(&s_done);
             for (uint32_t w = 0; w < kSpinLimit && !mbar_try_wait(&s_done, 0); ++w) {}
         }
         __syncwarp();
@@ -559,7 +657,7 @@ __global__ void __launch_bounds__(S::kThreads, S::kCtas)
         constexpr int kFly = 4;
         const int t64 = tid - 64;
         uint32_t n = 0;
-        for (int64_t tile = blockIdx.x; tile < tiles; tile += gridDim.x, ++n) {
+        for (int64_t tile = first; tile < tiles; tile += step, ++n) {
             const int mt = (int)(tile / p.nt_count);
             if (n >= 2 && !warp_wait(&s_aempty[n & 1], (n - 2) >> 1 & 1, failed)) break;
             uint8_t* codes = abuf + (n & 1) * S::a_buffer(nstages);
@@ -605,11 +703,11 @@ __global__ void __launch_bounds__(S::kThreads, S::kCtas)
         const int et = tid - 128;
         constexpr int kEt = 32 * S::kEpiWarps;
         uint32_t n = 0;
-        int2 of = blockIdx.x < tiles ? tile_of((int)(blockIdx.x / p.nt_count)) : make_int2(0, 0);
-        for (int64_t tile = blockIdx.x; tile < tiles && of.y; tile += gridDim.x, ++n) {
+        int2 of = first < tiles ? tile_of((int)(first / p.nt_count)) : make_int2(0, 0);
+        for (int64_t tile = first; tile < tiles && of.y; tile += step, ++n) {
             const int mt = (int)(tile / p.nt_count), nt = (int)(tile - (int64_t)mt * p.nt_count), mrows = of.y;
             const uint32_t acc = n % S::kAcc;
-            if (tile + gridDim.x < tiles) of = tile_of((int)((tile + gridDim.x) / p.nt_count));
+            if (tile + step < tiles) of = tile_of((int)((tile + step) / p.nt_count));
             if (warp == 4) {
                 const bool go = warp_wait(&s_accfull[acc], n / S::kAcc & 1, failed);
                 gemm::tc_fence_after();
@@ -713,11 +811,12 @@ __global__ void __launch_bounds__(S::kThreads, S::kCtas)
             __syncwarp();
         };
         uint32_t n = 0;
-        for (int64_t tile = blockIdx.x; tile < tiles; tile += gridDim.x, ++n) {
+        for (int64_t tile = first; tile < tiles; tile += step, ++n) {
             const int mt = (int)(tile / p.nt_count), nt = (int)(tile - (int64_t)mt * p.nt_count);
             const uint32_t acc = n % S::kAcc;
-            const int mrows = tile_of(mt).y;
-            if (mrows == 0) break;
+            const int all_rows = tile_of(mt).y;
+            if (all_rows == 0) break;
+            const int mrows = PAIR ? min(TM, max(0, all_rows - rank * TM)) : all_rows;
             if (!warp_wait(&s_accfull[acc], n / S::kAcc & 1, failed)) break;
             gemm::tc_fence_after();
             float v[S::kCols];
@@ -725,8 +824,11 @@ __global__ void __launch_bounds__(S::kThreads, S::kCtas)
             if (any) load_columns<S::kCols>(tmem + acc * NT + c0 + (quarter << 16), v);
             gemm::tc_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(&s_accempty[acc]);
-            const int64_t row = (int64_t)mt * TM + r;
+            if (lane == 0) {
+                if (PAIR) arrive_leader(&s_accempty[acc]);
+                else mbar_arrive(&s_accempty[acc]);
+            }
+            const int64_t row = (int64_t)mt * S::kTileRows + rank * TM + r;
             if (MODE == kGateUp) {
                 if (r >= mrows) continue;
 #pragma unroll
@@ -758,7 +860,7 @@ __global__ void __launch_bounds__(S::kThreads, S::kCtas)
                 continue;
             }
             if (S::kStaging && any && (MODE == kDown || p.tma_out)) {
-                const int y0 = mt * TM + (int)quarter;
+                const int y0 = mt * S::kTileRows + rank * TM + (int)quarter;
 #pragma unroll
                 for (int c = 0; c < S::kCols; c += 32) {
                     const int n0 = nt * NT + c0 + c;
@@ -811,9 +913,11 @@ __global__ void __launch_bounds__(S::kThreads, S::kCtas)
     if (s_failed && tid == 0) set_err(p.err, kErrFullWait);
     gemm::tc_fence_before();
     __syncthreads();
+    if (PAIR) cluster_sync();  // the peer's MMAs, reads and arrivals are over
     if (warp == 2) {
         gemm::tc_fence_after();
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(kTmemCols) : "memory");
+        if (PAIR) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(kTmemCols) : "memory");
+        else asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(kTmemCols) : "memory");
     }
 }
 
