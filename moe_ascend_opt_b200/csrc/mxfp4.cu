@@ -268,7 +268,8 @@ extern "C" int moe_mxfp4_matmul(const uint8_t* a, const uint8_t* a_scales, const
     }
     CUtensorMap ta, tb;
     if (int rc = encode(&ta, a, K / 2, M, 128)) return rc;
-    const bool wide = ceil_div(M, 128) * ceil_div(N, Pair::NT) >= sms;
+    // narrow tiles while all of them run at once (the rule at the shapes above)
+    const bool wide = ceil_div(M, 128) * ceil_div(N, Narrow::NT) > (int64_t)sms * Narrow::kCtas;
     p.mt_count = (int)ceil_div(M, wide ? Pair::kTileRows : Narrow::kTileRows);
     if (int rc = encode(&tb, b, K / 2, N, wide ? Pair::NT / 2 : Narrow::NT)) return rc;
     p.M = (int)M; p.N = (int)N; p.K = (int)K;
