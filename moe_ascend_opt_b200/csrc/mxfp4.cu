@@ -112,12 +112,22 @@ int sm_count(int dev, int* out) {
     return MOE_OK;
 }
 
-// Kernel shapes.  Wide: 128 x 256 tiles, for many rows (the tiles' loads from L2 bound it, which fall with
-// the tile's width); down has few stages a tile and many stores.  Narrow: 128 x 64, two CTAs per SM, for
-// dense products of too few wide tiles to fill the GPU.  Slim: 32 x 128, for experts with few rows each, where
-// the weights' stream from memory bounds the kernel: an MMA of 64 columns takes as long as one of 128, and two
-// CTAs with 32 x 64 tiles were held up by them.  Fused: 8 x 128, and small enough for a CTA of each
-// kernel on an SM, so that down's first weights arrive while gate_up runs.
+// Kernel shapes, and the rules that choose between them (times in us; layers have H = 2048, I = 768, 128
+// experts, top-8, and run in graphs).
+// Dense products.  Pair: 256 x 256 tiles of two CTAs, whose 35 KB a stage and CTA let six stages be in flight:
+// the ring's round trip (about 1 us plus a load's time) bounds wide tiles, so bytes per product count.  One-CTA
+// tiles of 128 x 256 (51 KB, four stages) took 59 at 8192 x 4096 x 4096 where pairs take 50 (5.5 PFLOP/s).
+// Narrow: 128 x 64, two CTAs per SM, for products whose narrow tiles all run at once:
+//   narrow | pairs: 1 x 4096 x 2048 5.5 | 7.5, 512 x 4096 x 4096 9.5 | 10.5, 1024 x 4096 x 4096 15.4 | 11.0.
+// Layers.  Wide: 128 x 256, from 32 rows an expert on; down has few stages a tile and many stores, so three
+// stages and four staging buffers.  Slim: 32 x 128, for fewer rows, where the weights' stream from memory
+// bounds the kernel: an MMA of 64 columns takes as long as one of 128, and two CTAs with 32 x 64 tiles were
+// held up by them.
+//   slim | wide, by rows an expert: 16 77 | 88, 32 99 | 99, 64 154 | 111.  (Pairs: 32 115, 128 148 | 138, 256 198 |
+//   193, 512 333 | 343 wide: not worth their kernels here.)
+// Fused: 8 x 128 and at most 16 pairs, small enough for a CTA of each kernel on an SM, so that down's first
+// weights arrive while gate_up runs; two launches instead of four, which is what an eager call pays for.
+//   fused | slim: T = 1 15.6 | 16.2, T = 2 22.1 | 21.3, T = 4 31.6 | 27.1.
 using Wide = mx::Shape<256, 128, 4, 8, 1, 1>;
 using WideDown = mx::Shape<256, 128, 3, 8, 1, 1, false, 4>;
 using Pair = mx::Shape<256, 128, 6, 8, 1, 1, false, 1, true>;
@@ -268,7 +278,7 @@ extern "C" int moe_mxfp4_matmul(const uint8_t* a, const uint8_t* a_scales, const
     }
     CUtensorMap ta, tb;
     if (int rc = encode(&ta, a, K / 2, M, 128)) return rc;
-    // narrow tiles while all of them run at once (the rule at the shapes above)
+    // narrow tiles while all of them run at once
     const bool wide = ceil_div(M, 128) * ceil_div(N, Narrow::NT) > (int64_t)sms * Narrow::kCtas;
     p.mt_count = (int)ceil_div(M, wide ? Pair::kTileRows : Narrow::kTileRows);
     if (int rc = encode(&tb, b, K / 2, N, wide ? Pair::NT / 2 : Narrow::NT)) return rc;

@@ -14,6 +14,16 @@
 // gate_up epilogue forms SiLU(gate) * up and quantises it without a word to other threads.
 // gate_up weights lie in 64-row groups of 32 gate rows and the 32 up rows of the same units.
 //
+// Large dense products run in pairs of CTAs (clusters of two): each fetches its 128 rows of A, half of B's rows
+// and its scales, all counted by CTA 0's barriers, and CTA 0 issues the MMAs of both (cta_group::2).  A thread
+// of CTA 1 that forwarded its stages to CTA 0 cost more than the sharing gave (64 us against 52 at
+// 8192 x 4096 x 4096).
+//
+// What bounds it: at many rows the ring's round trip, an MMA's end to the next data's arrival (about 1 us and a
+// load's latency for four to six stages), then the single accumulator's hand-over, about 1 us a tile; at few
+// rows the weights' stream.  Layers of H = 2048, I = 768, 128 experts, top-8: T = 4096 gate_up 76 us, down 59 us
+// (309 GFLOP of MMAs: 47 us at four times the measured bf16 rate); T = 201 of 64 experts gate_up 25, down 16 us.
+//
 // All waits are bounded; one that runs out sets the error word, and every role leaves its loop.
 #pragma once
 #include <cuda.h>
@@ -926,6 +936,8 @@ __global__ void __launch_bounds__(S::kThreads, S::kCtas)
 // quantised into the rows of their pairs.  A CTA takes a run of `tokens` tokens.  It needs, per
 // expert, the pairs before its run and the pairs in all: for short calls it counts all pairs
 // itself, for long ones the runs' counts come from mx_count_kernel.
+// T = 4096, H = 2048, top-8: 22 us (its 52 MB would take 8),
+// the counts 3.6 us; T = 201: 7.5 us.  A token is quantised once and written to the row of each of its pairs.
 constexpr int kPrepThreads = 512, kPrepWarps = kPrepThreads / 32, kPrepSelf = 4096;
 
 struct PrepParams {
@@ -1144,6 +1156,7 @@ __global__ void __launch_bounds__(kPrepThreads) mx_prep_kernel(const PrepParams 
 
 // y[t] = sum over the token's pairs, in their order, of w * part[row].  A warp takes 256 columns of a
 // token, a lane 8 of them; lane k holds the k-th pair's row and weight, and 8 parts are in flight.
+// T = 4096, H = 2048, top-8: 31 us for 155 MB, 5.0 TB/s; with fp32 parts twice the bytes.
 template <int DT, bool PART16>
 __global__ void __launch_bounds__(256, PART16 ? 3 : 2) mx_combine_kernel(const void* part, const uint8_t* pexp, const int32_t* ppos,
                                                          const float* tw, int T, int K, int H, void* y) {
