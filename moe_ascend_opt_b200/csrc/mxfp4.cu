@@ -3,8 +3,6 @@
 #include <atomic>
 #include <mutex>
 #include <new>
-#include <utility>
-#include <vector>
 
 #include "mx_layer.h"
 #include "mxfp4_gemm.cuh"
@@ -68,17 +66,14 @@ int encode_out(CUtensorMap* m, void* base, int64_t esz, int64_t cols, int64_t ro
 }
 
 // ------------------------------------------------------------------ launches
-// Opt-in shared memory of a kernel, once per kernel and device.
-int allow_smem(const void* fn, int bytes) {
-    static std::mutex mu;
-    static std::vector<std::pair<const void*, int>> done;
+// Opt-in shared memory of a kernel, once per device (a bit each).
+int allow_smem(const void* fn, int bytes, std::atomic<uint64_t>& devices) {
     int dev = 0;
     CUDA_TRY(cudaGetDevice(&dev));
-    std::lock_guard<std::mutex> lk(mu);
-    for (auto& d : done)
-        if (d.first == fn && d.second == dev) return MOE_OK;
+    const uint64_t bit = dev < 64 ? (uint64_t)1 << dev : 0;
+    if (devices.load(std::memory_order_acquire) & bit) return MOE_OK;
     CUDA_TRY(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
-    done.emplace_back(fn, dev);
+    devices.fetch_or(bit, std::memory_order_release);
     return MOE_OK;
 }
 
@@ -144,7 +139,8 @@ int launch_gemm(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap&
     auto fn = mx::mx_gemm_kernel<MODE, S>;
     constexpr bool WA = S::FUSED && MODE == mx::kGateUp;
     const int smem = S::smem(WA, (int)ceil_div(p.K, mx::kStageK));
-    if (int rc = allow_smem(reinterpret_cast<const void*>(fn), S::smem(WA, kFusedStages))) return rc;
+    static std::atomic<uint64_t> devices{0};
+    if (int rc = allow_smem(reinterpret_cast<const void*>(fn), S::smem(WA, kFusedStages), devices)) return rc;
     p.nt_count = (int)ceil_div(p.N, S::NT);
     const int64_t at_once = S::PAIR ? sms / 2 : sms * (S::FUSED ? 1 : S::kCtas);  // tiles
     const unsigned grid = (unsigned)(std::min(m_tiles * p.nt_count, at_once) * (S::PAIR ? 2 : 1));
@@ -313,7 +309,8 @@ struct MxLayer {
     CUtensorMap t1[2]{}, t2[2]{};
     uint8_t* ws = nullptr;
     size_t ws_bytes = 0;
-    std::vector<uint8_t*> retired;  // earlier workspaces: captured graphs may still hold them
+    uint8_t* retired[64] = {};  // earlier workspaces: captured graphs may still hold them
+    int n_retired = 0;
     size_t q1_expert() const { return (size_t)pn1 * st1 * mx::kPanel; }
     size_t q2_expert() const { return (size_t)pn2 * st2 * mx::kPanel; }
     size_t s1_expert() const { return (size_t)pn1 * st1 * mx::kPanelScales; }
@@ -439,6 +436,7 @@ int64_t slice_tokens(int64_t T, int64_t K) { return std::min(T, std::max<int64_t
 // graphs refer to it; sizes double, so that all of them hold at most twice the last.
 int grow(MxLayer* l, size_t bytes) {
     if (bytes <= l->ws_bytes) return MOE_OK;
+    if (l->n_retired == 64) return fail(MOE_ERR_STATE, "the workspace has grown too often");
     const size_t want = std::max(bytes, 2 * l->ws_bytes);
     uint8_t* p = nullptr;
     cudaError_t e = cudaMalloc(&p, want);
@@ -452,7 +450,7 @@ int grow(MxLayer* l, size_t bytes) {
         cudaGetLastError();
         return fail(MOE_ERR_CUDA, std::string("workspace of ") + std::to_string(bytes) + " bytes: " + cudaGetErrorString(e));
     }
-    if (l->ws) l->retired.push_back(l->ws);
+    if (l->ws) l->retired[l->n_retired++] = l->ws;
     l->ws = p;
     l->ws_bytes = got;
     return MOE_OK;
@@ -512,7 +510,8 @@ int forward_slice(MxLayer* l, const MxForward& f, const void* x, void* y, const 
     }
     const size_t psmem = ((size_t)(mx::kPrepWarps + 1) * E + (self ? T * f.K : r.tokens * f.K + 2 * E)) * 4;
     auto prep = f.act_dtype == MOE_BF16 ? mx::mx_prep_kernel<MOE_BF16> : mx::mx_prep_kernel<MOE_F16>;
-    if (int rc = allow_smem(reinterpret_cast<const void*>(prep), 128 * 1024)) return rc;
+    static std::atomic<uint64_t> prep_devices[2] = {};
+    if (int rc = allow_smem(reinterpret_cast<const void*>(prep), 128 * 1024, prep_devices[f.act_dtype == MOE_BF16])) return rc;
     if (int rc = launch(prep, runs, mx::kPrepThreads, psmem, f.pdl, st, r)) return rc;
     CUtensorMap tx, th, tx32, th32;  // boxes of a whole tile, and of 32 rows for tiles that are not full
     if (int rc = encode(&tx, w.xq, H / 2, w.mt * w.tile, w.tile)) return rc;
@@ -600,7 +599,7 @@ int mx_create(const moe_config& cfg, int num_sms, MxLayer** out) {
 void mx_destroy(MxLayer* l) {
     if (!l) return;
     for (uint8_t* p : {l->q1, l->s1, l->q2, l->s2, l->ws}) cudaFree(p);
-    for (uint8_t* p : l->retired) cudaFree(p);
+    for (uint8_t* p : l->retired) cudaFree(p);  // null where none is
     delete l;
 }
 

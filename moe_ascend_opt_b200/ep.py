@@ -213,6 +213,9 @@ class ExpertParallelMoE:
     def load_awq(self, *tensors):
         self.handle.store_awq(*tensors)
 
+    def load_mxfp4(self, w13, w13_scales, w2, w2_scales):
+        self.handle.store_mxfp4(w13, w13_scales, w2, w2_scales)
+
     def quantize_and_store_expert(self, e: int, proj: str, w):
         self.handle.quantize_and_store_expert(e, proj, w)
 

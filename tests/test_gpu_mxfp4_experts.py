@@ -319,6 +319,17 @@ def test_largest_and_smallest_sizes(E, H, I, K, T):
     close(y[torch.from_numpy(some).cuda()], want, tol)
 
 
+def test_expert_parallel_module():
+    from moe_ascend_opt_b200.ep import ExpertParallelMoE
+    E, H, I, K, T = 8, 128, 96, 4, 9
+    packed, _, _ = weights(E, H, I, 46)
+    x, ids, w = tokens(T, H, E, K, 47)
+    moe = ExpertParallelMoE(E, H, I, 3)
+    moe.load_mxfp4(*[torch.from_numpy(p) for p in packed])
+    want = ops.moe_forward(x, cuda(ids), cuda(w), handle(E, H, I, packed))
+    assert torch.equal(moe.forward(x, cuda(ids), cuda(w)), want)
+
+
 @pytest.mark.parametrize("T", [1, 3, 60, 300])
 def test_replicated_experts(T):
     """Ranks that share hot experts compute each pair once."""
