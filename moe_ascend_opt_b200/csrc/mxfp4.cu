@@ -114,20 +114,21 @@ int sm_count(int dev, int* out) {
 // tiles of 128 x 256 (51 KB, four stages) took 59 at 8192 x 4096 x 4096 where pairs take 50 (5.5 PFLOP/s).
 // Narrow: 128 x 64, two CTAs per SM, for products whose narrow tiles all run at once:
 //   narrow | pairs: 1 x 4096 x 2048 5.5 | 7.5, 512 x 4096 x 4096 9.5 | 10.5, 1024 x 4096 x 4096 15.4 | 11.0.
-// Layers.  Wide: 128 x 256, from 32 rows an expert on; down has few stages a tile and many stores, so three
+// Layers.  Wide: 128 x 256, from 56 rows an expert on; down has few stages a tile and many stores, so three
 // stages and four staging buffers.  Slim: 32 x 128, for fewer rows, where the weights' stream from memory
-// bounds the kernel: an MMA of 64 columns takes as long as one of 128, and two CTAs with 32 x 64 tiles were
-// held up by them.
-//   slim | wide, by rows an expert: 16 77 | 88, 32 99 | 99, 64 154 | 111.  (Pairs: 32 115, 128 148 | 138, 256 198 |
-//   193, 512 333 | 343 wide: not worth their kernels here.)
-// Fused: 8 x 128 and at most 16 pairs, small enough for a CTA of each kernel on an SM, so that down's first
+// bounds the kernel; two CTAs per SM with four stages each, so that down's first CTAs, and their weights, come in
+// as gate_up's leave (one CTA with nine stages: T = 4 27.1, 64 66.5, 256 76.8, now 24.6, 62.4, 72.6).  An MMA of 64
+// columns takes as long as one of 128, and 32 x 64 tiles were held up by them.
+//   slim | wide, by rows an expert: 16 73 | 88, 32 88 | 100, 48 106 | 108, 56 110 | 110, 64 123 | 112, 96 165 | 124.
+//   (Pairs: 32 115, 128 148 | 138 wide, 256 198 | 193, 512 333 | 343: not worth their kernels here.)
+// Fused: 8 x 128 and at most 8 pairs, small enough for a CTA of each kernel on an SM, so that down's first
 // weights arrive while gate_up runs; two launches instead of four, which is what an eager call pays for.
-//   fused | slim: T = 1 15.6 | 16.2, T = 2 22.1 | 21.3, T = 4 31.6 | 27.1.
+//   fused | slim: eager T = 1 23.3 | 25.6, T = 2 29.1 | 27.8; in graphs 15.8 | 15.3, 22.1 | 19.8.
 using Wide = mx::Shape<256, 128, 4, 8, 1, 1>;
 using WideDown = mx::Shape<256, 128, 3, 8, 1, 1, false, 4>;
 using Pair = mx::Shape<256, 128, 6, 8, 1, 1, false, 1, true>;
 using Narrow = mx::Shape<64, 128, 4, 4, 2, 2>;
-using Slim = mx::Shape<128, 32, 9, 4, 1, 2>;
+using Slim = mx::Shape<128, 32, 4, 4, 2, 1>;
 using FusedUp = mx::Shape<128, 8, 7, 4, 2, 1, true>;
 using FusedDown = mx::Shape<128, 8, 3, 4, 2, 1, true>;
 
@@ -378,10 +379,11 @@ __global__ void mx_store_rows_kernel(const void* w, int64_t n, int cols, int hal
 // their latencies are what counts; slim or wide tiles after a kernel that places the token rows, by the
 // rows that an expert can expect.
 enum Plan { kPlanFused, kPlanSlim, kPlanWide };
+constexpr int64_t kWideRows = 56;
 Plan plan_of(const MxLayer* l, int64_t T, int64_t K) {
     const int64_t P = T * K;
     if (P <= mx::kFusedPairs && l->st1 <= kFusedStages) return kPlanFused;
-    return P >= 32 * std::min(l->cfg.num_experts, P) ? kPlanWide : kPlanSlim;
+    return P >= kWideRows * std::min(l->cfg.num_experts, P) ? kPlanWide : kPlanSlim;
 }
 
 struct Workspace {
@@ -662,7 +664,7 @@ int mx_reserve(MxLayer* l, int64_t T, int64_t K) {
     // a shorter call may take another plan: the longest of each plan up to T
     const int64_t S = slice_tokens(T, K), E = l->cfg.num_experts;
     size_t bytes = 0;
-    for (int64_t t : {S, std::min(S, std::max<int64_t>(1, mx::kFusedPairs / K)), std::min(S, std::max<int64_t>(1, (32 * E - 1) / K))})
+    for (int64_t t : {S, std::min(S, std::max<int64_t>(1, mx::kFusedPairs / K)), std::min(S, std::max<int64_t>(1, (kWideRows * E - 1) / K))})
         bytes = std::max(bytes, carve(l, t, K, nullptr).bytes);
     return grow(l, bytes);
 }

@@ -35,7 +35,7 @@ namespace mx {
 
 enum Mode { kDense = 0, kGateUp = 1, kDown = 2 };
 constexpr int kStageK = 256;
-constexpr int kFusedPairs = 16;  // routed pairs of the calls whose two kernels route for themselves
+constexpr int kFusedPairs = 8;  // routed pairs of the calls whose two kernels route for themselves
 
 struct GemmParams {
     int M, N, K;         // dense: rows of a; N rows of b (of one expert); depth
@@ -330,14 +330,14 @@ MOE_DEV float silu_up(float g, float u) {
     return g * q * u;
 }
 
-// Routing of a fused call by the CTA itself: pieces of up to 8 pairs of one expert, in the order of
-// their first pairs, the pairs of a piece in their own order.
+// Routing of a fused call by the CTA itself: a piece per expert, in the order of their first pairs, the pairs
+// of a piece (at most 8, a tile's rows) in their own order.
 struct FusedRoute {
     int np;
     int e[kFusedPairs];                  // local expert of each pair, -1: another engine's
     int rank[kFusedPairs];               // among the pairs of its expert
     int piece_e[kFusedPairs], rows[kFusedPairs];
-    uint8_t pair[kFusedPairs * 8];       // pair of each row
+    uint8_t pair[kFusedPairs * kFusedPairs];  // pair of each row
 };
 
 template <bool FUSED>
@@ -372,12 +372,12 @@ MOE_DEV void fused_route(FusedRoute& f, const GemmParams& p, int threads) {
 #pragma unroll 8
         for (int j = 0; j <= i; ++j) {  // the piece's first pair comes at or before i
             const int rj = f.rank[j];
-            if (f.e[j] == e && rj == (rank & ~7)) piece = heads;
-            heads += rj >= 0 && (rj & 7) == 0;
+            if (f.e[j] == e && rj == 0) piece = heads;
+            heads += rj == 0;
         }
-        f.pair[piece * 8 + (rank & 7)] = (uint8_t)i;
-        atomicMax(&f.rows[piece], (rank & 7) + 1);
-        if ((rank & 7) == 0) {
+        f.pair[piece * kFusedPairs + rank] = (uint8_t)i;
+        atomicMax(&f.rows[piece], rank + 1);
+        if (rank == 0) {
             f.piece_e[piece] = e;
             atomicAdd(&f.np, 1);
         }
@@ -431,6 +431,7 @@ __global__ void __launch_bounds__(S::kThreads, S::kCtas)
     constexpr int NT = S::NT, TM = S::TM, STAGES = S::STAGES;
     constexpr bool PAIR = S::PAIR;
     static_assert(!PAIR || MODE == kDense, "pairs take dense products");
+    static_assert(!S::FUSED || TM == kFusedPairs, "all pairs of a fused call fit a tile");
     constexpr bool FUSED = S::FUSED, WRITE_A = FUSED && MODE == kGateUp;  // A from the token rows, by warps 2 and 3
     constexpr int kSfBase = S::kAcc * NT;  // TMEM: the accumulators, then each stage's scales
     constexpr int kTmemCols = kSfBase + STAGES * S::kSfCols <= 256 ? 256 : 512;
@@ -680,7 +681,7 @@ __global__ void __launch_bounds__(S::kThreads, S::kCtas)
                     const int u = u0 + 64 * f, r = u / per, k = (u - r * per) * 8;
                     q[f] = make_uint4(0u, 0u, 0u, 0u);
                     if (u < units && k < p.K) {
-                        const int64_t t = route.pair[mt * 8 + r] / p.topk;
+                        const int64_t t = route.pair[mt * kFusedPairs + r] / p.topk;
                         q[f] = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.x) + t * p.K + k));
                     }
                 }
@@ -770,7 +771,7 @@ __global__ void __launch_bounds__(S::kThreads, S::kCtas)
                 }
             } else {
                 for (int r = warp - 4; r < mrows; r += S::kEpiWarps) {
-                    const int64_t row = FUSED ? (int64_t)route.pair[mt * 8 + r] : (int64_t)mt * TM + r;  // fused parts lie by pair
+                    const int64_t row = FUSED ? (int64_t)route.pair[mt * kFusedPairs + r] : (int64_t)mt * TM + r;  // fused parts lie by pair
 #pragma unroll
                     for (int c = lane * 4; c < NT; c += 128)
                         if (nt * NT + c < p.N)  // rows are multiples of 32
