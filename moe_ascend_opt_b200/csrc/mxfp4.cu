@@ -530,6 +530,11 @@ int forward_slice(MxLayer* l, const MxForward& f, const void* x, void* y, const 
     mx::GemmParams g1 = p;
     g1.N = (int)(2 * I); g1.K = (int)H; g1.kb = (int)l->kb1;
     g1.sfa = w.xs; g1.sfb = l->s1; g1.hq = w.hq; g1.hs = w.hs; g1.hkb = (int)l->kb2;
+    if (self && !wide && f.pdl) {  // gate_up starts beside the token kernel, and finds its first weights by the ids
+        g1.ids = ids;
+        g1.T = (int)T; g1.topk = (int)f.K; g1.E = (int)E; g1.e_off = l->cfg.expert_offset;
+        g1.emap = f.emap; g1.emap_n = f.emap_n;
+    }
     if (int rc = wide ? launch_gemm<mx::kGateUp, Wide>(tx, l->t1[1], tx32, tx, tx, tx, g1, w.mt, l->sms, f.pdl, st)
                       : launch_gemm<mx::kGateUp, Slim>(tx, l->t1[0], tx, tx, tx, tx, g1, w.mt, l->sms, f.pdl, st))
         return rc;

@@ -72,6 +72,7 @@ template <int NT_, int TM_, int STAGES_, int EPI_, int CTAS_, int ACC_, bool FUS
 struct Shape {
     static constexpr int NT = NT_, TM = TM_, STAGES = STAGES_, kEpiWarps = EPI_, kCtas = CTAS_;
     static constexpr bool FUSED = FUSED_, PAIR = PAIR_;
+    static constexpr bool EARLY = TM == 32;  // gate_up fetches its first weights while the tokens are prepared
     static constexpr int BUFS = BUFS_;  // staging buffers of an epilogue warp
     static constexpr int kSfTiles = (NT + 127) / 128;  // scale tiles (128 rows) that cover a stage's B rows
     static constexpr int kA = TM * 128, kB = NT * 128 / (PAIR ? 2 : 1);
@@ -484,9 +485,41 @@ __global__ void __launch_bounds__(S::kThreads, S::kCtas)
     const uint32_t tmem = s_tmem;
     volatile int* failed = &s_failed;
     // down: the routing (ids, or the tiles' list) was complete before gate_up passed its own wait and let
-    // this kernel start, so the weights are fetched before the wait for gate_up's output
-    if (MODE != kDown) asm volatile("griddepcontrol.wait;" ::: "memory");
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    // this kernel start, so the weights are fetched before the wait for gate_up's output.  So does gate_up of a
+    // short call behind the token kernel, which let it start when the ids were there: it counts them itself to
+    // find its first tile's expert.
+    const bool ahead_of_list = MODE == kGateUp && S::EARLY && p.ids != nullptr;
+    int first_e = -1;
+    if (ahead_of_list) {
+        int* const hist = reinterpret_cast<int*>(smem + STAGES * kStage + S::tail(WRITE_A));  // the rows' place, idle so far
+        for (int e = tid; e < p.E; e += S::kThreads) hist[e] = 0;
+        __syncthreads();
+        const int P = p.T * p.topk;
+        for (int i = tid; i < P; i += S::kThreads) {
+            const int e = local_expert(__ldcg(p.ids + i), p.e_off, p.E, p.emap, p.emap_n, i, p.topk);
+            if (e >= 0) atomicAdd(&hist[e], 1);
+        }
+        __syncthreads();
+        if (warp == 0) {
+            const int mt0 = (int)(blockIdx.x / p.nt_count);
+            int before = 0;
+            for (int e0 = 0; e0 < p.E && first_e < 0; e0 += 32) {
+                const int n = e0 + lane < p.E ? (hist[e0 + lane] + TM - 1) / TM : 0;
+                int incl = n;
+#pragma unroll
+                for (int o = 1; o < 32; o <<= 1) {
+                    const int v = __shfl_up_sync(0xffffffffu, incl, o);
+                    if (lane >= o) incl += v;
+                }
+                const unsigned past = __ballot_sync(0xffffffffu, before + incl > mt0);
+                if (past) first_e = e0 + __ffs(past) - 1;
+                before += __shfl_sync(0xffffffffu, incl, 31);
+            }
+        }
+        __syncthreads();  // the rows' place is free
+    }
+    if (MODE != kDown && !(ahead_of_list && warp == 0)) asm volatile("griddepcontrol.wait;" ::: "memory");
+    if (!(ahead_of_list && warp == 0)) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     FusedRoute& route = reinterpret_cast<FusedRoute&>(s_route);  // an int where nothing is fused, never read
     if (FUSED) fused_route(route, p, S::kThreads);
 
@@ -531,11 +564,13 @@ __global__ void __launch_bounds__(S::kThreads, S::kCtas)
                 tma_2d_pair(base + oSfA, &tfa, s * 256, mt * 2 + rank, bar);
             }
         };
-        int2 next = first < tiles ? tile_of((int)(first / p.nt_count)) : make_int2(0, 0);
+        // of a first tile whose list is not there yet only the expert is known, and that it has rows
+        int2 next = ahead_of_list ? make_int2(first_e, first_e >= 0) : first < tiles ? tile_of((int)(first / p.nt_count)) : make_int2(0, 0);
         for (int64_t tile = first; ok && tile < tiles; tile += step) {
             const int mt = (int)(tile / p.nt_count), nt = (int)(tile - (int64_t)mt * p.nt_count);
             const int2 of = next;
-            if (tile + step < tiles) next = tile_of((int)((tile + step) / p.nt_count));  // a tile ahead of its use
+            const bool early = (MODE == kDown || ahead_of_list) && it == 0;
+            if (tile + step < tiles && !(ahead_of_list && early)) next = tile_of((int)((tile + step) / p.nt_count));  // a tile ahead of its use
             const int e = __shfl_sync(0xffffffffu, of.x, 0), rows = __shfl_sync(0xffffffffu, of.y, 0);
             if (rows == 0) break;
             const int copies = MODE == kDense || TM < 128 ? 4 : (rows + 31) >> 5;  // quarters of a 128-row tile
@@ -546,7 +581,6 @@ __global__ void __launch_bounds__(S::kThreads, S::kCtas)
             const int in_panel = nt * NT % kPanelRows;
             const uint8_t* sfb = MODE == kDense ? p.sfb + (int64_t)(nt * NT / 128) * p.kb * 512
                                                 : p.sfb + panel0 * kPanelScales + in_panel / 128 * 1024;
-            const bool early = MODE == kDown && it == 0;
             const int ahead = early ? min(STAGES, nstages) : 0;
             for (int s = 0; s < nstages; ++s, ++it) {
                 if (!warp_wait(&s_empty[st], parity, failed)) { ok = false; break; }
@@ -571,6 +605,7 @@ __global__ void __launch_bounds__(S::kThreads, S::kCtas)
                 __syncwarp();
                 if (!WRITE_A && s < ahead && s == ahead - 1) {
                     asm volatile("griddepcontrol.wait;" ::: "memory");
+                    if (ahead_of_list && tile + step < tiles) next = tile_of((int)((tile + step) / p.nt_count));
                     if (issue)
                         for (int a = 0; a < ahead; ++a) load_a(a, mt, a, copies);
                     __syncwarp();
@@ -581,7 +616,7 @@ __global__ void __launch_bounds__(S::kThreads, S::kCtas)
                 }
             }
         }
-        if (MODE == kDown && it == 0) asm volatile("griddepcontrol.wait;" ::: "memory");
+        if ((MODE == kDown || ahead_of_list) && it == 0) asm volatile("griddepcontrol.wait;" ::: "memory");
         // leave only when the copies have landed: a later owner of this shared memory must not be hit
         if (issue) {
             for (uint32_t b = 0; b < STAGES && b < it; ++b) {
