@@ -396,27 +396,25 @@ MOE_DEV void fused_combine(const FusedRoute& f, const GemmParams& p, int n0, int
     if (n >= p.N) return;
     for (int t = first; t < p.T; t += step) {
         float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (int k0 = 0; k0 < K; k0 += 8) {
-            float4 v[8];
-            float w[8];
+        float4 v[kFusedPairs];
+        float w[kFusedPairs];
 #pragma unroll
-            for (int k = 0; k < 8; ++k) {
-                const int i = t * K + k0 + k;
-                const bool have = k0 + k < K && f.e[min(i, p.T * K - 1)] >= 0;
-                v[k] = make_float4(0.f, 0.f, 0.f, 0.f);
-                w[k] = 0.f;
-                if (have) {
-                    v[k] = __ldcg(reinterpret_cast<const float4*>(part + (int64_t)i * p.N + n));
-                    w[k] = __ldg(p.tw + i);
-                }
+        for (int k = 0; k < kFusedPairs; ++k) {
+            const int i = t * K + k;
+            const bool have = k < K && f.e[min(i, p.T * p.topk - 1)] >= 0;
+            v[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+            w[k] = 0.f;
+            if (have) {
+                v[k] = __ldcg(reinterpret_cast<const float4*>(part + (int64_t)i * p.N + n));
+                w[k] = __ldg(p.tw + i);
             }
+        }
 #pragma unroll
-            for (int k = 0; k < 8; ++k) {
-                a.x = fmaf(w[k], v[k].x, a.x);
-                a.y = fmaf(w[k], v[k].y, a.y);
-                a.z = fmaf(w[k], v[k].z, a.z);
-                a.w = fmaf(w[k], v[k].w, a.w);
-            }
+        for (int k = 0; k < kFusedPairs; ++k) {
+            a.x = fmaf(w[k], v[k].x, a.x);
+            a.y = fmaf(w[k], v[k].y, a.y);
+            a.z = fmaf(w[k], v[k].z, a.z);
+            a.w = fmaf(w[k], v[k].w, a.w);
         }
         const int64_t at = (int64_t)t * p.N + n;
         if (DT == MOE_F32) *reinterpret_cast<float4*>(static_cast<float*>(p.y) + at) = a;
