@@ -522,6 +522,8 @@ __global__ void __launch_bounds__(S::kThreads, S::kCtas)
     if (!(ahead_of_list && warp == 0)) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     FusedRoute& route = reinterpret_cast<FusedRoute&>(s_route);  // an int where nothing is fused, never read
     if (FUSED) fused_route(route, p, S::kThreads);
+    // the producer alone goes ahead of gate_up's end: the bounded waits of the others must not count its time
+    if (MODE == kDown && warp != 0) asm volatile("griddepcontrol.wait;" ::: "memory");
 
     const int mt_count = FUSED ? route.np : p.mt_count;  // of an expert list its bound
     const int64_t tiles = (int64_t)mt_count * p.nt_count;
