@@ -12,7 +12,7 @@ using namespace moe;
 
 namespace {
 
-inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+using layer::ceil_div;
 
 // ------------------------------------------------------------------ tensor maps
 using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
@@ -132,7 +132,9 @@ using Slim = mx::Shape<128, 32, 4, 4, 2, 1>;
 using FusedUp = mx::Shape<128, 8, 7, 4, 2, 1, true>;
 using FusedDown = mx::Shape<128, 8, 3, 4, 2, 1, true>;
 
-constexpr int kFusedStages = 32;  // depth of fused calls: their A buffers hold it whole
+static_assert(FusedUp::TM == mx::kFusedRows && FusedDown::TM == mx::kFusedRows && Slim::TM == mx::kSlimRows &&
+                  Wide::TM == mx::kWideRows && WideDown::TM == mx::kWideRows,
+              "the workspace is laid out for these tiles");
 
 template <int MODE, class S>
 int launch_gemm(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& ta32, const CUtensorMap& to, const CUtensorMap& tfa,
@@ -141,7 +143,7 @@ int launch_gemm(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap&
     constexpr bool WA = S::FUSED && MODE == mx::kGateUp;
     const int smem = S::smem(WA, (int)ceil_div(p.K, mx::kStageK));
     static std::atomic<uint64_t> devices{0};
-    if (int rc = allow_smem(reinterpret_cast<const void*>(fn), S::smem(WA, kFusedStages), devices)) return rc;
+    if (int rc = allow_smem(reinterpret_cast<const void*>(fn), S::smem(WA, mx::kFusedStages), devices)) return rc;
     p.nt_count = (int)ceil_div(p.N, S::NT);
     const int64_t at_once = S::PAIR ? sms / 2 : sms * (S::FUSED ? 1 : S::kCtas);  // tiles
     const unsigned grid = (unsigned)(std::min(m_tiles * p.nt_count, at_once) * (S::PAIR ? 2 : 1));
@@ -320,8 +322,6 @@ struct MxLayer {
 
 namespace layer {
 
-constexpr int64_t kMaxPairs = 1 << 18;  // routed pairs of one pass; longer calls run in slices of tokens
-
 // Row of the input contract for row r of the layer: gate_up (map) rows lie in groups of 32 gate rows
 // and the 32 up rows of the same units.
 MOE_DEV int64_t source_row(int64_t r, int map, int64_t I) { return map ? ((r >> 5) & 1) * I + (r >> 6) * 32 + (r & 31) : r; }
@@ -375,64 +375,34 @@ __global__ void mx_store_rows_kernel(const void* w, int64_t n, int cols, int hal
     }
 }
 
-// How a call of T tokens runs.  Fused: two kernels that route for themselves, where the launches and
-// their latencies are what counts; slim or wide tiles after a kernel that places the token rows, by the
-// rows that an expert can expect.
-enum Plan { kPlanFused, kPlanSlim, kPlanWide };
-constexpr int64_t kWideRows = 56;
-Plan plan_of(const MxLayer* l, int64_t T, int64_t K) {
-    const int64_t P = T * K;
-    if (P <= mx::kFusedPairs && l->st1 <= kFusedStages) return kPlanFused;
-    return P >= kWideRows * std::min(l->cfg.num_experts, P) ? kPlanWide : kPlanSlim;
-}
-
 struct Workspace {
     int2* mt_list;
     int32_t *ppos, *counts;
     uint8_t *xq, *xs, *hq, *hs;
     uint8_t *part, *pexp;  // fp32 [rows][H], or 16-bit integers and exponents [rows][H / 32]
-    int64_t mt;  // bound of the number of m tiles
-    int tile;    // their rows
-    size_t bytes;
+    int64_t mt;
+    int tile;
 };
 
-// Tokens of one CTA of the token kernel: runs of 256 pairs or more and at most 512 runs in long
-// calls (every CTA reads all runs' counts), a 148th of a short call.
-int64_t prep_tokens(int64_t T, int64_t K) {
-    const int64_t P = T * K;
-    if (P <= mx::kPrepSelf) return ceil_div(T, 148);
-    return std::max<int64_t>(ceil_div(256, K), ceil_div(T, 512));
-}
+LayerShape shape_of(const MxLayer* l) { return {l->cfg.num_experts, l->cfg.hidden_size, l->cfg.intermediate_size}; }
 
-Workspace carve(const MxLayer* l, int64_t T, int64_t K, uint8_t* base) {
-    Workspace w{};
-    const int64_t P = T * K, H = l->cfg.hidden_size, I = l->cfg.intermediate_size;
-    const Plan plan = plan_of(l, T, K);
-    w.tile = plan == kPlanWide ? 128 : (plan == kPlanFused ? FusedUp::TM : Slim::TM);
-    w.mt = plan == kPlanFused ? P : P / w.tile + std::min(P, l->cfg.num_experts);
-    const int64_t rows = w.mt * w.tile;
-    size_t off = 0;
-    auto take = [&](size_t n) {
-        uint8_t* p = base + off;
-        off += (n + 1023) / 1024 * 1024;
-        return p;
-    };
-    w.hq = take(rows * (I / 2));
-    w.hs = take(w.mt * l->kb2 * 512);
-    w.part = take((size_t)(plan == kPlanFused ? P : rows) * H * 4);
-    if (plan != kPlanFused) {
-        w.pexp = take((size_t)rows * (H / 32));
-        w.mt_list = reinterpret_cast<int2*>(take(w.mt * 8));
-        w.ppos = reinterpret_cast<int32_t*>(take(P * 4));
-        w.counts = reinterpret_cast<int32_t*>(take(P > mx::kPrepSelf ? ceil_div(T, prep_tokens(T, K)) * l->cfg.num_experts * 4 : 0));
-        w.xq = take(rows * (H / 2));
-        w.xs = take(w.mt * l->kb1 * 512);
-    }
-    w.bytes = off;
-    return w;
+// The parts of the workspace for a call that runs in one pass.
+int carve(const MxLayer* l, int64_t T, int64_t K, Workspace& w) {
+    const Layout o = layout_of(shape_of(l), T, K);
+    if (o.bytes > l->ws_bytes) return fail(MOE_ERR_STATE, "the workspace is too small for this call");
+    w.mt_list = reinterpret_cast<int2*>(l->ws + o.mt_list);
+    w.ppos = reinterpret_cast<int32_t*>(l->ws + o.ppos);
+    w.counts = reinterpret_cast<int32_t*>(l->ws + o.counts);
+    w.xq = l->ws + o.xq;
+    w.xs = l->ws + o.xs;
+    w.hq = l->ws + o.hq;
+    w.hs = l->ws + o.hs;
+    w.part = l->ws + o.part;
+    w.pexp = l->ws + o.pexp;
+    w.mt = o.mt;
+    w.tile = o.tile;
+    return MOE_OK;
 }
-
-int64_t slice_tokens(int64_t T, int64_t K) { return std::min(T, std::max<int64_t>(1, kMaxPairs / K)); }
 
 // A workspace of at least `bytes`.  An outgrown one is kept until the engine goes, since captured
 // graphs refer to it; sizes double, so that all of them hold at most twice the last.
@@ -469,7 +439,8 @@ int combine_launch(const MxLayer* l, const MxForward& f, const float* tw, void* 
 int forward_fused(MxLayer* l, const MxForward& f, const void* x, void* y, const int32_t* ids, const float* tw, int64_t T,
                   cudaStream_t st) {
     const int64_t H = l->cfg.hidden_size, I = l->cfg.intermediate_size;
-    const Workspace w = carve(l, T, f.K, l->ws);
+    Workspace w;
+    if (int rc = carve(l, T, f.K, w)) return rc;
     CUtensorMap th;
     if (int rc = encode(&th, w.hq, I / 2, w.mt * w.tile, w.tile)) return rc;
     mx::GemmParams p{};
@@ -492,10 +463,11 @@ int forward_fused(MxLayer* l, const MxForward& f, const void* x, void* y, const 
 int forward_slice(MxLayer* l, const MxForward& f, const void* x, void* y, const int32_t* ids, const float* tw, int64_t T,
                   cudaStream_t st) {
     const int64_t E = l->cfg.num_experts, H = l->cfg.hidden_size, I = l->cfg.intermediate_size;
-    const Plan plan = plan_of(l, T, f.K);
+    const Plan plan = plan_of(shape_of(l), T, f.K);
     if (plan == kPlanFused) return forward_fused(l, f, x, y, ids, tw, T, st);
     const bool wide = plan == kPlanWide;
-    const Workspace w = carve(l, T, f.K, l->ws);
+    Workspace w;
+    if (int rc = carve(l, T, f.K, w)) return rc;
     mx::PrepParams r{};
     r.x = x; r.ids = ids;
     r.T = (int)T; r.K = (int)f.K; r.H = (int)H; r.E = (int)E; r.e_off = l->cfg.expert_offset;
@@ -666,18 +638,13 @@ int mx_export(MxLayer* l, int64_t expert, int32_t which, void* q_out, void* s_ou
 
 int mx_reserve(MxLayer* l, int64_t T, int64_t K) {
     if (T == 0) return MOE_OK;
-    // a shorter call may take another plan: the longest of each plan up to T
-    const int64_t S = slice_tokens(T, K), E = l->cfg.num_experts;
-    size_t bytes = 0;
-    for (int64_t t : {S, std::min(S, std::max<int64_t>(1, mx::kFusedPairs / K)), std::min(S, std::max<int64_t>(1, (kWideRows * E - 1) / K))})
-        bytes = std::max(bytes, carve(l, t, K, nullptr).bytes);
-    return grow(l, bytes);
+    return grow(l, reserve_bytes(shape_of(l), T, K));
 }
 
 int mx_forward(MxLayer* l, const MxForward& f, cudaStream_t st) {
     if (!aligned(f.x, 16) || !aligned(f.y, 16)) return fail(MOE_ERR_INVALID, "hidden and output must be 16-byte aligned");
     const int64_t S = slice_tokens(f.T, f.K), H = l->cfg.hidden_size;
-    const size_t need = carve(l, S, f.K, nullptr).bytes;
+    const size_t need = call_bytes(shape_of(l), f.T, f.K);
     if (need > l->ws_bytes) {
         cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
         CUDA_TRY(cudaStreamIsCapturing(st, &cap));

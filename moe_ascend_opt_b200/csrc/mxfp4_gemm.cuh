@@ -29,6 +29,7 @@
 #pragma once
 #include <cuda.h>
 
+#include "mx_plan.h"
 #include "mxfp4.cuh"
 
 namespace moe {
@@ -36,7 +37,6 @@ namespace mx {
 
 enum Mode { kDense = 0, kGateUp = 1, kDown = 2 };
 constexpr int kStageK = 256;
-constexpr int kFusedPairs = 8;  // routed pairs of the calls whose two kernels route for themselves
 
 struct GemmParams {
     int M, N, K;         // dense: rows of a; N rows of b (of one expert); depth
@@ -976,7 +976,7 @@ __global__ void __launch_bounds__(S::kThreads, S::kCtas)
 // itself, for long ones the runs' counts come from mx_count_kernel.
 // T = 4096, H = 2048, top-8: 22 us (its 52 MB would take 8),
 // the counts 3.6 us; T = 201: 7.5 us.  A token is quantised once and written to the row of each of its pairs.
-constexpr int kPrepThreads = 512, kPrepWarps = kPrepThreads / 32, kPrepSelf = 4096;
+constexpr int kPrepThreads = 512, kPrepWarps = kPrepThreads / 32;
 
 struct PrepParams {
     const void* x;

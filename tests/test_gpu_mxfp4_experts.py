@@ -409,3 +409,34 @@ def test_threads_with_streams_of_their_own():
     for t in threads:
         t.join()
     assert not bad
+
+
+def test_slices_of_different_runs():
+    """A long call whose last slice has more runs of the token kernel than the others: each token's row is that of
+    a call by itself."""
+    E, H, I, K, T = 1024, 32, 32, 51, 10260
+    packed, _, _ = weights(E, H, I, 52)
+    h = handle(E, H, I, packed)
+    x, ids, w = tokens(T, H, E, K, 53)
+    idc, wc = cuda(ids), cuda(w)
+    y = ops.moe_forward_partial(x, idc, wc, h)
+    for a, b in ((0, 300), (5000, 5300), (T - 300, T)):
+        assert torch.equal(y[a:b], ops.moe_forward_partial(x[a:b], idc[a:b].contiguous(), wc[a:b].contiguous(), h))
+    assert h.device_error() == 0
+
+
+def test_reserved_for_one_token_more():
+    """A captured call of fewer tokens than were reserved is accepted where the token kernel's runs change."""
+    E, H, I, K, T = 128, 64, 32, 8, 16384
+    packed, _, _ = weights(E, H, I, 54)
+    h = handle(E, H, I, packed)
+    x, ids, w = tokens(T, H, E, K, 55)
+    idc, wc = cuda(ids), cuda(w)
+    ctx = torch.classes.nanovllm.MoEGraphContext(h, T + 1, K, 1)
+    y = torch.zeros_like(x)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        ops.moe_forward_npu_graph_out(x, idc, wc, h, ctx, y)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(y, ops.moe_forward(x, idc, wc, h))

@@ -1,5 +1,7 @@
 """Refusals of the routing and MXFP4 entry points, without a GPU."""
 import ctypes as C
+import os
+import subprocess
 
 import pytest
 import torch
@@ -102,3 +104,61 @@ def test_ops_have_no_cpu_form():
                  lambda: torch.ops.nanovllm.mxfp4_tile_scales(torch.zeros(4, 2, dtype=torch.uint8))):
         with pytest.raises(NotImplementedError):
             call()
+
+
+PLAN = r"""
+#include "mx_plan.h"
+using namespace moe::layer;
+extern "C" int64_t layout_bytes(int64_t E, int64_t H, int64_t I, int64_t T, int64_t K) { return layout_of({E, H, I}, T, K).bytes; }
+extern "C" int64_t call_size(int64_t E, int64_t H, int64_t I, int64_t T, int64_t K) { return call_bytes({E, H, I}, T, K); }
+extern "C" int64_t reserve_size(int64_t E, int64_t H, int64_t I, int64_t T, int64_t K) { return reserve_bytes({E, H, I}, T, K); }
+extern "C" int64_t slice(int64_t T, int64_t K) { return slice_tokens(T, K); }
+extern "C" int64_t runs(int64_t T, int64_t K) { return ceil_div(T, prep_tokens(T, K)); }
+extern "C" int64_t runs_most(int64_t T, int64_t K) { return runs_bound(T, K); }
+// the first t in [lo, hi] whose layout is larger than `bytes`, or 0
+extern "C" int64_t first_above(int64_t E, int64_t H, int64_t I, int64_t K, int64_t lo, int64_t hi, int64_t bytes) {
+    for (int64_t t = lo; t <= hi; ++t)
+        if ((int64_t)layout_of({E, H, I}, t, K).bytes > bytes) return t;
+    return 0;
+}
+"""
+
+
+@pytest.fixture(scope="module")
+def plan(tmp_path_factory):
+    """The host arithmetic of the expert layer's workspace, compiled by itself."""
+    d = tmp_path_factory.mktemp("plan")
+    (d / "plan.cpp").write_text(PLAN)
+    csrc = os.path.join(os.path.dirname(moe_ascend_opt_b200.__file__), "csrc")
+    subprocess.check_call(["g++", "-O2", "-std=c++17", "-shared", "-fPIC", "-I", csrc, str(d / "plan.cpp"), "-o", str(d / "plan.so")])
+    lib = C.CDLL(str(d / "plan.so"))
+    for f in ("layout_bytes", "call_size", "reserve_size", "slice", "runs", "runs_most", "first_above"):
+        getattr(lib, f).restype = C.c_int64
+    return lambda name, *a: getattr(lib, name)(*[C.c_int64(v) for v in a])
+
+
+SHAPES = [(128, 2048, 768, 8), (1024, 32, 32, 51), (1024, 32, 32, 1), (1, 32, 32, 1), (3, 8224, 32, 2), (64, 2048, 768, 64), (8, 64, 32, 9)]
+
+
+@pytest.mark.parametrize("E,H,I,K", SHAPES)
+def test_reserve_covers_every_shorter_call(plan, E, H, I, K):
+    """What is reserved for T tokens holds every call of fewer: runs of the token kernel, plans and slices that change."""
+    S = plan("slice", 1 << 40, K)
+    ends = {1, 2, 8 // K, (56 * E - 1) // K, 56 * E // K, 4096 // K, 4096 // K + 1, S, S + 1, 3 * S}
+    ends |= {512 * n * max(1, 256 // K) + d for n in (1, 2) for d in (-1, 0, 1)} | {16384, 16385, 20000}
+    for T in sorted(t for t in ends if 0 < t):
+        assert plan("first_above", E, H, I, K, 1, min(T, S), plan("reserve_size", E, H, I, T, K)) == 0, T
+
+
+@pytest.mark.parametrize("E,H,I,K", SHAPES)
+def test_every_slice_of_a_call_fits(plan, E, H, I, K):
+    """The last slice of a long call is shorter and may need more than the others."""
+    S = plan("slice", 1 << 40, K)
+    for T in list(range(1, 400, 7)) + [S - 1, S, S + 1, 2 * S - 1] + [S + n for n in range(1, S, max(1, S // 700))]:
+        size = plan("call_size", E, H, I, T, K)
+        for t in {min(T, S), T % min(T, S)} - {0}:
+            assert plan("layout_bytes", E, H, I, t, K) <= size, (T, t)
+            if t * K > 4096:
+                assert plan("runs", t, K) <= plan("runs_most", t, K)
+    if (E, H, I, K) == (1024, 32, 32, 51):
+        assert plan("layout_bytes", E, H, I, 5120, K) <= plan("call_size", E, H, I, 10260, K)
