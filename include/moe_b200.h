@@ -118,8 +118,10 @@ int moe_engine_forward(moe_engine* eng, const void* x, void* y, const int32_t* t
 
 /* Dense MLP (a shared expert, or a dense FFN layer) through the same fused kernels:
  * y = down(SiLU(gate x) * up x) of local expert `expert` for every token, i.e.
- * moe_engine_forward with top_k = 1, that expert and weight 1 (the routing is kept in an
- * engine buffer, allocated on the first call with more tokens than before).  A shared expert
+ * moe_engine_forward with top_k = 1, that expert and weight 1.  Each expert's routing is an engine
+ * buffer of its own, written on its first call and on one with more tokens than it holds (a captured
+ * call included) and unchanged from then on, so that calls on any stream and captured ones keep
+ * their expert.  A shared expert
  * fuses into the routed layer without this call: load it as one more expert and pass its id
  * as an extra top-k column with its gate weight (1, or the model's shared-expert gate).
  * No counterpart in the reference, whose engine only serves routed experts. */

@@ -5,6 +5,7 @@
 
 #include <algorithm>
 #include <mutex>
+#include <new>
 #include <cstdio>
 #include <cstdlib>
 #include <cstring>
@@ -35,6 +36,16 @@ extern "C" const char* moe_last_error(void) { return g_last_error.c_str(); }
 static inline int64_t round_up(int64_t v, int64_t m) { return (v + m - 1) / m * m; }
 
 // ------------------------------------------------------------------ engine
+// The routing of dense calls of one expert: ids [cap] (the expert's global id) | weights [cap] (1.0).
+// Complete before the first call that takes it and never changed or freed while the engine lives, since
+// calls in flight and captured graphs read it; an outgrown one stays, and sizes double.
+struct DenseRoute {
+    int32_t gid;
+    int64_t cap;
+    int32_t* ids;
+    DenseRoute* next;
+};
+
 struct moe_engine {
     moe_config cfg{};
     int num_sms = 0;
@@ -73,8 +84,9 @@ struct moe_engine {
     int32_t emap_n = 0;
     std::vector<int32_t> emap_host;  // the map as set (flags included)
     int32_t rep_rank = 0, rep_world = 1;  // replicated experts: pairs with (token + id) % world == rank
-    void* dense_ids = nullptr;  // dense forward: routing ids [cap] (the expert) | weights [cap] (1.0)
-    int64_t dense_cap = 0, dense_expert = -1;
+    DenseRoute* dense = nullptr;  // routings of dense calls, the newest first
+    cudaStream_t dense_st = nullptr;  // writes them
+    std::mutex dense_mu;
     int32_t sk_cost_a = 3;  // its chunk cost model: streaming share per chunk vs one token of compute
     int32_t sk_min_chunks_per_cta = 2;  // use it from this many (unique expert x I/32) chunks per CTA
     // expert-parallel combine over peer memory (moe_engine_p2p_mailbox / _connect)
@@ -1426,7 +1438,12 @@ extern "C" int moe_engine_destroy(moe_engine* eng) {
     cudaFree(eng->agu);
     cudaFree(eng->adn);
     cudaFree(eng->clpart);
-    cudaFree(eng->dense_ids);
+    while (DenseRoute* r = eng->dense) {
+        eng->dense = r->next;
+        cudaFree(r->ids);
+        delete r;
+    }
+    if (eng->dense_st) cudaStreamDestroy(eng->dense_st);
     cudaFree(eng->clmeta);
     cudaFree(eng->emap);
     cudaFree(eng->part);
@@ -1954,6 +1971,44 @@ __global__ void fill_dense_route_kernel(int32_t* ids, float* w, int64_t n, int32
     }
 }
 
+// The routing of T tokens or more to expert gid.  A new one is filled on a stream of its own and waited for, so
+// that calls on any stream may read it; its allocation is allowed while a stream captures.
+static int dense_route(moe_engine* eng, int32_t gid, int64_t T, const DenseRoute** out) {
+    std::lock_guard<std::mutex> lk(eng->dense_mu);
+    for (const DenseRoute* r = eng->dense; r; r = r->next)
+        if (r->gid == gid && r->cap >= T) {
+            *out = r;
+            return MOE_OK;
+        }
+    int64_t cap = 64;
+    while (cap < T) cap *= 2;
+    DenseRoute* r = new (std::nothrow) DenseRoute{gid, cap, nullptr, nullptr};
+    if (!r) return fail(MOE_ERR_STATE, "out of host memory");
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+    cudaError_t e = cudaThreadExchangeStreamCaptureMode(&mode);
+    if (e == cudaSuccess) {
+        if (!eng->dense_st) e = cudaStreamCreateWithFlags(&eng->dense_st, cudaStreamNonBlocking);
+        if (e == cudaSuccess) e = cudaMalloc(&r->ids, (size_t)cap * 8);
+        if (e == cudaSuccess) {
+            fill_dense_route_kernel<<<(unsigned)((cap + 255) / 256), 256, 0, eng->dense_st>>>(
+                r->ids, reinterpret_cast<float*>(r->ids + cap), cap, gid);
+            e = cudaGetLastError();
+        }
+        if (e == cudaSuccess) e = cudaStreamSynchronize(eng->dense_st);
+        cudaThreadExchangeStreamCaptureMode(&mode);
+    }
+    if (e != cudaSuccess) {
+        cudaGetLastError();
+        cudaFree(r->ids);
+        delete r;
+        return fail(MOE_ERR_CUDA, std::string("routing of a dense call: ") + cudaGetErrorString(e));
+    }
+    r->next = eng->dense;
+    eng->dense = r;
+    *out = r;
+    return MOE_OK;
+}
+
 extern "C" int moe_engine_forward_dense(moe_engine* eng, int64_t expert, const void* x, void* y, int64_t T,
                                         int32_t act_dtype, int32_t out_dtype, void* stream) {
     if (int rc = check_engine(eng)) return rc;
@@ -1961,19 +2016,6 @@ extern "C" int moe_engine_forward_dense(moe_engine* eng, int64_t expert, const v
     if (T < 0) return fail(MOE_ERR_INVALID, "num_tokens must be >= 0");
     if (T == 0) return MOE_OK;
     DeviceGuard g(eng->cfg.device);
-    cudaStream_t st = static_cast<cudaStream_t>(stream);
-    if (T > eng->dense_cap) {
-        CUDA_TRY(cudaDeviceSynchronize());  // the old buffers may still be in use by queued work
-        cudaFree(eng->dense_ids);
-        eng->dense_ids = nullptr;
-        int64_t cap = std::max<int64_t>(64, eng->dense_cap);
-        while (cap < T) cap *= 2;
-        CUDA_TRY(cudaMalloc(&eng->dense_ids, (size_t)cap * 8));
-        eng->dense_cap = cap;
-        eng->dense_expert = -1;
-    }
-    int32_t* ids = reinterpret_cast<int32_t*>(eng->dense_ids);
-    float* w = reinterpret_cast<float*>(ids + eng->dense_cap);
     // global id of the expert for the routing (placement map or contiguous block)
     int32_t gid = (int32_t)(expert + eng->cfg.expert_offset);
     if (!eng->emap_host.empty()) {
@@ -1982,12 +2024,9 @@ extern "C" int moe_engine_forward_dense(moe_engine* eng, int64_t expert, const v
             if (eng->emap_host[gg] >= 0 && (eng->emap_host[gg] & ~kReplicaFlag) == expert) gid = (int32_t)gg;
         if (gid < 0) return fail(MOE_ERR_INVALID, "expert is not in this engine's placement map");
     }
-    if (eng->dense_expert != gid) {  // (re)fill on the stream; stays valid for later calls
-        fill_dense_route_kernel<<<(unsigned)((eng->dense_cap + 255) / 256), 256, 0, st>>>(ids, w, eng->dense_cap, gid);
-        CUDA_TRY(cudaGetLastError());
-        eng->dense_expert = gid;
-    }
-    return moe_engine_forward(eng, x, y, ids, w, T, 1, act_dtype, out_dtype, stream);
+    const DenseRoute* r = nullptr;
+    if (int rc = dense_route(eng, gid, T, &r)) return rc;
+    return moe_engine_forward(eng, x, y, r->ids, reinterpret_cast<const float*>(r->ids + r->cap), T, 1, act_dtype, out_dtype, stream);
 }
 
 extern "C" int moe_engine_last_time_ms(moe_engine* eng, double* ms) {

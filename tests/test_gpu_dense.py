@@ -62,3 +62,30 @@ def test_shared_expert_as_extra_column():
     y_ref = O.moe_forward_q(1, False, xf, ids9, w9, gq, gd, dq, dd)
     rel, cos = parity(y_fused.cpu().numpy(), y_ref)
     assert rel <= MAX_REL and cos >= MIN_COS, (rel, cos)
+
+
+@pytest.mark.parametrize("qt,T", [(1, 1), (1, 6), (0, 40)])
+def test_captured_dense_call_keeps_its_expert(qt, T):
+    """A captured dense call, of an expert that was called before or of a new one, is not changed by later dense calls."""
+    E, H, I = 4, 1024, 512
+    gq, gd, dq, dd = q_weights(qt, E, H, I, 90 + T)
+    h = torch.classes.nanovllm.MoEInfer(E, H, I, qt)
+    h.store_quantized_repack(torch.from_numpy(gq), torch.from_numpy(gd.view(np.int16)).view(torch.float16),
+                             torch.from_numpy(dq), torch.from_numpy(dd.view(np.int16)).view(torch.float16))
+    x = dev(tokens(T, H, E, 1, 90)[0].view(np.int16)).view(torch.bfloat16)
+    dense = torch.ops.nanovllm.moe_dense_forward
+    one = torch.ones(T, 1, device="cuda")
+    want = [torch.ops.nanovllm.moe_forward(x, torch.full((T, 1), e, device="cuda", dtype=torch.int32), one, h) for e in range(E)]
+    dense(x, 0, h)
+    torch.cuda.synchronize()
+    graphs, outs = [], []
+    for e in (0, 2):
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            outs.append(dense(x, e, h))
+    for e in (2, 1, 3):
+        assert torch.equal(dense(x, e, h), want[e])
+        for graph, out, of in zip(graphs, outs, (0, 2)):
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(out, want[of])

@@ -440,3 +440,70 @@ def test_reserved_for_one_token_more():
     graph.replay()
     torch.cuda.synchronize()
     assert torch.equal(y, ops.moe_forward(x, idc, wc, h))
+
+
+def test_dense_calls_in_graphs():
+    """A captured dense call keeps its expert: other experts, captures and longer calls in between change nothing."""
+    E, H, I, T = 4, 256, 128, 6
+    packed, _, _ = weights(E, H, I, 50)
+    h = handle(E, H, I, packed)
+    x = tokens(T, H, E, 1, 51)[0]
+    one = torch.ones(T, 1, device="cuda")
+
+    def routed(e):
+        return ops.moe_forward(x, torch.full((T, 1), e, device="cuda", dtype=torch.int32), one, h)
+
+    want = [routed(e) for e in range(E)]
+    assert torch.equal(ops.moe_dense_forward(x, 0, h), want[0])
+    graphs, outs = [], []
+    for e in (0, 2):  # an expert that was called before, and a new one
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            outs.append(ops.moe_dense_forward(x, e, h))
+    assert torch.equal(ops.moe_dense_forward(x, 2, h), want[2])  # not replayed yet
+    for e in (1, 3, 1):
+        assert torch.equal(ops.moe_dense_forward(x, e, h), want[e])
+        for graph, out, of in zip(graphs, outs, (0, 2)):
+            out.zero_()
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(out, want[of])
+
+
+def test_dense_calls_after_growth_and_on_streams():
+    """A captured dense call outlives longer calls of its expert; dense calls of two experts queued on two streams, and
+    from threads, each keep theirs."""
+    import threading
+    E, H, I, T = 3, 256, 128, 30
+    packed, _, _ = weights(E, H, I, 56)
+    h = handle(E, H, I, packed)
+    x = tokens(T, H, E, 1, 57)[0]
+    want = [ops.moe_dense_forward(x, e, h) for e in range(E)]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = ops.moe_dense_forward(x, 1, h)
+    ops.moe_dense_forward(tokens(3000, H, E, 1, 58)[0], 1, h)  # outgrows the captured routing
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(y, want[1])
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    outs = []
+    for i in range(20):
+        with torch.cuda.stream(streams[i % 2]):
+            outs.append(ops.moe_dense_forward(x, i % E, h))
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, want[i % E]) for i, o in enumerate(outs))
+    fresh, bad = handle(E, H, I, packed), []
+
+    def work(e):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(20):
+                if not torch.equal(ops.moe_dense_forward(x, e, fresh), want[e]):
+                    bad.append(e)
+
+    threads = [threading.Thread(target=work, args=(e,)) for e in range(E)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not bad
