@@ -117,7 +117,7 @@ struct moe_engine {
     uint8_t* gws = nullptr;
     size_t gws_bytes = 0;
     MxLayer* mx = nullptr;         // MXFP4: the layer's weights, workspace and kernels (mxfp4.cu)
-    cudaStream_t last_stream = nullptr;  // MXFP4: stream of the last forward (its end is ev1)
+    unsigned long long last_stream = 0;  // MXFP4: id of the last forward's stream (its end is ev1)
     std::mutex mx_mu;              // MXFP4: one thread at a time orders its call and launches it
     unsigned long long* timeline = nullptr;  // per-CTA phase stamps when enabled
     int timeline_ctas = 0;
@@ -1770,10 +1770,13 @@ extern "C" int moe_engine_forward(moe_engine* eng, const void* x, void* y, const
         CUDA_TRY(cudaStreamIsCapturing(st, &cap));
         const bool timed = cap == cudaStreamCaptureStatusNone;
         std::lock_guard<std::mutex> lk(eng->mx_mu);
+        unsigned long long id = 0;
         if (timed) {
-            // the workspace is the engine's: a call on another stream follows the last one (the
-            // per-thread stream is another one in each thread)
-            if (eng->timed && (eng->last_stream != st || st == cudaStreamPerThread)) CUDA_TRY(cudaStreamWaitEvent(st, eng->ev1, 0));
+            // the workspace is the engine's: a call on another stream follows the last one.  Streams are told
+            // apart by their ids: a destroyed one, whose work may still run, can give its handle to a new one, and
+            // the per-thread stream is another one in each thread.
+            CUDA_TRY(cudaStreamGetId(st, &id));
+            if (eng->timed && eng->last_stream != id) CUDA_TRY(cudaStreamWaitEvent(st, eng->ev1, 0));
             CUDA_TRY(cudaEventRecord(eng->ev0, st));
         }
         MxForward f{x, y, topk_ids, topk_w, T, K, act_dtype, out_dtype, eng->emap, eng->emap_n, eng->err,
@@ -1782,7 +1785,7 @@ extern "C" int moe_engine_forward(moe_engine* eng, const void* x, void* y, const
         if (timed) {  // after a failure too: what was launched before it still uses the workspace
             CUDA_TRY(cudaEventRecord(eng->ev1, st));
             eng->timed = true;
-            eng->last_stream = st;
+            eng->last_stream = id;
         }
         return rc;
     }

@@ -507,3 +507,32 @@ def test_dense_calls_after_growth_and_on_streams():
     for t in threads:
         t.join()
     assert not bad
+
+
+def test_streams_that_take_over_a_handle():
+    """Calls on a stream that is destroyed with work pending, then on a new stream that may have its handle."""
+    import ctypes
+    E, H, I, K, T = 8, 512, 256, 4, 4096
+    packed, _, _ = weights(E, H, I, 59)
+    h = handle(E, H, I, packed)
+    x, ids, w = tokens(T, H, E, K, 60)
+    idc, wc = cuda(ids), cuda(w)
+    short = (x[:2], idc[:2].contiguous(), wc[:2].contiguous())
+    want = ops.moe_forward(x, idc, wc, h), ops.moe_forward(*short, h)
+    torch.cuda.synchronize()
+    rt = torch.cuda.cudart()
+
+    def create():
+        p = ctypes.c_void_p()
+        assert int(rt.cudaStreamCreate(ctypes.addressof(p))) == 0
+        return p.value
+
+    outs = []
+    for _ in range(12):
+        a = create()
+        with torch.cuda.stream(torch.cuda.ExternalStream(a)):
+            outs.append([ops.moe_forward(*short, h)] + [ops.moe_forward(x, idc, wc, h) for _ in range(6)])
+        assert int(rt.cudaStreamDestroy(a)) == 0
+    torch.cuda.synchronize()
+    for first, *rest in outs:
+        assert torch.equal(first, want[1]) and all(torch.equal(o, want[0]) for o in rest)
