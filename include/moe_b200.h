@@ -99,8 +99,9 @@ int moe_engine_load_awq(moe_engine* eng, const void* w13_qweight, const void* w1
  * expert and a 16-bit output keep each pair's down row as 16-bit integers with an exponent per 32
  * columns until the sum (off by 2^-16 of the largest magnitude of the 32); others, and all with an
  * fp32 output, keep fp32.  x and y must be 16-byte aligned.  The workspace is the engine's: eager
- * calls on different streams, from one thread or several, are put in order; replays of captured
- * graphs that hold its calls must not overlap one another or such calls.
+ * calls on different streams, from one thread or several, are put in order, and so are the calls that
+ * one capture takes from several streams; replays of captured graphs that hold its calls must not
+ * overlap one another or eager calls.
  * A call that is captured needs moe_engine_reserve (or an earlier call of that size) first; the
  * graph stays valid when the workspace grows later.  The peer combine and the no-allocation
  * forward refuse such an engine. */

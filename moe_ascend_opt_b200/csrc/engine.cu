@@ -118,6 +118,9 @@ struct moe_engine {
     size_t gws_bytes = 0;
     MxLayer* mx = nullptr;         // MXFP4: the layer's weights, workspace and kernels (mxfp4.cu)
     unsigned long long last_stream = 0;  // MXFP4: id of the last forward's stream (its end is ev1)
+    unsigned long long cap_id = 0;       // MXFP4: capture and stream of the last captured forward
+    cudaStream_t cap_stream = nullptr;
+    cudaEvent_t cap_ev = nullptr;  // its end
     std::mutex mx_mu;              // MXFP4: one thread at a time orders its call and launches it
     unsigned long long* timeline = nullptr;  // per-CTA phase stamps when enabled
     int timeline_ctas = 0;
@@ -1420,6 +1423,8 @@ extern "C" int moe_engine_create(const moe_config* cfg, moe_engine** out) {
     if (rc == MOE_OK) rc = ensure_workspace(eng, 64);
     if (rc == MOE_OK && (cudaEventCreate(&eng->ev0) != cudaSuccess || cudaEventCreate(&eng->ev1) != cudaSuccess))
         rc = fail(MOE_ERR_CUDA, "cudaEventCreate failed");
+    if (rc == MOE_OK && eng->mx && cudaEventCreateWithFlags(&eng->cap_ev, cudaEventDisableTiming) != cudaSuccess)
+        rc = fail(MOE_ERR_CUDA, "cudaEventCreate failed");
     if (rc != MOE_OK) {
         moe_engine_destroy(eng);
         return rc;
@@ -1457,6 +1462,7 @@ extern "C" int moe_engine_destroy(moe_engine* eng) {
     cudaFree(eng->gws);
     if (eng->ev0) cudaEventDestroy(eng->ev0);
     if (eng->ev1) cudaEventDestroy(eng->ev1);
+    if (eng->cap_ev) cudaEventDestroy(eng->cap_ev);
     delete eng;
     return MOE_OK;
 }
@@ -1767,17 +1773,20 @@ extern "C" int moe_engine_forward(moe_engine* eng, const void* x, void* y, const
     if (T == 0) return MOE_OK;
     if (eng->mx) {
         cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
-        CUDA_TRY(cudaStreamIsCapturing(st, &cap));
+        unsigned long long id = 0, capture = 0;
+        CUDA_TRY(cudaStreamGetCaptureInfo(st, &cap, &capture));
         const bool timed = cap == cudaStreamCaptureStatusNone;
         std::lock_guard<std::mutex> lk(eng->mx_mu);
-        unsigned long long id = 0;
+        // The workspace is the engine's: a call on another stream follows the last one, eager calls the eager ones
+        // and calls of one capture each other, whose branches would run at once.  Streams are told apart by their
+        // ids: a destroyed one, whose work may still run, can give its handle to a new one, and the per-thread
+        // stream is another one in each thread.  (A capturing stream tells no id, and keeps its handle.)
         if (timed) {
-            // the workspace is the engine's: a call on another stream follows the last one.  Streams are told
-            // apart by their ids: a destroyed one, whose work may still run, can give its handle to a new one, and
-            // the per-thread stream is another one in each thread.
             CUDA_TRY(cudaStreamGetId(st, &id));
             if (eng->timed && eng->last_stream != id) CUDA_TRY(cudaStreamWaitEvent(st, eng->ev1, 0));
             CUDA_TRY(cudaEventRecord(eng->ev0, st));
+        } else if (eng->cap_id == capture && (eng->cap_stream != st || st == cudaStreamPerThread)) {
+            CUDA_TRY(cudaStreamWaitEvent(st, eng->cap_ev, 0));
         }
         MxForward f{x, y, topk_ids, topk_w, T, K, act_dtype, out_dtype, eng->emap, eng->emap_n, eng->err,
                     reinterpret_cast<unsigned int*>(reinterpret_cast<uint8_t*>(eng->bar) + 256), eng->pdl};
@@ -1786,6 +1795,10 @@ extern "C" int moe_engine_forward(moe_engine* eng, const void* x, void* y, const
             CUDA_TRY(cudaEventRecord(eng->ev1, st));
             eng->timed = true;
             eng->last_stream = id;
+        } else {
+            CUDA_TRY(cudaEventRecord(eng->cap_ev, st));
+            eng->cap_id = capture;
+            eng->cap_stream = st;
         }
         return rc;
     }

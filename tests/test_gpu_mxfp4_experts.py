@@ -536,3 +536,40 @@ def test_streams_that_take_over_a_handle():
     torch.cuda.synchronize()
     for first, *rest in outs:
         assert torch.equal(first, want[1]) and all(torch.equal(o, want[0]) for o in rest)
+
+
+def test_branches_of_one_graph():
+    """Calls that one capture takes from two streams without an order between them do not share the workspace at once."""
+    E, H, I, K = 8, 512, 256, 4
+    packed, _, _ = weights(E, H, I, 61)
+    h = handle(E, H, I, packed)
+    calls = []
+    for T in (2000, 30, 2):
+        x, ids, w = tokens(T, H, E, K, 62 + T)
+        calls.append((x, cuda(ids), cuda(w)))
+    want = [ops.moe_forward(*c, h) for c in calls] + [ops.moe_dense_forward(calls[0][0], 1, h)]
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    graph = torch.cuda.CUDAGraph()
+    outs = []
+    with torch.cuda.graph(graph):
+        main = torch.cuda.current_stream()
+        side.wait_stream(main)
+        for i in range(5):
+            outs.append((0, ops.moe_forward(*calls[0], h)))
+            with torch.cuda.stream(side):
+                outs.append((3, ops.moe_dense_forward(calls[0][0], 1, h)))
+                outs.append((1 + i % 2, ops.moe_forward(*calls[1 + i % 2], h)))
+        main.wait_stream(side)
+    for _ in range(3):
+        for _, o in outs:
+            o.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(o, want[i]) for i, o in outs)
+    again = torch.cuda.CUDAGraph()  # another capture does not wait for the first one's event
+    with torch.cuda.graph(again, stream=side):
+        o = ops.moe_forward(*calls[1], h)
+    again.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(o, want[1]) and torch.equal(ops.moe_forward(*calls[0], h), want[0])
