@@ -149,7 +149,7 @@ __device__ __noinline__ void route_row_exact(const RouteScoredParams& p, int64_t
 }
 
 
-// Floats as unsigned integers of the same order; 0 is below all of them.
+// Floats as unsigned integers of the same order; 0 is below all of them.  -0 falls below +0: callers have none.
 MOE_DEV uint32_t ordered(float v) {
     const uint32_t b = __float_as_uint(v);
     return b & 0x80000000u ? ~b : b | 0x80000000u;
@@ -230,7 +230,7 @@ __global__ void __launch_bounds__(kRouteWarps * 32) route_scored_kernel(const __
         for (int i = 0; i < NPL; ++i) l[i] = e0 + i < E ? load_logit(p.logits, base + e0 + i, DT) : -INFINITY;
     }
 #pragma unroll
-    for (int i = 0; i < NPL; ++i) l[i] = l[i] > -INFINITY ? fminf(l[i], kMostFloat) : -INFINITY;  // NaN: masked
+    for (int i = 0; i < NPL; ++i) l[i] = l[i] > -INFINITY ? fminf(l[i] + 0.f, kMostFloat) : -INFINITY;  // NaN: masked; -0 is 0
     const bool sums = p.groups > 1 && p.group_top > 1, scored = p.bias || sums;
     float top = 0.f, den = 1.f;
     if (!sigmoid) {

@@ -154,3 +154,34 @@ def test_agrees_with_softmax_router():
         a, b = torch.ops.nanovllm.moe_route(logits, 8, renorm), run(logits, None, 8, "softmax", renorm=renorm)
         assert torch.equal(a[0], b[0])
         torch.testing.assert_close(a[1], b[1], rtol=1e-5, atol=0)
+
+
+@pytest.mark.parametrize("dtype", sorted(TYPES))
+@pytest.mark.parametrize("E,groups,topk_groups,K", [(32, 1, 1, 16), (64, 1, 1, 30), (128, 4, 2, 24), (256, 8, 3, 8), (1024, 1, 1, 30), (60, 4, 2, 20)])
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+def test_signed_zeros_tie(score, E, groups, topk_groups, K, dtype):
+    """-0 and +0 are the same logit: logits times a 0/1 mask, rows of zeros and negatives, and rows whose last choice
+    is between one -0 and one +0, tie to the lower index."""
+    g = torch.Generator("cuda").manual_seed(E + K)
+    logits = torch.randn(80, E, generator=g, device="cuda")
+    logits[20:40] = -logits[20:40].abs()
+    logits[:40] *= torch.rand(40, E, generator=g, device="cuda") < 0.4
+    logits[40:60] = torch.where(torch.rand(20, E, generator=g, device="cuda") < 0.5, 0.0, -0.0)
+    per = E // groups
+    for t in range(60, 80):
+        logits[t] = -1.0 - logits[t].abs()
+        mine = torch.cat([gr * per + torch.randperm(per, generator=g, device="cuda") for gr in range(topk_groups)])
+        order = mine[torch.randperm(len(mine), generator=g, device="cuda")][:K + 1]
+        logits[t, order[:K - 1]] = 1.0 + torch.rand(K - 1, generator=g, device="cuda")
+        a, b = sorted(order[K - 1:].tolist())
+        logits[t, a], logits[t, b] = -0.0, 0.0
+    logits = logits.to(TYPES[dtype])
+    assert (logits.eq(0) & logits.signbit()).any()
+    check(logits, None, K, score, groups, topk_groups)
+    if groups > 1:
+        check(logits, None, K, score, groups, topk_groups, 2)
+        alone = torch.full((2, E), -1.0, device="cuda").to(TYPES[dtype])  # groups whose best are -0 and +0
+        alone[:, ::per] = 0.0
+        alone[:, :per * (groups // 2):per] = -0.0
+        check(alone, None, min(K, per), score, groups, 1)
+    check(logits, torch.zeros(E, device="cuda"), K, score, groups, topk_groups)
