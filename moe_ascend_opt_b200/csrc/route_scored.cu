@@ -269,7 +269,7 @@ __global__ void __launch_bounds__(kRouteWarps * 32) route_scored_kernel(const __
         }
 #pragma unroll
         for (int i = 0; i < NPL; ++i) {
-            // exp's argument and result lose 2e-7 of e and |v| 6e-8 of it, the reciprocal 1.2e-7 of s
+            // exp's result loses 2.4e-7 of e, its argument's rounding more where that is large; the reciprocal 1.2e-7 of s
             float s, e;
             asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"((sigmoid ? -l[i] : l[i] - top) * 1.44269504f));
             if (sigmoid) asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(s) : "f"(1.f + e));
@@ -279,7 +279,12 @@ __global__ void __launch_bounds__(kRouteWarps * 32) route_scored_kernel(const __
             key[i] = live ? (ordered(fminf(s + fminf(bias[i], kMostFloat), kMostFloat)) & ~kPlace) | (kPlace - i) : 0u;
         }
         most = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(most)));
-        tol = (sigmoid ? 1.4e-6f : 2.8e-6f) * most;
+        // what two scores may be off by, of the largest: 2 x 4.2e-7 and the argument's rounding, 7.3e-8 |l| of a score
+        // (softmax, of a difference: 1.33e-7), for the largest at most -log(most) times that and for smaller ones no
+        // more; a softmax's sum adds 6e-8 a term of its lane and 7.4e-7.  Below 1e-30, where approximations
+        // become zero, nothing is certain.
+        constexpr float base = sigmoid ? 1.4e-6f : 1.9e-6f + NPL * 6e-8f, slope = sigmoid ? 1.5e-7f : 2.7e-7f;
+        tol = most > 1e-30f ? most * (base - slope * __logf(most)) : INFINITY;
     } else {
 #pragma unroll
         for (int i = 0; i < NPL; ++i) key[i] = l[i] > -INFINITY ? (ordered(l[i]) & ~kPlace) | (kPlace - i) : 0u;

@@ -185,3 +185,45 @@ def test_signed_zeros_tie(score, E, groups, topk_groups, K, dtype):
         alone[:, :per * (groups // 2):per] = -0.0
         check(alone, None, min(K, per), score, groups, 1)
     check(logits, torch.zeros(E, device="cuda"), K, score, groups, topk_groups)
+
+
+@pytest.mark.parametrize("per", [4, 8])
+@pytest.mark.parametrize("low,high", [(-5, 3), (-45, -30), (-86, -45), (-110, -86)])
+def test_sums_of_small_scores(low, high, per):
+    """Groups by the sum of two sigmoid scores, the last that is kept and the first that is not nearly equal in it: far
+    below zero a score's relative error grows with its logit."""
+    T, G = 2000, 8
+    rng = np.random.default_rng(per - low)
+    l = low + (high - low) * rng.random((T, 1, 1)) - 3.0 - rng.random((T, G, per))
+    l[..., 0] += 3.0
+    l[..., 1] += 3.0
+    l = l.astype(np.float32).astype(np.float64)
+    s = 1 / (1 + np.exp(-l))
+    a, b = s[:, 0::2, :2].sum(-1), s[:, 1::2, 0]  # group 2j + 1 takes its second score from the sum of group 2j
+    rest = np.where(a > 1.1 * b, a - b, a / 2)
+    l[:, 1::2, 1] = np.log(rest / (1 - np.minimum(rest, 0.9)))
+    logits = torch.from_numpy(l.astype(np.float32).reshape(T, G * per)).cuda()
+    ids, _ = run(logits, None, 3 * per, "sigmoid", G, 3, 2)
+    ri, _ = R.route(logits.double().cpu().numpy(), None, 3 * per, "sigmoid", G, 3, 2)
+    np.testing.assert_array_equal(ids.cpu().numpy(), ri)
+
+
+@pytest.mark.parametrize("shift", [0.0, -10.0, -40.0, -70.0, -100.0])
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("E", [32, 256, 1024])
+def test_biases_that_level_small_scores(E, score, shift):
+    """Biases that bring pairs of choices to the same value, with scores far below one: all of a sigmoid's, and a
+    softmax's where the bias hides the largest logit.  A pair differs by the rounding of its biases."""
+    for seed in range(40):
+        g = torch.Generator("cuda").manual_seed(seed)
+        logits = shift + 0.05 * torch.randn(1, E, generator=g, device="cuda")
+        if score == "softmax":
+            logits[0, 3] = 1.0
+        s = torch.sigmoid(logits[0].double()) if score == "sigmoid" else torch.softmax(logits[0].double(), -1)
+        most = s[torch.arange(E, device="cuda") != 3].max()
+        level = 3.0 - 0.1 * (torch.randperm(E, generator=g, device="cuda") // 2).clamp(max=20)
+        bias = (level * most - s).float()
+        bias[3] = -float("inf")
+        ids, _ = run(logits, bias, 8, score)
+        ri, _ = R.route(logits.double().cpu().numpy(), bias.double().cpu().numpy(), 8, score)
+        np.testing.assert_array_equal(ids.cpu().numpy(), ri)
