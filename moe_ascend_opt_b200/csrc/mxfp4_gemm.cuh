@@ -320,10 +320,12 @@ MOE_DEV float part_low(uint32_t flipped) { return __uint_as_float(__byte_perm(fl
 MOE_DEV float part_high(uint32_t flipped) { return __uint_as_float(__byte_perm(flipped, 0x4b00u, 0x5432)) - 8421376.f; }
 
 // SiLU(g) * u.  exp(-g) = 2^t (1 + r ln 2) with t = -g log2(e) rounded and r what the rounding and
-// the constant lost, so that a large |g| costs no accuracy; below g = -88 exp overflows.
+// the constant lost, so that a large |g| costs no accuracy.  Past g = 128 exp(-g) adds nothing to 1, and t of the
+// largest g would be infinite; below g = -88 exp overflows, and SiLU, less than 6e-37, counts as 0.
 MOE_DEV float silu_up(float g, float u) {
-    const float t = -1.44269502f * g;
-    const float r = fmaf(g, -1.92596299e-8f, fmaf(g, -1.44269502f, -t));
+    const float c = fminf(g, 128.f);
+    const float t = -1.44269502f * c;
+    const float r = fmaf(c, -1.92596299e-8f, fmaf(c, -1.44269502f, -t));
     float e;
     asm("ex2.approx.f32 %0, %1;" : "=f"(e) : "f"(t));
     e = g < -88.f ? INFINITY : fmaf(e, 0.693147181f * r, e);

@@ -573,3 +573,18 @@ def test_branches_of_one_graph():
     again.replay()
     torch.cuda.synchronize()
     assert torch.equal(o, want[1]) and torch.equal(ops.moe_forward(*calls[0], h), want[0])
+
+
+@pytest.mark.parametrize("T", [1, 20, 300])
+def test_largest_gate(T):
+    """SiLU of a gate near the largest float is the gate: g = 6 * 2^125, h = .75 g, y = 4 * 2^125 * 2^-120."""
+    H = I = 32
+    c13, s13 = np.zeros((1, 2 * I, H), np.uint8), np.full((1, 2 * I, 1), 127, np.uint8)
+    c13[0, :I, 0], c13[0, I:, 0], s13[0, I:] = 2, 1, 0  # gate weight 1, up weight 2^-128
+    c2, s2 = np.zeros((1, H, I), np.uint8), np.full((1, H, 1), 7, np.uint8)
+    c2[0, :, 0] = 2
+    h = handle(1, H, I, (R.pack(c13), s13, R.pack(c2), s2))
+    x = torch.zeros(T, H, device="cuda", dtype=torch.bfloat16)
+    x[:, 0] = 2.5e38
+    y = ops.moe_forward(x, torch.zeros(T, 1, device="cuda", dtype=torch.int32), torch.ones(T, 1, device="cuda"), h)
+    assert (y == 128).all()
