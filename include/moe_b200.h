@@ -95,10 +95,8 @@ int moe_engine_load_awq(moe_engine* eng, const void* w13_qweight, const void* w1
  * The forward of such an engine quantises the token rows and h to MXFP4 too (both by the rule
  * of moe_quantize_rows_mxfp4) and multiplies codes by codes, accumulating in fp32:
  *   y = sum_k w_k * down(MX(SiLU(gate MX(x)) * (up MX(x)))).
- * A token row or an h block with an infinity or a NaN gives NaN.  Calls with 56 or more rows per
- * expert and a 16-bit output keep each pair's down row as 16-bit integers with an exponent per 32
- * columns until the sum (off by 2^-16 of the largest magnitude of the 32); others, and all with an
- * fp32 output, keep fp32.  x and y must be 16-byte aligned.  The workspace is the engine's: eager
+ * A token row or an h block with an infinity or a NaN gives NaN.  Parts and their sum are fp32, so a
+ * token's row does not depend on what else is in the call.  x and y must be 16-byte aligned.  The workspace is the engine's: eager
  * calls on different streams, from one thread or several, are put in order, and so are the calls that
  * one capture takes from several streams; replays of captured graphs that hold its calls must not
  * overlap one another or eager calls.

@@ -49,7 +49,7 @@ struct Layout {
     Plan plan;
     int tile;    // rows of an m tile
     int64_t mt;  // bound of the number of m tiles
-    size_t hq, hs, part, pexp, mt_list, ppos, counts, xq, xs, bytes;
+    size_t hq, hs, part, mt_list, ppos, counts, xq, xs, bytes;
 };
 inline Layout layout_of(const LayerShape& s, int64_t T, int64_t K) {
     Layout w{};
@@ -67,7 +67,6 @@ inline Layout layout_of(const LayerShape& s, int64_t T, int64_t K) {
     w.hs = take(w.mt * kb2 * 512);
     w.part = take((w.plan == kPlanFused ? P : rows) * s.H * 4);
     if (w.plan != kPlanFused) {
-        w.pexp = take(rows * (s.H / 32));
         w.mt_list = take(w.mt * 8);
         w.ppos = take(P * 4);
         w.counts = take(P > mx::kPrepSelf ? runs_bound(T, K) * s.E * 4 : 0);

@@ -379,7 +379,7 @@ struct Workspace {
     int2* mt_list;
     int32_t *ppos, *counts;
     uint8_t *xq, *xs, *hq, *hs;
-    uint8_t *part, *pexp;  // fp32 [rows][H], or 16-bit integers and exponents [rows][H / 32]
+    float* part;  // [rows][H]
     int64_t mt;
     int tile;
 };
@@ -397,8 +397,7 @@ int carve(const MxLayer* l, int64_t T, int64_t K, Workspace& w) {
     w.xs = l->ws + o.xs;
     w.hq = l->ws + o.hq;
     w.hs = l->ws + o.hs;
-    w.part = l->ws + o.part;
-    w.pexp = l->ws + o.pexp;
+    w.part = reinterpret_cast<float*>(l->ws + o.part);
     w.mt = o.mt;
     w.tile = o.tile;
     return MOE_OK;
@@ -428,11 +427,11 @@ int grow(MxLayer* l, size_t bytes) {
     return MOE_OK;
 }
 
-template <int DT, bool PART16>
+template <int DT>
 int combine_launch(const MxLayer* l, const MxForward& f, const float* tw, void* y, const Workspace& w, int64_t T, cudaStream_t st) {
     const int H = (int)l->cfg.hidden_size;
-    return launch(mx::mx_combine_kernel<DT, PART16>, (unsigned)std::min<int64_t>(ceil_div(T * ceil_div(H, 256), 8), l->sms * 16), 256, 0,
-                  f.pdl, st, (const void*)w.part, (const uint8_t*)w.pexp, (const int32_t*)w.ppos, tw, (int)T, (int)f.K, H, y);
+    return launch(mx::mx_combine_kernel<DT>, (unsigned)std::min<int64_t>(ceil_div(T * ceil_div(H, 256), 8), l->sms * 16), 256, 0,
+                  f.pdl, st, (const float*)w.part, (const int32_t*)w.ppos, tw, (int)T, (int)f.K, H, y);
 }
 
 // Two kernels: gate_up (routing, token rows quantised as they are needed), down with the weighted sum.
@@ -512,19 +511,16 @@ int forward_slice(MxLayer* l, const MxForward& f, const void* x, void* y, const 
         return rc;
     mx::GemmParams g2 = p;
     g2.N = (int)H; g2.K = (int)I; g2.kb = (int)l->kb2;
-    g2.sfa = w.hs; g2.sfb = l->s2; g2.out = w.part; g2.pexp = w.pexp;
-    const bool part16 = wide && f.out_dtype != MOE_F32;
-    g2.out_dtype = part16 ? MOE_F16 : MOE_F32;
+    g2.sfa = w.hs; g2.sfb = l->s2; g2.out = w.part; g2.out_dtype = MOE_F32;
     CUtensorMap tp = th;  // used by wide tiles
     if (wide)
-        if (int rc = encode_out(&tp, w.part, part16 ? 2 : 4, H, w.mt * w.tile)) return rc;
+        if (int rc = encode_out(&tp, w.part, 4, H, w.mt * w.tile)) return rc;
     if (int rc = wide ? launch_gemm<mx::kDown, WideDown>(th, l->t2[1], th32, tp, th, th, g2, w.mt, l->sms, f.pdl, st)
                       : launch_gemm<mx::kDown, Slim>(th, l->t2[0], th, tp, th, th, g2, w.mt, l->sms, f.pdl, st))
         return rc;
-    if (f.out_dtype == MOE_F32) return combine_launch<MOE_F32, false>(l, f, tw, y, w, T, st);
-    if (f.out_dtype == MOE_BF16)
-        return part16 ? combine_launch<MOE_BF16, true>(l, f, tw, y, w, T, st) : combine_launch<MOE_BF16, false>(l, f, tw, y, w, T, st);
-    return part16 ? combine_launch<MOE_F16, true>(l, f, tw, y, w, T, st) : combine_launch<MOE_F16, false>(l, f, tw, y, w, T, st);
+    return f.out_dtype == MOE_F32    ? combine_launch<MOE_F32>(l, f, tw, y, w, T, st)
+           : f.out_dtype == MOE_BF16 ? combine_launch<MOE_BF16>(l, f, tw, y, w, T, st)
+                                     : combine_launch<MOE_F16>(l, f, tw, y, w, T, st);
 }
 
 }  // namespace layer

@@ -21,7 +21,7 @@
 //
 // What bounds it: at many rows the ring's round trip, an MMA's end to the next data's arrival (about 1 us and a
 // load's latency for four to six stages), then the single accumulator's hand-over, about 1 us a tile; at few
-// rows the weights' stream.  Layers of H = 2048, I = 768, 128 experts, top-8: T = 4096 gate_up 76 us, down 59 us
+// rows the weights' stream.  Layers of H = 2048, I = 768, 128 experts, top-8: T = 4096 gate_up 77 us, down 65 us
 // (309 GFLOP of MMAs: 47 us at four times the measured bf16 rate); T = 201 of 64 experts gate_up 26, down 15 us
 // alone, 51 with the kernels around them, which overlap.
 //
@@ -45,10 +45,9 @@ struct GemmParams {
     const uint8_t* sfa;  // [m tiles][kb][512]
     const uint8_t* sfb;  // dense [ceil(N / 128)][kb][512]; experts [experts][ceil(N / 256)][stages][kPanelScales]
     const int2* mt_list;       // experts: expert and rows of each m tile; rows 0 ends it
-    void* out;           // dense [M][N] (out_dtype); down [m tile rows][N], fp32 or 16-bit parts
+    void* out;           // dense [M][N] (out_dtype); down [m tile rows][N] fp32 parts
     int out_dtype;
     int tma_out;         // dense, wide tiles: store through the map (rows of a multiple of 16 bytes)
-    uint8_t* pexp;       // down, 16-bit parts: exponent of each 32 columns [m tile rows][ceil(N / 32)]
     int I;               // gate_up: hq [m tile rows][I / 2], hs tiles with hkb tiles along I
     int hkb;
     uint8_t* hq;
@@ -293,31 +292,6 @@ MOE_DEV void store_row(void* out, int64_t at, const float* v, int n, bool vec) {
         }
     }
 }
-
-// A down row leaves wide tiles as 16-bit integers with one exponent per 32 columns: v = m 2^(e - 141),
-// e the exponent byte of the block's largest magnitude, so m is off by half a step of 2^-15 of that
-// power of two.  A sum of a token's parts so loses 2^-16 of the largest magnitude near each element where a
-// 16-bit output rounds to 2^-9 or 2^-12 of the element, and the parts' traffic is half of fp32's (which an
-// fp32 output keeps).  e = 255: the block held an infinity or a NaN, and is NaN.
-MOE_DEV uint32_t part_exponent(const float* v) {
-    uint32_t m = 0;
-#pragma unroll
-    for (int j = 0; j < 32; ++j) m = max(m, __float_as_uint(v[j]) & 0x7fffffffu);
-    return m >> 23;
-}
-// 2^(141 - e) and its inverse, e from 0 (a subnormal block counts as 15) to 254.
-MOE_DEV float part_scale(uint32_t e) { return __uint_as_float(min(268u - max(e, 15u), 253u) << 23); }
-MOE_DEV float part_unscale(uint32_t e) {
-    return e == 255u ? __uint_as_float(0x7fc00000u) : __uint_as_float((max(e, 15u) - 14u) << 23);
-}
-// Rounded v k, |v k| < 2^15, as the low 16 bits of a float near 1.5 2^23 (conversions run at an eighth of
-// the rate of sums); two of them a word, and a half of the word back as a float.
-MOE_DEV uint32_t part_pack(float a, float b, float k) {
-    const uint32_t x = __float_as_uint(fminf(a * k, 32767.f) + 12582912.f), y = __float_as_uint(fminf(b * k, 32767.f) + 12582912.f);
-    return __byte_perm(x, y, 0x5410);
-}
-MOE_DEV float part_low(uint32_t flipped) { return __uint_as_float(__byte_perm(flipped, 0x4b00u, 0x5410)) - 8421376.f; }
-MOE_DEV float part_high(uint32_t flipped) { return __uint_as_float(__byte_perm(flipped, 0x4b00u, 0x5432)) - 8421376.f; }
 
 // SiLU(g) * u.  exp(-g) = 2^t (1 + r ln 2) with t = -g log2(e) rounded and r what the rounding and
 // the constant lost, so that a large |g| costs no accuracy.  Past g = 128 exp(-g) adds nothing to 1, and t of the
@@ -911,36 +885,34 @@ __global__ void __launch_bounds__(S::kThreads, S::kCtas)
             }
             if (S::kStaging && any && (MODE == kDown || p.tma_out)) {
                 const int y0 = mt * S::kTileRows + rank * TM + (int)quarter;
+                auto store_fp32 = [&](const float* f, int n0) {
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        if (n0 + 16 * h >= p.N) break;
+                        uint32_t w[16];
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) w[j] = __float_as_uint(f[16 * h + j]);
+                        stage_row(w);
+                        if (lane == 0) tma_store_2d(&to, smem_u32(staging), n0 + 16 * h, y0);
+                    }
+                };
 #pragma unroll
                 for (int c = 0; c < S::kCols; c += 32) {
                     const int n0 = nt * NT + c0 + c;
                     if (n0 >= p.N) break;
-                    uint32_t w[16];
-                    if (p.out_dtype == MOE_F32) {
-#pragma unroll
-                        for (int h = 0; h < 2; ++h) {
-                            if (n0 + 16 * h >= p.N) break;
-#pragma unroll
-                            for (int j = 0; j < 16; ++j) w[j] = __float_as_uint(v[c + 16 * h + j]);
-                            stage_row(w);
-                            if (lane == 0) tma_store_2d(&to, smem_u32(staging), n0 + 16 * h, y0);
-                        }
-                        continue;
-                    }
-                    if (MODE == kDown) {
-                        const uint32_t e = part_exponent(v + c);
-                        const float k = part_scale(e);
-#pragma unroll
-                        for (int j = 0; j < 16; ++j) w[j] = part_pack(v[c + 2 * j], v[c + 2 * j + 1], k);
-                        if (r < mrows) p.pexp[row * ((p.N + 31) >> 5) + (n0 >> 5)] = (uint8_t)e;
+                    if constexpr (MODE == kDown) {
+                        store_fp32(v + c, n0);
+                    } else if (p.out_dtype == MOE_F32) {
+                        store_fp32(v + c, n0);
                     } else {
+                        uint32_t w[16];
 #pragma unroll
                         for (int j = 0; j < 16; ++j)
                             w[j] = p.out_dtype == MOE_BF16 ? pack16<MOE_BF16>(v[c + 2 * j], v[c + 2 * j + 1])
                                                            : pack16<MOE_F16>(v[c + 2 * j], v[c + 2 * j + 1]);
+                        stage_row(w);
+                        if (lane == 0) tma_store_2d(&to, smem_u32(staging), n0, y0);
                     }
-                    stage_row(w);
-                    if (lane == 0) tma_store_2d(&to, smem_u32(staging), n0, y0);
                 }
                 continue;
             }
@@ -1196,14 +1168,15 @@ __global__ void __launch_bounds__(kPrepThreads) mx_prep_kernel(const PrepParams 
 
 // y[t] = sum over the token's pairs, in their order, of w * part[row].  A warp takes 256 columns of a
 // token, a lane 8 of them; lane k holds the k-th pair's row and weight, and 8 parts are in flight.
-// T = 4096, H = 2048, top-8: 31 us for 155 MB, 5.0 TB/s; with fp32 parts twice the bytes.
-template <int DT, bool PART16>
-__global__ void __launch_bounds__(256, PART16 ? 3 : 2) mx_combine_kernel(const void* part, const uint8_t* pexp, const int32_t* ppos,
-                                                         const float* tw, int T, int K, int H, void* y) {
+// T = 4096, H = 2048, top-8: 45 us for 285 MB, 6.3 TB/s.  (Parts of 16 bits with an exponent per 32 columns took 31,
+// but lost a column beside one a few hundred times larger more than the output's rounding does.)
+template <int DT>
+__global__ void __launch_bounds__(256, 2) mx_combine_kernel(const float* part, const int32_t* ppos, const float* tw, int T, int K, int H,
+                                                            void* y) {
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     constexpr int kFly = 8;
-    const int lane = threadIdx.x & 31, chunks = (H + 255) >> 8, nb = H >> 5;
+    const int lane = threadIdx.x & 31, chunks = (H + 255) >> 8;
     const int64_t total = (int64_t)T * chunks;
     for (int64_t i = (blockIdx.x * (int64_t)blockDim.x + threadIdx.x) >> 5; i < total; i += (int64_t)gridDim.x * blockDim.x >> 5) {
         const int64_t t = i / chunks;
@@ -1216,43 +1189,25 @@ __global__ void __launch_bounds__(256, PART16 ? 3 : 2) mx_combine_kernel(const v
             const float myw = k0 + lane < K ? __ldg(tw + t * K + k0 + lane) : 0.f;
             for (int k1 = 0; k1 < min(32, K - k0); k1 += kFly) {
                 // no branch stands between the loads: of an absent pair row 0 is read, and weighs nothing
-                uint4 q[kFly][PART16 ? 1 : 2];
+                float4 q[kFly][2];
                 int pos[kFly];
-                uint32_t e[kFly];
-                float w[kFly];
 #pragma unroll
                 for (int f = 0; f < kFly; ++f) {
                     pos[f] = __shfl_sync(0xffffffffu, mypos, k1 + f);
-                    const int64_t row = max(pos[f], 0);
-                    if (PART16) {
-                        q[f][0] = __ldcs(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(part) + row * H + at8));
-                        e[f] = __ldcg(pexp + row * nb + (at8 >> 5));
-                    } else {
-                        const uint4* src = reinterpret_cast<const uint4*>(static_cast<const float*>(part) + row * H + at8);
-                        q[f][0] = __ldcs(src);
-                        q[f][PART16 ? 0 : 1] = __ldcs(src + 1);
-                        e[f] = 0;
-                    }
+                    const float4* src = reinterpret_cast<const float4*>(part + (int64_t)max(pos[f], 0) * H + at8);
+                    q[f][0] = __ldcs(src);
+                    q[f][1] = __ldcs(src + 1);
                 }
 #pragma unroll
                 for (int f = 0; f < kFly; ++f) {
-                    w[f] = __shfl_sync(0xffffffffu, myw, k1 + f);
-                    if (PART16) w[f] *= part_unscale(e[f]);
+                    float w = __shfl_sync(0xffffffffu, myw, k1 + f);
                     if (pos[f] < 0) {
-                        w[f] = 0.f;
-                        q[f][0] = q[f][PART16 ? 0 : 1] = make_uint4(0u, 0u, 0u, 0u);
+                        w = 0.f;
+                        q[f][0] = q[f][1] = make_float4(0.f, 0.f, 0.f, 0.f);
                     }
-                }
+                    const float v[8] = {q[f][0].x, q[f][0].y, q[f][0].z, q[f][0].w, q[f][1].x, q[f][1].y, q[f][1].z, q[f][1].w};
 #pragma unroll
-                for (int f = 0; f < kFly; ++f) {
-                    const uint32_t* r = reinterpret_cast<const uint32_t*>(&q[f][0]);
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        const uint32_t word = r[PART16 ? j / 2 : j];
-                        const float v = !PART16 ? __uint_as_float(word)
-                                                : (j & 1 ? part_high(word ^ 0x80008000u) : part_low(word ^ 0x80008000u));
-                        a[j] = fmaf(w[f], v, a[j]);
-                    }
+                    for (int j = 0; j < 8; ++j) a[j] = fmaf(w, v[j], a[j]);
                 }
             }
         }

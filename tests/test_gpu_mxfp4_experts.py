@@ -588,3 +588,35 @@ def test_largest_gate(T):
     x[:, 0] = 2.5e38
     y = ops.moe_forward(x, torch.zeros(T, 1, device="cuda", dtype=torch.int32), torch.ones(T, 1, device="cuda"), h)
     assert (y == 128).all()
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
+@pytest.mark.parametrize("T", [8, 40, 300])
+def test_columns_beside_a_large_one(T, dtype):
+    """An output column 2^12 times its neighbours takes no bits from them, however many rows the call has: parts
+    and sums hold 32 bits, the output is rounded once."""
+    E, H, I, K = 4, 96, 64, 2
+    rng = np.random.default_rng(48)
+    c13, s13 = R.quantize(0.05 * rng.standard_normal((E, 2 * I, H)))
+    w2 = 0.02 * rng.standard_normal((E, H, I))
+    w2[:, 5] *= 4096.0
+    w2[:, 70] *= 4096.0
+    c2, s2 = R.quantize(w2)
+    h = handle(E, H, I, (R.pack(c13), s13, R.pack(c2), s2))
+    x, ids, w = tokens(T, H, E, K, 49, dtype)
+    want, tol = R.experts(x.double().cpu().numpy(), ids, w, R.decode(c13, s13), R.decode(c2, s2), "float32")
+    tol = tol + R.HALF[dtype] * (np.abs(want) + tol) + (2.0 ** -25 if dtype == "float16" else 0.0)
+    close(ops.moe_forward(x, cuda(ids), cuda(w), h), want, tol)
+
+
+def test_sixteen_bit_rows_do_not_depend_on_the_batch():
+    """As for fp32 outputs: the plan that a call of many rows takes gives the bits of the plan for few."""
+    E, H, I, K, T = 4, 256, 160, 2, 400
+    packed, _, _ = weights(E, H, I, 63)
+    h = handle(E, H, I, packed)
+    for dtype in ("bfloat16", "float16"):
+        x, ids, w = tokens(T, H, E, K, 64, dtype)
+        idc, wc = cuda(ids), cuda(w)
+        full = ops.moe_forward(x, idc, wc, h)
+        for n in (1, 3, 64, 129):
+            assert torch.equal(full[:n], ops.moe_forward(x[:n], idc[:n].contiguous(), wc[:n].contiguous(), h))
