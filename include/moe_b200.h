@@ -295,6 +295,11 @@ int moe_engine_p2p_covers(moe_engine* eng, int64_t num_tokens);
 int moe_engine_set_expert_map(moe_engine* eng, const int32_t* local_of_global, int64_t num_global);
 /* This engine's rank and the world size for the replicated experts of its map (default 0 of 1). */
 int moe_engine_set_replica_split(moe_engine* eng, int32_t rank, int32_t world);
+/* Number of experts of the whole layer of which this engine holds a part (set by
+ * moe_engine_set_expert_map; for contiguous blocks call this before moe_engine_reserve; by default the
+ * engine's own).  Results do not depend on it: the MXFP4 layer takes from it how many rows an expert of
+ * the calls' pairs gets, and so its tiles; the other formats ignore it. */
+int moe_engine_set_layer_experts(moe_engine* eng, int64_t num_global);
 
 #ifdef __cplusplus
 }

@@ -28,7 +28,7 @@ SYMBOLS = [
     "moe_engine_set_expert_map", "moe_route_gemm_topk", "moe_engine_save", "moe_engine_load_file",
     "moe_engine_set_replica_split", "moe_engine_forward_dense",
     "moe_engine_load_mxfp4", "moe_route_scored", "moe_quantize_rows_mxfp4", "moe_dequantize_rows_mxfp4",
-    "moe_mxfp4_tile_scales", "moe_mxfp4_matmul",
+    "moe_mxfp4_tile_scales", "moe_mxfp4_matmul", "moe_engine_set_layer_experts",
 ]
 
 
@@ -83,6 +83,7 @@ def lib() -> C.CDLL:
             "moe_engine_set_replica_split": [_P, _I32, _I32],
             "moe_engine_forward_dense": [_P, _I64, _P, _P, _I64, _I32, _I32, _P],
             "moe_engine_load_file": [_P, C.c_char_p],
+            "moe_engine_set_layer_experts": [_P, _I64],
             "moe_engine_load_mxfp4": [_P, _P, _P, _P, _P, _I32, _P],
             "moe_route_scored": [_P, _I32, _P, _I64, _I64, _I64, _I32, _I64, _I64, _I32, _I32, C.c_float, _P, _P, _P],
             "moe_quantize_rows_mxfp4": [_P, _I32, _I64, _I64, _I32, _P, _P, _P],
@@ -169,6 +170,9 @@ class Engine:
 
     def set_replica_split(self, rank, world):
         call("moe_engine_set_replica_split", self.h, rank, world)
+
+    def set_layer_experts(self, num_global):
+        call("moe_engine_set_layer_experts", self.h, num_global)
 
     def forward_dense(self, expert, x, y, act_dtype, out_dtype, stream=None):
         call("moe_engine_forward_dense", self.h, expert, x.data_ptr(), y.data_ptr(), x.shape[0], act_dtype, out_dtype,

@@ -1757,9 +1757,9 @@ void fill_peer_combine(moe_engine* eng, PeerCombine& pc) {
     }
 }
 
-extern "C" int moe_engine_forward(moe_engine* eng, const void* x, void* y, const int32_t* topk_ids,
-                                  const float* topk_w, int64_t T, int64_t K, int32_t act_dtype, int32_t out_dtype,
-                                  void* stream) {
+// dense: every pair is this engine's
+static int forward_routed(moe_engine* eng, const void* x, void* y, const int32_t* topk_ids, const float* topk_w, int64_t T, int64_t K,
+                          int32_t act_dtype, int32_t out_dtype, void* stream, bool dense) {
     if (int rc = check_engine(eng)) return rc;
     if (!eng->loaded) return fail(MOE_ERR_STATE, "no weights loaded");
     if (T < 0 || K <= 0 || K > 64) return fail(MOE_ERR_INVALID, "num_tokens must be >= 0 and 1 <= top_k <= 64");
@@ -1789,7 +1789,7 @@ extern "C" int moe_engine_forward(moe_engine* eng, const void* x, void* y, const
             CUDA_TRY(cudaStreamWaitEvent(st, eng->cap_ev, 0));
         }
         MxForward f{x, y, topk_ids, topk_w, T, K, act_dtype, out_dtype, eng->emap, eng->emap_n, eng->err,
-                    reinterpret_cast<unsigned int*>(reinterpret_cast<uint8_t*>(eng->bar) + 256), eng->pdl};
+                    reinterpret_cast<unsigned int*>(reinterpret_cast<uint8_t*>(eng->bar) + 256), eng->pdl, dense};
         const int rc = mx_forward(eng->mx, f, st);
         if (timed) {  // after a failure too: what was launched before it still uses the workspace
             CUDA_TRY(cudaEventRecord(eng->ev1, st));
@@ -1978,6 +1978,12 @@ extern "C" int moe_engine_forward(moe_engine* eng, const void* x, void* y, const
     return MOE_OK;
 }
 
+extern "C" int moe_engine_forward(moe_engine* eng, const void* x, void* y, const int32_t* topk_ids,
+                                  const float* topk_w, int64_t T, int64_t K, int32_t act_dtype, int32_t out_dtype,
+                                  void* stream) {
+    return forward_routed(eng, x, y, topk_ids, topk_w, T, K, act_dtype, out_dtype, stream, false);
+}
+
 // Dense MLP through the same fused kernels: every token routed to one expert with weight 1.
 __global__ void fill_dense_route_kernel(int32_t* ids, float* w, int64_t n, int32_t expert) {
     const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
@@ -2042,7 +2048,7 @@ extern "C" int moe_engine_forward_dense(moe_engine* eng, int64_t expert, const v
     }
     const DenseRoute* r = nullptr;
     if (int rc = dense_route(eng, gid, T, &r)) return rc;
-    return moe_engine_forward(eng, x, y, r->ids, reinterpret_cast<const float*>(r->ids + r->cap), T, 1, act_dtype, out_dtype, stream);
+    return forward_routed(eng, x, y, r->ids, reinterpret_cast<const float*>(r->ids + r->cap), T, 1, act_dtype, out_dtype, stream, true);
 }
 
 extern "C" int moe_engine_last_time_ms(moe_engine* eng, double* ms) {
@@ -2486,7 +2492,19 @@ extern "C" int moe_engine_set_expert_map(moe_engine* eng, const int32_t* local_o
         if (v < 0 || l >= E || seen[l]++) return fail(MOE_ERR_INVALID, "expert map must send each local expert id once");
     }
     eng->emap_host.assign(local_of_global, local_of_global + num_global);
+    if (int rc = moe_engine_set_layer_experts(eng, std::max(num_global, E))) return rc;
     return upload_expert_map(eng);
+}
+
+extern "C" int moe_engine_set_layer_experts(moe_engine* eng, int64_t num_global) {
+    if (int rc = check_engine(eng)) return rc;
+    if (num_global < eng->cfg.num_experts || num_global > (1 << 20))
+        return fail(MOE_ERR_INVALID, "a layer has at least the engine's experts, and at most 2^20");
+    if (eng->mx) {
+        std::lock_guard<std::mutex> lk(eng->mx_mu);
+        mx_set_layer_experts(eng->mx, num_global);
+    }
+    return MOE_OK;
 }
 
 extern "C" int moe_engine_set_replica_split(moe_engine* eng, int32_t rank, int32_t world) {

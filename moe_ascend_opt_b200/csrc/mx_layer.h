@@ -28,6 +28,7 @@ struct MxForward {
     int32_t* err;
     unsigned int* cnt;  // counters [H / 64 or more], zero between calls
     bool pdl;
+    bool dense;         // every pair is this engine's
 };
 
 int mx_create(const moe_config& cfg, int num_sms, MxLayer** out);
@@ -36,6 +37,7 @@ int mx_load(MxLayer* l, const uint8_t* w13_q, const uint8_t* w13_s, const uint8_
 int mx_quantize_store(MxLayer* l, int64_t expert, int32_t proj, const void* w, int32_t dtype, cudaStream_t st);
 int mx_export(MxLayer* l, int64_t expert, int32_t which, void* q_out, void* s_out);
 void mx_buffers(MxLayer* l, MxBuffer (&b)[kMxBuffers]);
+void mx_set_layer_experts(MxLayer* l, int64_t n);
 int mx_reserve(MxLayer* l, int64_t T, int64_t K);
 int mx_forward(MxLayer* l, const MxForward& f, cudaStream_t st);
 

@@ -21,17 +21,19 @@ inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 struct LayerShape {
     int64_t E, H, I;
+    int64_t all = 0;  // experts that the call's pairs are spread over, of which this engine holds E (0: no others)
 };
 
 // How a call of T tokens runs.  Fused: two kernels that route for themselves, where the launches and
 // their latencies are what counts; slim or wide tiles after a kernel that places the token rows, by the
-// rows that an expert can expect.
+// rows that an expert can expect: the call's pairs over the experts of the whole layer, since a call on a part
+// of them is given the pairs of the others too.
 enum Plan { kPlanFused, kPlanSlim, kPlanWide };
 constexpr int64_t kWideExpert = 56;  // wide tiles from this many rows an expert on
 inline Plan plan_of(const LayerShape& s, int64_t T, int64_t K) {
     const int64_t P = T * K;
     if (P <= mx::kFusedPairs && ceil_div(s.H, 256) <= mx::kFusedStages) return kPlanFused;
-    return P >= kWideExpert * std::min(s.E, P) ? kPlanWide : kPlanSlim;
+    return P >= kWideExpert * std::max(s.E, s.all) ? kPlanWide : kPlanSlim;
 }
 
 // Tokens of one CTA of the token kernel: runs of 256 pairs or more and at most 512 runs in long
@@ -85,12 +87,16 @@ inline size_t call_bytes(const LayerShape& s, int64_t T, int64_t K) {
     return tail ? std::max(bytes, layout_of(s, tail, K).bytes) : bytes;
 }
 
-// Bytes for every call of 1 to T tokens: the longest of each plan.
-inline size_t reserve_bytes(const LayerShape& s, int64_t T, int64_t K) {
-    const int64_t S = slice_tokens(T, K);
+// Bytes for every call of 1 to T tokens, the longest of each plan: routed ones, and dense ones, whose pairs are
+// all this engine's.
+inline size_t reserve_bytes(LayerShape s, int64_t T, int64_t K) {
     size_t bytes = 0;
-    for (int64_t t : {S, std::min(S, std::max<int64_t>(1, mx::kFusedPairs / K)), std::min(S, std::max<int64_t>(1, (kWideExpert * s.E - 1) / K))})
-        bytes = std::max(bytes, layout_of(s, t, K).bytes);
+    for (int dense = 0; dense < 2; ++dense) {
+        const int64_t k = dense ? 1 : K, S = slice_tokens(T, k);
+        if (dense) s.all = 0;
+        for (int64_t t : {S, mx::kFusedPairs / k, (kWideExpert * std::max(s.E, s.all) - 1) / k})
+            bytes = std::max(bytes, layout_of(s, std::min(S, std::max<int64_t>(1, t)), k).bytes);
+    }
     return bytes;
 }
 

@@ -119,8 +119,9 @@ int sm_count(int dev, int* out) {
 // bounds the kernel; two CTAs per SM with four stages each, so that down's first CTAs, and their weights, come in
 // as gate_up's leave (one CTA with nine stages: T = 4 27.1, 64 66.5, 256 76.8, now 24.6, 62.4, 72.6).  An MMA of 64
 // columns takes as long as one of 128, and 32 x 64 tiles were held up by them.
-//   slim | wide, by rows an expert: 16 73 | 88, 32 88 | 100, 48 106 | 108, 56 110 | 110, 64 123 | 112, 96 165 | 124.
-//   (Pairs: 32 115, 128 148 | 138 wide, 256 198 | 193, 512 333 | 343: not worth their kernels here.)
+//   slim | wide, by rows an expert: 16 70 | 86, 32 87 | 100, 48 109 | 111, 56 119 | 114, 64 131 | 118, 96 169 | 135;
+//   16 of the 128 experts, an eighth of the pairs: 7 20.7 | 26.8, 32 32 | 34, 56 36.9 | 39.8, 80 43.5 | 44.5, 96 48.5 | 47.5.
+//   (Pairs, with 16-bit parts: 32 115, 128 148 | 138 wide, 256 198 | 193, 512 333 | 343: not worth their kernels here.)
 // Fused: 8 x 128 and at most 8 pairs, small enough for a CTA of each kernel on an SM, so that down's first
 // weights arrive while gate_up runs; two launches instead of four, which is what an eager call pays for.
 //   fused | slim: eager T = 1 23.3 | 25.6, T = 2 29.1 | 27.8; in graphs 15.8 | 15.3, 22.1 | 19.8.
@@ -305,6 +306,7 @@ namespace moe {
 struct MxLayer {
     moe_config cfg{};
     int sms = 0;
+    int64_t all_experts = 0;   // of the whole layer
     int64_t kb1 = 0, kb2 = 0;  // scale tiles along K of gate_up (1) and down (2)
     int64_t st1 = 0, st2 = 0, pn1 = 0, pn2 = 0;  // panels along K and N
     // panels of codes and their scales; maps of 128 and of 256 rows
@@ -384,11 +386,13 @@ struct Workspace {
     int tile;
 };
 
-LayerShape shape_of(const MxLayer* l) { return {l->cfg.num_experts, l->cfg.hidden_size, l->cfg.intermediate_size}; }
+LayerShape shape_of(const MxLayer* l, bool dense) {
+    return {l->cfg.num_experts, l->cfg.hidden_size, l->cfg.intermediate_size, dense ? 0 : l->all_experts};
+}
 
 // The parts of the workspace for a call that runs in one pass.
-int carve(const MxLayer* l, int64_t T, int64_t K, Workspace& w) {
-    const Layout o = layout_of(shape_of(l), T, K);
+int carve(const MxLayer* l, const MxForward& f, int64_t T, Workspace& w) {
+    const Layout o = layout_of(shape_of(l, f.dense), T, f.K);
     if (o.bytes > l->ws_bytes) return fail(MOE_ERR_STATE, "the workspace is too small for this call");
     w.mt_list = reinterpret_cast<int2*>(l->ws + o.mt_list);
     w.ppos = reinterpret_cast<int32_t*>(l->ws + o.ppos);
@@ -439,7 +443,7 @@ int forward_fused(MxLayer* l, const MxForward& f, const void* x, void* y, const 
                   cudaStream_t st) {
     const int64_t H = l->cfg.hidden_size, I = l->cfg.intermediate_size;
     Workspace w;
-    if (int rc = carve(l, T, f.K, w)) return rc;
+    if (int rc = carve(l, f, T, w)) return rc;
     CUtensorMap th;
     if (int rc = encode(&th, w.hq, I / 2, w.mt * w.tile, w.tile)) return rc;
     mx::GemmParams p{};
@@ -462,11 +466,11 @@ int forward_fused(MxLayer* l, const MxForward& f, const void* x, void* y, const 
 int forward_slice(MxLayer* l, const MxForward& f, const void* x, void* y, const int32_t* ids, const float* tw, int64_t T,
                   cudaStream_t st) {
     const int64_t E = l->cfg.num_experts, H = l->cfg.hidden_size, I = l->cfg.intermediate_size;
-    const Plan plan = plan_of(shape_of(l), T, f.K);
+    const Plan plan = plan_of(shape_of(l, f.dense), T, f.K);
     if (plan == kPlanFused) return forward_fused(l, f, x, y, ids, tw, T, st);
     const bool wide = plan == kPlanWide;
     Workspace w;
-    if (int rc = carve(l, T, f.K, w)) return rc;
+    if (int rc = carve(l, f, T, w)) return rc;
     mx::PrepParams r{};
     r.x = x; r.ids = ids;
     r.T = (int)T; r.K = (int)f.K; r.H = (int)H; r.E = (int)E; r.e_off = l->cfg.expert_offset;
@@ -632,15 +636,17 @@ int mx_export(MxLayer* l, int64_t expert, int32_t which, void* q_out, void* s_ou
     return MOE_OK;
 }
 
+void mx_set_layer_experts(MxLayer* l, int64_t n) { l->all_experts = n; }
+
 int mx_reserve(MxLayer* l, int64_t T, int64_t K) {
     if (T == 0) return MOE_OK;
-    return grow(l, reserve_bytes(shape_of(l), T, K));
+    return grow(l, reserve_bytes(shape_of(l, false), T, K));
 }
 
 int mx_forward(MxLayer* l, const MxForward& f, cudaStream_t st) {
     if (!aligned(f.x, 16) || !aligned(f.y, 16)) return fail(MOE_ERR_INVALID, "hidden and output must be 16-byte aligned");
     const int64_t S = slice_tokens(f.T, f.K), H = l->cfg.hidden_size;
-    const size_t need = call_bytes(shape_of(l), f.T, f.K);
+    const size_t need = call_bytes(shape_of(l, f.dense), f.T, f.K);
     if (need > l->ws_bytes) {
         cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
         CUDA_TRY(cudaStreamIsCapturing(st, &cap));

@@ -118,6 +118,7 @@ struct MoEInferHandle : torch::CustomClassHolder {
         cfg.device = device;
         cfg.expert_offset = (int32_t)expert_offset();
         check_rc(moe_engine_create(&cfg, &eng), "moe_engine_create");
+        check_rc(moe_engine_set_layer_experts(eng, E), "moe_engine_set_layer_experts");
         if (!placement.empty()) {
             std::vector<int32_t> m(E, -1);
             for (size_t l = 0; l < placement.size(); ++l) m[placement[l]] = (int32_t)l;

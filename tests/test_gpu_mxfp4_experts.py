@@ -620,3 +620,34 @@ def test_sixteen_bit_rows_do_not_depend_on_the_batch():
         full = ops.moe_forward(x, idc, wc, h)
         for n in (1, 3, 64, 129):
             assert torch.equal(full[:n], ops.moe_forward(x[:n], idc[:n].contiguous(), wc[:n].contiguous(), h))
+
+
+@pytest.mark.parametrize("T", [20, 300, 1000])
+def test_a_ranks_rows_are_the_layers(T):
+    """A rank's fp32 part has the bits of the whole engine's with the other ranks' pairs left out, whatever tiles
+    either takes; the C engine with its number of experts told, too."""
+    E, H, I, K, W = 64, 128, 96, 4, 8
+    packed, _, _ = weights(E, H, I, 65)
+    whole = handle(E, H, I, packed)
+    x, ids, w = tokens(T, H, E, K, 66)
+    idc, wc = cuda(ids), cuda(w)
+    for r in (0, 5):
+        lo, hi = r * E // W, (r + 1) * E // W
+        want = ops.moe_forward_partial(x, cuda(np.where((ids >= lo) & (ids < hi), ids, -1)), wc, whole)
+        rank = torch.classes.nanovllm.MoEInfer(E, H, I, 3)
+        rank.set_expert_parallel(r, W)
+        rank.store_mxfp4(*[torch.from_numpy(p) for p in packed])
+        assert torch.equal(ops.moe_forward_partial(x, idc, wc, rank), want)
+        eng = capi.Engine(E // W, H, I, capi.MXFP4, expert_offset=lo)
+        eng.load_mxfp4(*[torch.from_numpy(p[lo:hi].copy()) for p in packed])
+        for n in (E, E // W):
+            eng.set_layer_experts(n)
+            y = torch.empty(T, H, device="cuda")
+            eng.forward(x, y, idc, wc, capi.BF16, capi.F32)
+            assert torch.equal(y, want)
+        with pytest.raises(capi.MoeError, match="at least the engine"):
+            eng.set_layer_experts(E // W - 1)
+    one = torch.ones(T, 1, device="cuda")
+    for e in (0, 9):
+        want = ops.moe_forward(x, torch.full((T, 1), e, device="cuda", dtype=torch.int32), one, whole)
+        assert torch.equal(ops.moe_dense_forward(x, e, whole), want)

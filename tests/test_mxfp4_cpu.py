@@ -162,3 +162,48 @@ def test_every_slice_of_a_call_fits(plan, E, H, I, K):
                 assert plan("runs", t, K) <= plan("runs_most", t, K)
     if (E, H, I, K) == (1024, 32, 32, 51):
         assert plan("layout_bytes", E, H, I, 5120, K) <= plan("call_size", E, H, I, 10260, K)
+
+
+RANK = r"""
+#include "mx_plan.h"
+using namespace moe::layer;
+extern "C" int64_t plan(int64_t E, int64_t all, int64_t T, int64_t K) { return plan_of({E, 2048, 768, all}, T, K); }
+extern "C" int64_t reserve_size(int64_t E, int64_t all, int64_t T, int64_t K) { return reserve_bytes({E, 2048, 768, all}, T, K); }
+extern "C" int64_t call_size(int64_t E, int64_t all, int64_t T, int64_t K) { return call_bytes({E, 2048, 768, all}, T, K); }
+"""
+FUSED, SLIM, WIDE = 0, 1, 2
+
+
+@pytest.fixture(scope="module")
+def rank_plan(tmp_path_factory):
+    d = tmp_path_factory.mktemp("rank")
+    (d / "rank.cpp").write_text(RANK)
+    csrc = os.path.join(os.path.dirname(moe_ascend_opt_b200.__file__), "csrc")
+    subprocess.check_call(["g++", "-O2", "-std=c++17", "-shared", "-fPIC", "-I", csrc, str(d / "rank.cpp"), "-o", str(d / "rank.so")])
+    lib = C.CDLL(str(d / "rank.so"))
+    for f in ("plan", "reserve_size", "call_size"):
+        getattr(lib, f).restype = C.c_int64
+    return lambda name, *a: getattr(lib, name)(*[C.c_int64(v) for v in a])
+
+
+@pytest.mark.parametrize("W", [1, 2, 8])
+def test_plan_of_a_rank(rank_plan, W):
+    """A rank of W is given every rank's pairs and keeps a W-th: its tiles are those of the rows that its experts get."""
+    E, K = 128, 8
+    assert rank_plan("plan", E // W, E, 1, K) == FUSED
+    for rows in (1, 7, 55):
+        assert rank_plan("plan", E // W, E, rows * E // K, K) == SLIM
+    for rows in (56, 57, 400):
+        assert rank_plan("plan", E // W, E, rows * E // K, K) == WIDE
+    assert rank_plan("plan", E, 0, 1000, K) == WIDE and rank_plan("plan", E, 0, 800, K) == SLIM
+
+
+@pytest.mark.parametrize("E,all_", [(1, 1), (2, 0), (3, 24), (16, 128), (128, 0)])
+def test_reserve_of_a_rank(rank_plan, E, all_):
+    """It covers the routed calls and the dense ones, whose pairs are all the rank's."""
+    for K in (1, 2, 8):
+        if K <= max(E, all_):
+            for T in (1, 8, 9, 55, 56, 57, 500, 3000):
+                size = rank_plan("reserve_size", E, all_, T, K)
+                assert all(rank_plan("call_size", E, 0, t, 1) <= size and rank_plan("call_size", E, all_, t, K) <= size
+                           for t in range(1, T + 1)), (T, K)
