@@ -407,6 +407,7 @@ __global__ void __launch_bounds__(S::kThreads, S::kCtas)
     constexpr int NT = S::NT, TM = S::TM, STAGES = S::STAGES;
     constexpr bool PAIR = S::PAIR;
     static_assert(!PAIR || MODE == kDense, "pairs take dense products");
+    static_assert(MODE != kDown || TM < 128 || S::kStaging > 0, "down's tiles of 128 rows leave through shared memory");
     static_assert(!S::FUSED || TM == kFusedPairs, "all pairs of a fused call fit a tile");
     constexpr bool FUSED = S::FUSED, WRITE_A = FUSED && MODE == kGateUp;  // A from the token rows, by warps 2 and 3
     constexpr int kSfBase = S::kAcc * NT;  // TMEM: the accumulators, then each stage's scales
@@ -916,14 +917,14 @@ __global__ void __launch_bounds__(S::kThreads, S::kCtas)
                 }
                 continue;
             }
-            if (r < mrows) {
-                const int esz = MODE == kDown || p.out_dtype == MOE_F32 ? 4 : 2;
+            if (MODE == kDense && r < mrows) {
+                const int esz = p.out_dtype == MOE_F32 ? 4 : 2;
                 const bool vec = (int64_t)p.N * esz % 16 == 0;
 #pragma unroll
                 for (int c = 0; c < S::kCols; c += 32) {
                     const int n0 = nt * NT + c0 + c, left = min(32, p.N - n0);
                     if (left <= 0) break;
-                    if (MODE == kDown || p.out_dtype == MOE_F32) store_row<MOE_F32>(p.out, row * p.N + n0, v + c, left, vec);
+                    if (p.out_dtype == MOE_F32) store_row<MOE_F32>(p.out, row * p.N + n0, v + c, left, vec);
                     else if (p.out_dtype == MOE_BF16) store_row<MOE_BF16>(p.out, row * p.N + n0, v + c, left, vec);
                     else store_row<MOE_F16>(p.out, row * p.N + n0, v + c, left, vec);
                 }
