@@ -37,10 +37,10 @@ inline Plan plan_of(const LayerShape& s, int64_t T, int64_t K) {
 }
 
 // Tokens of one CTA of the token kernel: runs of 256 pairs or more and at most 512 runs in long
-// calls (every CTA reads all runs' counts), a 148th of a short call.
-inline int64_t prep_tokens(int64_t T, int64_t K) {
+// calls (every CTA reads all runs' counts), a CTA for each SM in a short call.
+inline int64_t prep_tokens(int64_t T, int64_t K, int sms) {
     const int64_t P = T * K;
-    if (P <= mx::kPrepSelf) return ceil_div(T, 148);
+    if (P <= mx::kPrepSelf) return ceil_div(T, sms);
     return std::max<int64_t>(ceil_div(256, K), ceil_div(T, 512));
 }
 // A bound of the runs of a long call that, unlike their number, does not fall as T grows.

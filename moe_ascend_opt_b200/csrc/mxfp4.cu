@@ -475,7 +475,7 @@ int forward_slice(MxLayer* l, const MxForward& f, const void* x, void* y, const 
     r.x = x; r.ids = ids;
     r.T = (int)T; r.K = (int)f.K; r.H = (int)H; r.E = (int)E; r.e_off = l->cfg.expert_offset;
     r.emap = f.emap; r.emap_n = f.emap_n;
-    r.tokens = (int)prep_tokens(T, f.K);
+    r.tokens = (int)prep_tokens(T, f.K, l->sms);
     r.tile_log2 = wide ? 7 : 5;
     r.mt_list = w.mt_list; r.mt_bound = (int)w.mt; r.ppos = w.ppos;
     r.xq = w.xq; r.xs = w.xs; r.kb = (int)l->kb1;

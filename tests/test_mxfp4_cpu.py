@@ -113,7 +113,7 @@ extern "C" int64_t layout_bytes(int64_t E, int64_t H, int64_t I, int64_t T, int6
 extern "C" int64_t call_size(int64_t E, int64_t H, int64_t I, int64_t T, int64_t K) { return call_bytes({E, H, I}, T, K); }
 extern "C" int64_t reserve_size(int64_t E, int64_t H, int64_t I, int64_t T, int64_t K) { return reserve_bytes({E, H, I}, T, K); }
 extern "C" int64_t slice(int64_t T, int64_t K) { return slice_tokens(T, K); }
-extern "C" int64_t runs(int64_t T, int64_t K) { return ceil_div(T, prep_tokens(T, K)); }
+extern "C" int64_t runs(int64_t T, int64_t K) { return ceil_div(T, prep_tokens(T, K, 148)); }
 extern "C" int64_t runs_most(int64_t T, int64_t K) { return runs_bound(T, K); }
 // the first t in [lo, hi] whose layout is larger than `bytes`, or 0
 extern "C" int64_t first_above(int64_t E, int64_t H, int64_t I, int64_t K, int64_t lo, int64_t hi, int64_t bytes) {
