@@ -1788,7 +1788,7 @@ static int forward_routed(moe_engine* eng, const void* x, void* y, const int32_t
         } else if (eng->cap_id == capture && (eng->cap_stream != st || st == cudaStreamPerThread)) {
             CUDA_TRY(cudaStreamWaitEvent(st, eng->cap_ev, 0));
         }
-        MxForward f{x, y, topk_ids, topk_w, T, K, act_dtype, out_dtype, eng->emap, eng->emap_n, eng->err,
+        MxForward f{x, y, topk_ids, topk_w, T, K, act_dtype, out_dtype, dense ? nullptr : eng->emap, eng->emap_n, eng->err,
                     reinterpret_cast<unsigned int*>(reinterpret_cast<uint8_t*>(eng->bar) + 256), eng->pdl, dense};
         const int rc = mx_forward(eng->mx, f, st);
         if (timed) {  // after a failure too: what was launched before it still uses the workspace
@@ -2038,9 +2038,10 @@ extern "C" int moe_engine_forward_dense(moe_engine* eng, int64_t expert, const v
     if (T < 0) return fail(MOE_ERR_INVALID, "num_tokens must be >= 0");
     if (T == 0) return MOE_OK;
     DeviceGuard g(eng->cfg.device);
-    // global id of the expert for the routing (placement map or contiguous block)
+    // global id of the expert for the routing (placement map or contiguous block; an MXFP4 layer takes dense calls
+    // past the map, which would give a replicated expert's tokens to other ranks)
     int32_t gid = (int32_t)(expert + eng->cfg.expert_offset);
-    if (!eng->emap_host.empty()) {
+    if (!eng->mx && !eng->emap_host.empty()) {
         gid = -1;
         for (size_t gg = 0; gg < eng->emap_host.size(); ++gg)
             if (eng->emap_host[gg] >= 0 && (eng->emap_host[gg] & ~kReplicaFlag) == expert) gid = (int32_t)gg;

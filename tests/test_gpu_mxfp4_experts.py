@@ -651,3 +651,21 @@ def test_a_ranks_rows_are_the_layers(T):
     for e in (0, 9):
         want = ops.moe_forward(x, torch.full((T, 1), e, device="cuda", dtype=torch.int32), one, whole)
         assert torch.equal(ops.moe_dense_forward(x, e, whole), want)
+
+
+@pytest.mark.parametrize("T", [5, 100])
+def test_dense_call_of_a_replicated_expert(T):
+    """It takes every token on the rank that makes it, not the rank's share of routed pairs."""
+    E, H, I, W = 6, 128, 96, 3
+    packed, _, _ = weights(E, H, I, 67)
+    whole = handle(E, H, I, packed)
+    x, _, _ = tokens(T, H, E, 1, 68)
+    h = torch.classes.nanovllm.MoEInfer(E, H, I, 3)
+    h.set_expert_parallel(1, W)
+    h.set_expert_placement([4, 0, 5])
+    h.set_expert_replicas([0])
+    h.store_mxfp4(*[torch.from_numpy(p) for p in packed])
+    for e in (4, 0, 5):
+        assert torch.equal(ops.moe_dense_forward(x, e, h), ops.moe_dense_forward(x, e, whole))
+    with pytest.raises(RuntimeError, match="not held"):
+        ops.moe_dense_forward(x, 1, h)
