@@ -337,6 +337,7 @@ at::Tensor moe_dense_forward(const at::Tensor& hidden, int64_t expert, const c10
     TORCH_CHECK(moe->eng, "no weights loaded");
     TORCH_CHECK(hidden.is_cuda() && hidden.dim() == 2 && hidden.size(1) == moe->H && hidden.is_contiguous(),
                 "hidden must be a contiguous CUDA [T, H] tensor");
+    TORCH_CHECK(hidden.get_device() == moe->device, "hidden must be on the engine's device");
     TORCH_CHECK(hidden.scalar_type() == at::kHalf || hidden.scalar_type() == at::kBFloat16,
                 "hidden must be float16 or bfloat16");
     c10::cuda::CUDAGuard g(moe->device);
