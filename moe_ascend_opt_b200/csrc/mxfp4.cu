@@ -111,7 +111,7 @@ int sm_count(int dev, int* out) {
 // experts, top-8, and run in graphs).
 // Dense products.  Pair: 256 x 256 tiles of two CTAs, whose 35 KB a stage and CTA let six stages be in flight:
 // the ring's round trip (about 1 us plus a load's time) bounds wide tiles, so bytes per product count.  One-CTA
-// tiles of 128 x 256 (51 KB, four stages) took 59 at 8192 x 4096 x 4096 where pairs take 50 (5.5 PFLOP/s).
+// tiles of 128 x 256 (51 KB, four stages) took 59 at 8192 x 4096 x 4096 where pairs take 50 (5.5 PFLOP/s; both with operands in L2, 60 without).
 // Narrow: 128 x 64, two CTAs per SM, for products whose narrow tiles all run at once:
 //   narrow | pairs: 1 x 4096 x 2048 5.5 | 7.5, 512 x 4096 x 4096 9.5 | 10.5, 1024 x 4096 x 4096 15.4 | 11.0.
 // Layers.  Wide: 128 x 256, from 56 rows an expert on; down has few stages a tile and many stores, so three

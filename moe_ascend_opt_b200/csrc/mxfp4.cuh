@@ -147,7 +147,7 @@ __global__ void tile_scales_kernel(const uint8_t* s, int64_t rows, int nb, uint8
 }
 
 // Codes and scales -> rows, 8 elements a thread; memory traffic again: 24577 x 768 to bf16 (48 MB, most of it
-// written) take 10.5 us, 4.6 TB/s.
+// written) take 10.5 us, 4.6 TB/s, with one load in flight a thread.
 template <int DT, bool TILED>
 __global__ void __launch_bounds__(256) dequantize_kernel(const uint8_t* q, const uint8_t* s, int64_t rows, int cols, void* y) {
     const int64_t n = rows * (cols >> 3);
