@@ -95,11 +95,11 @@ int moe_engine_load_awq(moe_engine* eng, const void* w13_qweight, const void* w1
  * The forward of such an engine quantises the token rows and h to MXFP4 too (both by the rule
  * of moe_quantize_rows_mxfp4) and multiplies codes by codes, accumulating in fp32:
  *   y = sum_k w_k * down(MX(SiLU(gate MX(x)) * (up MX(x)))).
- * A token row or an h block with an infinity or a NaN gives NaN.  Parts and their sum are fp32, so a
- * token's row does not depend on what else is in the call.  x and y must be 16-byte aligned.  The workspace is the engine's: eager
- * calls on different streams, from one thread or several, are put in order, and so are the calls that
- * one capture takes from several streams; replays of captured graphs that hold its calls must not
- * overlap one another or eager calls.
+ * A token row or an h block with an infinity or a NaN gives NaN.  Parts and their sum are fp32, and
+ * a token's row does not depend on what else is in the call.  x and y must be 16-byte aligned.
+ * The workspace is the engine's: eager calls on different streams, from one thread or several, are
+ * put in order, and so are the calls that one capture takes from several streams; replays of
+ * captured graphs that hold its calls must not overlap one another or eager calls.
  * A call that is captured needs moe_engine_reserve (or an earlier call of that size) first; the
  * graph stays valid when the workspace grows later.  The peer combine and the no-allocation
  * forward refuse such an engine. */
@@ -120,7 +120,8 @@ int moe_engine_forward(moe_engine* eng, const void* x, void* y, const int32_t* t
  * moe_engine_forward with top_k = 1, that expert and weight 1.  Each expert's routing is an engine
  * buffer of its own, written on its first call and on one with more tokens than it holds (a captured
  * call included) and unchanged from then on, so that calls on any stream and captured ones keep
- * their expert.  A shared expert
+ * their expert.  (A replicated expert's call takes every token on an MXFP4 engine, this rank's share
+ * of them on the others.)  A shared expert
  * fuses into the routed layer without this call: load it as one more expert and pass its id
  * as an extra top-k column with its gate weight (1, or the model's shared-expert gate).
  * No counterpart in the reference, whose engine only serves routed experts. */

@@ -118,7 +118,7 @@ struct moe_engine {
     size_t gws_bytes = 0;
     MxLayer* mx = nullptr;         // MXFP4: the layer's weights, workspace and kernels (mxfp4.cu)
     unsigned long long last_stream = 0;  // MXFP4: id of the last forward's stream (its end is ev1)
-    unsigned long long cap_id = 0;       // MXFP4: capture and stream of the last captured forward
+    unsigned long long cap_id = ~0ull;   // MXFP4: capture and stream of the last captured forward
     cudaStream_t cap_stream = nullptr;
     cudaEvent_t cap_ev = nullptr;  // its end
     std::mutex mx_mu;              // MXFP4: one thread at a time orders its call and launches it
